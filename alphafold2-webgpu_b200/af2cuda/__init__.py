@@ -11,6 +11,10 @@ from .attention import (AttentionGpu, AttentionInput, AttentionResult, Attention
 from .block import encode_evoformer_pair_block_tensors
 from .bundle import TriangleReferenceBundle, load_triangle_reference_bundle_from_files
 from .device import Device
+from .gradients import encode_clip_gradients_tensors, encode_gradient_norm_tensors, gradient_norm_workspace_bytes
+from .layers import (dense_saved_bytes, dense_workspace_bytes, encode_dense_backward_tensors, encode_dense_tensors,
+                     encode_gated_transition_backward_tensors, encode_gated_transition_tensors,
+                     gated_transition_saved_bytes, gated_transition_workspace_bytes)
 from .triangle import (TriangleGpuOptions, TriangleGpuResult, TriangleMultiplicationIncomingGpu,
                        TriangleMultiplicationOutgoingGpu, encode_triangle_multiplication,
                        encode_triangle_multiplication_tensors, triangle_weight_count, triangle_workspace_bytes)
@@ -49,4 +53,8 @@ __all__ = [
     "quantize_q8_block", "read_tensor_range", "tensor_byte_length", "tensor_elements", "write_tensor_manifest",
     "encode_outer_product_mean_weight_tensors", "encode_triangle_multiplication_weight_tensors", "opm_tensor_sizes",
     "stored_weights", "triangle_tensor_sizes", "PeerLost", "PeerMonitor", "comm_set_timeout", "comm_abort",
+    "dense_saved_bytes", "dense_workspace_bytes", "encode_dense_tensors", "encode_dense_backward_tensors",
+    "encode_gated_transition_tensors", "encode_gated_transition_backward_tensors", "gated_transition_saved_bytes",
+    "gated_transition_workspace_bytes", "encode_gradient_norm_tensors", "encode_clip_gradients_tensors",
+    "gradient_norm_workspace_bytes",
 ]

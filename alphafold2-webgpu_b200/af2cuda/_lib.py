@@ -98,6 +98,21 @@ class LinearShape(ctypes.Structure):
     _fields_ = [("rows", _i64), ("inner", _i64), ("columns", _i64)]
 
 
+class LayerOptions(ctypes.Structure):
+    _fields_ = [("activation", ctypes.c_int32), ("reserved", ctypes.c_int32), ("x_stride", _i64),
+                ("residual_stride", _i64), ("out_stride", _i64), ("d_x_stride", _i64)]
+
+
+class GatedWeights(ctypes.Structure):
+    _fields_ = [("gate_weight", _vp), ("gate_bias", _vp), ("value_weight", _vp), ("value_bias", _vp),
+                ("output_weight", _vp), ("output_bias", _vp)]
+
+
+class GatedGradients(ctypes.Structure):
+    _fields_ = [("x", _vp), ("gate_weight", _vp), ("gate_bias", _vp), ("value_weight", _vp), ("value_bias", _vp),
+                ("output_weight", _vp), ("output_bias", _vp)]
+
+
 SIGNATURES = {
     "af2_version": (_i32, []),
     "af2_status_string": (ctypes.c_char_p, [_i32]),
@@ -166,6 +181,25 @@ SIGNATURES = {
                              ctypes.POINTER(AttentionOptions), _vp, _i32, _vp, _vp]),
     "af2_evoformer_pair_block": (_i32, [_vp, ctypes.POINTER(PairBlockShape), ctypes.POINTER(PairBlockWeights), _vp, _i32,
                                         _vp, _vp, _i32, _vp, ctypes.POINTER(PairBlockOptions), _vp]),
+    "af2_dense_saved_bytes": (_i32, [ctypes.POINTER(LinearShape), _i32, _i32, ctypes.POINTER(ctypes.c_uint64)]),
+    "af2_dense_workspace_bytes": (_i32, [ctypes.POINTER(LinearShape), _i32, _i32, _i32,
+                                         ctypes.POINTER(ctypes.c_uint64)]),
+    "af2_dense": (_i32, [_vp, ctypes.POINTER(LinearShape), _i32, _vp, _vp, _vp, _vp, ctypes.POINTER(LayerOptions), _vp,
+                         _vp, _vp, _vp]),
+    "af2_dense_backward": (_i32, [_vp, ctypes.POINTER(LinearShape), _i32, _vp, _vp, _vp, _vp,
+                                  ctypes.POINTER(LayerOptions), _vp, _vp, _vp, _vp, _vp]),
+    "af2_gated_transition_saved_bytes": (_i32, [ctypes.POINTER(TransitionShape), _i32,
+                                                ctypes.POINTER(ctypes.c_uint64)]),
+    "af2_gated_transition_workspace_bytes": (_i32, [ctypes.POINTER(TransitionShape), _i32, _i32,
+                                                    ctypes.POINTER(ctypes.c_uint64)]),
+    "af2_gated_transition": (_i32, [_vp, ctypes.POINTER(TransitionShape), _i32, _vp, ctypes.POINTER(GatedWeights), _vp,
+                                    ctypes.POINTER(LayerOptions), _vp, _vp, _vp, _vp]),
+    "af2_gated_transition_backward": (_i32, [_vp, ctypes.POINTER(TransitionShape), _i32, _vp, _vp,
+                                             ctypes.POINTER(GatedWeights), _vp, ctypes.POINTER(LayerOptions),
+                                             ctypes.POINTER(GatedGradients), _vp, _vp]),
+    "af2_gradient_norm_workspace_bytes": (_i32, [_i64, ctypes.POINTER(ctypes.c_uint64)]),
+    "af2_gradient_norm": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp]),
+    "af2_clip_gradients": (_i32, [_vp, _vp, _vp, _i64, _f64, _vp, _vp, _vp]),
     "af2_linear_workspace_bytes": (_i32, [ctypes.POINTER(LinearShape), _i32, ctypes.POINTER(ctypes.c_uint64)]),
     "af2_linear": (_i32, [_vp, ctypes.POINTER(LinearShape), _vp, _i32, ctypes.POINTER(Matrix), _vp, _i32, _i32, _vp,
                           _i32, _vp, _vp]),

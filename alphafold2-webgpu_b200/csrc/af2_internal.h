@@ -67,6 +67,9 @@ enum ProfileKernel {
   kProfAttentionProject,
   kProfAttentionFlash,
   kProfAttentionOutput,
+  kProfLayerGemm,
+  kProfLayerElementwise,
+  kProfGradientNorm,
   kProfCount
 };
 const char *profile_name(int id);
@@ -114,6 +117,11 @@ struct af2_ctx {
   // af2_set_weight_cache: prepared weights kept per weights pointer and shape, made once
   bool weight_cache = false;
   std::vector<af2::CachedWeights> cached_weights;
+  // scratch of the layers with learned weights: `layer_done` is recorded after each call that
+  // uses it, and a call on another stream waits for it first
+  af2::DeviceBuffer layer_scratch;
+  cudaEvent_t layer_done = nullptr;
+  cudaStream_t layer_stream = nullptr;
 };
 
 namespace af2 {
@@ -409,6 +417,71 @@ AttentionLayout attention_layout(int64_t batch, int64_t queries, int64_t channel
 af2_status attention_launch(af2_ctx *ctx, const AttentionLayout &L, int transpose, const void *x, int x_dtype,
                             const float *mask, const float *packed, double eps, int residual, void *out,
                             int out_dtype, void *workspace, cudaStream_t stream);
+
+// ---- layers with learned weights (layers.cu: entry points; dense.cu: kernels) ----
+
+// Scratch of one call: the caller's workspace, or the context's with its use on other streams
+// waited for.  release() after the last launch.
+class LayerScratch {
+ public:
+  LayerScratch(af2_ctx *ctx, cudaStream_t stream) : ctx_(ctx), stream_(stream) {}
+  af2_status acquire(void *workspace, size_t bytes);
+  af2_status release();
+  uint8_t *base() const { return base_; }
+
+ private:
+  af2_ctx *ctx_;
+  cudaStream_t stream_;
+  uint8_t *base_ = nullptr;
+  bool owned_ = false, capturing_ = false;
+};
+
+struct DenseForward {
+  int64_t rows = 0, inner = 0, columns = 0;
+  int dtype = 0, activation = 0;
+  const void *x = nullptr, *weight = nullptr, *bias = nullptr, *residual = nullptr;
+  int64_t x_stride = 0, residual_stride = 0, out_stride = 0;
+  void *out = nullptr, *saved = nullptr;
+};
+struct DenseBackward {
+  int64_t rows = 0, inner = 0, columns = 0;
+  int dtype = 0, activation = 0;
+  const void *d_out = nullptr, *x = nullptr, *weight = nullptr, *saved = nullptr;
+  int64_t d_out_stride = 0, x_stride = 0, d_x_stride = 0;
+  void *d_x = nullptr, *d_weight = nullptr, *d_bias = nullptr;
+};
+struct GatedForward {
+  int64_t rows = 0, channels = 0, hidden = 0;
+  int dtype = 0, activation = 0;
+  const void *x = nullptr, *residual = nullptr;
+  af2_gated_weights w = {};
+  int64_t x_stride = 0, residual_stride = 0, out_stride = 0;
+  void *out = nullptr, *saved = nullptr;
+};
+struct GatedBackward {
+  int64_t rows = 0, channels = 0, hidden = 0;
+  int dtype = 0, activation = 0;
+  const void *d_out = nullptr, *x = nullptr, *saved = nullptr;
+  af2_gated_weights w = {};
+  af2_gated_gradients g = {};
+  int64_t d_out_stride = 0, x_stride = 0, d_x_stride = 0;
+};
+uint64_t dense_saved_bytes(int64_t rows, int64_t columns, int dtype, int activation);
+uint64_t dense_workspace_bytes(int64_t rows, int64_t inner, int64_t columns, int dtype, int activation, bool backward);
+uint64_t gated_saved_bytes(int64_t rows, int64_t hidden, int dtype);
+uint64_t gated_workspace_bytes(int64_t rows, int64_t channels, int64_t hidden, int dtype, bool backward);
+af2_status dense_forward_launch(af2_ctx *ctx, const DenseForward &p, void *workspace, cudaStream_t stream);
+af2_status dense_backward_launch(af2_ctx *ctx, const DenseBackward &p, void *workspace, cudaStream_t stream);
+af2_status gated_forward_launch(af2_ctx *ctx, const GatedForward &p, void *workspace, cudaStream_t stream);
+af2_status gated_backward_launch(af2_ctx *ctx, const GatedBackward &p, void *workspace, cudaStream_t stream);
+
+// ---- gradient norm and clipping (gradients.cu) ----
+
+uint64_t gradient_norm_workspace_bytes(int64_t count);
+// clip: scale into outputs (or in place when outputs is NULL); otherwise the norm alone.
+af2_status gradient_norm_launch(af2_ctx *ctx, const af2_tensor_ref *tensors, const af2_tensor_ref *outputs,
+                                int64_t count, bool clip, float max_norm, float *norm, void *workspace,
+                                cudaStream_t stream);
 
 // ---- row-sharded operators (comm.cu) ----
 

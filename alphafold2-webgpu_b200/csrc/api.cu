@@ -113,7 +113,8 @@ const char *profile_name(int id) {
       "q8.decode",           "weights.prepare",      "activations.convert",  "linear",
       "opm.normalize",       "opm.project",          "opm.count",         "opm.outer",
       "opm.output",          "opm.fused",            "transition.linear",
-      "attention.normalize", "attention.project",    "attention.flash",   "attention.output"};
+      "attention.normalize", "attention.project",    "attention.flash",   "attention.output",
+      "layer.gemm",          "layer.elementwise",    "gradients.norm"};
   return (id >= 0 && id < kProfCount) ? names[id] : nullptr;
 }
 
@@ -349,6 +350,8 @@ void af2_destroy(af2_ctx *ctx) {
   comm_destroy(ctx);
   clear_weight_cache(ctx);
   if (ctx->workspace.ptr) cudaFree(ctx->workspace.ptr);
+  if (ctx->layer_scratch.ptr) cudaFree(ctx->layer_scratch.ptr);
+  if (ctx->layer_done) cudaEventDestroy(ctx->layer_done);
   for (auto &s : ctx->staging)
     if (s.ptr) cudaFree(s.ptr);
   if (ctx->err_word) cudaFree(ctx->err_word);

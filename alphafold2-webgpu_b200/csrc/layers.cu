@@ -1,0 +1,417 @@
+// layers.cu -- entry points of the layers with learned weights (the dense
+// layer and the gated transition, forward and backward) and of the gradient
+// norm: argument checks, scratch, and the hand-over to the launchers in
+// dense.cu and gradients.cu.
+//
+// No counterpart in the reference, which runs fixed weights forward only; the
+// checks follow its conventions (positive safe integers, a RangeError-class
+// status with the reason in the message).
+#include <cmath>
+#include <new>
+#include <string>
+
+#include "af2_internal.h"
+
+namespace af2 {
+
+af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
+  if (workspace) {
+    base_ = static_cast<uint8_t *>(workspace);
+    return AF2_OK;
+  }
+  if (bytes == 0) return AF2_OK;
+  if (!ctx_->layer_done) {
+    cudaError_t e = cudaEventCreateWithFlags(&ctx_->layer_done, cudaEventDisableTiming);
+    if (e != cudaSuccess) {
+      ctx_->layer_done = nullptr;
+      return cuda_fail(ctx_, e, "create the layer scratch's event");
+    }
+  }
+  // inside a stream capture the order between streams is the graph's, not this context's
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaError_t e = cudaStreamIsCapturing(stream_, &capture); e != cudaSuccess)
+    return cuda_fail(ctx_, e, "query the stream's capture");
+  capturing_ = capture != cudaStreamCaptureStatusNone;
+  if (ctx_->layer_scratch.bytes < bytes) {
+    if (capturing_)
+      return fail(ctx_, AF2_ERR_UNSUPPORTED, "the context's scratch cannot grow inside a stream capture; pass a "
+                                             "workspace, or make the same call once before the capture");
+    // earlier calls on any stream may still use the buffer that is about to be freed
+    if (ctx_->layer_scratch.ptr)
+      if (cudaError_t e = cudaEventSynchronize(ctx_->layer_done); e != cudaSuccess)
+        return cuda_fail(ctx_, e, "wait for the layer scratch");
+    if (af2_status st = ensure(ctx_, ctx_->layer_scratch, bytes, "layer scratch"); st != AF2_OK) return st;
+  } else if (!capturing_ && ctx_->layer_stream != stream_) {
+    if (cudaError_t e = cudaStreamWaitEvent(stream_, ctx_->layer_done, 0); e != cudaSuccess)
+      return cuda_fail(ctx_, e, "order the layer scratch between streams");
+  }
+  base_ = static_cast<uint8_t *>(ctx_->layer_scratch.ptr);
+  owned_ = true;
+  return AF2_OK;
+}
+
+af2_status LayerScratch::release() {
+  if (!owned_ || capturing_) return AF2_OK;
+  ctx_->layer_stream = stream_;
+  if (cudaError_t e = cudaEventRecord(ctx_->layer_done, stream_); e != cudaSuccess)
+    return cuda_fail(ctx_, e, "record the layer scratch's use");
+  return AF2_OK;
+}
+
+namespace {
+
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1024, kMaxWidth = 65536;
+
+bool known_dtype(int dtype) { return dtype == AF2_F32 || dtype == AF2_F16 || dtype == AF2_BF16; }
+size_t element_bytes(int dtype) { return dtype == AF2_F32 ? 4 : 2; }
+
+// No exception leaves a C entry.
+template <typename F>
+af2_status guarded(af2_ctx *ctx, F &&f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc &) {
+    return AF2_ERR_OUT_OF_MEMORY;
+  } catch (...) {
+    return AF2_ERR_CUDA;
+  }
+}
+
+af2_status check_sizes(af2_ctx *ctx, int64_t rows, int64_t a, int64_t b, int dtype, const char *what) {
+  if (rows < 0 || a <= 0 || b <= 0)
+    return fail(ctx, AF2_ERR_INVALID_ARGUMENT,
+                std::string(what) + " widths must be positive and its rows not negative; received " +
+                    std::to_string(rows) + " rows, " + std::to_string(a) + " and " + std::to_string(b));
+  if (!known_dtype(dtype)) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "dtype must be AF2_F32, AF2_F16 or AF2_BF16");
+  if (rows > kMaxRows || a > kMaxWidth || b > kMaxWidth)
+    return fail(ctx, AF2_ERR_UNSUPPORTED, std::string(what) + " beyond 2^31 - 1024 rows or widths of 65536");
+  return AF2_OK;
+}
+
+af2_status check_activation(af2_ctx *ctx, int activation) {
+  if (activation < AF2_ACTIVATION_NONE || activation > AF2_ACTIVATION_GELU)
+    return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "unknown activation " + std::to_string(activation));
+  return AF2_OK;
+}
+
+struct NamedTensor {
+  const char *name;
+  const void *ptr;
+  bool required;
+};
+
+// Required tensors are there, and each is aligned to its element.
+template <int N>
+af2_status check_tensors(af2_ctx *ctx, const NamedTensor (&tensors)[N], int dtype) {
+  for (const NamedTensor &t : tensors) {
+    if (!t.ptr && t.required) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, std::string(t.name) + " is NULL");
+    if (reinterpret_cast<uintptr_t>(t.ptr) % element_bytes(dtype) != 0)
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, std::string(t.name) + " is not aligned to its element type");
+  }
+  return AF2_OK;
+}
+
+af2_status check_block(af2_ctx *ctx, const void *ptr, const char *name) {
+  if (reinterpret_cast<uintptr_t>(ptr) % 256 != 0)
+    return fail(ctx, AF2_ERR_INVALID_ARGUMENT, std::string(name) + " must be 256-byte aligned");
+  return AF2_OK;
+}
+
+struct Strides {
+  int activation = AF2_ACTIVATION_NONE;
+  int64_t x = 0, residual = 0, out = 0, d_x = 0;
+};
+
+af2_status read_options(af2_ctx *ctx, const af2_layer_options *o, int64_t x_width, int64_t out_width, bool residual,
+                        bool backward, Strides *s) {
+  s->x = s->d_x = x_width;
+  s->residual = s->out = out_width;
+  if (!o) return AF2_OK;
+  if (af2_status st = check_activation(ctx, o->activation); st != AF2_OK) return st;
+  if (o->reserved != 0) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "the reserved option must be 0");
+  const struct { const char *name; int64_t value, width; bool used; } strides[4] = {
+      {"x_stride", o->x_stride, x_width, true},
+      {"residual_stride", o->residual_stride, out_width, residual},
+      {"out_stride", o->out_stride, out_width, true},
+      {"d_x_stride", o->d_x_stride, x_width, backward}};
+  for (const auto &v : strides)
+    if (v.used && (v.value < v.width || v.value > (int64_t(1) << 40)))
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, std::string(v.name) + " " + std::to_string(v.value) +
+                                                     " is outside the rows' width " + std::to_string(v.width) +
+                                                     " to 2^40");
+  s->activation = o->activation;
+  s->x = o->x_stride;
+  s->residual = o->residual_stride;
+  s->out = o->out_stride;
+  s->d_x = o->d_x_stride;
+  return AF2_OK;
+}
+
+// Runs `launch(scratch)` with the call's scratch.
+template <typename F>
+af2_status with_scratch(af2_ctx *ctx, void *workspace, uint64_t bytes, cudaStream_t stream, F &&launch) {
+  LayerScratch scratch(ctx, stream);
+  if (af2_status st = scratch.acquire(workspace, bytes); st != AF2_OK) return st;
+  const af2_status st = launch(static_cast<void *>(scratch.base()));
+  const af2_status rel = scratch.release();
+  return st != AF2_OK ? st : rel;
+}
+
+cudaStream_t stream_of(af2_ctx *ctx, void *stream) {
+  return stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
+}
+
+af2_status check_set(af2_ctx *ctx, const af2_tensor_ref *t, int64_t count, const char *what) {
+  for (int64_t i = 0; i < count; ++i) {
+    const std::string name = std::string(what) + " " + std::to_string(i);
+    if (!known_dtype(t[i].dtype))
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + ": dtype must be AF2_F32, AF2_F16 or AF2_BF16");
+    if (t[i].count < 0 || t[i].count > (int64_t(1) << 48))
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + " has " + std::to_string(t[i].count) + " elements");
+    if (t[i].count > 0 && !t[i].data) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + " is NULL");
+    if (reinterpret_cast<uintptr_t>(t[i].data) % element_bytes(t[i].dtype) != 0)
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + " is not aligned to its element type");
+  }
+  return AF2_OK;
+}
+
+}  // namespace
+}  // namespace af2
+
+using namespace af2;
+
+extern "C" {
+
+af2_status af2_dense_saved_bytes(const af2_linear_shape *shape, int dtype, int activation, uint64_t *bytes) {
+  return guarded(nullptr, [&]() -> af2_status {
+    if (!shape || !bytes) return AF2_ERR_INVALID_ARGUMENT;
+    if (af2_status st = check_sizes(nullptr, shape->rows, shape->inner, shape->columns, dtype, ""); st != AF2_OK)
+      return st;
+    if (af2_status st = check_activation(nullptr, activation); st != AF2_OK) return st;
+    *bytes = dense_saved_bytes(shape->rows, shape->columns, dtype, activation);
+    return AF2_OK;
+  });
+}
+
+af2_status af2_dense_workspace_bytes(const af2_linear_shape *shape, int dtype, int activation, int backward,
+                                     uint64_t *bytes) {
+  return guarded(nullptr, [&]() -> af2_status {
+    if (!shape || !bytes) return AF2_ERR_INVALID_ARGUMENT;
+    if (af2_status st = check_sizes(nullptr, shape->rows, shape->inner, shape->columns, dtype, ""); st != AF2_OK)
+      return st;
+    if (af2_status st = check_activation(nullptr, activation); st != AF2_OK) return st;
+    *bytes = dense_workspace_bytes(shape->rows, shape->inner, shape->columns, dtype, activation, backward != 0);
+    return AF2_OK;
+  });
+}
+
+af2_status af2_dense(af2_ctx *ctx, const af2_linear_shape *shape, int dtype, const void *x, const void *weight,
+                     const void *bias, const void *residual, const af2_layer_options *options, void *out, void *saved,
+                     void *workspace, void *stream) {
+  if (!ctx) return AF2_ERR_INVALID_ARGUMENT;
+  return guarded(ctx, [&]() -> af2_status {
+    if (!shape) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "shape is NULL");
+    af2_status st = check_sizes(ctx, shape->rows, shape->inner, shape->columns, dtype, "the dense layer's");
+    if (st != AF2_OK) return st;
+    const bool some = shape->rows > 0;
+    const NamedTensor tensors[] = {{"x", x, some},       {"weight", weight, true},
+                                   {"bias", bias, false}, {"residual", residual, false},
+                                   {"out", out, some}};
+    if ((st = check_tensors(ctx, tensors, dtype)) != AF2_OK) return st;
+    Strides s;
+    if ((st = read_options(ctx, options, shape->inner, shape->columns, residual != nullptr, false, &s)) != AF2_OK)
+      return st;
+    if ((st = check_block(ctx, saved, "saved")) != AF2_OK || (st = check_block(ctx, workspace, "workspace")) != AF2_OK)
+      return st;
+    if (!some) return AF2_OK;
+    cudaSetDevice(ctx->device);
+    const DenseForward p{shape->rows, shape->inner, shape->columns, dtype, s.activation, x,   weight,
+                         bias,        residual,     s.x,            s.residual, s.out,  out, saved};
+    const cudaStream_t cs = stream_of(ctx, stream);
+    return with_scratch(ctx, workspace,
+                        dense_workspace_bytes(p.rows, p.inner, p.columns, dtype, s.activation, false), cs,
+                        [&](void *ws) { return dense_forward_launch(ctx, p, ws, cs); });
+  });
+}
+
+af2_status af2_dense_backward(af2_ctx *ctx, const af2_linear_shape *shape, int dtype, const void *d_out, const void *x,
+                              const void *weight, const void *saved, const af2_layer_options *options, void *d_x,
+                              void *d_weight, void *d_bias, void *workspace, void *stream) {
+  if (!ctx) return AF2_ERR_INVALID_ARGUMENT;
+  return guarded(ctx, [&]() -> af2_status {
+    if (!shape) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "shape is NULL");
+    af2_status st = check_sizes(ctx, shape->rows, shape->inner, shape->columns, dtype, "the dense layer's");
+    if (st != AF2_OK) return st;
+    Strides s;
+    if ((st = read_options(ctx, options, shape->inner, shape->columns, false, d_x != nullptr, &s)) != AF2_OK)
+      return st;
+    const bool some = shape->rows > 0;
+    const NamedTensor tensors[] = {
+        {"d_out", d_out, some},
+        {"x", x, some && d_weight},
+        {"weight", weight, some && d_x},
+        {"saved", saved, some && s.activation != AF2_ACTIVATION_NONE},
+        {"d_x", d_x, false},
+        {"d_weight", d_weight, false},
+        {"d_bias", d_bias, false}};
+    if ((st = check_tensors(ctx, tensors, dtype)) != AF2_OK) return st;
+    if ((st = check_block(ctx, saved, "saved")) != AF2_OK || (st = check_block(ctx, workspace, "workspace")) != AF2_OK)
+      return st;
+    cudaSetDevice(ctx->device);
+    const DenseBackward p{shape->rows, shape->inner, shape->columns, dtype, s.activation, d_out, x,       weight,
+                          saved,       s.out,        s.x,            s.d_x, d_x,          d_weight, d_bias};
+    const cudaStream_t cs = stream_of(ctx, stream);
+    return with_scratch(ctx, workspace,
+                        dense_workspace_bytes(p.rows, p.inner, p.columns, dtype, s.activation, true), cs,
+                        [&](void *ws) { return dense_backward_launch(ctx, p, ws, cs); });
+  });
+}
+
+af2_status af2_gated_transition_saved_bytes(const af2_transition_shape *shape, int dtype, uint64_t *bytes) {
+  return guarded(nullptr, [&]() -> af2_status {
+    if (!shape || !bytes) return AF2_ERR_INVALID_ARGUMENT;
+    if (af2_status st = check_sizes(nullptr, shape->rows, shape->channels, shape->hidden_channels, dtype, "");
+        st != AF2_OK)
+      return st;
+    *bytes = gated_saved_bytes(shape->rows, shape->hidden_channels, dtype);
+    return AF2_OK;
+  });
+}
+
+af2_status af2_gated_transition_workspace_bytes(const af2_transition_shape *shape, int dtype, int backward,
+                                                uint64_t *bytes) {
+  return guarded(nullptr, [&]() -> af2_status {
+    if (!shape || !bytes) return AF2_ERR_INVALID_ARGUMENT;
+    if (af2_status st = check_sizes(nullptr, shape->rows, shape->channels, shape->hidden_channels, dtype, "");
+        st != AF2_OK)
+      return st;
+    *bytes = gated_workspace_bytes(shape->rows, shape->channels, shape->hidden_channels, dtype, backward != 0);
+    return AF2_OK;
+  });
+}
+
+af2_status af2_gated_transition(af2_ctx *ctx, const af2_transition_shape *shape, int dtype, const void *x,
+                                const af2_gated_weights *weights, const void *residual,
+                                const af2_layer_options *options, void *out, void *saved, void *workspace,
+                                void *stream) {
+  if (!ctx) return AF2_ERR_INVALID_ARGUMENT;
+  return guarded(ctx, [&]() -> af2_status {
+    if (!shape || !weights) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "shape or weights is NULL");
+    af2_status st = check_sizes(ctx, shape->rows, shape->channels, shape->hidden_channels, dtype,
+                                "the gated transition's");
+    if (st != AF2_OK) return st;
+    const bool some = shape->rows > 0;
+    const NamedTensor tensors[] = {{"x", x, some},
+                                   {"gate_weight", weights->gate_weight, true},
+                                   {"gate_bias", weights->gate_bias, false},
+                                   {"value_weight", weights->value_weight, true},
+                                   {"value_bias", weights->value_bias, false},
+                                   {"output_weight", weights->output_weight, true},
+                                   {"output_bias", weights->output_bias, false},
+                                   {"residual", residual, false},
+                                   {"out", out, some}};
+    if ((st = check_tensors(ctx, tensors, dtype)) != AF2_OK) return st;
+    Strides s;
+    if ((st = read_options(ctx, options, shape->channels, shape->channels, residual != nullptr, false, &s)) != AF2_OK)
+      return st;
+    if ((st = check_block(ctx, saved, "saved")) != AF2_OK || (st = check_block(ctx, workspace, "workspace")) != AF2_OK)
+      return st;
+    if (!some) return AF2_OK;
+    cudaSetDevice(ctx->device);
+    const GatedForward p{shape->rows, shape->channels, shape->hidden_channels, dtype, s.activation, x,
+                         residual,    *weights,        s.x,                    s.residual, s.out,   out, saved};
+    const cudaStream_t cs = stream_of(ctx, stream);
+    return with_scratch(ctx, workspace, gated_workspace_bytes(p.rows, p.channels, p.hidden, dtype, false), cs,
+                        [&](void *ws) { return gated_forward_launch(ctx, p, ws, cs); });
+  });
+}
+
+af2_status af2_gated_transition_backward(af2_ctx *ctx, const af2_transition_shape *shape, int dtype,
+                                         const void *d_out, const void *x, const af2_gated_weights *weights,
+                                         const void *saved, const af2_layer_options *options,
+                                         const af2_gated_gradients *gradients, void *workspace, void *stream) {
+  if (!ctx) return AF2_ERR_INVALID_ARGUMENT;
+  return guarded(ctx, [&]() -> af2_status {
+    if (!shape || !weights || !gradients)
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "shape, weights or gradients is NULL");
+    af2_status st = check_sizes(ctx, shape->rows, shape->channels, shape->hidden_channels, dtype,
+                                "the gated transition's");
+    if (st != AF2_OK) return st;
+    const bool some = shape->rows > 0;
+    const NamedTensor tensors[] = {{"d_out", d_out, some},
+                                   {"x", x, some},
+                                   {"saved", saved, some},
+                                   {"gate_weight", weights->gate_weight, some},
+                                   {"value_weight", weights->value_weight, some},
+                                   {"output_weight", weights->output_weight, some},
+                                   {"the gradient of x", gradients->x, false},
+                                   {"the gradient of gate_weight", gradients->gate_weight, false},
+                                   {"the gradient of gate_bias", gradients->gate_bias, false},
+                                   {"the gradient of value_weight", gradients->value_weight, false},
+                                   {"the gradient of value_bias", gradients->value_bias, false},
+                                   {"the gradient of output_weight", gradients->output_weight, false},
+                                   {"the gradient of output_bias", gradients->output_bias, false}};
+    if ((st = check_tensors(ctx, tensors, dtype)) != AF2_OK) return st;
+    Strides s;
+    if ((st = read_options(ctx, options, shape->channels, shape->channels, false, gradients->x != nullptr, &s)) !=
+        AF2_OK)
+      return st;
+    if ((st = check_block(ctx, saved, "saved")) != AF2_OK || (st = check_block(ctx, workspace, "workspace")) != AF2_OK)
+      return st;
+    cudaSetDevice(ctx->device);
+    const GatedBackward p{shape->rows, shape->channels, shape->hidden_channels, dtype, s.activation, d_out, x,
+                          saved,       *weights,        *gradients,             s.out, s.x,          s.d_x};
+    const cudaStream_t cs = stream_of(ctx, stream);
+    return with_scratch(ctx, workspace, gated_workspace_bytes(p.rows, p.channels, p.hidden, dtype, true), cs,
+                        [&](void *ws) { return gated_backward_launch(ctx, p, ws, cs); });
+  });
+}
+
+af2_status af2_gradient_norm_workspace_bytes(int64_t count, uint64_t *bytes) {
+  if (!bytes || count < 0 || count > (int64_t(1) << 24)) return AF2_ERR_INVALID_ARGUMENT;
+  *bytes = gradient_norm_workspace_bytes(count);
+  return AF2_OK;
+}
+
+static af2_status gradient_call(af2_ctx *ctx, const af2_tensor_ref *tensors, const af2_tensor_ref *outputs,
+                                int64_t count, bool clip, double max_norm, float *norm, void *workspace,
+                                void *stream) {
+  if (!ctx) return AF2_ERR_INVALID_ARGUMENT;
+  return guarded(ctx, [&]() -> af2_status {
+    if (count < 0 || count > (int64_t(1) << 24))
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "the set has " + std::to_string(count) + " tensors");
+    if (count > 0 && !tensors) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "tensors is NULL");
+    if (!norm || reinterpret_cast<uintptr_t>(norm) % 4 != 0)
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "norm must be an f32 on the device");
+    if (clip && (!(max_norm >= 0) || !std::isfinite(max_norm)))
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "max_norm must be finite and not negative; received " +
+                                                     std::to_string(max_norm));
+    af2_status st = check_set(ctx, tensors, count, "tensor");
+    if (st != AF2_OK) return st;
+    if (outputs) {
+      if ((st = check_set(ctx, outputs, count, "output")) != AF2_OK) return st;
+      for (int64_t i = 0; i < count; ++i)
+        if (outputs[i].count != tensors[i].count || outputs[i].dtype != tensors[i].dtype)
+          return fail(ctx, AF2_ERR_INVALID_ARGUMENT,
+                      "output " + std::to_string(i) + " differs from its tensor in size or type");
+    }
+    if ((st = check_block(ctx, workspace, "workspace")) != AF2_OK) return st;
+    cudaSetDevice(ctx->device);
+    const cudaStream_t cs = stream_of(ctx, stream);
+    return with_scratch(ctx, workspace, gradient_norm_workspace_bytes(count), cs, [&](void *ws) {
+      return gradient_norm_launch(ctx, tensors, outputs, count, clip, static_cast<float>(max_norm), norm, ws, cs);
+    });
+  });
+}
+
+af2_status af2_gradient_norm(af2_ctx *ctx, const af2_tensor_ref *tensors, int64_t count, float *norm, void *workspace,
+                             void *stream) {
+  return gradient_call(ctx, tensors, nullptr, count, false, 0.0, norm, workspace, stream);
+}
+
+af2_status af2_clip_gradients(af2_ctx *ctx, const af2_tensor_ref *tensors, const af2_tensor_ref *outputs,
+                              int64_t count, double max_norm, float *norm, void *workspace, void *stream) {
+  return gradient_call(ctx, tensors, outputs, count, true, max_norm, norm, workspace, stream);
+}
+
+}  // extern "C"

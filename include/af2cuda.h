@@ -608,7 +608,14 @@ typedef struct af2_linear_shape {
     int64_t columns;
 } af2_linear_shape;
 
-typedef enum af2_activation { AF2_ACTIVATION_NONE = 0, AF2_ACTIVATION_RELU = 1 } af2_activation;
+typedef enum af2_activation {
+    AF2_ACTIVATION_NONE = 0,
+    AF2_ACTIVATION_RELU = 1,
+    /* af2_dense and af2_gated_transition only: */
+    AF2_ACTIVATION_SIGMOID = 2,
+    AF2_ACTIVATION_SILU = 3, /* z sigmoid(z) */
+    AF2_ACTIVATION_GELU = 4  /* z Phi(z), Phi the standard normal distribution (the erf form) */
+} af2_activation;
 
 AF2_API af2_status af2_linear_workspace_bytes(const af2_linear_shape *shape, int a_dtype, uint64_t *bytes);
 
@@ -621,6 +628,139 @@ AF2_API af2_status af2_linear_workspace_bytes(const af2_linear_shape *shape, int
 AF2_API af2_status af2_linear(af2_ctx *ctx, const af2_linear_shape *shape, const void *a, int a_dtype,
                               const af2_matrix *weight, const float *bias, int activation, int residual, void *out,
                               int out_dtype, void *workspace, void *stream);
+
+/* ---- layers with learned weights ------------------------------------------ */
+
+/*
+ * The dense layer and the gated transition, with their backward passes, for
+ * weights that change from step to step: every tensor of a call -- activations,
+ * weights, biases, gradients -- has the one type `dtype` (f32, f16 or bf16),
+ * weights are [in, out] row-major and used as they are stored, and nothing is
+ * kept from one call for the next.  No counterpart in the reference, whose
+ * weights are fixed.
+ *
+ * Arithmetic: 16-bit tensors are multiplied as they are, f32 tensors to f32
+ * accuracy; sums, biases, activations and the residual are f32, rounded once
+ * to `dtype`.  The hidden activations of a 16-bit gated transition and the
+ * gradients at its pre-activations are rounded to `dtype` where they become a
+ * product's operand.
+ *
+ * rows = 0 is valid: outputs of no rows are not touched, and the gradients of
+ * the weights are zero.  Outputs must not overlap inputs, except that out may
+ * be the residual itself.
+ */
+typedef struct af2_layer_options {
+    int32_t activation; /* af2_activation; of the gate in af2_gated_transition */
+    int32_t reserved;   /* 0 */
+    /* Elements from one row to the next, at least the row's width.  The
+     * backward passes use x_stride for x, out_stride for d_out and write d_x
+     * with d_x_stride. */
+    int64_t x_stride;
+    int64_t residual_stride;
+    int64_t out_stride;
+    int64_t d_x_stride;
+} af2_layer_options;
+
+/* Bytes of `saved`: what the forward pass leaves for the backward pass (0 for
+ * AF2_ACTIVATION_NONE).  Its layout is the library's. */
+AF2_API af2_status af2_dense_saved_bytes(const af2_linear_shape *shape, int dtype, int activation, uint64_t *bytes);
+/* Scratch bytes of the forward (backward = 0) or the backward pass. */
+AF2_API af2_status af2_dense_workspace_bytes(const af2_linear_shape *shape, int dtype, int activation, int backward,
+                                             uint64_t *bytes);
+
+/*
+ * out = act(x weight + bias) (+ residual): x [rows, inner], weight [inner,
+ * columns], bias [columns] or NULL, residual and out [rows, columns].  saved:
+ * NULL, or af2_dense_saved_bytes() bytes, 256-byte aligned, for the backward
+ * pass.  options NULL: contiguous rows, no activation.  workspace NULL =
+ * context-owned (calls on different streams are then ordered among
+ * themselves), else af2_dense_workspace_bytes() bytes, 256-byte aligned.
+ */
+AF2_API af2_status af2_dense(af2_ctx *ctx, const af2_linear_shape *shape, int dtype, const void *x,
+                             const void *weight, const void *bias, const void *residual,
+                             const af2_layer_options *options, void *out, void *saved, void *workspace, void *stream);
+
+/*
+ * The gradients of af2_dense: d_out [rows, columns] arrives at out (and is
+ * the residual's gradient as it stands); d_x [rows, inner], d_weight [inner,
+ * columns] and d_bias [columns] are written, each unless NULL.  saved: what
+ * the forward pass left (may be NULL for AF2_ACTIVATION_NONE).
+ */
+AF2_API af2_status af2_dense_backward(af2_ctx *ctx, const af2_linear_shape *shape, int dtype, const void *d_out,
+                                      const void *x, const void *weight, const void *saved,
+                                      const af2_layer_options *options, void *d_x, void *d_weight, void *d_bias,
+                                      void *workspace, void *stream);
+
+/* The gated transition's tensors: gate and value weights [channels,
+ * hidden_channels], output weight [hidden_channels, channels]; biases
+ * [hidden_channels], [hidden_channels] and [channels], each may be NULL. */
+typedef struct af2_gated_weights {
+    const void *gate_weight, *gate_bias;
+    const void *value_weight, *value_bias;
+    const void *output_weight, *output_bias;
+} af2_gated_weights;
+
+/* Where the backward pass writes; each may be NULL. */
+typedef struct af2_gated_gradients {
+    void *x;
+    void *gate_weight, *gate_bias;
+    void *value_weight, *value_bias;
+    void *output_weight, *output_bias;
+} af2_gated_gradients;
+
+AF2_API af2_status af2_gated_transition_saved_bytes(const af2_transition_shape *shape, int dtype, uint64_t *bytes);
+AF2_API af2_status af2_gated_transition_workspace_bytes(const af2_transition_shape *shape, int dtype, int backward,
+                                                        uint64_t *bytes);
+
+/*
+ * out = (act(x Wg + bg) * (x Wv + bv)) Wo + bo (+ residual) on x [rows,
+ * channels]: the transition with a gated hidden layer.  Other arguments as
+ * af2_dense.
+ */
+AF2_API af2_status af2_gated_transition(af2_ctx *ctx, const af2_transition_shape *shape, int dtype, const void *x,
+                                        const af2_gated_weights *weights, const void *residual,
+                                        const af2_layer_options *options, void *out, void *saved, void *workspace,
+                                        void *stream);
+
+/* The gradients of af2_gated_transition; `saved` is what the forward pass left.  weights' biases are not read. */
+AF2_API af2_status af2_gated_transition_backward(af2_ctx *ctx, const af2_transition_shape *shape, int dtype,
+                                                 const void *d_out, const void *x, const af2_gated_weights *weights,
+                                                 const void *saved, const af2_layer_options *options,
+                                                 const af2_gated_gradients *gradients, void *workspace, void *stream);
+
+/* ---- the norm of a set of gradients, and clipping -------------------------- */
+
+/* One contiguous tensor of a set: `count` elements of `dtype` at `data`, aligned to its element. */
+typedef struct af2_tensor_ref {
+    void *data;
+    int64_t count;
+    int32_t dtype;
+    int32_t reserved; /* 0 */
+} af2_tensor_ref;
+
+/* Scratch bytes of both calls for `count` tensors. */
+AF2_API af2_status af2_gradient_norm_workspace_bytes(int64_t count, uint64_t *bytes);
+
+/*
+ * norm[0] (f32, on the device) = the square root of the sum of the squares of
+ * every element of the `count` tensors (a host array of refs, read before the
+ * call returns).  Squares are summed in f64, so no finite f32 input overflows,
+ * in an order that depends on the sizes alone; an infinity or a NaN among the
+ * elements makes the norm infinite or NaN.  No tensors: 0.
+ */
+AF2_API af2_status af2_gradient_norm(af2_ctx *ctx, const af2_tensor_ref *tensors, int64_t count, float *norm,
+                                     void *workspace, void *stream);
+
+/*
+ * The norm as above, and every tensor scaled by min(1, max_norm / (norm +
+ * 1e-6)), computed in f32 and rounded once to the output's type.  outputs:
+ * NULL scales in place (and writes nothing when the factor is 1), else
+ * `count` refs of the same counts and types, each the same memory as its input or
+ * disjoint from every input.  A NaN norm makes every element NaN, an infinite one
+ * makes the finite elements zero.  max_norm must be finite and not negative.
+ */
+AF2_API af2_status af2_clip_gradients(af2_ctx *ctx, const af2_tensor_ref *tensors, const af2_tensor_ref *outputs,
+                                      int64_t count, double max_norm, float *norm, void *workspace, void *stream);
 
 #ifdef __cplusplus
 }
