@@ -297,6 +297,15 @@ __device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap
       "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
+// The same for a 3-D map.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1,
+                                                 int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_addr(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols)
                : "memory");
@@ -483,6 +492,11 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(int m, int n) {
 
 // The same with A MN-major (transpose-A bit).
 __host__ __device__ constexpr uint32_t idesc_f16_f32_amn(int m, int n) { return idesc_f16_f32(m, n) | (1u << 15); }
+
+// The same for either 16-bit type (the same one for A and B) and either order of each operand.
+__host__ __device__ constexpr uint32_t idesc_16_f32(int m, int n, bool bf16, bool a_mn, bool b_mn) {
+  return idesc_f16_f32(m, n) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u);
+}
 
 // Byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a 128B-swizzled tile.
 __device__ __forceinline__ uint32_t sw128_offset(uint32_t row, uint32_t chunk) {

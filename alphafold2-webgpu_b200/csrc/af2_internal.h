@@ -467,13 +467,13 @@ struct GatedBackward {
   int64_t d_out_stride = 0, x_stride = 0, d_x_stride = 0;
 };
 uint64_t dense_saved_bytes(int64_t rows, int64_t columns, int dtype, int activation);
-uint64_t dense_workspace_bytes(int64_t rows, int64_t inner, int64_t columns, int dtype, int activation, bool backward);
 uint64_t gated_saved_bytes(int64_t rows, int64_t hidden, int dtype);
-uint64_t gated_workspace_bytes(int64_t rows, int64_t channels, int64_t hidden, int dtype, bool backward);
-af2_status dense_forward_launch(af2_ctx *ctx, const DenseForward &p, void *workspace, cudaStream_t stream);
-af2_status dense_backward_launch(af2_ctx *ctx, const DenseBackward &p, void *workspace, cudaStream_t stream);
-af2_status gated_forward_launch(af2_ctx *ctx, const GatedForward &p, void *workspace, cudaStream_t stream);
-af2_status gated_backward_launch(af2_ctx *ctx, const GatedBackward &p, void *workspace, cudaStream_t stream);
+// Each runs its pass in `scratch`, or with ctx NULL only counts: *bytes = the scratch that the pass
+// with these tensors takes (tensors that TMA cannot read as they lie are copied there first).
+af2_status dense_forward(af2_ctx *ctx, const DenseForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream);
+af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, uint64_t *bytes, cudaStream_t stream);
+af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream);
+af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, uint64_t *bytes, cudaStream_t stream);
 
 // ---- gradient norm and clipping (gradients.cu) ----
 

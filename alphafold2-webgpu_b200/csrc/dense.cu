@@ -6,356 +6,639 @@
 //           dh = dy Wo^T, dv = dh act(g), dg = dh v act'(g),
 //           dx = dg Wg^T + dv Wv^T, dWg = x^T dg, dWv = x^T dv, dWo = h^T dy
 //
-// Simplest form: one tiled product in f32 on the CUDA cores for every operand
-// order, its sums kept in f32 in the scratch, and one elementwise pass for
-// each of the rest.
+// Every product is a layer_gemm launch on the operands as they are stored; the
+// 16-bit types' activations, slopes and gates are in its epilogues.  Tensors
+// that TMA cannot read (rows not in 16-byte pieces) are copied to padded rows
+// first, and f32 ones are split into bf16 terms by the same pass.
+//
+// What a forward pass saves, in the 16-bit types: the pre-activations' upper 24
+// bits (their f32 rounded to 2^-16), so that the backward pass rounds to 16
+// bits only what becomes a product's operand; and the gated transition's h, an
+// operand already.
+#include <algorithm>
 #include <type_traits>
 
-#include "af2_internal.h"
+#include "layer_gemm.h"
 #include "layer_math.cuh"
 
 namespace af2 {
 namespace {
 
-// C[m][n] (+)= sum_k A(m, k) B(k, n); A(m, k) = a[m * a_m + k * a_k], B(k, n) = b[k * b_k + n * b_n].
-struct Product {
-  const void *a, *b;
-  int64_t a_m, a_k, b_k, b_n;
-  int64_t m, n, k;
-  float *c;  // [m][n]
-  int accumulate;
+size_t element_size(int dtype) { return dtype == AF2_F32 ? 4 : 2; }
+uint64_t part(uint64_t bytes) { return align_up(bytes, 256); }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---- copies to operands ---------------------------------------------------------
+
+constexpr int kMaxPackJobs = 6;
+struct PackJob {
+  const void *src;
+  int64_t stride;  // elements
+  int64_t rows, width;
+  void *dst;       // [pieces][rows][pitch] of 16 bits
+  int64_t pitch, piece_stride;
+  int64_t first;   // 8-column groups of the jobs before this one
+};
+struct PackArgs {
+  PackJob job[kMaxPackJobs];
+  int count;
+  int64_t groups;
 };
 
-constexpr int kTile = 64, kDepth = 16;
-
-template <typename TA, typename TB>
-__global__ void __launch_bounds__(256) product_kernel(const Product p) {
-  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kTile;
-  const TA *a = static_cast<const TA *>(p.a);
-  const TB *b = static_cast<const TB *>(p.b);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
-    for (int i = threadIdx.x; i < kTile * kDepth; i += 256) {
-      // the contiguous index of each operand runs fastest over the threads
-      const int am = p.a_k == 1 ? i / kDepth : i % kTile, ak = p.a_k == 1 ? i % kDepth : i / kTile;
-      const int64_t m = m0 + am, ka = k0 + ak;
-      sa[ak][am] = m < p.m && ka < p.k ? to_f32<TA>(a[m * p.a_m + ka * p.a_k]) : 0.f;
-      const int bn = p.b_k == 1 ? i / kDepth : i % kTile, bk = p.b_k == 1 ? i % kDepth : i / kTile;
-      const int64_t n = n0 + bn, kb = k0 + bk;
-      sb[bk][bn] = n < p.n && kb < p.k ? to_f32<TB>(b[kb * p.b_k + n * p.b_n]) : 0.f;
-    }
-    __syncthreads();
+// The three bf16 terms of eight f32: x = t0 + t1 + t2 up to 2^-24 of |x|.  A finite x whose rounding
+// to bf16 would overflow takes the largest bf16 first; an infinite or NaN x is whole in t0.
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 (&t)[3]) {
+  uint32_t w[3][4];
 #pragma unroll
-    for (int k = 0; k < kDepth; ++k)
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int k = 0; k < 3; ++k) {
+      constexpr float kMost = 0x1.fep127f;
+      w[k][i] = pack2_t<__nv_bfloat16>(isfinite(a) ? fminf(fmaxf(a, -kMost), kMost) : a,
+                                       isfinite(b) ? fminf(fmaxf(b, -kMost), kMost) : b);
+      const float2 r = unpack2<__nv_bfloat16>(w[k][i]);
+      a = isfinite(r.x) ? a - r.x : 0.f;
+      b = isfinite(r.y) ? b - r.y : 0.f;
+    }
+  }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m >= p.m || n >= p.n) continue;
-      float *c = p.c + m * p.n + n;
-      *c = p.accumulate ? *c + acc[i][j] : acc[i][j];
-    }
+  for (int k = 0; k < 3; ++k) t[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
 }
 
-__device__ __forceinline__ int64_t grid_index() {
-  return static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-}
-__device__ __forceinline__ int64_t grid_stride() { return static_cast<int64_t>(gridDim.x) * blockDim.x; }
-
-// out = act(acc + bias) (+ residual); saved = acc + bias
-template <typename T, int ACT>
-__global__ void dense_finish_kernel(const float *acc, int64_t rows, int64_t cols, const T *bias, const T *residual,
-                                    int64_t residual_stride, T *out, int64_t out_stride, float *saved) {
-  for (int64_t i = grid_index(); i < rows * cols; i += grid_stride()) {
-    const int64_t r = i / cols, c = i - r * cols;
-    const float z = acc[i] + (bias ? to_f32<T>(bias[c]) : 0.f);
-    if (saved) saved[i] = z;
-    float y = activate<ACT>(z);
-    if (residual) y += to_f32<T>(residual[r * residual_stride + c]);
-    out[r * out_stride + c] = from_f32<T>(y);
-  }
-}
-
-// dz = dy act'(z), in f32
-template <typename T, int ACT>
-__global__ void dense_slope_kernel(const T *dy, int64_t dy_stride, const float *z, int64_t rows, int64_t cols,
-                                   float *dz) {
-  for (int64_t i = grid_index(); i < rows * cols; i += grid_stride()) {
-    const int64_t r = i / cols, c = i - r * cols;
-    float value, slope = 1.f;
-    if (ACT != AF2_ACTIVATION_NONE) activate_slope<ACT>(z[i], value, slope);
-    dz[i] = to_f32<T>(dy[r * dy_stride + c]) * slope;
-  }
-}
-
-// saved [rows][2 cols] = the biased pre-activations (gate, value); h = act(gate) value
-template <typename T, int ACT>
-__global__ void gate_kernel(const float *g, const float *v, int64_t rows, int64_t cols, const T *bg, const T *bv,
-                            T *h, float *saved) {
-  for (int64_t i = grid_index(); i < rows * cols; i += grid_stride()) {
-    const int64_t r = i / cols, c = i - r * cols;
-    const float gate = g[i] + (bg ? to_f32<T>(bg[c]) : 0.f), value = v[i] + (bv ? to_f32<T>(bv[c]) : 0.f);
-    if (saved) {
-      saved[r * 2 * cols + c] = gate;
-      saved[r * 2 * cols + cols + c] = value;
-    }
-    h[i] = from_f32<T>(activate<ACT>(gate) * value);
-  }
-}
-
-// dh [rows][cols] and saved [rows][2 cols] -> dgv [rows][2 cols] (dg, dv) and h
-template <typename T, int ACT>
-__global__ void gate_backward_kernel(const float *dh, const float *saved, int64_t rows, int64_t cols, float *dgv,
-                                     T *h) {
-  for (int64_t i = grid_index(); i < rows * cols; i += grid_stride()) {
-    const int64_t r = i / cols, c = i - r * cols;
-    const float g = saved[r * 2 * cols + c], v = saved[r * 2 * cols + cols + c];
-    float value, slope;
-    activate_slope<ACT>(g, value, slope);
-    dgv[r * 2 * cols + c] = dh[i] * v * slope;
-    dgv[r * 2 * cols + cols + c] = dh[i] * value;
-    h[i] = from_f32<T>(value * v);
-  }
-}
-
-// rounds rows of f32 sums to T
 template <typename T>
-__global__ void round_kernel(const float *src, int64_t rows, int64_t cols, T *dst, int64_t dst_stride) {
-  for (int64_t i = grid_index(); i < rows * cols; i += grid_stride()) {
-    const int64_t r = i / cols, c = i - r * cols;
-    dst[r * dst_stride + c] = from_f32<T>(src[i]);
+__device__ __forceinline__ void load8(const T *p, int n, float (&x)[8]) {
+  if (n >= 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+      unpack8<T>(*reinterpret_cast<const uint4 *>(p), x);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? to_f32<T>(p[i]) : 0.f;
   }
 }
 
-// dst[c] = sum over the rows of src; one block per 32 columns, rows strided over its 32 warps
-template <typename TS, typename T>
-__global__ void __launch_bounds__(1024) column_sum_kernel(const TS *src, int64_t stride, int64_t rows, int64_t cols,
-                                                          T *dst) {
-  __shared__ float part[32][33];
+// Eight values as an operand: rounded to T, or f32 as three bf16 terms `piece_stride` elements apart.
+template <typename T>
+__device__ __forceinline__ void store_operand8(void *dst, int64_t at, int64_t piece_stride, const float (&x)[8]) {
+  uint16_t *d = static_cast<uint16_t *>(dst) + at;
+  if constexpr (sizeof(T) == 4) {
+    uint4 t[3];
+    split8(x, t);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) *reinterpret_cast<uint4 *>(d + k * piece_stride) = t[k];
+  } else {
+    *reinterpret_cast<uint4 *>(d) = make_uint4(pack2_t<T>(x[0], x[1]), pack2_t<T>(x[2], x[3]),
+                                               pack2_t<T>(x[4], x[5]), pack2_t<T>(x[6], x[7]));
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs p) {
+  for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g < p.groups;
+       g += static_cast<int64_t>(gridDim.x) * 256) {
+    int j = 0;
+    while (j + 1 < p.count && g >= p.job[j + 1].first) ++j;
+    const PackJob &job = p.job[j];
+    const int64_t per_row = job.pitch / 8, at = g - job.first, r = at / per_row, c = (at - r * per_row) * 8;
+    float x[8];
+    load8<T>(static_cast<const T *>(job.src) + r * job.stride + c,
+             static_cast<int>(min(static_cast<int64_t>(8), job.width - c)), x);
+    store_operand8<T>(job.dst, r * job.pitch + c, job.piece_stride, x);
+  }
+}
+
+// ---- passes over rows, with column sums --------------------------------------------
+
+constexpr int kSumRows = 64;  // rows of a block
+
+// Block (x, y): columns [256 y, + 256) of rows [64 x, + 64); a thread has eight columns of every
+// eighth row.  body(row, column, sums) for each; then sums[s] over the rows go to
+// partial[x][s][pitch], in a fixed order.
+template <int SETS, typename F>
+__device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, float *partial, int64_t pitch, F &&body) {
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + tx) * 8, r0 = static_cast<int64_t>(blockIdx.x) * kSumRows;
+  float sums[SETS][8] = {};
+  if (c < width)
+    for (int64_t r = r0 + ty; r < min(rows, r0 + kSumRows); r += 8) body(r, c, sums);
+  if (!partial) return;
+  __shared__ float all[8][32][9];
+#pragma unroll
+  for (int s = 0; s < SETS; ++s) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all[ty][tx][i] = sums[s][i];
+    __syncthreads();
+    // thread t sums column t of the block's 256
+    const int cx = threadIdx.x >> 3, ci = threadIdx.x & 7;
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) total += all[w][cx][ci];
+    const int64_t col = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x;
+    if (col < pitch) partial[(static_cast<int64_t>(blockIdx.x) * SETS + s) * pitch + col] = total;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t stride, int64_t rows, int64_t width,
+                                                         float *partial, int64_t pitch) {
+  for_row_groups<1>(rows, width, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
+    float x[8];
+    load8<T>(src + r * stride + c, static_cast<int>(min(static_cast<int64_t>(8), width - c)), x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[0][i] += x[i];
+  });
+}
+
+// dst[c] = the sum over `chunks` of partial[chunk][set][pitch] at c; block: 32 columns, 32 warps
+template <typename T>
+__global__ void __launch_bounds__(1024) column_finish_kernel(const float *partial, int64_t chunks, int sets, int set,
+                                                             int64_t pitch, int64_t cols, T *dst) {
+  __shared__ float all[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float sum = 0.f;
   if (c < cols)
-    for (int64_t r = warp; r < rows; r += 32) sum += to_f32<TS>(src[r * stride + c]);
-  part[warp][lane] = sum;
+    for (int64_t k = warp; k < chunks; k += 32) sum += partial[(k * sets + set) * pitch + c];
+  all[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && c < cols) {
     float total = 0.f;
-    for (int w = 0; w < 32; ++w) total += part[w][lane];
+    for (int w = 0; w < 32; ++w) total += all[w][lane];
     dst[c] = from_f32<T>(total);
   }
 }
 
-struct Launcher {
-  af2_ctx *ctx;
-  cudaStream_t stream;
-  af2_status status = AF2_OK;
+// Eight saved pre-activations.
+template <typename T>
+__device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int64_t r, int64_t c, float (&z)[8]) {
+  const int64_t at = plane * s.stride + r * s.pitch + c;
+  if constexpr (sizeof(T) == 4) {
+    load8<float>(s.f32 + at, 8, z);
+  } else {
+    const uint4 h = *reinterpret_cast<const uint4 *>(s.hi + at);
+    const uint2 l = *reinterpret_cast<const uint2 *>(s.lo + at);
+    const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[2] = {l.x, l.y};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      z[i] = __uint_as_float(((i & 1) ? hw[i >> 1] & 0xffff0000u : hw[i >> 1] << 16) |
+                             (((lw[i >> 2] >> (8 * (i & 3))) & 0xffu) << 8));
+  }
+}
 
-  void check(const char *what) {
-    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess && status == AF2_OK) status = cuda_fail(ctx, e, what);
+// dz = dy act'(z) as an operand, with its column sums
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t dy_stride, const SavedPlanes saved,
+                                                          int64_t rows, int64_t width, void *dz, int64_t dz_pitch,
+                                                          int64_t dz_piece, float *partial, int64_t pitch) {
+  for_row_groups<1>(rows, width, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
+    const int n = static_cast<int>(min(static_cast<int64_t>(8), width - c));
+    float d[8], z[8];
+    load8<T>(dy + r * dy_stride + c, n, d);
+    load_saved8<T>(saved, 0, r, c, z);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float value, slope;
+      activate_slope<ACT>(z[i], value, slope);
+      d[i] = i < n ? d[i] * slope : 0.f;
+      sums[0][i] += d[i];
+    }
+    store_operand8<T>(dz, r * dz_pitch + c, dz_piece, d);
+  });
+}
+
+// f32: h = act(g) v as an operand, from the saved planes
+template <int ACT>
+__global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, int64_t rows, int64_t width, void *h,
+                                                       int64_t h_pitch, int64_t h_piece) {
+  for_row_groups<1>(rows, width, nullptr, 0, [&](int64_t r, int64_t c, float (&)[1][8]) {
+    float g[8], v[8];
+    load_saved8<float>(saved, 0, r, c, g);
+    load_saved8<float>(saved, 1, r, c, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = activate<ACT>(g[i]) * v[i];
+    store_operand8<float>(h, r * h_pitch + c, h_piece, g);
+  });
+}
+
+// f32: dg and dv as operands, `dgv_set` elements apart, from dh [rows][saved.pitch] and the saved planes
+template <int ACT>
+__global__ void __launch_bounds__(256) gate_backward_f32_kernel(const float *dh, const SavedPlanes saved, int64_t rows,
+                                                                int64_t width, uint16_t *dgv, int64_t dgv_pitch,
+                                                                int64_t dgv_piece, int64_t dgv_set, float *partial,
+                                                                int64_t pitch) {
+  for_row_groups<2>(rows, width, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[2][8]) {
+    float d[8], g[8], v[8];
+    load8<float>(dh + r * saved.pitch + c, 8, d);
+    load_saved8<float>(saved, 0, r, c, g);
+    load_saved8<float>(saved, 1, r, c, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float value, slope;
+      activate_slope<ACT>(g[i], value, slope);
+      const bool in = c + i < width;  // past the width nothing was written
+      g[i] = in ? d[i] * v[i] * slope : 0.f;
+      v[i] = in ? d[i] * value : 0.f;
+      sums[0][i] += g[i];
+      sums[1][i] += v[i];
+    }
+    store_operand8<float>(dgv, r * dgv_pitch + c, dgv_piece, g);
+    store_operand8<float>(dgv + dgv_set, r * dgv_pitch + c, dgv_piece, v);
+  });
+}
+
+// ---- one pass of a layer --------------------------------------------------------------
+
+// Lays the scratch out and launches; without a context it only counts the scratch.
+class Pass {
+ public:
+  Pass(af2_ctx *ctx, int dtype, void *scratch, cudaStream_t stream)
+      : ctx_(ctx), dtype_(dtype), base_(static_cast<uint8_t *>(scratch)), stream_(stream) {}
+
+  af2_status status = AF2_OK;
+  uint64_t used = 0;
+
+  bool live() const { return ctx_ && status == AF2_OK; }
+  bool f32() const { return dtype_ == AF2_F32; }
+  int pieces() const { return f32() ? 3 : 1; }
+
+  uint8_t *take(uint64_t bytes) {
+    uint8_t *p = base_ + used;
+    used += part(bytes);
+    return p;
   }
-  int blocks(int64_t elements) const {
-    return static_cast<int>(std::min<int64_t>((elements + 255) / 256, 16 * ctx->sm_count));
+  // Room for an operand of this width made by a kernel.
+  GemmOperand make_operand(int64_t rows, int64_t width) {
+    GemmOperand o;
+    o.pitch = operand_pitch(width);
+    o.piece_stride = rows * o.pitch;
+    o.ptr = take(2ull * pieces() * rows * o.pitch);
+    return o;
   }
-  template <typename TA, typename TB>
-  void product(const Product &p) {
-    LaunchScope scope(ctx, stream, kProfLayerGemm);
-    const dim3 grid(static_cast<unsigned>((p.m + kTile - 1) / kTile), static_cast<unsigned>((p.n + kTile - 1) / kTile));
-    product_kernel<TA, TB><<<grid, 256, 0, stream>>>(p);
-    check("layer product");
+  // A tensor of the call's type as an operand: itself, or a copy (pack() launches the copies).
+  GemmOperand operand(const void *src, int64_t stride, int64_t rows, int64_t width) {
+    if (!f32() && reinterpret_cast<uintptr_t>(src) % 16 == 0 && stride % 8 == 0 && stride < (int64_t(1) << 38)) {
+      GemmOperand o;
+      o.ptr = src;
+      o.pitch = stride;
+      return o;
+    }
+    const GemmOperand o = make_operand(rows, width);
+    jobs_.job[jobs_.count++] = {src, stride, rows, width, const_cast<void *>(o.ptr), o.pitch, o.piece_stride,
+                                jobs_.groups};
+    jobs_.groups += rows * (o.pitch / 8);
+    return o;
   }
+  void pack() {
+    if (live() && jobs_.count) {
+      const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(jobs_.groups, 256), 16 * ctx_->sm_count));
+      LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
+      with_element(dtype_, [&](auto *tag) {
+        pack_kernel<std::remove_pointer_t<decltype(tag)>><<<blocks, 256, 0, stream_>>>(jobs_);
+      });
+      check("layer operand copies");
+    }
+    jobs_ = PackArgs{};
+  }
+
+  LayerGemm product(int64_t m, int64_t n, int64_t k) const {
+    LayerGemm g;
+    g.m = m;
+    g.n = n;
+    g.k = k;
+    g.bf16 = dtype_ != AF2_F16;
+    g.pieces = pieces();
+    g.out_dtype = dtype_;
+    return g;
+  }
+  static GemmOperand mn(GemmOperand o) {
+    o.mn_major = true;
+    return o;
+  }
+  void run(LayerGemm g) {
+    const uint64_t mark = used;
+    g.scratch = take(layer_gemm_scratch(g));
+    if (live()) status = layer_gemm_launch(ctx_, g, stream_);
+    peak_ = std::max(peak_, used);
+    used = mark;  // launches follow one another on the stream: the next may use the same place
+  }
+  uint64_t total() const { return std::max(peak_, used); }
+
+  SavedPlanes planes(void *saved, int64_t rows, int64_t width, int count) const {
+    SavedPlanes s;
+    s.pitch = saved_pitch(width);
+    s.stride = rows * s.pitch;
+    if (f32()) {
+      s.f32 = static_cast<float *>(saved);
+    } else {
+      s.hi = static_cast<uint16_t *>(saved);
+      s.lo = static_cast<uint8_t *>(saved) + part(2ull * count * s.stride);
+    }
+    return s;
+  }
+
   template <typename F>
-  void elementwise(F &&f) {
-    LaunchScope scope(ctx, stream, kProfLayerElementwise);
-    f();
-    check("layer elementwise kernel");
+  void rows_kernel(int64_t rows, int64_t width, F &&launch) {
+    if (!live()) return;
+    LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
+    const dim3 grid(static_cast<unsigned>(ceil_div(rows, kSumRows)), static_cast<unsigned>(ceil_div(width, 256)));
+    launch(grid);
+    check("layer row pass");
+  }
+  // The column sums of a tensor, or of partial sums (`sets` sets of `chunks` rows).
+  float *sum_room(int64_t rows, int64_t width, int sets) {
+    return reinterpret_cast<float *>(take(4ull * sets * ceil_div(rows, kSumRows) * saved_pitch(width)));
+  }
+  void finish_sums(const float *partial, int64_t chunks, int sets, int set, int64_t width, void *dst) {
+    if (!live() || !dst) return;
+    LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
+    with_element(dtype_, [&](auto *tag) {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      column_finish_kernel<T><<<static_cast<unsigned>(ceil_div(width, 32)), 1024, 0, stream_>>>(
+          partial, chunks, sets, set, saved_pitch(width), width, static_cast<T *>(dst));
+    });
+    check("layer column sums");
+  }
+  void column_sums(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst) {
+    if (!dst) return;
+    float *partial = sum_room(rows, width, 1);
+    rows_kernel(rows, width, [&](dim3 grid) {
+      with_element(dtype_, [&](auto *tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        column_sum_kernel<T><<<grid, 256, 0, stream_>>>(static_cast<const T *>(src), stride, rows, width, partial,
+                                                        saved_pitch(width));
+      });
+    });
+    finish_sums(partial, ceil_div(rows, kSumRows), 1, 0, width, dst);
   }
   void zero(void *ptr, size_t bytes) {
-    if (!ptr || status != AF2_OK) return;
-    if (cudaError_t e = cudaMemsetAsync(ptr, 0, bytes, stream); e != cudaSuccess) status = cuda_fail(ctx, e, "zero");
+    if (!ptr || !live()) return;
+    if (cudaError_t e = cudaMemsetAsync(ptr, 0, bytes, stream_); e != cudaSuccess)
+      status = cuda_fail(ctx_, e, "zero a gradient");
   }
+  void check(const char *what) {
+    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess && status == AF2_OK) status = cuda_fail(ctx_, e, what);
+  }
+  cudaStream_t stream() const { return stream_; }
+
+ private:
+  af2_ctx *ctx_;
+  int dtype_;
+  uint8_t *base_;
+  cudaStream_t stream_;
+  PackArgs jobs_{};
+  uint64_t peak_ = 0;
 };
 
-size_t element_size(int dtype) { return dtype == AF2_F32 ? 4 : 2; }
-uint64_t part(uint64_t bytes) { return align_up(bytes, 256); }
+uint64_t planes_bytes(int64_t rows, int64_t width, int dtype, int count) {
+  const uint64_t n = static_cast<uint64_t>(count) * rows * saved_pitch(width);
+  return dtype == AF2_F32 ? part(4 * n) : part(2 * n) + part(n);
+}
+uint64_t hidden_bytes(int64_t rows, int64_t hidden, int dtype) {
+  return part(2ull * (dtype == AF2_F32 ? 3 : 1) * rows * operand_pitch(hidden));
+}
 
 }  // namespace
 
 uint64_t dense_saved_bytes(int64_t rows, int64_t columns, int dtype, int activation) {
-  return activation == AF2_ACTIVATION_NONE ? 0 : 4ull * rows * columns;
+  return activation == AF2_ACTIVATION_NONE ? 0 : planes_bytes(rows, columns, dtype, 1);
 }
-uint64_t dense_workspace_bytes(int64_t rows, int64_t inner, int64_t columns, int dtype, int activation,
-                               bool backward) {
-  if (!backward) return part(4ull * rows * columns);
-  return part(4ull * rows * columns) + part(4ull * rows * inner) + part(4ull * inner * columns);
-}
-uint64_t gated_saved_bytes(int64_t rows, int64_t hidden, int dtype) { return 8ull * rows * hidden; }
-uint64_t gated_workspace_bytes(int64_t rows, int64_t channels, int64_t hidden, int dtype, bool backward) {
-  const uint64_t h = part(element_size(dtype) * rows * hidden);
-  if (!backward) return h + 2 * part(4ull * rows * hidden) + part(4ull * rows * channels);
-  return h + part(4ull * rows * hidden) + part(8ull * rows * hidden) + part(4ull * rows * channels) +
-         part(4ull * channels * hidden);
+uint64_t gated_saved_bytes(int64_t rows, int64_t hidden, int dtype) {
+  return hidden_bytes(rows, hidden, dtype) + planes_bytes(rows, hidden, dtype, 2);
 }
 
-af2_status dense_forward_launch(af2_ctx *ctx, const DenseForward &p, void *workspace, cudaStream_t stream) {
-  Launcher l{ctx, stream};
-  float *acc = static_cast<float *>(workspace);
-  with_element(p.dtype, [&](auto *tag) {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    l.product<T, T>({p.x, p.weight, p.x_stride, 1, p.columns, 1, p.rows, p.columns, p.inner, acc, 0});
-    with_activation(p.activation, [&](auto act) {
-      l.elementwise([&] {
-        dense_finish_kernel<T, act.value><<<l.blocks(p.rows * p.columns), 256, 0, stream>>>(
-            acc, p.rows, p.columns, static_cast<const T *>(p.bias), static_cast<const T *>(p.residual),
-            p.residual_stride, static_cast<T *>(p.out), p.out_stride,
-            act.value == AF2_ACTIVATION_NONE ? nullptr : static_cast<float *>(p.saved));
-      });
-    });
-  });
+af2_status dense_forward(af2_ctx *ctx, const DenseForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
+  Pass l(ctx, p.dtype, scratch, stream);
+  LayerGemm g = l.product(p.rows, p.columns, p.inner);
+  g.a[0] = l.operand(p.x, p.x_stride, p.rows, p.inner);
+  g.b[0] = Pass::mn(l.operand(p.weight, p.columns, p.inner, p.columns));
+  l.pack();
+  g.activation = p.activation;
+  g.bias[0] = p.bias;
+  g.residual = p.residual;
+  g.residual_stride = p.residual_stride;
+  g.out[0] = p.out;
+  g.out_stride = p.out_stride;
+  if (p.saved && p.activation != AF2_ACTIVATION_NONE) g.saved = l.planes(p.saved, p.rows, p.columns, 1);
+  l.run(g);
+  *bytes = l.total();
   return l.status;
 }
 
-af2_status dense_backward_launch(af2_ctx *ctx, const DenseBackward &p, void *workspace, cudaStream_t stream) {
-  Launcher l{ctx, stream};
+af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
+  Pass l(ctx, p.dtype, scratch, stream);
   const size_t e = element_size(p.dtype);
   if (p.rows == 0) {
     l.zero(p.d_weight, e * p.inner * p.columns);
     l.zero(p.d_bias, e * p.columns);
+    *bytes = 0;
     return l.status;
   }
-  uint8_t *ws = static_cast<uint8_t *>(workspace);
-  float *dz = reinterpret_cast<float *>(ws);
-  float *dx = reinterpret_cast<float *>(ws + part(4ull * p.rows * p.columns));
-  float *dw = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(dx) + part(4ull * p.rows * p.inner));
-  with_element(p.dtype, [&](auto *tag) {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    with_activation(p.activation, [&](auto act) {
-      l.elementwise([&] {
-        dense_slope_kernel<T, act.value><<<l.blocks(p.rows * p.columns), 256, 0, stream>>>(
-            static_cast<const T *>(p.d_out), p.d_out_stride, static_cast<const float *>(p.saved), p.rows, p.columns,
-            dz);
-      });
-    });
-    if (p.d_x) {
-      l.product<float, T>({dz, p.weight, p.columns, 1, 1, p.columns, p.rows, p.inner, p.columns, dx, 0});
-      l.elementwise([&] {
-        round_kernel<T><<<l.blocks(p.rows * p.inner), 256, 0, stream>>>(dx, p.rows, p.inner, static_cast<T *>(p.d_x),
-                                                                        p.d_x_stride);
-      });
-    }
-    if (p.d_weight) {
-      l.product<T, float>({p.x, dz, 1, p.x_stride, p.columns, 1, p.inner, p.columns, p.rows, dw, 0});
-      l.elementwise([&] {
-        round_kernel<T><<<l.blocks(p.inner * p.columns), 256, 0, stream>>>(dw, p.inner, p.columns,
-                                                                           static_cast<T *>(p.d_weight), p.columns);
-      });
-    }
-    if (p.d_bias)
-      l.elementwise([&] {
-        column_sum_kernel<float, T><<<static_cast<unsigned>((p.columns + 31) / 32), 1024, 0, stream>>>(
-            dz, p.columns, p.rows, p.columns, static_cast<T *>(p.d_bias));
-      });
-  });
-  return l.status;
-}
-
-af2_status gated_forward_launch(af2_ctx *ctx, const GatedForward &p, void *workspace, cudaStream_t stream) {
-  Launcher l{ctx, stream};
-  uint8_t *ws = static_cast<uint8_t *>(workspace);
-  float *g = reinterpret_cast<float *>(ws + part(element_size(p.dtype) * p.rows * p.hidden));
-  float *v = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(g) + part(4ull * p.rows * p.hidden));
-  float *y = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(v) + part(4ull * p.rows * p.hidden));
-  with_element(p.dtype, [&](auto *tag) {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    T *h = reinterpret_cast<T *>(ws);
-    l.product<T, T>({p.x, p.w.gate_weight, p.x_stride, 1, p.hidden, 1, p.rows, p.hidden, p.channels, g, 0});
-    l.product<T, T>({p.x, p.w.value_weight, p.x_stride, 1, p.hidden, 1, p.rows, p.hidden, p.channels, v, 0});
-    with_activation(p.activation, [&](auto act) {
-      l.elementwise([&] {
-        gate_kernel<T, act.value><<<l.blocks(p.rows * p.hidden), 256, 0, stream>>>(
-            g, v, p.rows, p.hidden, static_cast<const T *>(p.w.gate_bias), static_cast<const T *>(p.w.value_bias), h,
-            static_cast<float *>(p.saved));
-      });
-    });
-    l.product<T, T>({h, p.w.output_weight, p.hidden, 1, p.channels, 1, p.rows, p.channels, p.hidden, y, 0});
-    l.elementwise([&] {
-      dense_finish_kernel<T, AF2_ACTIVATION_NONE><<<l.blocks(p.rows * p.channels), 256, 0, stream>>>(
-          y, p.rows, p.channels, static_cast<const T *>(p.w.output_bias), static_cast<const T *>(p.residual),
-          p.residual_stride, static_cast<T *>(p.out), p.out_stride, nullptr);
-    });
-  });
-  return l.status;
-}
-
-af2_status gated_backward_launch(af2_ctx *ctx, const GatedBackward &p, void *workspace, cudaStream_t stream) {
-  Launcher l{ctx, stream};
-  const size_t e = element_size(p.dtype);
-  if (p.rows == 0) {
-    const size_t w = e * p.channels * p.hidden;
-    l.zero(p.g.gate_weight, w);
-    l.zero(p.g.value_weight, w);
-    l.zero(p.g.output_weight, w);
-    l.zero(p.g.gate_bias, e * p.hidden);
-    l.zero(p.g.value_bias, e * p.hidden);
-    l.zero(p.g.output_bias, e * p.channels);
-    return l.status;
-  }
-  uint8_t *ws = static_cast<uint8_t *>(workspace);
-  float *dh = reinterpret_cast<float *>(ws + part(e * p.rows * p.hidden));
-  float *dgv = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(dh) + part(4ull * p.rows * p.hidden));
-  float *dx = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(dgv) + part(8ull * p.rows * p.hidden));
-  float *dw = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(dx) + part(4ull * p.rows * p.channels));
-  const int64_t c = p.channels, hid = p.hidden;
-  with_element(p.dtype, [&](auto *tag) {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    T *h = reinterpret_cast<T *>(ws);
-    auto round_to = [&](const float *src, int64_t rows, int64_t cols, void *dst, int64_t stride) {
-      l.elementwise([&] {
-        round_kernel<T><<<l.blocks(rows * cols), 256, 0, stream>>>(src, rows, cols, static_cast<T *>(dst), stride);
-      });
-    };
-    l.product<T, T>({p.d_out, p.w.output_weight, p.d_out_stride, 1, 1, c, p.rows, hid, c, dh, 0});
-    with_activation(p.activation, [&](auto act) {
-      l.elementwise([&] {
-        gate_backward_kernel<T, act.value><<<l.blocks(p.rows * hid), 256, 0, stream>>>(
-            dh, static_cast<const float *>(p.saved), p.rows, hid, dgv, h);
-      });
-    });
-    if (p.g.x) {
-      l.product<float, T>({dgv, p.w.gate_weight, 2 * hid, 1, 1, hid, p.rows, c, hid, dx, 0});
-      l.product<float, T>({dgv + hid, p.w.value_weight, 2 * hid, 1, 1, hid, p.rows, c, hid, dx, 1});
-      round_to(dx, p.rows, c, p.g.x, p.d_x_stride);
-    }
-    for (int i = 0; i < 2; ++i) {
-      void *dst = i ? p.g.value_weight : p.g.gate_weight, *bias = i ? p.g.value_bias : p.g.gate_bias;
-      if (dst) {
-        l.product<T, float>({p.x, dgv + i * hid, 1, p.x_stride, 2 * hid, 1, c, hid, p.rows, dw, 0});
-        round_to(dw, c, hid, dst, hid);
-      }
-      if (bias)
-        l.elementwise([&] {
-          column_sum_kernel<float, T><<<static_cast<unsigned>((hid + 31) / 32), 1024, 0, stream>>>(
-              dgv + i * hid, 2 * hid, p.rows, hid, static_cast<T *>(bias));
+  GemmOperand dz, x, w;
+  if (p.d_weight) x = l.operand(p.x, p.x_stride, p.rows, p.inner);
+  if (p.d_x) w = l.operand(p.weight, p.columns, p.inner, p.columns);
+  if (p.activation == AF2_ACTIVATION_NONE) {
+    if (p.d_x || p.d_weight) dz = l.operand(p.d_out, p.d_out_stride, p.rows, p.columns);
+    l.pack();
+    l.column_sums(p.d_out, p.d_out_stride, p.rows, p.columns, p.d_bias);
+  } else {
+    l.pack();
+    dz = l.make_operand(p.rows, p.columns);
+    const SavedPlanes saved = l.planes(const_cast<void *>(p.saved), p.rows, p.columns, 1);
+    float *partial = p.d_bias ? l.sum_room(p.rows, p.columns, 1) : nullptr;
+    l.rows_kernel(p.rows, p.columns, [&](dim3 grid) {
+      with_element(p.dtype, [&](auto *tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        with_activation(p.activation, [&](auto act) {
+          dense_slope_kernel<T, decltype(act)::value><<<grid, 256, 0, stream>>>(
+              static_cast<const T *>(p.d_out), p.d_out_stride, saved, p.rows, p.columns, const_cast<void *>(dz.ptr),
+              dz.pitch, dz.piece_stride, partial, saved_pitch(p.columns));
         });
-    }
-    if (p.g.output_weight) {
-      l.product<T, T>({h, p.d_out, 1, hid, p.d_out_stride, 1, hid, c, p.rows, dw, 0});
-      round_to(dw, hid, c, p.g.output_weight, c);
-    }
-    if (p.g.output_bias)
-      l.elementwise([&] {
-        column_sum_kernel<T, T><<<static_cast<unsigned>((c + 31) / 32), 1024, 0, stream>>>(
-            static_cast<const T *>(p.d_out), p.d_out_stride, p.rows, c, static_cast<T *>(p.g.output_bias));
       });
-  });
+    });
+    l.finish_sums(partial, ceil_div(p.rows, kSumRows), 1, 0, p.columns, p.d_bias);
+  }
+  if (p.d_x) {
+    LayerGemm g = l.product(p.rows, p.inner, p.columns);
+    g.a[0] = dz;
+    g.b[0] = w;
+    g.out[0] = p.d_x;
+    g.out_stride = p.d_x_stride;
+    l.run(g);
+  }
+  if (p.d_weight) {
+    LayerGemm g = l.product(p.inner, p.columns, p.rows);
+    g.a[0] = Pass::mn(x);
+    g.b[0] = Pass::mn(dz);
+    g.out[0] = p.d_weight;
+    g.out_stride = p.columns;
+    l.run(g);
+  }
+  *bytes = l.total();
+  return l.status;
+}
+
+af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
+  Pass l(ctx, p.dtype, scratch, stream);
+  const GemmOperand x = l.operand(p.x, p.x_stride, p.rows, p.channels);
+  const GemmOperand wg = l.operand(p.w.gate_weight, p.hidden, p.channels, p.hidden);
+  const GemmOperand wv = l.operand(p.w.value_weight, p.hidden, p.channels, p.hidden);
+  const GemmOperand wo = l.operand(p.w.output_weight, p.channels, p.hidden, p.channels);
+  l.pack();
+  GemmOperand h;
+  if (p.saved) {
+    h.ptr = p.saved;
+    h.pitch = operand_pitch(p.hidden);
+    h.piece_stride = p.rows * h.pitch;
+  } else {
+    h = l.make_operand(p.rows, p.hidden);
+  }
+  uint8_t *const planes_at =
+      p.saved ? static_cast<uint8_t *>(p.saved) + hidden_bytes(p.rows, p.hidden, p.dtype)
+              : (l.f32() ? l.take(planes_bytes(p.rows, p.hidden, p.dtype, 2)) : nullptr);
+  LayerGemm g = l.product(p.rows, p.hidden, p.channels);
+  g.a[0] = x;
+  g.b[0] = Pass::mn(wg);
+  g.b[1] = Pass::mn(wv);
+  g.bias[0] = p.w.gate_bias;
+  g.bias[1] = p.w.value_bias;
+  if (l.f32()) {
+    const SavedPlanes s = l.planes(planes_at, p.rows, p.hidden, 2);
+    g.batch = 2;
+    g.out[0] = s.f32;
+    g.out[1] = s.f32 + s.stride;
+    g.out_stride = s.pitch;
+    l.run(g);
+    l.rows_kernel(p.rows, p.hidden, [&](dim3 grid) {
+      with_activation(p.activation, [&](auto act) {
+        gate_f32_kernel<decltype(act)::value><<<grid, 256, 0, stream>>>(s, p.rows, p.hidden, const_cast<void *>(h.ptr),
+                                                                        h.pitch, h.piece_stride);
+      });
+    });
+  } else {
+    g.epilogue = kEpilogueGate;
+    g.activation = p.activation;
+    g.out[0] = const_cast<void *>(h.ptr);
+    g.out_stride = h.pitch;
+    if (p.saved) g.saved = l.planes(planes_at, p.rows, p.hidden, 2);
+    l.run(g);
+  }
+  LayerGemm y = l.product(p.rows, p.channels, p.hidden);
+  y.a[0] = h;
+  y.b[0] = Pass::mn(wo);
+  y.bias[0] = p.w.output_bias;
+  y.residual = p.residual;
+  y.residual_stride = p.residual_stride;
+  y.out[0] = p.out;
+  y.out_stride = p.out_stride;
+  l.run(y);
+  *bytes = l.total();
+  return l.status;
+}
+
+af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
+  Pass l(ctx, p.dtype, scratch, stream);
+  const int64_t c = p.channels, hid = p.hidden;
+  if (p.rows == 0) {
+    const size_t e = element_size(p.dtype);
+    for (void *w : {p.g.gate_weight, p.g.value_weight, p.g.output_weight}) l.zero(w, e * c * hid);
+    for (void *b : {p.g.gate_bias, p.g.value_bias}) l.zero(b, e * hid);
+    l.zero(p.g.output_bias, e * c);
+    *bytes = 0;
+    return l.status;
+  }
+  const bool gradients_at_hidden = p.g.x || p.g.gate_weight || p.g.gate_bias || p.g.value_weight || p.g.value_bias;
+  const GemmOperand dy = l.operand(p.d_out, p.d_out_stride, p.rows, c);
+  GemmOperand x, wg, wv, wo, dgv[2];
+  if (p.g.gate_weight || p.g.value_weight) x = l.operand(p.x, p.x_stride, p.rows, c);
+  if (p.g.x) {
+    wg = l.operand(p.w.gate_weight, hid, c, hid);
+    wv = l.operand(p.w.value_weight, hid, c, hid);
+  }
+  if (gradients_at_hidden) wo = l.operand(p.w.output_weight, c, hid, c);
+  l.pack();
+  GemmOperand h;
+  h.ptr = p.saved;
+  h.pitch = operand_pitch(hid);
+  h.piece_stride = p.rows * h.pitch;
+  uint8_t *planes_at = static_cast<uint8_t *>(const_cast<void *>(p.saved)) + hidden_bytes(p.rows, hid, p.dtype);
+  const SavedPlanes saved = l.planes(planes_at, p.rows, hid, 2);
+
+  l.column_sums(p.d_out, p.d_out_stride, p.rows, c, p.g.output_bias);
+  if (gradients_at_hidden) {
+    dgv[0] = l.make_operand(p.rows, hid);
+    dgv[1] = l.make_operand(p.rows, hid);
+    const bool sums = p.g.gate_bias || p.g.value_bias;
+    LayerGemm g = l.product(p.rows, hid, c);
+    g.a[0] = dy;
+    g.b[0] = wo;
+    float *partial = nullptr;
+    int64_t chunks = 0;
+    if (l.f32()) {
+      chunks = ceil_div(p.rows, kSumRows);
+      if (sums) partial = l.sum_room(p.rows, hid, 2);
+      float *dh = reinterpret_cast<float *>(l.take(4ull * p.rows * saved.pitch));
+      g.out[0] = dh;
+      g.out_stride = saved.pitch;
+      l.run(g);
+      l.rows_kernel(p.rows, hid, [&](dim3 grid) {
+        with_activation(p.activation, [&](auto act) {
+          gate_backward_f32_kernel<decltype(act)::value><<<grid, 256, 0, stream>>>(
+              dh, saved, p.rows, hid, static_cast<uint16_t *>(const_cast<void *>(dgv[0].ptr)), dgv[0].pitch,
+              dgv[0].piece_stride,
+              static_cast<const uint16_t *>(dgv[1].ptr) - static_cast<const uint16_t *>(dgv[0].ptr), partial,
+              saved.pitch);
+        });
+      });
+    } else {
+      chunks = ceil_div(p.rows, 32);
+      if (sums) partial = reinterpret_cast<float *>(l.take(8ull * chunks * saved.pitch));
+      g.epilogue = kEpilogueGateBackward;
+      g.activation = p.activation;
+      g.saved = saved;
+      g.out[0] = const_cast<void *>(dgv[0].ptr);
+      g.out[1] = const_cast<void *>(dgv[1].ptr);
+      g.out_stride = dgv[0].pitch;
+      g.column_partial = partial;
+      l.run(g);
+    }
+    l.finish_sums(partial, chunks, 2, 0, hid, p.g.gate_bias);
+    l.finish_sums(partial, chunks, 2, 1, hid, p.g.value_bias);
+  }
+  if (p.g.x) {
+    LayerGemm g = l.product(p.rows, c, hid);
+    g.segments = 2;
+    g.a[0] = dgv[0];
+    g.a[1] = dgv[1];
+    g.b[0] = wg;
+    g.b[1] = wv;
+    g.out[0] = p.g.x;
+    g.out_stride = p.d_x_stride;
+    l.run(g);
+  }
+  if (p.g.gate_weight || p.g.value_weight) {
+    LayerGemm g = l.product(c, hid, p.rows);
+    g.a[0] = Pass::mn(x);
+    int n = 0;
+    if (p.g.gate_weight) g.b[n] = Pass::mn(dgv[0]), g.out[n++] = p.g.gate_weight;
+    if (p.g.value_weight) g.b[n] = Pass::mn(dgv[1]), g.out[n++] = p.g.value_weight;
+    g.batch = n;
+    g.out_stride = hid;
+    l.run(g);
+  }
+  if (p.g.output_weight) {
+    LayerGemm g = l.product(hid, c, p.rows);
+    g.a[0] = Pass::mn(h);
+    g.b[0] = Pass::mn(dy);
+    g.out[0] = p.g.output_weight;
+    g.out_stride = c;
+    l.run(g);
+  }
+  *bytes = l.total();
   return l.status;
 }
 

@@ -1,0 +1,62 @@
+// layer_gemm.h -- the products behind the layers with learned weights.
+#pragma once
+
+#include "af2_internal.h"
+
+namespace af2 {
+
+// One 16-bit operand as TMA reads it: rows of `pitch` elements (a multiple of 8, 16-byte aligned).
+// K-major: [outer][pitch] with k contiguous; MN-major: [k][pitch] with the outer index contiguous.
+// pieces > 1: an f32 operand as that many bf16 terms (high to low), `piece_stride` elements apart.
+struct GemmOperand {
+  const void *ptr = nullptr;
+  int64_t pitch = 0;
+  bool mn_major = false;
+  int64_t piece_stride = 0;
+};
+
+// How a tile leaves the accumulators.
+enum GemmEpilogue {
+  kEpilogueOut = 0,       // out = act(acc + bias) (+ residual), saved = acc + bias
+  kEpilogueGate = 1,      // b[0], b[1] are the gate's and the value's weights: out = act(g) v, saved = g, v
+  kEpilogueGateBackward,  // acc = dh: with the saved g and v, out = dg and dv
+};
+
+// Pre-activations kept for the backward pass of the 16-bit types: the upper 24 bits of each f32, as
+// planes of its upper 16 (`hi`) and of the next 8 (`lo`), rows of `pitch` elements, `stride`
+// elements from the gate's plane to the value's.  The f32 type keeps f32 in `f32` instead.
+struct SavedPlanes {
+  uint16_t *hi = nullptr;
+  uint8_t *lo = nullptr;
+  float *f32 = nullptr;
+  int64_t pitch = 0, stride = 0;
+};
+
+struct LayerGemm {
+  int64_t m = 0, n = 0, k = 0;  // n: of one batch entry (the gate: hidden channels)
+  int segments = 1;             // sums over a[s] b[s], s < segments, each of depth k
+  int batch = 1;                // products a[0] b[z] -> out[z], z < batch
+  GemmOperand a[2], b[2];
+  bool bf16 = false;            // the operands' type
+  int pieces = 1;               // 1, or 3: f32 operands in bf16 terms
+  GemmEpilogue epilogue = kEpilogueOut;
+  int activation = 0;
+  int out_dtype = 0;
+  void *out[2] = {nullptr, nullptr};
+  int64_t out_stride = 0;
+  const void *bias[2] = {nullptr, nullptr};  // of out_dtype, or NULL
+  const void *residual = nullptr;            // of out_dtype
+  int64_t residual_stride = 0;
+  SavedPlanes saved;                         // written by Out and Gate, read by GateBackward
+  float *column_partial = nullptr;           // GateBackward: [ceil(m / 32)][2 * saved.pitch] column sums, or NULL
+  uint8_t *scratch = nullptr;                // split sums: layer_gemm_scratch() bytes
+};
+
+// Row pitch (elements) of a 16-bit operand of `width`, and of the saved planes.
+inline int64_t operand_pitch(int64_t width) { return align_up(width, 8); }
+inline int64_t saved_pitch(int64_t width) { return align_up(width, 32); }
+
+uint64_t layer_gemm_scratch(const LayerGemm &g);
+af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stream);
+
+}  // namespace af2

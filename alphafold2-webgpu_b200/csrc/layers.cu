@@ -147,15 +147,22 @@ af2_status read_options(af2_ctx *ctx, const af2_layer_options *o, int64_t x_widt
   return AF2_OK;
 }
 
-// Runs `launch(scratch)` with the call's scratch.
-template <typename F>
-af2_status with_scratch(af2_ctx *ctx, void *workspace, uint64_t bytes, cudaStream_t stream, F &&launch) {
+// Runs `pass` (see dense_forward) on p with the call's scratch.
+template <typename P>
+af2_status run_pass(af2_ctx *ctx, void *workspace, cudaStream_t stream, const P &p,
+                    af2_status (*pass)(af2_ctx *, const P &, void *, uint64_t *, cudaStream_t)) {
+  uint64_t bytes = 0;
+  if (!workspace)
+    if (af2_status st = pass(nullptr, p, nullptr, &bytes, stream); st != AF2_OK) return st;
   LayerScratch scratch(ctx, stream);
   if (af2_status st = scratch.acquire(workspace, bytes); st != AF2_OK) return st;
-  const af2_status st = launch(static_cast<void *>(scratch.base()));
+  const af2_status st = pass(ctx, p, scratch.base(), &bytes, stream);
   const af2_status rel = scratch.release();
   return st != AF2_OK ? st : rel;
 }
+
+// Stands for a tensor at an unknown address when scratch is sized: one that TMA cannot read in place.
+void *const kAnywhere = reinterpret_cast<void *>(uintptr_t(4));
 
 cudaStream_t stream_of(af2_ctx *ctx, void *stream) {
   return stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
@@ -200,8 +207,13 @@ af2_status af2_dense_workspace_bytes(const af2_linear_shape *shape, int dtype, i
     if (af2_status st = check_sizes(nullptr, shape->rows, shape->inner, shape->columns, dtype, ""); st != AF2_OK)
       return st;
     if (af2_status st = check_activation(nullptr, activation); st != AF2_OK) return st;
-    *bytes = dense_workspace_bytes(shape->rows, shape->inner, shape->columns, dtype, activation, backward != 0);
-    return AF2_OK;
+    void *const any = kAnywhere;
+    const int64_t rows = shape->rows, in = shape->inner, cols = shape->columns;
+    if (backward)
+      return dense_backward(nullptr, {rows, in, cols, dtype, activation, any, any, any, any, cols, in, in, any, any, any},
+                            nullptr, bytes, nullptr);
+    return dense_forward(nullptr, {rows, in, cols, dtype, activation, any, any, any, any, in, cols, cols, any, any},
+                         nullptr, bytes, nullptr);
   });
 }
 
@@ -228,9 +240,7 @@ af2_status af2_dense(af2_ctx *ctx, const af2_linear_shape *shape, int dtype, con
     const DenseForward p{shape->rows, shape->inner, shape->columns, dtype, s.activation, x,   weight,
                          bias,        residual,     s.x,            s.residual, s.out,  out, saved};
     const cudaStream_t cs = stream_of(ctx, stream);
-    return with_scratch(ctx, workspace,
-                        dense_workspace_bytes(p.rows, p.inner, p.columns, dtype, s.activation, false), cs,
-                        [&](void *ws) { return dense_forward_launch(ctx, p, ws, cs); });
+    return run_pass(ctx, workspace, cs, p, dense_forward);
   });
 }
 
@@ -261,9 +271,7 @@ af2_status af2_dense_backward(af2_ctx *ctx, const af2_linear_shape *shape, int d
     const DenseBackward p{shape->rows, shape->inner, shape->columns, dtype, s.activation, d_out, x,       weight,
                           saved,       s.out,        s.x,            s.d_x, d_x,          d_weight, d_bias};
     const cudaStream_t cs = stream_of(ctx, stream);
-    return with_scratch(ctx, workspace,
-                        dense_workspace_bytes(p.rows, p.inner, p.columns, dtype, s.activation, true), cs,
-                        [&](void *ws) { return dense_backward_launch(ctx, p, ws, cs); });
+    return run_pass(ctx, workspace, cs, p, dense_backward);
   });
 }
 
@@ -285,8 +293,21 @@ af2_status af2_gated_transition_workspace_bytes(const af2_transition_shape *shap
     if (af2_status st = check_sizes(nullptr, shape->rows, shape->channels, shape->hidden_channels, dtype, "");
         st != AF2_OK)
       return st;
-    *bytes = gated_workspace_bytes(shape->rows, shape->channels, shape->hidden_channels, dtype, backward != 0);
-    return AF2_OK;
+    void *const any = kAnywhere;
+    const int64_t rows = shape->rows, c = shape->channels, h = shape->hidden_channels;
+    const af2_gated_weights w{any, any, any, any, any, any};
+    if (backward)
+      return gated_backward(nullptr, {rows, c, h, dtype, 0, any, any, any, w, {any, any, any, any, any, any, any}, c, c, c},
+                            nullptr, bytes, nullptr);
+    uint64_t saving = 0;  // the forward pass that saves nothing needs the most
+    if (af2_status st = gated_forward(nullptr, {rows, c, h, dtype, 0, any, any, w, c, c, c, any, any}, nullptr, &saving,
+                                      nullptr);
+        st != AF2_OK)
+      return st;
+    const af2_status st = gated_forward(nullptr, {rows, c, h, dtype, 0, any, any, w, c, c, c, any, nullptr}, nullptr,
+                                        bytes, nullptr);
+    if (*bytes < saving) *bytes = saving;
+    return st;
   });
 }
 
@@ -321,8 +342,7 @@ af2_status af2_gated_transition(af2_ctx *ctx, const af2_transition_shape *shape,
     const GatedForward p{shape->rows, shape->channels, shape->hidden_channels, dtype, s.activation, x,
                          residual,    *weights,        s.x,                    s.residual, s.out,   out, saved};
     const cudaStream_t cs = stream_of(ctx, stream);
-    return with_scratch(ctx, workspace, gated_workspace_bytes(p.rows, p.channels, p.hidden, dtype, false), cs,
-                        [&](void *ws) { return gated_forward_launch(ctx, p, ws, cs); });
+    return run_pass(ctx, workspace, cs, p, gated_forward);
   });
 }
 
@@ -362,8 +382,7 @@ af2_status af2_gated_transition_backward(af2_ctx *ctx, const af2_transition_shap
     const GatedBackward p{shape->rows, shape->channels, shape->hidden_channels, dtype, s.activation, d_out, x,
                           saved,       *weights,        *gradients,             s.out, s.x,          s.d_x};
     const cudaStream_t cs = stream_of(ctx, stream);
-    return with_scratch(ctx, workspace, gated_workspace_bytes(p.rows, p.channels, p.hidden, dtype, true), cs,
-                        [&](void *ws) { return gated_backward_launch(ctx, p, ws, cs); });
+    return run_pass(ctx, workspace, cs, p, gated_backward);
   });
 }
 
@@ -398,9 +417,11 @@ static af2_status gradient_call(af2_ctx *ctx, const af2_tensor_ref *tensors, con
     if ((st = check_block(ctx, workspace, "workspace")) != AF2_OK) return st;
     cudaSetDevice(ctx->device);
     const cudaStream_t cs = stream_of(ctx, stream);
-    return with_scratch(ctx, workspace, gradient_norm_workspace_bytes(count), cs, [&](void *ws) {
-      return gradient_norm_launch(ctx, tensors, outputs, count, clip, static_cast<float>(max_norm), norm, ws, cs);
-    });
+    LayerScratch scratch(ctx, cs);
+    if ((st = scratch.acquire(workspace, gradient_norm_workspace_bytes(count))) != AF2_OK) return st;
+    st = gradient_norm_launch(ctx, tensors, outputs, count, clip, static_cast<float>(max_norm), norm, scratch.base(), cs);
+    const af2_status rel = scratch.release();
+    return st != AF2_OK ? st : rel;
   });
 }
 
