@@ -11,10 +11,10 @@
 // that TMA cannot read (rows not in 16-byte pieces) are copied to padded rows
 // first, and f32 ones are split into bf16 terms by the same pass.
 //
-// What a forward pass saves, in the 16-bit types: the pre-activations' upper 24
-// bits (their f32 rounded to 2^-16), so that the backward pass rounds to 16
-// bits only what becomes a product's operand; and the gated transition's h, an
-// operand already.
+// What a forward pass saves: the factors that the backward pass multiplies by
+// (dense: act'(z); gated: v act'(g) and act(g); the f32 gated transition g and v
+// themselves), 24 bits of each in the 16-bit types, and the gated transition's
+// h, an operand already.
 #include <algorithm>
 #include <type_traits>
 
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(1024) column_finish_kernel(const float *partia
   }
 }
 
-// Eight saved pre-activations.
+// Eight saved values.
 template <typename T>
 __device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int64_t r, int64_t c, float (&z)[8]) {
   const int64_t at = plane * s.stride + r * s.pitch + c;
@@ -190,8 +190,8 @@ __device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int
   }
 }
 
-// dz = dy act'(z) as an operand, with its column sums
-template <typename T, int ACT>
+// dz = dy act'(z), the slope saved, as an operand, with its column sums
+template <typename T>
 __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t dy_stride, const SavedPlanes saved,
                                                           int64_t rows, int64_t width, void *dz, int64_t dz_pitch,
                                                           int64_t dz_piece, float *partial, int64_t pitch) {
@@ -202,9 +202,7 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
     load_saved8<T>(saved, 0, r, c, z);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float value, slope;
-      activate_slope<ACT>(z[i], value, slope);
-      d[i] = i < n ? d[i] * slope : 0.f;
+      d[i] = i < n ? d[i] * z[i] : 0.f;
       sums[0][i] += d[i];
     }
     store_operand8<T>(dz, r * dz_pitch + c, dz_piece, d);
@@ -220,7 +218,11 @@ __global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, 
     load_saved8<float>(saved, 0, r, c, g);
     load_saved8<float>(saved, 1, r, c, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = activate<ACT>(g[i]) * v[i];
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = activate2<ACT, false>(make_float2(g[2 * i], g[2 * i + 1]));
+      g[2 * i] = a.x * v[2 * i];
+      g[2 * i + 1] = a.y * v[2 * i + 1];
+    }
     store_operand8<float>(h, r * h_pitch + c, h_piece, g);
   });
 }
@@ -238,11 +240,11 @@ __global__ void __launch_bounds__(256) gate_backward_f32_kernel(const float *dh,
     load_saved8<float>(saved, 1, r, c, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float value, slope;
-      activate_slope<ACT>(g[i], value, slope);
+      float2 value, slope;
+      activate_slope2<ACT, false>(f2(g[i]), value, slope);
       const bool in = c + i < width;  // past the width nothing was written
-      g[i] = in ? d[i] * v[i] * slope : 0.f;
-      v[i] = in ? d[i] * value : 0.f;
+      g[i] = in ? d[i] * v[i] * slope.x : 0.f;
+      v[i] = in ? d[i] * value.x : 0.f;
       sums[0][i] += g[i];
       sums[1][i] += v[i];
     }
@@ -453,11 +455,9 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
     l.rows_kernel(p.rows, p.columns, [&](dim3 grid) {
       with_element(p.dtype, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        with_activation(p.activation, [&](auto act) {
-          dense_slope_kernel<T, decltype(act)::value><<<grid, 256, 0, stream>>>(
-              static_cast<const T *>(p.d_out), p.d_out_stride, saved, p.rows, p.columns, const_cast<void *>(dz.ptr),
-              dz.pitch, dz.piece_stride, partial, saved_pitch(p.columns));
-        });
+        dense_slope_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T *>(p.d_out), p.d_out_stride, saved, p.rows,
+                                                        p.columns, const_cast<void *>(dz.ptr), dz.pitch,
+                                                        dz.piece_stride, partial, saved_pitch(p.columns));
       });
     });
     l.finish_sums(partial, ceil_div(p.rows, kSumRows), 1, 0, p.columns, p.d_bias);

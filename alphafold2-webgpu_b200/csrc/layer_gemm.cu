@@ -5,18 +5,21 @@
 // A cluster of two CTAs computes a 256 x BN tile with M = 256 MMAs
 // (cta_group::2): CTA r holds rows 128 r .. of A's tile and half of B's rows,
 // so each SM reads half of the B tile that it multiplies by.  Warp 0 of each
-// CTA issues TMA loads, warp 1 of the even CTA the MMAs, warps 2-9 drain the
-// accumulators (two warps per TMEM lane quarter, half of the columns each);
-// two accumulators, so one tile's epilogue overlaps the next tile's MMAs.
-// Operands are taken as they are stored: K-major rows as one 128-byte-swizzled
-// block per K step of 64, MN-major ones as 64-wide blocks of 64 k each (the
-// tensor core's transposed order), so no weight and no activation is ever
-// transposed in memory.
+// CTA issues TMA loads, warp 1 of the even CTA the MMAs, warps 2-17 drain the
+// accumulators (four warps per TMEM lane quarter, every fourth block of 32
+// columns each: eight warps left the multi-function unit and the issue slots
+// two thirds idle); two accumulators, so one tile's epilogue overlaps the next
+// tile's MMAs.  Operands are taken as they are stored: K-major rows as one
+// 128-byte-swizzled block per K step of 64, MN-major ones as 64-wide blocks of
+// 64 k each (the tensor core's transposed order), so no weight and no
+// activation is ever transposed in memory.  What an epilogue reads (residual,
+// saved factors) comes by TMA into the same block of shared memory that its
+// result leaves from.
 //
 // f32 tensors are multiplied as three bf16 terms each, x = x0 + x1 + x2, and
 // the six products whose weight is at least 2^-16 of the largest are summed,
 // the small ones first: what is left out is below 2^-24 of |x||y|, f32's own
-// rounding.
+// rounding.  (An infinite f32 element makes its sums NaN or infinite.)
 #include <algorithm>
 #include <type_traits>
 
@@ -27,26 +30,47 @@ namespace af2 {
 namespace {
 
 constexpr int BM = 128, PAIR_M = 256, BK = 64;
-constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr int EPI_WARPS = 16, THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint32_t A_BYTES = BM * 128;
 constexpr int kPairs = 74;  // CTA pairs of a B200; only the choice of tiles and splits depends on it
 
-// Stages of the operand ring and bytes of one epilogue warp's staging.
-template <int EPI, int BN>
+// The kernels behind the epilogues: Gate with and without what the backward pass needs.
+enum Kind { kOut, kGate, kGateSave, kGateBackward };
+
+// Stages of the operand ring and bytes of one epilogue warp's staging: 32 x 32 blocks of 16 bits
+// (2 KB), two of them; with factors to save or to read three (h and the factors' upper halves; the
+// factors' upper halves and their 1 KB of lower bytes), paid for with a stage.
+template <int KIND, int BN>
 struct Shape {
   static constexpr uint32_t B_BYTES = (BN / 2) * 128;
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = EPI == kEpilogueGateBackward ? 4 : BN == 256 ? 6 : 8;
-  // Out, Gate: two 32 x 32 blocks of 16 bits (or one of 32); GateBackward: two slots of the four
-  // planes' blocks (g and v: 2 KB of upper halves, 1 KB of lower bytes), the results written over them
-  static constexpr uint32_t SLOT_BYTES = EPI == kEpilogueGateBackward ? 6144 : 2048;
+  static constexpr uint32_t SLOT_BYTES = KIND == kGateSave || KIND == kGateBackward ? 6144 : 4096;
+  static constexpr int STAGES = (229376 - EPI_WARPS * SLOT_BYTES) / STAGE_BYTES;
   static constexpr uint32_t OFF_STAGE = STAGES * STAGE_BYTES;
-  static constexpr uint32_t OFF_BAR = OFF_STAGE + EPI_WARPS * 2 * SLOT_BYTES;
+  static constexpr uint32_t OFF_BAR = OFF_STAGE + EPI_WARPS * SLOT_BYTES;
   static constexpr uint32_t BYTES = OFF_BAR + 512 + 1024;
 };
 
 struct Maps {
-  CUtensorMap a[2], b[2], out[2], hi, lo;
+  CUtensorMap a[2], b[2], out[2], residual, hi, lo;
+};
+
+// n / d and n % d for n below 2^30, d fixed for a launch: the quotient by a multiply-high with
+// ceil(2^(32 + s) / d), 2^s >= d, whose error stays below 1 / d there.
+struct Divisor {
+  uint32_t d = 1, mul = 0, shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t divisor) : d(divisor) {
+    while ((1u << shift) < d) ++shift;
+    // 2^32 < 2^(32 + s) / d < 2^33: the leading 2^32 is added by the quotient itself
+    mul = static_cast<uint32_t>(((uint64_t(1) << (32 + shift)) + d - 1) / d - (uint64_t(1) << 32));
+  }
+  __device__ __forceinline__ int split(int &n) const {  // n becomes the quotient; returns the remainder
+    const uint32_t q = (__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift;
+    const int r = n - static_cast<int>(q * d);
+    n = static_cast<int>(q);
+    return r;
+  }
 };
 
 struct Args {
@@ -61,12 +85,13 @@ struct Args {
   int64_t saved_pitch, saved_stride;
   float *column_partial;
   int64_t m;
-  int n, k_blocks, splits, combos, segments, batch;
-  int tiles_m, tiles_n, total_tiles;
+  int n, k_blocks, splits, combos, segments;
+  Divisor tiles_m, tiles_n, batches;
+  int total_tiles;
   int a_mn, b_mn, bf16, activation;
-  int tma_out;     // out rows are 16-byte aligned: whole blocks leave by TMA
-  int vector_res;  // residual rows are 16-byte aligned
-  int vector_bias;
+  int tma_out;       // out rows are 16-byte aligned: whole blocks leave by TMA
+  int tma_residual;  // the residual's blocks come by TMA
+  int vector_bias;   // 16-byte aligned
   int partial;     // out[0] is [split][batch][m][n] of f32 sums (no bias, activation or residual)
   unsigned int *err;
 };
@@ -76,147 +101,111 @@ __constant__ const int8_t kTermA[6] = {2, 0, 1, 1, 0, 0};
 __constant__ const int8_t kTermB[6] = {0, 2, 1, 0, 1, 0};
 
 struct Tile {
-  int split, z, mi, ni, kb0, kb1;
+  int split, z, mi, ni;
 };
 __device__ __forceinline__ Tile tile_at(const Args &p, int t) {
   Tile r;
-  r.ni = t % p.tiles_n;
-  t /= p.tiles_n;
-  r.mi = t % p.tiles_m;
-  t /= p.tiles_m;
-  r.z = t % p.batch;
-  r.split = t / p.batch;
-  r.kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * r.split / p.splits);
-  r.kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (r.split + 1) / p.splits);
+  r.ni = p.tiles_n.split(t);
+  r.mi = p.tiles_m.split(t);
+  r.z = p.batches.split(t);
+  r.split = t;
   return r;
 }
-
-template <typename F>
-__device__ __forceinline__ void activation_switch(int activation, F &&f) {
-  switch (activation) {
-    case AF2_ACTIVATION_RELU: f(std::integral_constant<int, AF2_ACTIVATION_RELU>()); break;
-    case AF2_ACTIVATION_SIGMOID: f(std::integral_constant<int, AF2_ACTIVATION_SIGMOID>()); break;
-    case AF2_ACTIVATION_SILU: f(std::integral_constant<int, AF2_ACTIVATION_SILU>()); break;
-    case AF2_ACTIVATION_GELU: f(std::integral_constant<int, AF2_ACTIVATION_GELU>()); break;
-    default: f(std::integral_constant<int, AF2_ACTIVATION_NONE>()); break;
-  }
+// The tile's range of K steps.
+__device__ __forceinline__ int k_begin(const Args &p, int split) {
+  return static_cast<int>(static_cast<int64_t>(p.k_blocks) * split / p.splits);
 }
 
-// x[i] += row[c0 + i] for the columns below `cols`; `vector`: row + c0 is 16-byte aligned.
+// 32 values of a row as raw 16-bit pairs; zeros past `cols`.
 template <typename T>
-__device__ __forceinline__ void add_row32(const T *row, int c0, int cols, bool vector, float (&x)[32]) {
+__device__ __forceinline__ void load_raw32(const T *row, int c0, int cols, bool vector, uint32_t (&w)[16]) {
   if (vector && c0 + 32 <= cols) {
-    constexpr int PER = 16 / sizeof(T);
     const uint4 *p = reinterpret_cast<const uint4 *>(row + c0);
 #pragma unroll
-    for (int w = 0; w < 32 / PER; ++w) {
-      const uint4 u = p[w];
-      const T *e = reinterpret_cast<const T *>(&u);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) x[w * PER + i] += to_f32<T>(e[i]);
+    for (int i = 0; i < 4; ++i) {
+      const uint4 u = __ldg(p + i);
+      w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
     }
   } else {
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (c0 + i < cols) x[i] += to_f32<T>(row[c0 + i]);
-  }
-}
-
-// The upper 16 bits of two f32 as one word (the first in its lower half), and the third bytes of four.
-__device__ __forceinline__ uint32_t upper_halves(float a, float b) {
-  return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-}
-__device__ __forceinline__ uint32_t third_bytes(float a, float b, float c, float d) {
-  return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0051),
-                     __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0051), 0x5410);
-}
-// The f32 whose upper half is half `i` of `hi` and whose third byte is byte `j` of `lo`.
-template <int I, int J>
-__device__ __forceinline__ float from_planes(uint32_t hi, uint32_t lo) {
-  // bytes (low to high): 0, lo[J], hi[2I], hi[2I + 1]; byte_perm sources 0-3 = hi, 4-7 = lo
-  constexpr uint32_t sel = ((2 * I + 1) << 12) | ((2 * I) << 8) | ((4 + J) << 4);
-  return __uint_as_float(__byte_perm(hi, lo, sel) & 0xffffff00u);
-}
-
-// One row (`lane`) of a 32 x 32 block of 16-bit values in a 64B-swizzled slot: its four 16-byte pieces.
-__device__ __forceinline__ uint4 *slot_piece(uint8_t *slot, int lane, int c) {
-  return reinterpret_cast<uint4 *>(slot + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4));
-}
-__device__ __forceinline__ void slot_write(uint8_t *slot, int lane, const uint32_t (&w)[16]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    *slot_piece(slot, lane, c) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-}
-
-// An epilogue warp's ring of two 2 KB blocks on their way out.
-struct StoreRing {
-  uint8_t *ptr;
-  uint32_t addr;
-  int next = 0;
-
-  // The next block, free for writing.
-  __device__ __forceinline__ int take(int lane) {
-    if (lane == 0) bulk_wait_read_but_one();
-    __syncwarp();
-    return next;
-  }
-  __device__ __forceinline__ void store16(const CUtensorMap *map, int lane, const uint32_t (&w)[16], int c0, int r0,
-                                          int z, bool inside) {
-    const int b = take(lane);
-    slot_write(ptr + b * 2048, lane, w);
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (inside) tma_store_3d(map, addr + b * 2048, c0, r0, z);
-      bulk_commit();
-    }
-    next ^= 1;
-  }
-  // A 32 x 32 block of f32 over both blocks (128B-swizzled rows).
-  __device__ __forceinline__ void store32(const CUtensorMap *map, int lane, const float (&y)[32], int c0, int r0,
-                                          int z, bool inside) {
-    if (lane == 0) bulk_wait_read_all();
-    __syncwarp();
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-      *reinterpret_cast<float4 *>(ptr + sw128_offset(lane, c)) =
-          make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (inside) tma_store_3d(map, addr, c0, r0, z);
-      bulk_commit();
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t a = c0 + 2 * i < cols ? p[c0 + 2 * i] : 0, b = c0 + 2 * i + 1 < cols ? p[c0 + 2 * i + 1] : 0;
+      w[i] = a | (b << 16);
     }
   }
-};
+}
 
-// The planes of 32 saved pre-activations of one row: upper halves through the ring, third bytes directly.
-__device__ __forceinline__ void save_planes(const Maps &maps, const Args &p, StoreRing &ring, int lane,
-                                            const float (&z)[32], int c0, int r0, int plane, int64_t m, bool inside) {
-  uint32_t hi[16];
+// A f32 is kept to 24 bits as its upper 16 and its third byte (cut, not rounded: no carry can turn a
+// NaN into a number).  The upper halves of two as one word, the third bytes of four as one.
+__device__ __forceinline__ uint32_t upper_halves(float2 v) {
+  return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
+}
+__device__ __forceinline__ uint32_t third_bytes(float2 a, float2 b) {
+  return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0051),
+                     __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0051), 0x5410);
+}
+// Two f32 from a word of upper halves and bytes 2 PAIR, 2 PAIR + 1 of a word of third bytes.
+template <int PAIR>
+__device__ __forceinline__ float2 from_planes(uint32_t hi, uint32_t lo) {
+  // bytes low to high: (masked), lo[.], hi[.], hi[.]; byte_perm sources 0-3 = hi, 4-7 = lo
+  constexpr uint32_t s0 = 0x1000 | ((4 + 2 * PAIR) << 4), s1 = 0x3200 | ((5 + 2 * PAIR) << 4);
+  return make_float2(__uint_as_float(__byte_perm(hi, lo, s0) & 0xffffff00u),
+                     __uint_as_float(__byte_perm(hi, lo, s1) & 0xffffff00u));
+}
+
+// 16-byte piece c of row `row` of a 32 x 32 block of 16 bits (64B-swizzled), and one element of it.
+__device__ __forceinline__ uint4 *piece16(uint8_t *block, int row, int c) {
+  return reinterpret_cast<uint4 *>(block + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ uint16_t *element16(uint8_t *block, int row, int col) {
+  return reinterpret_cast<uint16_t *>(piece16(block, row, col >> 3)) + (col & 7);
+}
+// The same of a block of f32 (128B-swizzled, 4 KB).
+__device__ __forceinline__ float4 *piece32(uint8_t *block, int row, int c) {
+  return reinterpret_cast<float4 *>(block + sw128_offset(row, c));
+}
+__device__ __forceinline__ float *element32(uint8_t *block, int row, int col) {
+  return reinterpret_cast<float *>(piece32(block, row, col >> 2)) + (col & 3);
+}
+
+// Rows that TMA cannot address, moved between memory and a block with the lanes along each row.
+template <typename T, bool IN>
+__device__ __forceinline__ void move_rows(uint8_t *block, T *at, int64_t stride, int rows, int cols, int lane) {
+  if (lane < cols)
+    for (int r = 0; r < rows; ++r) {
+      T *s;
+      if constexpr (sizeof(T) == 4)
+        s = element32(block, r, lane);
+      else
+        s = reinterpret_cast<T *>(element16(block, r, lane));
+      T *g = at + r * stride + lane;
+      if constexpr (IN)
+        *s = *g;
+      else
+        *g = *s;
+    }
+}
+
+// x[i] of lane l becomes, in x[0] of lane i, the sum over the lanes: 31 exchanges for 32 columns.
+__device__ __forceinline__ float lane_sums(float (&x)[32], int lane) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) hi[i] = upper_halves(z[2 * i], z[2 * i + 1]);
-  ring.store16(&maps.hi, lane, hi, c0, r0, plane, inside);
-  if (inside && m < p.m) {
-    uint4 *dst = reinterpret_cast<uint4 *>(p.saved_lo + plane * p.saved_stride + m * p.saved_pitch + c0);
-    uint32_t lo[8];
+  for (int o = 16; o; o >>= 1) {
+    const bool upper = lane & o;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lo[i] = third_bytes(z[4 * i], z[4 * i + 1], z[4 * i + 2], z[4 * i + 3]);
-    dst[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    dst[1] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+    for (int i = 0; i < o; ++i) {
+      const float keep = upper ? x[i + o] : x[i], send = upper ? x[i] : x[i + o];
+      x[i] = keep + __shfl_xor_sync(kFull, send, o);
+    }
   }
+  return x[0];
 }
 
-template <typename T>
-__device__ __forceinline__ void pack_row(const float (&y)[32], uint32_t (&w)[16]) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = pack2_t<T>(y[2 * i], y[2 * i + 1]);
-}
-
-template <int EPI, typename OT, int BN>
+template <int KIND, typename OT, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     layer_gemm_kernel(const __grid_constant__ Maps maps, const Args p) {
-  using S = Shape<EPI, BN>;
+  using S = Shape<KIND, BN>;
+  constexpr bool GATE = KIND == kGate || KIND == kGateSave;
   constexpr int STAGES = S::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
@@ -224,7 +213,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const uint32_t bar0 = sbase + S::OFF_BAR;
   // full: the leader's only (both CTAs' loads complete on it); empty, acc_full: both CTAs
   // (multicast commits); acc_empty: the leader's, one arrival per epilogue warp of the pair;
-  // load: one per epilogue warp and slot, for the planes it reads
+  // load: one per epilogue warp and block, for what it reads
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (STAGES + s); };
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * STAGES + b); };
@@ -248,9 +237,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       mbar_init(acc_empty(b), 2 * EPI_WARPS);
     }
     mbar_init(drain, 1);
-    if (EPI == kEpilogueGateBackward)
-      for (int w = 0; w < EPI_WARPS; ++w)
-        for (int b = 0; b < 2; ++b) mbar_init(load(w, b), 1);
+    for (int w = 0; w < EPI_WARPS; ++w)
+      for (int b = 0; b < 2; ++b) mbar_init(load(w, b), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -272,14 +260,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       bool ok = true;
       for (int t = pair; t < p.total_tiles && ok; t += npairs) {
         const Tile tile = tile_at(p, t);
+        const int kb0 = p.splits > 1 ? k_begin(p, tile.split) : 0;
+        const int kb1 = p.splits > 1 ? k_begin(p, tile.split + 1) : p.k_blocks;
         const int arow = tile.mi * PAIR_M + rank * BM;
-        const int brow = EPI == kEpilogueGate ? tile.ni * (BN / 2) : tile.ni * BN + rank * (BN / 2);
+        const int brow = GATE ? tile.ni * (BN / 2) : tile.ni * BN + rank * (BN / 2);
         for (int c = 0; c < p.combos && ok; ++c) {
           const int ta = p.combos > 1 ? kTermA[c] : 0, tb = p.combos > 1 ? kTermB[c] : 0;
           for (int seg = 0; seg < p.segments && ok; ++seg) {
             const CUtensorMap *am = &maps.a[seg];
-            const CUtensorMap *bm = &maps.b[EPI == kEpilogueGate ? rank : seg + tile.z];
-            for (int kb = tile.kb0; kb < tile.kb1; ++kb, ++it) {
+            const CUtensorMap *bm = &maps.b[GATE ? rank : seg + tile.z];
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
               // the stage is free in this CTA once the pair's MMAs have read it (multicast commit)
               if (!mbar_wait(empty(s), ph, abort_flag, p.err, kErrWaitProducer)) {
                 ok = false;
@@ -328,8 +318,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       uint32_t ph = 0, bph = 0;
       bool ok = true;
       for (int t = pair; t < p.total_tiles && ok; t += npairs) {
-        const Tile tile = tile_at(p, t);
-        const int iters = (tile.kb1 - tile.kb0) * p.segments * p.combos;
+        int steps = p.k_blocks;
+        if (p.splits > 1) {
+          const int split = tile_at(p, t).split;
+          steps = k_begin(p, split + 1) - k_begin(p, split);
+        }
+        const int iters = steps * p.segments * p.combos;
         if (!warp_wait(acc_empty(buf), bph ^ 1, abort_flag, p.err, kErrWaitMma)) break;
         tc_fence_after();
         const uint32_t d = tmem + buf * 256;
@@ -362,9 +356,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       mbar_wait_drain(drain, 0, p.err);
     }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2, ew = warp - 2;
-    StoreRing ring{smem + S::OFF_STAGE + ew * 2 * S::SLOT_BYTES, sbase + S::OFF_STAGE + ew * 2 * S::SLOT_BYTES};
-    int tile_it = 0, loads = 0;
+    // Each warp: its lane quarter's 32 rows, column blocks cw, cw + 4, ... of 32.
+    const int q = warp & 3, cw = (warp - 2) >> 2, ew = warp - 2;
+    uint8_t *const block = smem + S::OFF_STAGE + ew * S::SLOT_BYTES;
+    const uint32_t block_addr = sbase + S::OFF_STAGE + ew * S::SLOT_BYTES;
+    int tile_it = 0, stores = 0;  // stores: through the two blocks in turn
+    uint32_t load_phase[2] = {0, 0};
     for (int t = pair; t < p.total_tiles; t += npairs, ++tile_it) {
       const Tile tile = tile_at(p, t);
       const int buf = tile_it & 1;
@@ -372,178 +369,336 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const int64_t m = static_cast<int64_t>(r0) + lane;
       const bool rows_ok = r0 < p.m, row_ok = m < p.m;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
+      const uint32_t acc_phase = (tile_it >> 1) & 1;
 
-      if constexpr (EPI == kEpilogueGateBackward) {
-        // planes of the chunk that starts at column c0, into slot loads & 1
-        auto fetch = [&](int c0, int slot) {
+      if constexpr (KIND == kGateBackward) {
+        // dg = dh p and dv = dh a with the saved factors p = v act'(g) and a = act(g).  A block's
+        // factors come into the warp's slot and the products leave from the same place.
+        const int col0 = tile.ni * BN + cw * 32;
+        auto fetch = [&](int c0) {
           if (lane == 0) {
-            bulk_wait_read_all();  // the results of the chunk that used this slot have left it
-            const uint32_t dst = ring.addr + slot * S::SLOT_BYTES, bar = load(ew, slot);
+            bulk_wait_read_all();  // the results before them have left the slot
+            const uint32_t bar = load(ew, 0);
             mbar_arrive_expect_tx(bar, 6144);
-            tma_load_3d(dst, &maps.hi, bar, c0, r0, 0);
-            tma_load_3d(dst + 2048, &maps.hi, bar, c0, r0, 1);
-            tma_load_3d(dst + 4096, &maps.lo, bar, c0, r0, 0);
-            tma_load_3d(dst + 5120, &maps.lo, bar, c0, r0, 1);
+            tma_load_3d(block_addr, &maps.hi, bar, c0, r0, 0);
+            tma_load_3d(block_addr + 2048, &maps.hi, bar, c0, r0, 1);
+            tma_load_3d(block_addr + 4096, &maps.lo, bar, c0, r0, 0);
+            tma_load_3d(block_addr + 5120, &maps.lo, bar, c0, r0, 1);
           }
         };
-        constexpr int CHUNKS = BN / 64;
-        const int col0 = tile.ni * BN + half * (BN / 2);
-        const int chunks = rows_ok ? min(CHUNKS, max(0, (p.n - col0 + 31) / 32)) : 0;
-        if (chunks > 0) fetch(col0, loads & 1);
-        if (!warp_wait(acc_full(buf), (tile_it >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue)) {
-          if (chunks > 0 && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, p.err);
+        const bool any = rows_ok && col0 < p.n;
+        if (any) fetch(col0);
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) {
+          if (any && lane == 0) mbar_wait_drain(load(ew, 0), load_phase[0], p.err);
           break;
         }
         tc_fence_after();
         bool ok = true;
-        for (int chunk = 0; chunk < chunks; ++chunk, ++loads) {
-          const int slot = loads & 1, c0 = col0 + chunk * 32;
-          if (chunk + 1 < chunks) fetch(c0 + 32, slot ^ 1);
+#pragma unroll 1
+        for (int j = 0; j < BN / 128; ++j) {
+          const int c0 = col0 + j * 128;
+          if (!rows_ok || c0 >= p.n) break;
+          if (j) fetch(c0);
           uint32_t v[32];
-          tmem_ld32(taddr + half * (BN / 2) + chunk * 32, v);
-          ok = warp_wait(load(ew, slot), (loads >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
+          tmem_ld32(taddr + cw * 32 + j * 128, v);
+          ok = warp_wait(load(ew, 0), load_phase[0], abort_flag, p.err, kErrWaitEpilogue);
           tmem_ld_wait();
-          if (!ok) {
-            if (chunk + 1 < chunks && lane == 0) mbar_wait_drain(load(ew, slot ^ 1), ((loads + 1) >> 1) & 1, p.err);
-            break;
-          }
-          uint8_t *sl = ring.ptr + slot * S::SLOT_BYTES;
-          uint32_t dg[16], dv[16];
-          activation_switch(p.activation, [&](auto act) {
-            constexpr int ACT = decltype(act)::value;
+          if (!ok) break;
+          load_phase[0] ^= 1;
+#pragma unroll
+          for (int plane = 0; plane < 2; ++plane) {
+            float d[32];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {  // 8 columns each
-              const uint4 gh = *slot_piece(sl, lane, c), vh = *slot_piece(sl + 2048, lane, c);
-              const uint2 gl = *reinterpret_cast<const uint2 *>(sl + 4096 + lane * 32 + c * 8);
-              const uint2 vl = *reinterpret_cast<const uint2 *>(sl + 5120 + lane * 32 + c * 8);
-              const uint32_t ghw[4] = {gh.x, gh.y, gh.z, gh.w}, vhw[4] = {vh.x, vh.y, vh.z, vh.w};
+              uint4 *piece = piece16(block + plane * 2048, lane, c);
+              const uint4 hi = *piece;
+              const uint2 lo = *reinterpret_cast<const uint2 *>(block + 4096 + plane * 1024 + lane * 32 + c * 8);
+              float2 f[4] = {from_planes<0>(hi.x, lo.x), from_planes<1>(hi.y, lo.x), from_planes<0>(hi.z, lo.y),
+                             from_planes<1>(hi.w, lo.y)};
+              uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const uint32_t glw = i < 2 ? gl.x : gl.y, vlw = i < 2 ? vl.x : vl.y;
-                float g0, g1, v0, v1;
-                if (i & 1) {
-                  g0 = from_planes<0, 2>(ghw[i], glw), g1 = from_planes<1, 3>(ghw[i], glw);
-                  v0 = from_planes<0, 2>(vhw[i], vlw), v1 = from_planes<1, 3>(vhw[i], vlw);
-                } else {
-                  g0 = from_planes<0, 0>(ghw[i], glw), g1 = from_planes<1, 1>(ghw[i], glw);
-                  v0 = from_planes<0, 0>(vhw[i], vlw), v1 = from_planes<1, 1>(vhw[i], vlw);
-                }
-                float a0, s0, a1, s1;
-                activate_slope<ACT>(g0, a0, s0);
-                activate_slope<ACT>(g1, a1, s1);
-                const float d0 = __uint_as_float(v[8 * c + 2 * i]), d1 = __uint_as_float(v[8 * c + 2 * i + 1]);
-                dg[4 * c + i] = pack2_t<OT>(d0 * v0 * s0, d1 * v1 * s1);
-                dv[4 * c + i] = pack2_t<OT>(d0 * a0, d1 * a1);
+                f[i] = f2mul(f[i], make_float2(__uint_as_float(v[8 * c + 2 * i]), __uint_as_float(v[8 * c + 2 * i + 1])));
+                w[i] = pack2_t<OT>(f[i].x, f[i].y);
+                d[8 * c + 2 * i] = f[i].x;
+                d[8 * c + 2 * i + 1] = f[i].y;
               }
+              *piece = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          });
-          __syncwarp();
-          slot_write(sl, lane, dg);
-          slot_write(sl + 2048, lane, dv);
+            if (p.column_partial) {
+              // the bias gradients' sums, of the products before they are rounded
+              const float sum = lane_sums(d, lane);
+              p.column_partial[(static_cast<int64_t>(r0 >> 5) * 2 + plane) * p.saved_pitch + c0 + lane] = sum;
+            }
+          }
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
-            const uint32_t src = ring.addr + slot * S::SLOT_BYTES;
-            tma_store_3d(&maps.out[0], src, c0, r0, 0);
-            tma_store_3d(&maps.out[1], src + 2048, c0, r0, 0);
+            tma_store_3d(&maps.out[0], block_addr, c0, r0, 0);
+            tma_store_3d(&maps.out[1], block_addr + 2048, c0, r0, 0);
             bulk_commit();
-          }
-          if (p.column_partial) {
-            // the block's column sums: lane l takes columns 2 (l % 16), + 1 of rows l / 16, + 2, ...
-            const int pc = lane & 15, par = lane >> 4;
-#pragma unroll
-            for (int plane = 0; plane < 2; ++plane) {
-              float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int row = 2 * i + par;
-                const uint32_t w = *reinterpret_cast<const uint32_t *>(
-                    sl + plane * 2048 + row * 64 + (((pc >> 2) ^ ((row >> 1) & 3)) << 4) + (pc & 3) * 4);
-                sum = f2add(sum, unpack2<OT>(w));
-              }
-              sum.x += __shfl_xor_sync(kFull, sum.x, 16);
-              sum.y += __shfl_xor_sync(kFull, sum.y, 16);
-              if (par == 0)
-                *reinterpret_cast<float2 *>(p.column_partial + (static_cast<int64_t>(r0 >> 5) * 2 + plane) *
-                                                                   p.saved_pitch + c0 + 2 * pc) = sum;
-            }
           }
         }
         if (!ok) break;
-      } else {
-        if (!warp_wait(acc_full(buf), (tile_it >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
+      } else if constexpr (GATE) {
+        // h = act(g) v; columns [0, BN / 2) of the accumulator are g, the others v
+        const int cc = cw * 32, c0 = tile.ni * (BN / 2) + cc;
+        const bool inside = cc < BN / 2 && rows_ok && c0 < p.n;
+        uint32_t bg[16], bv[16];
+        if (inside) {
+          if (p.bias[0]) load_raw32(static_cast<const OT *>(p.bias[0]), c0, p.n, p.vector_bias, bg);
+          if (p.bias[1]) load_raw32(static_cast<const OT *>(p.bias[1]), c0, p.n, p.vector_bias, bv);
+        }
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) break;
         tc_fence_after();
-        if constexpr (EPI == kEpilogueGate) {
-#pragma unroll 1
-          for (int chunk = 0; chunk < BN / 128; ++chunk) {
-            const int cc = half * (BN / 4) + chunk * 32, c0 = tile.ni * (BN / 2) + cc;
-            uint32_t gr[32], vr[32];
-            tmem_ld32(taddr + cc, gr);
-            tmem_ld32(taddr + BN / 2 + cc, vr);
-            tmem_ld_wait();
-            const bool inside = rows_ok && c0 < p.n;
-            float(&g)[32] = reinterpret_cast<float(&)[32]>(gr);
-            float(&v)[32] = reinterpret_cast<float(&)[32]>(vr);
-            if (p.bias[0]) add_row32(static_cast<const OT *>(p.bias[0]), c0, p.n, p.vector_bias, g);
-            if (p.bias[1]) add_row32(static_cast<const OT *>(p.bias[1]), c0, p.n, p.vector_bias, v);
-            if (p.saved_hi) {
-              save_planes(maps, p, ring, lane, g, c0, r0, 0, m, inside);
-              save_planes(maps, p, ring, lane, v, c0, r0, 1, m, inside);
-            }
-            activation_switch(p.activation, [&](auto act) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) g[i] = activate<decltype(act)::value>(g[i]) * v[i];
-            });
-            uint32_t w[16];
-            pack_row<OT>(g, w);
-            ring.store16(&maps.out[0], lane, w, c0, r0, 0, inside);
+        if (inside) {
+          const int b = KIND == kGateSave ? 0 : (stores++ & 1) * 2048;
+          if (lane == 0) {
+            if (KIND == kGateSave)
+              bulk_wait_read_all();
+            else
+              bulk_wait_read_but_one();
           }
-        } else {
-          const int z = p.partial ? tile.split * p.batch + tile.z : 0;
-          const CUtensorMap *omap = &maps.out[p.partial ? 0 : tile.z];
-#pragma unroll 1
-          for (int chunk = 0; chunk < BN / 64; ++chunk) {
-            const int cc = half * (BN / 2) + chunk * 32, c0 = tile.ni * BN + cc;
-            if (c0 >= p.n || !rows_ok) break;
-            uint32_t r[32];
-            tmem_ld32(taddr + cc, r);
+          __syncwarp();
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {  // 16 columns each
+            uint32_t g[16], v[16];
+            tmem_ld16(taddr + cc + part * 16, g);
+            tmem_ld16(taddr + BN / 2 + cc + part * 16, v);
             tmem_ld_wait();
-            float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
-            if (!p.partial) {
-              if (p.bias[tile.z]) add_row32(static_cast<const OT *>(p.bias[tile.z]), c0, p.n, p.vector_bias, y);
-              if (p.saved_hi) save_planes(maps, p, ring, lane, y, c0, r0, 0, m, true);
-              if (p.saved_f32 && row_ok) {
-                float4 *dst = reinterpret_cast<float4 *>(p.saved_f32 + m * p.saved_pitch + c0);
+            uint32_t h[8], ph[8], ah[8], pl[4], al[4];
+            with_activation(p.activation, [&](auto act) {
+              constexpr int ACT = decltype(act)::value;
+              float2 last_p = f2(0.f), last_a = f2(0.f);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+              for (int i = 0; i < 8; ++i) {
+                float2 gz = make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+                float2 vz = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                if (p.bias[0]) gz = f2add(gz, unpack2<OT>(bg[part * 8 + i]));
+                if (p.bias[1]) vz = f2add(vz, unpack2<OT>(bv[part * 8 + i]));
+                float2 a;
+                if constexpr (KIND == kGateSave) {
+                  float2 slope;
+                  activate_slope2<ACT, true>(gz, a, slope);
+                  slope = f2mul(slope, vz);
+                  ph[i] = upper_halves(slope);
+                  ah[i] = upper_halves(a);
+                  if (i & 1) {
+                    pl[i >> 1] = third_bytes(last_p, slope);
+                    al[i >> 1] = third_bytes(last_a, a);
+                  }
+                  last_p = slope;
+                  last_a = a;
+                } else {
+                  a = activate2<ACT, true>(gz);
+                }
+                a = f2mul(a, vz);
+                h[i] = pack2_t<OT>(a.x, a.y);
               }
-              activation_switch(p.activation, [&](auto act) {
+            });
 #pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = activate<decltype(act)::value>(y[i]);
-              });
-              if (p.residual && row_ok)
-                add_row32(static_cast<const OT *>(p.residual) + m * p.residual_stride, c0, p.n, p.vector_res, y);
-            }
-            if (p.tma_out) {
-              if constexpr (sizeof(OT) == 4) {
-                ring.store32(omap, lane, y, c0, r0, z, true);
-              } else {
-                uint32_t w[16];
-                pack_row<OT>(y, w);
-                ring.store16(omap, lane, w, c0, r0, z, true);
+            for (int c = 0; c < 2; ++c) {
+              *piece16(block + b, lane, part * 2 + c) = make_uint4(h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+              if constexpr (KIND == kGateSave) {
+                *piece16(block + 2048, lane, part * 2 + c) =
+                    make_uint4(ph[4 * c], ph[4 * c + 1], ph[4 * c + 2], ph[4 * c + 3]);
+                *piece16(block + 4096, lane, part * 2 + c) =
+                    make_uint4(ah[4 * c], ah[4 * c + 1], ah[4 * c + 2], ah[4 * c + 3]);
               }
-            } else if (row_ok) {
-              OT *orow = static_cast<OT *>(p.out[tile.z]) + m * p.out_stride;
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (c0 + i < p.n) orow[c0 + i] = from_f32<OT>(y[i]);
             }
+            if constexpr (KIND == kGateSave) if (row_ok) {
+              uint8_t *lo = p.saved_lo + m * p.saved_pitch + c0 + part * 16;
+              *reinterpret_cast<uint4 *>(lo) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+              *reinterpret_cast<uint4 *>(lo + p.saved_stride) = make_uint4(al[0], al[1], al[2], al[3]);
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&maps.out[0], block_addr + b, c0, r0, 0);
+            if constexpr (KIND == kGateSave) {
+              tma_store_3d(&maps.hi, block_addr + 2048, c0, r0, 0);
+              tma_store_3d(&maps.hi, block_addr + 4096, c0, r0, 1);
+            }
+            bulk_commit();
           }
         }
+      } else {
+        // out = act(acc + bias) (+ residual)
+        const int z = p.partial ? tile.split * static_cast<int>(p.batches.d) + tile.z : 0;
+        const CUtensorMap *omap = &maps.out[p.partial ? 0 : tile.z];
+        const int col0 = tile.ni * BN + cw * 32;
+        if (p.tma_residual && rows_ok && lane == 0) {
+          bulk_wait_read_all();
+#pragma unroll
+          for (int j = 0; j < BN / 128; ++j)
+            if (col0 + j * 128 < p.n) {
+              mbar_arrive_expect_tx(load(ew, j), 2048);
+              tma_load_3d(block_addr + j * 2048, &maps.residual, load(ew, j), col0 + j * 128, r0, 0);
+            }
+        }
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) {
+          if (p.tma_residual && rows_ok && lane == 0)
+            for (int j = 0; j < BN / 128; ++j)
+              if (col0 + j * 128 < p.n) mbar_wait_drain(load(ew, j), load_phase[j], p.err);
+          break;
+        }
+        tc_fence_after();
+        bool ok = true;
+#pragma unroll
+        for (int j = 0; j < BN / 128; ++j) {
+          const int c0 = col0 + j * 128;
+          if (!rows_ok || c0 >= p.n || !ok) continue;
+          uint32_t r[32];
+          tmem_ld32(taddr + cw * 32 + j * 128, r);
+          tmem_ld_wait();
+          float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
+          const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0)), cols = min(32, p.n - c0);
+          if (!p.partial) {
+            if (p.bias[tile.z]) {
+              const OT *bias = static_cast<const OT *>(p.bias[tile.z]);
+              if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] += i < cols ? bias[c0 + i] : 0.f;
+              } else {
+                uint32_t bw[16];
+                load_raw32(bias, c0, p.n, p.vector_bias, bw);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float2 b2 = unpack2<OT>(bw[i]);
+                  y[2 * i] += b2.x;
+                  y[2 * i + 1] += b2.y;
+                }
+              }
+            }
+            if (p.activation != AF2_ACTIVATION_NONE) {
+              const bool save = p.saved_hi || p.saved_f32;
+              if (save) {  // the slopes, in the place of the values until they are stored
+                if (lane == 0) bulk_wait_read_all();
+                __syncwarp();
+                with_activation(p.activation, [&](auto act) {
+                  constexpr int ACT = decltype(act)::value;
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) {
+                    float2 s[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                      float2 v2;
+                      activate_slope2<ACT, sizeof(OT) == 2>(make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]), v2,
+                                                            s[i]);
+                      y[8 * c + 2 * i] = v2.x;
+                      y[8 * c + 2 * i + 1] = v2.y;
+                    }
+                    if constexpr (sizeof(OT) == 4) {
+                      if (row_ok) {
+                        float4 *dst = reinterpret_cast<float4 *>(p.saved_f32 + m * p.saved_pitch + c0 + 8 * c);
+                        dst[0] = make_float4(s[0].x, s[0].y, s[1].x, s[1].y);
+                        dst[1] = make_float4(s[2].x, s[2].y, s[3].x, s[3].y);
+                      }
+                    } else {
+                      *piece16(block, lane, c) = make_uint4(upper_halves(s[0]), upper_halves(s[1]), upper_halves(s[2]),
+                                                            upper_halves(s[3]));
+                      if (row_ok)
+                        *reinterpret_cast<uint2 *>(p.saved_lo + m * p.saved_pitch + c0 + 8 * c) =
+                            make_uint2(third_bytes(s[0], s[1]), third_bytes(s[2], s[3]));
+                    }
+                  }
+                });
+                if constexpr (sizeof(OT) == 2) {
+                  fence_async_smem();
+                  __syncwarp();
+                  if (lane == 0) {
+                    tma_store_3d(&maps.hi, block_addr, c0, r0, 0);
+                    bulk_commit();
+                  }
+                }
+              } else {
+                with_activation(p.activation, [&](auto act) {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) {
+                    const float2 v2 = activate2<decltype(act)::value, sizeof(OT) == 2>(make_float2(y[2 * i], y[2 * i + 1]));
+                    y[2 * i] = v2.x;
+                    y[2 * i + 1] = v2.y;
+                  }
+                });
+              }
+            }
+          }
+          // the block that the result leaves from, with the residual in it where there is one
+          uint32_t at = 0;
+          if constexpr (sizeof(OT) == 2)
+            at = 2048u * (p.saved_hi       ? 1  // the first block may still hold slopes
+                          : p.tma_residual ? j
+                                           : stores++ & 1);
+          uint8_t *const dst = block + at;
+          const uint32_t dst_addr = block_addr + at;
+          if (p.tma_residual) {
+            ok = warp_wait(load(ew, j), load_phase[j], abort_flag, p.err, kErrWaitEpilogue);
+            load_phase[j] ^= 1;
+            if (!ok) continue;
+          } else {
+            if (lane == 0) {
+              if (sizeof(OT) == 4)
+                bulk_wait_read_all();
+              else
+                bulk_wait_read_but_one();
+            }
+            __syncwarp();
+            if (p.residual) {
+              move_rows<OT, true>(dst, const_cast<OT *>(static_cast<const OT *>(p.residual)) +
+                                           static_cast<int64_t>(r0) * p.residual_stride + c0,
+                                  p.residual_stride, rows, cols, lane);
+              __syncwarp();
+            }
+          }
+          if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              float4 o = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+              float4 *piece = piece32(dst, lane, c);
+              if (p.residual) {
+                const float4 res = *piece;
+                o.x += res.x, o.y += res.y, o.z += res.z, o.w += res.w;
+              }
+              *piece = o;
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint4 *piece = piece16(dst, lane, c);
+              uint32_t w[4];
+              if (p.residual) {
+                const uint4 u = *piece;
+                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float2 o = make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]);
+                if (p.residual) o = f2add(o, unpack2<OT>(w[i]));
+                w[i] = pack2_t<OT>(o.x, o.y);
+              }
+              *piece = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          if (p.tma_out) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(omap, dst_addr, c0, r0, z);
+              bulk_commit();
+            }
+          } else {
+            __syncwarp();
+            move_rows<OT, false>(dst, static_cast<OT *>(p.out[tile.z]) + static_cast<int64_t>(r0) * p.out_stride + c0,
+                                 p.out_stride, rows, cols, lane);
+            __syncwarp();
+          }
+        }
+        if (!ok) break;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_leader(acc_empty(buf));
+      if (lane == 0) mbar_arrive_leader_relaxed(acc_empty(buf));
     }
     if (lane == 0) bulk_wait_all();
   }
@@ -556,8 +711,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   }
 }
 
-// out = act(sum of the splits' partial sums + bias) (+ residual), saved = the pre-activation.  One
-// thread per four columns.
+// out = act(sum of the splits' partial sums + bias) (+ residual), saved = the slope.  One thread per
+// four columns.
 struct ReduceArgs {
   const float *partial;  // [split][batch][m][pitch]
   int splits, batch, activation;
@@ -598,13 +753,19 @@ __global__ void __launch_bounds__(256) reduce_kernel(const ReduceArgs p) {
       const int64_t c = c0 + j;
       if (c >= p.n) break;
       if (bias) y[j] += to_f32<OT>(bias[c]);
+      float slope = 1.f;
+      with_activation(p.activation, [&](auto act) {
+        float2 value, slopes;
+        activate_slope2<decltype(act)::value, sizeof(OT) == 2>(make_float2(y[j], y[j]), value, slopes);
+        y[j] = value.x;
+        slope = slopes.x;
+      });
       if (p.saved_hi) {
-        const uint32_t bits = __float_as_uint(y[j]);
+        const uint32_t bits = __float_as_uint(slope);
         p.saved_hi[m * p.saved_pitch + c] = static_cast<uint16_t>(bits >> 16);
         p.saved_lo[m * p.saved_pitch + c] = static_cast<uint8_t>(bits >> 8);
       }
-      if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c] = y[j];
-      activation_switch(p.activation, [&](auto act) { y[j] = activate<decltype(act)::value>(y[j]); });
+      if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c] = slope;
       if (res) y[j] += to_f32<OT>(res[c]);
       out[c] = from_f32<OT>(y[j]);
     }
@@ -657,10 +818,10 @@ bool operand_map(CUtensorMap *map, const GemmOperand &o, int64_t outer, int64_t 
   return encode_map_3d(map, t, o.ptr, k, outer, pieces, row, piece, BK, box_outer, 1, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int EPI, typename OT, int BN>
+template <int KIND, typename OT, int BN>
 af2_status launch(af2_ctx *ctx, const Maps &maps, const Args &p, cudaStream_t stream) {
-  constexpr uint32_t smem = Shape<EPI, BN>::BYTES;
-  auto kernel = layer_gemm_kernel<EPI, OT, BN>;
+  constexpr uint32_t smem = Shape<KIND, BN>::BYTES;
+  auto kernel = layer_gemm_kernel<KIND, OT, BN>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       e != cudaSuccess)
     return cuda_fail(ctx, e, "layer product shared memory");
@@ -671,15 +832,16 @@ af2_status launch(af2_ctx *ctx, const Maps &maps, const Args &p, cudaStream_t st
   return AF2_OK;
 }
 
-template <typename OT>
-af2_status launch_out(af2_ctx *ctx, int bn, const Maps &maps, const Args &p, cudaStream_t stream) {
-  return bn == 256 ? launch<kEpilogueOut, OT, 256>(ctx, maps, p, stream)
-                   : launch<kEpilogueOut, OT, 128>(ctx, maps, p, stream);
+template <int KIND, typename OT>
+af2_status launch_bn(af2_ctx *ctx, int bn, const Maps &maps, const Args &p, cudaStream_t stream) {
+  if constexpr (KIND == kGateBackward) return launch<KIND, OT, 256>(ctx, maps, p, stream);
+  return bn == 256 ? launch<KIND, OT, 256>(ctx, maps, p, stream) : launch<KIND, OT, 128>(ctx, maps, p, stream);
 }
-template <typename OT>
-af2_status launch_gate(af2_ctx *ctx, int bn, const Maps &maps, const Args &p, cudaStream_t stream) {
-  return bn == 256 ? launch<kEpilogueGate, OT, 256>(ctx, maps, p, stream)
-                   : launch<kEpilogueGate, OT, 128>(ctx, maps, p, stream);
+// A 16-bit output type.
+template <int KIND>
+af2_status launch_16(af2_ctx *ctx, int dtype, int bn, const Maps &maps, const Args &p, cudaStream_t stream) {
+  return dtype == AF2_F16 ? launch_bn<KIND, __half>(ctx, bn, maps, p, stream)
+                          : launch_bn<KIND, __nv_bfloat16>(ctx, bn, maps, p, stream);
 }
 
 CUtensorMapDataType map_type(int dtype) {
@@ -706,10 +868,10 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
   p.splits = plan.splits;
   p.combos = g.pieces > 1 ? 6 : 1;
   p.segments = g.segments;
-  p.batch = g.batch;
-  p.tiles_m = static_cast<int>(ceil_div(g.m, PAIR_M));
-  p.tiles_n = static_cast<int>(ceil_div(g.n, gate ? plan.bn / 2 : plan.bn));
-  const int64_t total = static_cast<int64_t>(p.splits) * p.batch * p.tiles_m * p.tiles_n;
+  p.batches = Divisor(g.batch);
+  p.tiles_m = Divisor(static_cast<uint32_t>(ceil_div(g.m, PAIR_M)));
+  p.tiles_n = Divisor(static_cast<uint32_t>(ceil_div(g.n, gate ? plan.bn / 2 : plan.bn)));
+  const int64_t total = static_cast<int64_t>(p.splits) * g.batch * p.tiles_m.d * p.tiles_n.d;
   if (total > 0x3fffffff) return fail(ctx, AF2_ERR_UNSUPPORTED, "the product has too many tiles");
   p.total_tiles = static_cast<int>(total);
   p.a_mn = g.a[0].mn_major;
@@ -736,7 +898,11 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
     p.activation = g.activation;
     p.residual = g.residual;
     p.residual_stride = g.residual_stride;
-    p.vector_res = aligned16(g.residual, g.residual_stride, out_bytes);
+    if (g.residual && !g.saved.hi && out_bytes == 2 && aligned16(g.residual, g.residual_stride, 2)) {
+      p.tma_residual = 1;
+      maps_ok &= encode_map_3d(&maps.residual, map_type(g.out_dtype), g.residual, g.n, g.m, 1, g.residual_stride * 2,
+                               g.residual_stride * 2, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
+    }
     p.out_stride = g.out_stride;
     p.vector_bias = 1;
     p.tma_out = 1;
@@ -770,16 +936,15 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
 
   af2_status st = AF2_OK;
   if (g.epilogue == kEpilogueGateBackward)
-    st = g.out_dtype == AF2_F16 ? launch<kEpilogueGateBackward, __half, 256>(ctx, maps, p, stream)
-                                : launch<kEpilogueGateBackward, __nv_bfloat16, 256>(ctx, maps, p, stream);
+    st = launch_16<kGateBackward>(ctx, g.out_dtype, plan.bn, maps, p, stream);
+  else if (gate && g.saved.hi)
+    st = launch_16<kGateSave>(ctx, g.out_dtype, plan.bn, maps, p, stream);
   else if (gate)
-    st = g.out_dtype == AF2_F16 ? launch_gate<__half>(ctx, plan.bn, maps, p, stream)
-                                : launch_gate<__nv_bfloat16>(ctx, plan.bn, maps, p, stream);
+    st = launch_16<kGate>(ctx, g.out_dtype, plan.bn, maps, p, stream);
   else if (p.partial || g.out_dtype == AF2_F32)
-    st = launch_out<float>(ctx, plan.bn, maps, p, stream);
+    st = launch_bn<kOut, float>(ctx, plan.bn, maps, p, stream);
   else
-    st = g.out_dtype == AF2_F16 ? launch_out<__half>(ctx, plan.bn, maps, p, stream)
-                                : launch_out<__nv_bfloat16>(ctx, plan.bn, maps, p, stream);
+    st = launch_16<kOut>(ctx, g.out_dtype, plan.bn, maps, p, stream);
   if (st != AF2_OK || plan.splits == 1) return st;
 
   ReduceArgs r{};

@@ -17,14 +17,16 @@ struct GemmOperand {
 
 // How a tile leaves the accumulators.
 enum GemmEpilogue {
-  kEpilogueOut = 0,       // out = act(acc + bias) (+ residual), saved = acc + bias
-  kEpilogueGate = 1,      // b[0], b[1] are the gate's and the value's weights: out = act(g) v, saved = g, v
-  kEpilogueGateBackward,  // acc = dh: with the saved g and v, out = dg and dv
+  kEpilogueOut = 0,       // out = act(acc + bias) (+ residual), saved = act'(acc + bias)
+  kEpilogueGate = 1,      // b[0], b[1] are the gate's and the value's weights: out = act(g) v,
+                          // saved = v act'(g) and act(g): what the backward pass multiplies dh by
+  kEpilogueGateBackward,  // acc = dh: out = dh times each of the two saved factors (dg and dv)
 };
 
-// Pre-activations kept for the backward pass of the 16-bit types: the upper 24 bits of each f32, as
-// planes of its upper 16 (`hi`) and of the next 8 (`lo`), rows of `pitch` elements, `stride`
-// elements from the gate's plane to the value's.  The f32 type keeps f32 in `f32` instead.
+// Factors kept for the backward pass.  The 16-bit types keep the upper 24 bits of each f32, as planes
+// of its upper 16 (`hi`) and of the next 8 (`lo`), rows of `pitch` elements, `stride` elements from
+// the first factor's plane to the second's; so the backward pass rounds to 16 bits only what becomes
+// a product's operand.  The f32 type keeps f32 in `f32`.
 struct SavedPlanes {
   uint16_t *hi = nullptr;
   uint8_t *lo = nullptr;

@@ -1,5 +1,22 @@
 // layer_math.cuh -- the activations of the layers with learned weights and
 // their slopes, in f32.
+//
+//   relu:    max(z, 0);  1 where z > 0
+//   sigmoid: s;          s (1 - s)            s = 1 / (1 + e^-z)
+//   silu:    z s;        s (1 + z (1 - s))
+//   gelu:    z Phi(z);   Phi(z) + z phi(z)    Phi, phi of the standard normal
+//
+// Two forms.  FAST = false, for f32 tensors: sigmoidf (a few ulp) and CUDA's
+// erff.  FAST = true, for 16-bit tensors, relative error below 2^-16 where the
+// value matters to them, on two elements at a time, because the epilogues that
+// call it are bound by the multi-function unit and by issue slots:
+//   - two sigmoids share one reciprocal: with d = 1 + e^-z, 1 / d0 = d1 / (d0 d1).
+//     The exponent is held below 2^60 so that the product cannot overflow; a
+//     sigmoid below 2^-60 (z < -41) is 2^-60.
+//   - Phi(-u) = e^(-u^2 / 2) t Q(t), t = 1 / (1 + 0.31 u), u >= 0: the form of
+//     Hastings' approximations with a polynomial of degree 5 fitted to
+//     Phi(-u) e^(u^2 / 2) / t on u in [0, 14] for the least largest relative
+//     error, 4.7e-6; the exponential serves the slope too.
 #pragma once
 
 #include <math.h>
@@ -9,48 +26,96 @@
 
 namespace af2 {
 
-// Value of the activation at z.  sigmoidf is within a few ulp (af2_device.cuh), erff CUDA's own.
-template <int ACT>
-__device__ __forceinline__ float activate(float z) {
-  if constexpr (ACT == AF2_ACTIVATION_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-  if constexpr (ACT == AF2_ACTIVATION_SIGMOID) return sigmoidf(z);
-  if constexpr (ACT == AF2_ACTIVATION_SILU) return z * sigmoidf(z);
-  if constexpr (ACT == AF2_ACTIVATION_GELU) return z * fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f);
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The sigmoids of two values; a NaN gives 2^-60 (its product with z is NaN again).
+__device__ __forceinline__ float2 sigmoid2_fast(float2 z) {
+  const float2 x = f2mul(z, f2(-1.4426950408889634f));
+  const float2 d = f2add(make_float2(ex2_approx(fminf(x.x, 60.f)), ex2_approx(fminf(x.y, 60.f))), f2(1.f));
+  const float r = rcp_approx(d.x * d.y);
+  return f2mul(f2(r), make_float2(d.y, d.x));
+}
+
+// Phi and, for the slope, e^(-z^2 / 2).
+__device__ __forceinline__ float2 normal_cdf2_fast(float2 z, float2 &e) {
+  const float2 arg = f2mul(f2mul(z, z), f2(-0.72134752044448170f));
+  e = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
+  const float2 d = f2fma(make_float2(fabsf(z.x), fabsf(z.y)), f2(0.31f), f2(1.f));
+  const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+  float2 q = f2fma(f2(-0.07392890751361847f), t, f2(0.1804496943950653f));
+  q = f2fma(q, t, f2(0.015745392069220543f));
+  q = f2fma(q, t, f2(0.13342945277690887f));
+  q = f2fma(q, t, f2(0.12044135481119156f));
+  q = f2fma(q, t, f2(0.12386069446802139f));
+  const float2 w = f2mul(f2mul(q, t), e);
+  return make_float2(z.x < 0.f ? w.x : 1.f - w.x, z.y < 0.f ? w.y : 1.f - w.y);
+}
+
+__device__ __forceinline__ float relu(float z) { return z > 0.f ? z : (z != z ? z : 0.f); }
+
+// Values at two places.
+template <int ACT, bool FAST>
+__device__ __forceinline__ float2 activate2(float2 z) {
+  if constexpr (ACT == AF2_ACTIVATION_RELU) return make_float2(relu(z.x), relu(z.y));
+  if constexpr (ACT == AF2_ACTIVATION_SIGMOID) return make_float2(sigmoidf(z.x), sigmoidf(z.y));
+  if constexpr (ACT == AF2_ACTIVATION_SILU)
+    return f2mul(z, FAST ? sigmoid2_fast(z) : make_float2(sigmoidf(z.x), sigmoidf(z.y)));
+  if constexpr (ACT == AF2_ACTIVATION_GELU) {
+    if constexpr (FAST) {
+      float2 e;
+      return f2mul(z, normal_cdf2_fast(z, e));
+    }
+    return make_float2(z.x * fmaf(0.5f, erff(z.x * 0.70710678118654752f), 0.5f),
+                       z.y * fmaf(0.5f, erff(z.y * 0.70710678118654752f), 0.5f));
+  }
   return z;
 }
 
-// Value and slope together.
-//   relu:    max(z, 0);  1 where z > 0
-//   sigmoid: s;          s (1 - s)
-//   silu:    z s;        s (1 + z (1 - s))
-//   gelu:    z Phi(z);   Phi(z) + z phi(z)
-template <int ACT>
-__device__ __forceinline__ void activate_slope(float z, float &value, float &slope) {
+// Values and slopes at two places.
+template <int ACT, bool FAST>
+__device__ __forceinline__ void activate_slope2(float2 z, float2 &value, float2 &slope) {
   if constexpr (ACT == AF2_ACTIVATION_NONE) {
     value = z;
-    slope = 1.f;
+    slope = f2(1.f);
   } else if constexpr (ACT == AF2_ACTIVATION_RELU) {
-    value = z > 0.f ? z : (z != z ? z : 0.f);
-    slope = z > 0.f ? 1.f : 0.f;
+    value = make_float2(relu(z.x), relu(z.y));
+    slope = make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
   } else if constexpr (ACT == AF2_ACTIVATION_GELU) {
-    const float cdf = fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f);
-    value = z * cdf;
-    slope = fmaf(z * 0.39894228040143268f, exp2f(z * z * -0.72134752044448170f), cdf);
+    float2 cdf, e;
+    if constexpr (FAST) {
+      cdf = normal_cdf2_fast(z, e);
+    } else {
+      cdf = make_float2(fmaf(0.5f, erff(z.x * 0.70710678118654752f), 0.5f),
+                        fmaf(0.5f, erff(z.y * 0.70710678118654752f), 0.5f));
+      e = make_float2(exp2f(z.x * z.x * -0.72134752044448170f), exp2f(z.y * z.y * -0.72134752044448170f));
+    }
+    value = f2mul(z, cdf);
+    slope = f2fma(f2mul(z, f2(0.39894228040143268f)), e, cdf);
   } else {
-    const float s = sigmoidf(z);
+    const float2 s = FAST && ACT == AF2_ACTIVATION_SILU ? sigmoid2_fast(z) : make_float2(sigmoidf(z.x), sigmoidf(z.y));
+    const float2 rest = f2fma(s, f2(-1.f), f2(1.f));
     if constexpr (ACT == AF2_ACTIVATION_SIGMOID) {
       value = s;
-      slope = s * (1.f - s);
+      slope = f2mul(s, rest);
     } else {
-      value = z * s;
-      slope = s * fmaf(z, 1.f - s, 1.f);
+      value = f2mul(z, s);
+      slope = f2mul(s, f2fma(z, rest, f2(1.f)));
     }
   }
 }
 
-// Calls f with the activation as a compile-time constant.
+// Calls f with the activation as a compile-time constant (host and device).
 template <typename F>
-inline void with_activation(int activation, F &&f) {
+__host__ __device__ __forceinline__ void with_activation(int activation, F &&f) {
   switch (activation) {
     case AF2_ACTIVATION_RELU: f(std::integral_constant<int, AF2_ACTIVATION_RELU>()); break;
     case AF2_ACTIVATION_SIGMOID: f(std::integral_constant<int, AF2_ACTIVATION_SIGMOID>()); break;
