@@ -13,11 +13,11 @@
 //
 // What a forward pass saves: the factors that the backward pass multiplies by
 // (dense: act'(z); gated: v act'(g) and act(g); the f32 gated transition g and v
-// themselves), 24 bits of each in the 16-bit types, and the gated transition's
-// h, an operand already.
+// themselves), and the gated transition's h, an operand already.
 #include <algorithm>
 #include <type_traits>
 
+#include "layer_factor.cuh"
 #include "layer_gemm.h"
 #include "layer_math.cuh"
 
@@ -154,39 +154,59 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t s
   });
 }
 
-// dst[c] = the sum over `chunks` of partial[chunk][set][pitch] at c; block: 32 columns, 32 warps
+// dst[set][c] = the sum over `chunks` of partial[chunk][set][pitch] at c.  Block (x, y): 32 columns of
+// set y, 32 warps with eight loads in flight each (two rows of blocks are few: latency bounds them).
+struct FinishArgs {
+  const float *partial;
+  int64_t chunks, pitch, cols;
+  int sets;
+  void *dst[2];
+};
 template <typename T>
-__global__ void __launch_bounds__(1024) column_finish_kernel(const float *partial, int64_t chunks, int sets, int set,
-                                                             int64_t pitch, int64_t cols, T *dst) {
+__global__ void __launch_bounds__(1024) column_finish_kernel(const FinishArgs p) {
   __shared__ float all[32][33];
+  T *dst = static_cast<T *>(p.dst[blockIdx.y]);
+  if (!dst) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane, row = p.sets * p.pitch;
+  const float *src = p.partial + blockIdx.y * p.pitch + c;
   float sum = 0.f;
-  if (c < cols)
-    for (int64_t k = warp; k < chunks; k += 32) sum += partial[(k * sets + set) * pitch + c];
+  if (c < p.cols) {
+    int64_t k = warp;
+    for (; k + 7 * 32 < p.chunks; k += 8 * 32) {
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = src[(k + 32 * i) * row];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += x[i];
+    }
+    for (; k < p.chunks; k += 32) sum += src[k * row];
+  }
   all[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && c < cols) {
+  if (warp == 0 && c < p.cols) {
     float total = 0.f;
+#pragma unroll
     for (int w = 0; w < 32; ++w) total += all[w][lane];
     dst[c] = from_f32<T>(total);
   }
 }
 
-// Eight saved values.
+// Eight saved values (16-bit types: slopes).
 template <typename T>
 __device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int64_t r, int64_t c, float (&z)[8]) {
   const int64_t at = plane * s.stride + r * s.pitch + c;
   if constexpr (sizeof(T) == 4) {
     load8<float>(s.f32 + at, 8, z);
   } else {
-    const uint4 h = *reinterpret_cast<const uint4 *>(s.hi + at);
-    const uint2 l = *reinterpret_cast<const uint2 *>(s.lo + at);
-    const uint32_t hw[4] = {h.x, h.y, h.z, h.w}, lw[2] = {l.x, l.y};
+    const uint4 u = *reinterpret_cast<const uint4 *>(s.half + at);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      z[i] = __uint_as_float(((i & 1) ? hw[i >> 1] & 0xffff0000u : hw[i >> 1] << 16) |
-                             (((lw[i >> 2] >> (8 * (i & 3))) & 0xffu) << 8));
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = Factor<T>::slope_value(w[i]);
+      z[2 * i] = v.x;
+      z[2 * i + 1] = v.y;
+    }
   }
 }
 
@@ -337,8 +357,9 @@ class Pass {
     if (f32()) {
       s.f32 = static_cast<float *>(saved);
     } else {
-      s.hi = static_cast<uint16_t *>(saved);
-      s.lo = static_cast<uint8_t *>(saved) + part(2ull * count * s.stride);
+      s.half = static_cast<uint16_t *>(saved);
+      s.scale = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(saved) + part(2ull * count * s.stride));
+      s.scale_rows = align_up(rows, 32);
     }
     return s;
   }
@@ -355,13 +376,14 @@ class Pass {
   float *sum_room(int64_t rows, int64_t width, int sets) {
     return reinterpret_cast<float *>(take(4ull * sets * ceil_div(rows, kSumRows) * saved_pitch(width)));
   }
-  void finish_sums(const float *partial, int64_t chunks, int sets, int set, int64_t width, void *dst) {
-    if (!live() || !dst) return;
+  void finish_sums(const float *partial, int64_t chunks, int64_t width, void *dst, int sets = 1,
+                   void *second = nullptr) {
+    if (!live() || !(dst || second)) return;
+    const FinishArgs f{partial, chunks, saved_pitch(width), width, sets, {dst, second}};
     LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
+    const dim3 grid(static_cast<unsigned>(ceil_div(width, 32)), sets);
     with_element(dtype_, [&](auto *tag) {
-      using T = std::remove_pointer_t<decltype(tag)>;
-      column_finish_kernel<T><<<static_cast<unsigned>(ceil_div(width, 32)), 1024, 0, stream_>>>(
-          partial, chunks, sets, set, saved_pitch(width), width, static_cast<T *>(dst));
+      column_finish_kernel<std::remove_pointer_t<decltype(tag)>><<<grid, 1024, 0, stream_>>>(f);
     });
     check("layer column sums");
   }
@@ -375,7 +397,7 @@ class Pass {
                                                         saved_pitch(width));
       });
     });
-    finish_sums(partial, ceil_div(rows, kSumRows), 1, 0, width, dst);
+    finish_sums(partial, ceil_div(rows, kSumRows), width, dst);
   }
   void zero(void *ptr, size_t bytes) {
     if (!ptr || !live()) return;
@@ -398,7 +420,8 @@ class Pass {
 
 uint64_t planes_bytes(int64_t rows, int64_t width, int dtype, int count) {
   const uint64_t n = static_cast<uint64_t>(count) * rows * saved_pitch(width);
-  return dtype == AF2_F32 ? part(4 * n) : part(2 * n) + part(n);
+  if (dtype == AF2_F32) return part(4 * n);
+  return part(2 * n) + (count > 1 ? part(align_up(rows, 32) * saved_pitch(width) / 8) : 0);
 }
 uint64_t hidden_bytes(int64_t rows, int64_t hidden, int dtype) {
   return part(2ull * (dtype == AF2_F32 ? 3 : 1) * rows * operand_pitch(hidden));
@@ -460,7 +483,7 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
                                                         dz.piece_stride, partial, saved_pitch(p.columns));
       });
     });
-    l.finish_sums(partial, ceil_div(p.rows, kSumRows), 1, 0, p.columns, p.d_bias);
+    l.finish_sums(partial, ceil_div(p.rows, kSumRows), p.columns, p.d_bias);
   }
   if (p.d_x) {
     LayerGemm g = l.product(p.rows, p.inner, p.columns);
@@ -606,8 +629,7 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
       g.column_partial = partial;
       l.run(g);
     }
-    l.finish_sums(partial, chunks, 2, 0, hid, p.g.gate_bias);
-    l.finish_sums(partial, chunks, 2, 1, hid, p.g.value_bias);
+    l.finish_sums(partial, chunks, hid, p.g.gate_bias, 2, p.g.value_bias);
   }
   if (p.g.x) {
     LayerGemm g = l.product(p.rows, c, hid);

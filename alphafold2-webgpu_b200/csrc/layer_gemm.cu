@@ -6,9 +6,11 @@
 // (cta_group::2): CTA r holds rows 128 r .. of A's tile and half of B's rows,
 // so each SM reads half of the B tile that it multiplies by.  Warp 0 of each
 // CTA issues TMA loads, warp 1 of the even CTA the MMAs, warps 2-17 drain the
-// accumulators (four warps per TMEM lane quarter, every fourth block of 32
-// columns each: eight warps left the multi-function unit and the issue slots
-// two thirds idle); two accumulators, so one tile's epilogue overlaps the next
+// two accumulators: where a pair has more than one tile, one group of eight
+// warps (two per TMEM lane quarter) each, so that the loads, arithmetic and
+// stores of one group fall between those of the other (all sixteen warps on one
+// tile keep in step, each unit idle while they use the next); else all on the
+// one tile.  One tile's epilogue overlaps the next
 // tile's MMAs.  Operands are taken as they are stored: K-major rows as one
 // 128-byte-swizzled block per K step of 64, MN-major ones as 64-wide blocks of
 // 64 k each (the tensor core's transposed order), so no weight and no
@@ -23,6 +25,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "layer_factor.cuh"
 #include "layer_gemm.h"
 #include "layer_math.cuh"
 
@@ -38,13 +41,13 @@ constexpr int kPairs = 74;  // CTA pairs of a B200; only the choice of tiles and
 enum Kind { kOut, kGate, kGateSave, kGateBackward };
 
 // Stages of the operand ring and bytes of one epilogue warp's staging: 32 x 32 blocks of 16 bits
-// (2 KB), two of them; with factors to save or to read three (h and the factors' upper halves; the
-// factors' upper halves and their 1 KB of lower bytes), paid for with a stage.
+// (2 KB), two of them (GateBackward: one of each factor); three where h and two factors leave
+// together, paid for with a stage.
 template <int KIND, int BN>
 struct Shape {
   static constexpr uint32_t B_BYTES = (BN / 2) * 128;
   static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr uint32_t SLOT_BYTES = KIND == kGateSave || KIND == kGateBackward ? 6144 : 4096;
+  static constexpr uint32_t SLOT_BYTES = KIND == kGateSave ? 6144 : 4096;
   static constexpr int STAGES = (229376 - EPI_WARPS * SLOT_BYTES) / STAGE_BYTES;
   static constexpr uint32_t OFF_STAGE = STAGES * STAGE_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_STAGE + EPI_WARPS * SLOT_BYTES;
@@ -52,7 +55,7 @@ struct Shape {
 };
 
 struct Maps {
-  CUtensorMap a[2], b[2], out[2], residual, hi, lo;
+  CUtensorMap a[2], b[2], out[2], residual, half;
 };
 
 // n / d and n % d for n below 2^30, d fixed for a launch: the quotient by a multiply-high with
@@ -79,10 +82,9 @@ struct Args {
   const void *bias[2];
   const void *residual;
   int64_t residual_stride;
-  uint16_t *saved_hi;
-  uint8_t *saved_lo;
+  uint32_t *saved_scale;
   float *saved_f32;
-  int64_t saved_pitch, saved_stride;
+  int64_t saved_pitch, scale_rows;
   float *column_partial;
   int64_t m;
   int n, k_blocks, splits, combos, segments;
@@ -92,6 +94,8 @@ struct Args {
   int tma_out;       // out rows are 16-byte aligned: whole blocks leave by TMA
   int tma_residual;  // the residual's blocks come by TMA
   int vector_bias;   // 16-byte aligned
+  int save;          // Out: the slopes are kept
+  int alternate;     // the two groups of epilogue warps take tiles in turn
   int partial;     // out[0] is [split][batch][m][n] of f32 sums (no bias, activation or residual)
   unsigned int *err;
 };
@@ -116,42 +120,21 @@ __device__ __forceinline__ int k_begin(const Args &p, int split) {
   return static_cast<int>(static_cast<int64_t>(p.k_blocks) * split / p.splits);
 }
 
-// 32 values of a row as raw 16-bit pairs; zeros past `cols`.
+// 16 values of a row as raw 16-bit pairs; zeros past `cols`.  `vector`: row + c0 is 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void load_raw32(const T *row, int c0, int cols, bool vector, uint32_t (&w)[16]) {
-  if (vector && c0 + 32 <= cols) {
+__device__ __forceinline__ void load_raw16(const T *row, int c0, int cols, bool vector, uint32_t (&w)[8]) {
+  if (vector && c0 + 16 <= cols) {
     const uint4 *p = reinterpret_cast<const uint4 *>(row + c0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 u = __ldg(p + i);
-      w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-    }
+    const uint4 u = __ldg(p), x = __ldg(p + 1);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w, w[4] = x.x, w[5] = x.y, w[6] = x.z, w[7] = x.w;
   } else {
     const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const uint32_t a = c0 + 2 * i < cols ? p[c0 + 2 * i] : 0, b = c0 + 2 * i + 1 < cols ? p[c0 + 2 * i + 1] : 0;
       w[i] = a | (b << 16);
     }
   }
-}
-
-// A f32 is kept to 24 bits as its upper 16 and its third byte (cut, not rounded: no carry can turn a
-// NaN into a number).  The upper halves of two as one word, the third bytes of four as one.
-__device__ __forceinline__ uint32_t upper_halves(float2 v) {
-  return __byte_perm(__float_as_uint(v.x), __float_as_uint(v.y), 0x7632);
-}
-__device__ __forceinline__ uint32_t third_bytes(float2 a, float2 b) {
-  return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0051),
-                     __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0051), 0x5410);
-}
-// Two f32 from a word of upper halves and bytes 2 PAIR, 2 PAIR + 1 of a word of third bytes.
-template <int PAIR>
-__device__ __forceinline__ float2 from_planes(uint32_t hi, uint32_t lo) {
-  // bytes low to high: (masked), lo[.], hi[.], hi[.]; byte_perm sources 0-3 = hi, 4-7 = lo
-  constexpr uint32_t s0 = 0x1000 | ((4 + 2 * PAIR) << 4), s1 = 0x3200 | ((5 + 2 * PAIR) << 4);
-  return make_float2(__uint_as_float(__byte_perm(hi, lo, s0) & 0xffffff00u),
-                     __uint_as_float(__byte_perm(hi, lo, s1) & 0xffffff00u));
 }
 
 // 16-byte piece c of row `row` of a 32 x 32 block of 16 bits (64B-swizzled), and one element of it.
@@ -234,7 +217,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 2 * EPI_WARPS);
+      mbar_init(acc_empty(b), p.alternate ? EPI_WARPS : 2 * EPI_WARPS);  // both CTAs' warps on a tile
     }
     mbar_init(drain, 1);
     for (int w = 0; w < EPI_WARPS; ++w)
@@ -356,72 +339,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       mbar_wait_drain(drain, 0, p.err);
     }
   } else {
-    // Each warp: its lane quarter's 32 rows, column blocks cw, cw + 4, ... of 32.
-    const int q = warp & 3, cw = (warp - 2) >> 2, ew = warp - 2;
+    // Each warp: its lane quarter's 32 rows, every second (one of the two warps of its group and
+    // quarter) or fourth block of 32 columns.
+    const int q = warp & 3, ew = warp - 2, group = ew >> 3;
+    const int first = p.alternate ? (ew >> 2) & 1 : ew >> 2, step = p.alternate ? 2 : 4;
+    constexpr int WIDTH = GATE ? BN / 2 : BN;  // output columns of a tile
     uint8_t *const block = smem + S::OFF_STAGE + ew * S::SLOT_BYTES;
     const uint32_t block_addr = sbase + S::OFF_STAGE + ew * S::SLOT_BYTES;
-    int tile_it = 0, stores = 0;  // stores: through the two blocks in turn
-    uint32_t load_phase[2] = {0, 0};
+    int tile_it = 0, stores = 0, loads = 0;  // stores, loads: through the two blocks in turn
     for (int t = pair; t < p.total_tiles; t += npairs, ++tile_it) {
-      const Tile tile = tile_at(p, t);
       const int buf = tile_it & 1;
+      if (p.alternate && buf != group) continue;
+      const Tile tile = tile_at(p, t);
       const int r0 = tile.mi * PAIR_M + rank * BM + q * 32;  // the warp's first row
       const int64_t m = static_cast<int64_t>(r0) + lane;
-      const bool rows_ok = r0 < p.m, row_ok = m < p.m;
+      const int n0 = tile.ni * WIDTH;
+      // this warp's blocks of the tile: first, first + step, ... below `end`
+      const int end = r0 < p.m ? min(WIDTH / 32, (p.n - n0 + 31) >> 5) : 0;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
       const uint32_t acc_phase = (tile_it >> 1) & 1;
+      bool ok = true;
 
       if constexpr (KIND == kGateBackward) {
         // dg = dh p and dv = dh a with the saved factors p = v act'(g) and a = act(g).  A block's
-        // factors come into the warp's slot and the products leave from the same place.
-        const int col0 = tile.ni * BN + cw * 32;
-        auto fetch = [&](int c0) {
+        // factors come into the warp's two blocks and the products leave from the same place.
+        auto fetch = [&](int b) {
           if (lane == 0) {
-            bulk_wait_read_all();  // the results before them have left the slot
-            const uint32_t bar = load(ew, 0);
-            mbar_arrive_expect_tx(bar, 6144);
-            tma_load_3d(block_addr, &maps.hi, bar, c0, r0, 0);
-            tma_load_3d(block_addr + 2048, &maps.hi, bar, c0, r0, 1);
-            tma_load_3d(block_addr + 4096, &maps.lo, bar, c0, r0, 0);
-            tma_load_3d(block_addr + 5120, &maps.lo, bar, c0, r0, 1);
+            bulk_wait_read_all();  // the products before them have left
+            mbar_arrive_expect_tx(load(ew, 0), 4096);
+            tma_load_3d(block_addr, &maps.half, load(ew, 0), n0 + b * 32, r0, 0);
+            tma_load_3d(block_addr + 2048, &maps.half, load(ew, 0), n0 + b * 32, r0, 1);
           }
         };
-        const bool any = rows_ok && col0 < p.n;
-        if (any) fetch(col0);
+        if (first < end) fetch(first);
         if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) {
-          if (any && lane == 0) mbar_wait_drain(load(ew, 0), load_phase[0], p.err);
+          if (first < end && lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, p.err);
           break;
         }
         tc_fence_after();
-        bool ok = true;
 #pragma unroll 1
-        for (int j = 0; j < BN / 128; ++j) {
-          const int c0 = col0 + j * 128;
-          if (!rows_ok || c0 >= p.n) break;
-          if (j) fetch(c0);
+        for (int b = first; b < end; b += step) {
+          const int c0 = n0 + b * 32;
+          if (b != first) fetch(b);
           uint32_t v[32];
-          tmem_ld32(taddr + cw * 32 + j * 128, v);
-          ok = warp_wait(load(ew, 0), load_phase[0], abort_flag, p.err, kErrWaitEpilogue);
+          tmem_ld32(taddr + b * 32, v);
+          const uint32_t scales = p.saved_scale[(c0 >> 5) * p.scale_rows + m];
+          ok = warp_wait(load(ew, 0), loads++ & 1, abort_flag, p.err, kErrWaitEpilogue);
           tmem_ld_wait();
           if (!ok) break;
-          load_phase[0] ^= 1;
 #pragma unroll
           for (int plane = 0; plane < 2; ++plane) {
             float d[32];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {  // 8 columns each
+              const float scale = Factor<OT>::scale((scales >> (16 * plane + 8 * (c >> 1))) & 0xffu);
               uint4 *piece = piece16(block + plane * 2048, lane, c);
-              const uint4 hi = *piece;
-              const uint2 lo = *reinterpret_cast<const uint2 *>(block + 4096 + plane * 1024 + lane * 32 + c * 8);
-              float2 f[4] = {from_planes<0>(hi.x, lo.x), from_planes<1>(hi.y, lo.x), from_planes<0>(hi.z, lo.y),
-                             from_planes<1>(hi.w, lo.y)};
-              uint32_t w[4];
+              const uint4 u = *piece;
+              uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                f[i] = f2mul(f[i], make_float2(__uint_as_float(v[8 * c + 2 * i]), __uint_as_float(v[8 * c + 2 * i + 1])));
-                w[i] = pack2_t<OT>(f[i].x, f[i].y);
-                d[8 * c + 2 * i] = f[i].x;
-                d[8 * c + 2 * i + 1] = f[i].y;
+                const float2 dh = make_float2(__uint_as_float(v[8 * c + 2 * i]), __uint_as_float(v[8 * c + 2 * i + 1]));
+                const float2 f = f2mul(Factor<OT>::value(w[i], scale), dh);
+                w[i] = pack2_t<OT>(f.x, f.y);
+                d[8 * c + 2 * i] = f.x;
+                d[8 * c + 2 * i + 1] = f.y;
               }
               *piece = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -442,200 +423,186 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (!ok) break;
       } else if constexpr (GATE) {
         // h = act(g) v; columns [0, BN / 2) of the accumulator are g, the others v
-        const int cc = cw * 32, c0 = tile.ni * (BN / 2) + cc;
-        const bool inside = cc < BN / 2 && rows_ok && c0 < p.n;
-        uint32_t bg[16], bv[16];
-        if (inside) {
-          if (p.bias[0]) load_raw32(static_cast<const OT *>(p.bias[0]), c0, p.n, p.vector_bias, bg);
-          if (p.bias[1]) load_raw32(static_cast<const OT *>(p.bias[1]), c0, p.n, p.vector_bias, bv);
-        }
         if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) break;
         tc_fence_after();
-        if (inside) {
-          const int b = KIND == kGateSave ? 0 : (stores++ & 1) * 2048;
-          if (lane == 0) {
-            if (KIND == kGateSave)
-              bulk_wait_read_all();
-            else
-              bulk_wait_read_but_one();
-          }
-          __syncwarp();
+#pragma unroll 1
+        for (int b = first; b < end; b += step) {
+          const int c0 = n0 + b * 32;
+          const uint32_t at = KIND == kGateSave ? 0 : (stores++ & 1) * 2048;
+          uint32_t scales = 0;
 #pragma unroll
           for (int part = 0; part < 2; ++part) {  // 16 columns each
-            uint32_t g[16], v[16];
-            tmem_ld16(taddr + cc + part * 16, g);
-            tmem_ld16(taddr + BN / 2 + cc + part * 16, v);
+            uint32_t g[16], v[16], bg[8] = {}, bv[8] = {};
+            tmem_ld16(taddr + b * 32 + part * 16, g);
+            tmem_ld16(taddr + WIDTH + b * 32 + part * 16, v);
+            if (p.bias[0]) load_raw16(static_cast<const OT *>(p.bias[0]), c0 + part * 16, p.n, p.vector_bias, bg);
+            if (p.bias[1]) load_raw16(static_cast<const OT *>(p.bias[1]), c0 + part * 16, p.n, p.vector_bias, bv);
             tmem_ld_wait();
-            uint32_t h[8], ph[8], ah[8], pl[4], al[4];
+            uint32_t h[8], pw[8], aw[8];
             with_activation(p.activation, [&](auto act) {
               constexpr int ACT = decltype(act)::value;
-              float2 last_p = f2(0.f), last_a = f2(0.f);
+              float2 pf[8], af[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                float2 gz = make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-                float2 vz = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                if (p.bias[0]) gz = f2add(gz, unpack2<OT>(bg[part * 8 + i]));
-                if (p.bias[1]) vz = f2add(vz, unpack2<OT>(bv[part * 8 + i]));
-                float2 a;
+                const float2 gz = f2add(make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])),
+                                        unpack2<OT>(bg[i]));
+                const float2 vz = f2add(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])),
+                                        unpack2<OT>(bv[i]));
                 if constexpr (KIND == kGateSave) {
-                  float2 slope;
-                  activate_slope2<ACT, true>(gz, a, slope);
-                  slope = f2mul(slope, vz);
-                  ph[i] = upper_halves(slope);
-                  ah[i] = upper_halves(a);
-                  if (i & 1) {
-                    pl[i >> 1] = third_bytes(last_p, slope);
-                    al[i >> 1] = third_bytes(last_a, a);
-                  }
-                  last_p = slope;
-                  last_a = a;
+                  activate_slope2<ACT, true>(gz, af[i], pf[i]);
+                  pf[i] = f2mul(pf[i], vz);
                 } else {
-                  a = activate2<ACT, true>(gz);
+                  af[i] = activate2<ACT, true>(gz);
                 }
-                a = f2mul(a, vz);
-                h[i] = pack2_t<OT>(a.x, a.y);
+                const float2 hz = f2mul(af[i], vz);
+                h[i] = pack2_t<OT>(hz.x, hz.y);
               }
+              if constexpr (KIND == kGateSave)
+                scales |= Factor<OT>::block(pf, pw) << (8 * part) | Factor<OT>::block(af, aw) << (16 + 8 * part);
             });
+            if (part == 0) {
+              // the blocks are free once what left from them before has been read
+              if (lane == 0) {
+                if (KIND == kGateSave)
+                  bulk_wait_read_all();
+                else
+                  bulk_wait_read_but_one();
+              }
+              __syncwarp();
+            }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              *piece16(block + b, lane, part * 2 + c) = make_uint4(h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+              const int pc = part * 2 + c;
+              *piece16(block + at, lane, pc) = make_uint4(h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
               if constexpr (KIND == kGateSave) {
-                *piece16(block + 2048, lane, part * 2 + c) =
-                    make_uint4(ph[4 * c], ph[4 * c + 1], ph[4 * c + 2], ph[4 * c + 3]);
-                *piece16(block + 4096, lane, part * 2 + c) =
-                    make_uint4(ah[4 * c], ah[4 * c + 1], ah[4 * c + 2], ah[4 * c + 3]);
+                *piece16(block + 2048, lane, pc) = make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]);
+                *piece16(block + 4096, lane, pc) = make_uint4(aw[4 * c], aw[4 * c + 1], aw[4 * c + 2], aw[4 * c + 3]);
               }
-            }
-            if constexpr (KIND == kGateSave) if (row_ok) {
-              uint8_t *lo = p.saved_lo + m * p.saved_pitch + c0 + part * 16;
-              *reinterpret_cast<uint4 *>(lo) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
-              *reinterpret_cast<uint4 *>(lo + p.saved_stride) = make_uint4(al[0], al[1], al[2], al[3]);
             }
           }
           fence_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_3d(&maps.out[0], block_addr + b, c0, r0, 0);
+            tma_store_3d(&maps.out[0], block_addr + at, c0, r0, 0);
             if constexpr (KIND == kGateSave) {
-              tma_store_3d(&maps.hi, block_addr + 2048, c0, r0, 0);
-              tma_store_3d(&maps.hi, block_addr + 4096, c0, r0, 1);
+              tma_store_3d(&maps.half, block_addr + 2048, c0, r0, 0);
+              tma_store_3d(&maps.half, block_addr + 4096, c0, r0, 1);
             }
             bulk_commit();
           }
+          if constexpr (KIND == kGateSave) p.saved_scale[(c0 >> 5) * p.scale_rows + m] = scales;
         }
       } else {
         // out = act(acc + bias) (+ residual)
         const int z = p.partial ? tile.split * static_cast<int>(p.batches.d) + tile.z : 0;
         const CUtensorMap *omap = &maps.out[p.partial ? 0 : tile.z];
-        const int col0 = tile.ni * BN + cw * 32;
-        if (p.tma_residual && rows_ok && lane == 0) {
-          bulk_wait_read_all();
-#pragma unroll
-          for (int j = 0; j < BN / 128; ++j)
-            if (col0 + j * 128 < p.n) {
-              mbar_arrive_expect_tx(load(ew, j), 2048);
-              tma_load_3d(block_addr + j * 2048, &maps.residual, load(ew, j), col0 + j * 128, r0, 0);
-            }
-        }
+        // the residual's blocks come ahead, each into the block that its result leaves from
+        auto fetch = [&](int b, int at) {
+          if (lane == 0) {
+            bulk_wait_read_all();
+            mbar_arrive_expect_tx(load(ew, at & 1), 2048);
+            tma_load_3d(block_addr + (at & 1) * 2048, &maps.residual, load(ew, at & 1), n0 + b * 32, r0, 0);
+          }
+        };
+        if (p.tma_residual && first < end) fetch(first, loads);
         if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) {
-          if (p.tma_residual && rows_ok && lane == 0)
-            for (int j = 0; j < BN / 128; ++j)
-              if (col0 + j * 128 < p.n) mbar_wait_drain(load(ew, j), load_phase[j], p.err);
+          if (p.tma_residual && first < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, p.err);
           break;
         }
         tc_fence_after();
-        bool ok = true;
-#pragma unroll
-        for (int j = 0; j < BN / 128; ++j) {
-          const int c0 = col0 + j * 128;
-          if (!rows_ok || c0 >= p.n || !ok) continue;
+#pragma unroll 1
+        for (int b = first; b < end; b += step) {
+          const int c0 = n0 + b * 32;
           uint32_t r[32];
-          tmem_ld32(taddr + cw * 32 + j * 128, r);
-          tmem_ld_wait();
+          tmem_ld32(taddr + b * 32, r);
+          if (p.tma_residual && b + step < end) fetch(b + step, loads + 1);
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
           const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0)), cols = min(32, p.n - c0);
-          if (!p.partial) {
-            if (p.bias[tile.z]) {
-              const OT *bias = static_cast<const OT *>(p.bias[tile.z]);
-              if constexpr (sizeof(OT) == 4) {
+          const OT *bias = p.partial ? nullptr : static_cast<const OT *>(p.bias[tile.z]);
+          if constexpr (sizeof(OT) == 2) {
+            uint32_t bw[2][8] = {};
+            if (bias) {
+              load_raw16(bias, c0, p.n, p.vector_bias, bw[0]);
+              load_raw16(bias, c0 + 16, p.n, p.vector_bias, bw[1]);
+            }
+            tmem_ld_wait();
+            if (bias) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] += i < cols ? bias[c0 + i] : 0.f;
-              } else {
-                uint32_t bw[16];
-                load_raw32(bias, c0, p.n, p.vector_bias, bw);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float2 b2 = unpack2<OT>(bw[i]);
-                  y[2 * i] += b2.x;
-                  y[2 * i + 1] += b2.y;
-                }
+              for (int i = 0; i < 16; ++i) {
+                const float2 s2 = f2add(make_float2(y[2 * i], y[2 * i + 1]), unpack2<OT>(bw[i >> 3][i & 7]));
+                y[2 * i] = s2.x;
+                y[2 * i + 1] = s2.y;
               }
             }
-            if (p.activation != AF2_ACTIVATION_NONE) {
-              const bool save = p.saved_hi || p.saved_f32;
-              if (save) {  // the slopes, in the place of the values until they are stored
-                if (lane == 0) bulk_wait_read_all();
-                __syncwarp();
-                with_activation(p.activation, [&](auto act) {
-                  constexpr int ACT = decltype(act)::value;
+          } else {
+            tmem_ld_wait();
+            if (bias) {
 #pragma unroll
-                  for (int c = 0; c < 4; ++c) {
-                    float2 s[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                      float2 v2;
-                      activate_slope2<ACT, sizeof(OT) == 2>(make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]), v2,
-                                                            s[i]);
-                      y[8 * c + 2 * i] = v2.x;
-                      y[8 * c + 2 * i + 1] = v2.y;
-                    }
-                    if constexpr (sizeof(OT) == 4) {
-                      if (row_ok) {
-                        float4 *dst = reinterpret_cast<float4 *>(p.saved_f32 + m * p.saved_pitch + c0 + 8 * c);
-                        dst[0] = make_float4(s[0].x, s[0].y, s[1].x, s[1].y);
-                        dst[1] = make_float4(s[2].x, s[2].y, s[3].x, s[3].y);
-                      }
-                    } else {
-                      *piece16(block, lane, c) = make_uint4(upper_halves(s[0]), upper_halves(s[1]), upper_halves(s[2]),
-                                                            upper_halves(s[3]));
-                      if (row_ok)
-                        *reinterpret_cast<uint2 *>(p.saved_lo + m * p.saved_pitch + c0 + 8 * c) =
-                            make_uint2(third_bytes(s[0], s[1]), third_bytes(s[2], s[3]));
-                    }
-                  }
-                });
-                if constexpr (sizeof(OT) == 2) {
-                  fence_async_smem();
-                  __syncwarp();
-                  if (lane == 0) {
-                    tma_store_3d(&maps.hi, block_addr, c0, r0, 0);
-                    bulk_commit();
-                  }
-                }
-              } else {
-                with_activation(p.activation, [&](auto act) {
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) {
-                    const float2 v2 = activate2<decltype(act)::value, sizeof(OT) == 2>(make_float2(y[2 * i], y[2 * i + 1]));
-                    y[2 * i] = v2.x;
-                    y[2 * i + 1] = v2.y;
-                  }
-                });
-              }
+              for (int i = 0; i < 32; ++i) y[i] += i < cols ? bias[c0 + i] : 0.f;
             }
           }
-          // the block that the result leaves from, with the residual in it where there is one
+          if (!p.partial && p.activation != AF2_ACTIVATION_NONE) {
+            if (p.save) {  // the slopes, through the first block (16 bits) or directly (f32)
+              if (lane == 0) bulk_wait_read_all();
+              __syncwarp();
+              with_activation(p.activation, [&](auto act) {
+                constexpr int ACT = decltype(act)::value;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  float2 s[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    float2 v2;
+                    activate_slope2<ACT, sizeof(OT) == 2>(make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]), v2, s[i]);
+                    y[8 * c + 2 * i] = v2.x;
+                    y[8 * c + 2 * i + 1] = v2.y;
+                  }
+                  if constexpr (sizeof(OT) == 4) {
+                    if (m < p.m) {
+                      float4 *dst = reinterpret_cast<float4 *>(p.saved_f32 + m * p.saved_pitch + c0 + 8 * c);
+                      dst[0] = make_float4(s[0].x, s[0].y, s[1].x, s[1].y);
+                      dst[1] = make_float4(s[2].x, s[2].y, s[3].x, s[3].y);
+                    }
+                  } else {
+                    *piece16(block, lane, c) =
+                        make_uint4(Factor<OT>::slope(s[0]), Factor<OT>::slope(s[1]), Factor<OT>::slope(s[2]),
+                                   Factor<OT>::slope(s[3]));
+                  }
+                }
+              });
+              if constexpr (sizeof(OT) == 2) {
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_3d(&maps.half, block_addr, c0, r0, 0);
+                  bulk_commit();
+                }
+              }
+            } else {
+              with_activation(p.activation, [&](auto act) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float2 v2 = activate2<decltype(act)::value, sizeof(OT) == 2>(make_float2(y[2 * i], y[2 * i + 1]));
+                  y[2 * i] = v2.x;
+                  y[2 * i + 1] = v2.y;
+                }
+              });
+            }
+          }
+          // the block that the result leaves from (f32: both), with the residual in it where there is one
           uint32_t at = 0;
           if constexpr (sizeof(OT) == 2)
-            at = 2048u * (p.saved_hi       ? 1  // the first block may still hold slopes
-                          : p.tma_residual ? j
-                                           : stores++ & 1);
+            at = 2048u * (p.tma_residual ? loads & 1
+                          : p.save       ? 1  // the first block may still hold slopes
+                                         : stores++ & 1);
           uint8_t *const dst = block + at;
-          const uint32_t dst_addr = block_addr + at;
           if (p.tma_residual) {
-            ok = warp_wait(load(ew, j), load_phase[j], abort_flag, p.err, kErrWaitEpilogue);
-            load_phase[j] ^= 1;
-            if (!ok) continue;
+            ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
+            ++loads;
+            if (!ok) {
+              if (b + step < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, p.err);
+              break;
+            }
           } else {
             if (lane == 0) {
               if (sizeof(OT) == 4)
@@ -684,7 +651,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              tma_store_3d(omap, dst_addr, c0, r0, z);
+              tma_store_3d(omap, block_addr + at, c0, r0, z);
               bulk_commit();
             }
           } else {
@@ -722,8 +689,7 @@ struct ReduceArgs {
   const void *bias[2];
   const void *residual;
   int64_t residual_stride;
-  uint16_t *saved_hi;
-  uint8_t *saved_lo;
+  uint16_t *saved_half;
   float *saved_f32;
   int64_t saved_pitch;
 };
@@ -760,10 +726,9 @@ __global__ void __launch_bounds__(256) reduce_kernel(const ReduceArgs p) {
         y[j] = value.x;
         slope = slopes.x;
       });
-      if (p.saved_hi) {
-        const uint32_t bits = __float_as_uint(slope);
-        p.saved_hi[m * p.saved_pitch + c] = static_cast<uint16_t>(bits >> 16);
-        p.saved_lo[m * p.saved_pitch + c] = static_cast<uint8_t>(bits >> 8);
+      if constexpr (sizeof(OT) == 2) {
+        if (p.saved_half)
+          p.saved_half[m * p.saved_pitch + c] = static_cast<uint16_t>(Factor<OT>::slope(f2(slope)));
       }
       if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c] = slope;
       if (res) y[j] += to_f32<OT>(res[c]);
@@ -819,13 +784,14 @@ bool operand_map(CUtensorMap *map, const GemmOperand &o, int64_t outer, int64_t 
 }
 
 template <int KIND, typename OT, int BN>
-af2_status launch(af2_ctx *ctx, const Maps &maps, const Args &p, cudaStream_t stream) {
+af2_status launch(af2_ctx *ctx, const Maps &maps, Args p, cudaStream_t stream) {
   constexpr uint32_t smem = Shape<KIND, BN>::BYTES;
   auto kernel = layer_gemm_kernel<KIND, OT, BN>;
   if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       e != cudaSuccess)
     return cuda_fail(ctx, e, "layer product shared memory");
   const int pairs = std::min(p.total_tiles, std::max(1, ctx->sm_count / 2));
+  p.alternate = p.total_tiles > pairs;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
   kernel<<<2 * pairs, THREADS, smem, stream>>>(maps, p);
   if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cuda_fail(ctx, e, "layer product");
@@ -898,7 +864,7 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
     p.activation = g.activation;
     p.residual = g.residual;
     p.residual_stride = g.residual_stride;
-    if (g.residual && !g.saved.hi && out_bytes == 2 && aligned16(g.residual, g.residual_stride, 2)) {
+    if (g.residual && !g.saved.half && out_bytes == 2 && aligned16(g.residual, g.residual_stride, 2)) {
       p.tma_residual = 1;
       maps_ok &= encode_map_3d(&maps.residual, map_type(g.out_dtype), g.residual, g.n, g.m, 1, g.residual_stride * 2,
                                g.residual_stride * 2, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -918,18 +884,15 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
                                  g.out_stride * out_bytes, 32, 32, 1,
                                  out_bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     p.saved_f32 = g.saved.f32;
-    p.saved_hi = g.saved.hi;
-    p.saved_lo = g.saved.lo;
+    p.save = g.saved.half || g.saved.f32;
+    p.saved_f32 = g.saved.f32;
+    p.saved_scale = g.saved.scale;
     p.saved_pitch = g.saved.pitch;
-    p.saved_stride = g.saved.stride;
-    if (g.saved.hi) {
-      const int planes = g.epilogue == kEpilogueOut ? 1 : 2;
-      maps_ok &= encode_map_3d(&maps.hi, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.saved.hi, g.saved.pitch, g.m, planes,
-                               g.saved.pitch * 2, g.saved.stride * 2, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
-      if (g.epilogue == kEpilogueGateBackward)
-        maps_ok &= encode_map_3d(&maps.lo, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.saved.lo, g.saved.pitch, g.m, planes,
-                                 g.saved.pitch, g.saved.stride, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
-    }
+    p.scale_rows = g.saved.scale_rows;
+    if (g.saved.half)
+      maps_ok &= encode_map_3d(&maps.half, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.saved.half, g.saved.pitch, g.m,
+                               g.epilogue == kEpilogueOut ? 1 : 2, g.saved.pitch * 2, g.saved.stride * 2, 32, 32, 1,
+                               CU_TENSOR_MAP_SWIZZLE_64B);
     p.column_partial = g.column_partial;
   }
   if (!maps_ok) return fail(ctx, AF2_ERR_CUDA, "cannot describe the layer's tensors to the TMA unit");
@@ -937,7 +900,7 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
   af2_status st = AF2_OK;
   if (g.epilogue == kEpilogueGateBackward)
     st = launch_16<kGateBackward>(ctx, g.out_dtype, plan.bn, maps, p, stream);
-  else if (gate && g.saved.hi)
+  else if (gate && g.saved.half)
     st = launch_16<kGateSave>(ctx, g.out_dtype, plan.bn, maps, p, stream);
   else if (gate)
     st = launch_16<kGate>(ctx, g.out_dtype, plan.bn, maps, p, stream);
@@ -962,8 +925,7 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
   r.out_stride = g.out_stride;
   r.residual = g.residual;
   r.residual_stride = g.residual_stride;
-  r.saved_hi = g.saved.hi;
-  r.saved_lo = g.saved.lo;
+  r.saved_half = g.saved.half;
   r.saved_f32 = g.saved.f32;
   r.saved_pitch = g.saved.pitch;
   const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(g.batch * g.m * pitch / 4, 256), 8 * ctx->sm_count));

@@ -23,15 +23,16 @@ enum GemmEpilogue {
   kEpilogueGateBackward,  // acc = dh: out = dh times each of the two saved factors (dg and dv)
 };
 
-// Factors kept for the backward pass.  The 16-bit types keep the upper 24 bits of each f32, as planes
-// of its upper 16 (`hi`) and of the next 8 (`lo`), rows of `pitch` elements, `stride` elements from
-// the first factor's plane to the second's; so the backward pass rounds to 16 bits only what becomes
-// a product's operand.  The f32 type keeps f32 in `f32`.
+// Factors kept for the backward pass, rows of `pitch` elements; the second factor's plane `stride`
+// elements after the first's.  The f32 type keeps f32 in `f32`.  The 16-bit types keep 16 bits
+// (layer_factor.cuh) in `half`; the gated transition's factors, of any size, with an exponent byte for
+// every 16 columns of a row, four of them (two factors x two halves) as a word per row and 32 columns in
+// `scale` [pitch / 32][scale_rows].
 struct SavedPlanes {
-  uint16_t *hi = nullptr;
-  uint8_t *lo = nullptr;
+  uint16_t *half = nullptr;
+  uint32_t *scale = nullptr;
   float *f32 = nullptr;
-  int64_t pitch = 0, stride = 0;
+  int64_t pitch = 0, stride = 0, scale_rows = 0;
 };
 
 struct LayerGemm {
