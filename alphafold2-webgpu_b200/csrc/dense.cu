@@ -17,6 +17,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "few_rows.h"
 #include "layer_factor.cuh"
 #include "layer_gemm.h"
 #include "layer_math.cuh"
@@ -438,6 +439,18 @@ uint64_t gated_saved_bytes(int64_t rows, int64_t hidden, int dtype) {
 
 af2_status dense_forward(af2_ctx *ctx, const DenseForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
   Pass l(ctx, p.dtype, scratch, stream);
+  if (p.rows <= kFewRows && !(p.saved && p.activation != AF2_ACTIVATION_NONE)) {
+    *bytes = 0;
+    if (!ctx) return AF2_OK;
+    FewRows f;
+    f.rows = p.rows, f.inner = p.inner, f.columns = p.columns;
+    f.dtype = p.dtype, f.activation = p.activation;
+    f.x = p.x, f.x_stride = p.x_stride;
+    f.weight[0] = p.weight, f.bias[0] = p.bias;
+    f.residual = p.residual, f.residual_stride = p.residual_stride;
+    f.out = p.out, f.out_stride = p.out_stride;
+    return few_rows_launch(ctx, f, stream);
+  }
   LayerGemm g = l.product(p.rows, p.columns, p.inner);
   g.a[0] = l.operand(p.x, p.x_stride, p.rows, p.inner);
   g.b[0] = Pass::mn(l.operand(p.weight, p.columns, p.inner, p.columns));
@@ -507,6 +520,28 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
 
 af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
   Pass l(ctx, p.dtype, scratch, stream);
+  if (p.rows <= kFewRows && !p.saved) {
+    void *h = l.take(element_size(p.dtype) * p.rows * p.hidden);
+    *bytes = l.total();
+    if (!ctx) return AF2_OK;
+    FewRows f;
+    f.rows = p.rows, f.inner = p.channels, f.columns = p.hidden;
+    f.dtype = p.dtype, f.activation = p.activation;
+    f.x = p.x, f.x_stride = p.x_stride;
+    f.weight[0] = p.w.gate_weight, f.weight[1] = p.w.value_weight;
+    f.bias[0] = p.w.gate_bias, f.bias[1] = p.w.value_bias;
+    f.out = h, f.out_stride = p.hidden;
+    if (af2_status st = few_rows_launch(ctx, f, stream); st != AF2_OK) return st;
+    FewRows y;
+    y.rows = p.rows, y.inner = p.hidden, y.columns = p.channels;
+    y.dtype = p.dtype;
+    y.x = h, y.x_stride = p.hidden;
+    y.weight[0] = p.w.output_weight, y.bias[0] = p.w.output_bias;
+    y.residual = p.residual, y.residual_stride = p.residual_stride;
+    y.out = p.out, y.out_stride = p.out_stride;
+    y.follows = true;
+    return few_rows_launch(ctx, y, stream);
+  }
   const GemmOperand x = l.operand(p.x, p.x_stride, p.rows, p.channels);
   const GemmOperand wg = l.operand(p.w.gate_weight, p.hidden, p.channels, p.hidden);
   const GemmOperand wv = l.operand(p.w.value_weight, p.hidden, p.channels, p.hidden);
