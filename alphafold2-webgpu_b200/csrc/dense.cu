@@ -344,7 +344,8 @@ class Pass {
   }
   void run(LayerGemm g) {
     const uint64_t mark = used;
-    g.scratch = take(layer_gemm_scratch(g));
+    layer_gemm_plan(&g);
+    g.scratch = take(g.scratch_bytes);
     if (live()) status = layer_gemm_launch(ctx_, g, stream_);
     peak_ = std::max(peak_, used);
     used = mark;  // launches follow one another on the stream: the next may use the same place

@@ -23,6 +23,7 @@
 // the small ones first: what is left out is below 2^-24 of |x||y|, f32's own
 // rounding.  (An infinite f32 element makes its sums NaN or infinite.)
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "layer_factor.cuh"
@@ -737,37 +738,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const ReduceArgs p) {
   }
 }
 
-// Tile width and number of splits of the depth, from what a launch costs in SM clocks: a K step of
-// 64 takes 512 (BN = 256) or about 300 (BN = 128) clocks, a tile's start and its last epilogue about
-// 2500, and split sums are written, read and reduced by another kernel.
-struct Plan {
-  int bn = 256, splits = 1;
-};
-
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-Plan make_plan(const LayerGemm &g) {
-  Plan best;
-  double best_cost = 0;
-  const int64_t k_blocks = ceil_div(g.k, BK), combos = g.pieces > 1 ? 6 : 1;
-  const bool gate = g.epilogue == kEpilogueGate, may_split = g.epilogue == kEpilogueOut;
-  for (int bn : {256, 128}) {
-    if (g.epilogue == kEpilogueGateBackward && bn == 128) continue;
-    const int64_t tiles = g.batch * ceil_div(g.m, PAIR_M) * ceil_div(g.n, gate ? bn / 2 : bn);
-    const int64_t max_splits = may_split ? std::min<int64_t>({ceil_div(k_blocks, 4), ceil_div(2 * kPairs, tiles), 64}) : 1;
-    for (int64_t s = 1; s <= std::max<int64_t>(max_splits, 1); ++s) {
-      const double waves = static_cast<double>(ceil_div(tiles * s, kPairs));
-      const double steps = static_cast<double>(ceil_div(k_blocks, s) * g.segments * combos);
-      double cost = waves * steps * (bn == 256 ? 512 : 300) + waves * 800 + 2500;
-      if (s > 1) cost += 5000 + 8.0 * s * g.batch * g.m * align_up(g.n, 4) / 2500;
-      if (best_cost == 0 || cost < best_cost) {
-        best_cost = cost;
-        best = {bn, static_cast<int>(s)};
-      }
-    }
-  }
-  return best;
-}
 
 bool aligned16(const void *ptr, int64_t stride, int element) {
   return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && (stride * element) % 16 == 0 &&
@@ -787,9 +758,14 @@ template <int KIND, typename OT, int BN>
 af2_status launch(af2_ctx *ctx, const Maps &maps, Args p, cudaStream_t stream) {
   constexpr uint32_t smem = Shape<KIND, BN>::BYTES;
   auto kernel = layer_gemm_kernel<KIND, OT, BN>;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      e != cudaSuccess)
-    return cuda_fail(ctx, e, "layer product shared memory");
+  static std::atomic<uint64_t> allowed{0};  // devices on which this kernel has its shared memory
+  const uint64_t bit = uint64_t(1) << (ctx->device & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit) || ctx->device > 63) {
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e != cudaSuccess)
+      return cuda_fail(ctx, e, "layer product shared memory");
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int pairs = std::min(p.total_tiles, std::max(1, ctx->sm_count / 2));
   p.alternate = p.total_tiles > pairs;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
@@ -818,25 +794,45 @@ CUtensorMapDataType map_type(int dtype) {
 
 }  // namespace
 
-uint64_t layer_gemm_scratch(const LayerGemm &g) {
-  const Plan plan = make_plan(g);
-  return plan.splits > 1 ? align_up(4ull * plan.splits * g.batch * g.m * align_up(g.n, 4), 256) : 0;
+// Tile width and number of splits of the depth, from what a launch costs in SM clocks: a K step of
+// 64 takes 512 (BN = 256) or about 300 (BN = 128) clocks, a tile's start and its last epilogue about
+// 2500, and split sums are written, read and reduced by another kernel.
+void layer_gemm_plan(LayerGemm *g) {
+  double best = 0;
+  const int64_t k_blocks = ceil_div(g->k, BK), combos = g->pieces > 1 ? 6 : 1;
+  const bool gate = g->epilogue == kEpilogueGate;
+  for (int bn : {256, 128}) {
+    if (g->epilogue == kEpilogueGateBackward && bn == 128) continue;
+    const int64_t tiles = g->batch * ceil_div(g->m, PAIR_M) * ceil_div(g->n, gate ? bn / 2 : bn);
+    for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
+      if (s > 1 && (g->epilogue != kEpilogueOut || s * 4 > k_blocks || tiles * (s - 1) >= 2 * kPairs)) break;
+      const double waves = static_cast<double>(ceil_div(tiles * s, kPairs));
+      const double steps = static_cast<double>(ceil_div(k_blocks, s) * g->segments * combos);
+      double cost = waves * steps * (bn == 256 ? 512 : 300) + waves * 800 + 2500;
+      if (s > 1) cost += 5000 + 8.0 * s * g->batch * g->m * align_up(g->n, 4) / 2500;
+      if (best == 0 || cost < best) {
+        best = cost;
+        g->tile_n = bn;
+        g->splits = s;
+      }
+    }
+  }
+  g->scratch_bytes = g->splits > 1 ? align_up(4ull * g->splits * g->batch * g->m * align_up(g->n, 4), 256) : 0;
 }
 
 af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stream) {
-  const Plan plan = make_plan(g);
   const bool gate = g.epilogue == kEpilogueGate;
   Maps maps{};
   Args p{};
   p.m = g.m;
   p.n = static_cast<int>(g.n);
   p.k_blocks = static_cast<int>(ceil_div(g.k, BK));
-  p.splits = plan.splits;
+  p.splits = g.splits;
   p.combos = g.pieces > 1 ? 6 : 1;
   p.segments = g.segments;
   p.batches = Divisor(g.batch);
   p.tiles_m = Divisor(static_cast<uint32_t>(ceil_div(g.m, PAIR_M)));
-  p.tiles_n = Divisor(static_cast<uint32_t>(ceil_div(g.n, gate ? plan.bn / 2 : plan.bn)));
+  p.tiles_n = Divisor(static_cast<uint32_t>(ceil_div(g.n, gate ? g.tile_n / 2 : g.tile_n)));
   const int64_t total = static_cast<int64_t>(p.splits) * g.batch * p.tiles_m.d * p.tiles_n.d;
   if (total > 0x3fffffff) return fail(ctx, AF2_ERR_UNSUPPORTED, "the product has too many tiles");
   p.total_tiles = static_cast<int>(total);
@@ -849,16 +845,16 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
   for (int i = 0; i < g.segments; ++i)
     maps_ok &= operand_map(&maps.a[i], g.a[i], g.m, g.k, g.bf16, g.pieces, BM);
   for (int i = 0; i < bsets; ++i)
-    maps_ok &= operand_map(&maps.b[i], g.b[i], g.n, g.k, g.bf16, g.pieces, plan.bn / 2);
+    maps_ok &= operand_map(&maps.b[i], g.b[i], g.n, g.k, g.bf16, g.pieces, g.tile_n / 2);
 
   const int out_bytes = g.out_dtype == AF2_F32 ? 4 : 2;
   const int64_t pitch = align_up(g.n, 4);
   const int outs = g.epilogue == kEpilogueGateBackward ? 2 : g.batch;
-  if (plan.splits > 1) {
+  if (g.splits > 1) {
     p.partial = 1;
     p.tma_out = 1;
     maps_ok &= encode_map_3d(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.scratch, g.n, g.m,
-                             plan.splits * g.batch, pitch * 4, g.m * pitch * 4, 32, 32, 1,
+                             g.splits * g.batch, pitch * 4, g.m * pitch * 4, 32, 32, 1,
                              CU_TENSOR_MAP_SWIZZLE_128B);
   } else {
     p.activation = g.activation;
@@ -899,20 +895,20 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
 
   af2_status st = AF2_OK;
   if (g.epilogue == kEpilogueGateBackward)
-    st = launch_16<kGateBackward>(ctx, g.out_dtype, plan.bn, maps, p, stream);
+    st = launch_16<kGateBackward>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
   else if (gate && g.saved.half)
-    st = launch_16<kGateSave>(ctx, g.out_dtype, plan.bn, maps, p, stream);
+    st = launch_16<kGateSave>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
   else if (gate)
-    st = launch_16<kGate>(ctx, g.out_dtype, plan.bn, maps, p, stream);
+    st = launch_16<kGate>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
   else if (p.partial || g.out_dtype == AF2_F32)
-    st = launch_bn<kOut, float>(ctx, plan.bn, maps, p, stream);
+    st = launch_bn<kOut, float>(ctx, g.tile_n, maps, p, stream);
   else
-    st = launch_16<kOut>(ctx, g.out_dtype, plan.bn, maps, p, stream);
-  if (st != AF2_OK || plan.splits == 1) return st;
+    st = launch_16<kOut>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
+  if (st != AF2_OK || g.splits == 1) return st;
 
   ReduceArgs r{};
   r.partial = reinterpret_cast<const float *>(g.scratch);
-  r.splits = plan.splits;
+  r.splits = g.splits;
   r.batch = g.batch;
   r.activation = g.activation;
   r.m = g.m;

@@ -52,14 +52,17 @@ struct LayerGemm {
   int64_t residual_stride = 0;
   SavedPlanes saved;                         // written by Out and Gate, read by GateBackward
   float *column_partial = nullptr;           // GateBackward: [ceil(m / 32)][2 * saved.pitch] column sums, or NULL
-  uint8_t *scratch = nullptr;                // split sums: layer_gemm_scratch() bytes
+  // layer_gemm_plan: the tile's width, the parts the depth is cut into and the split sums' bytes
+  int tile_n = 0, splits = 0;
+  uint64_t scratch_bytes = 0;
+  uint8_t *scratch = nullptr;
 };
 
 // Row pitch (elements) of a 16-bit operand of `width`, and of the saved planes.
 inline int64_t operand_pitch(int64_t width) { return align_up(width, 8); }
 inline int64_t saved_pitch(int64_t width) { return align_up(width, 32); }
 
-uint64_t layer_gemm_scratch(const LayerGemm &g);
+void layer_gemm_plan(LayerGemm *g);
 af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stream);
 
 }  // namespace af2

@@ -168,16 +168,20 @@ cudaStream_t stream_of(af2_ctx *ctx, void *stream) {
   return stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
 }
 
+// (The message is put together for a tensor that fails only: a set has hundreds.)
 af2_status check_set(af2_ctx *ctx, const af2_tensor_ref *t, int64_t count, const char *what) {
   for (int64_t i = 0; i < count; ++i) {
-    const std::string name = std::string(what) + " " + std::to_string(i);
+    std::string wrong;
     if (!known_dtype(t[i].dtype))
-      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + ": dtype must be AF2_F32, AF2_F16 or AF2_BF16");
-    if (t[i].count < 0 || t[i].count > (int64_t(1) << 48))
-      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + " has " + std::to_string(t[i].count) + " elements");
-    if (t[i].count > 0 && !t[i].data) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + " is NULL");
-    if (reinterpret_cast<uintptr_t>(t[i].data) % element_bytes(t[i].dtype) != 0)
-      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, name + " is not aligned to its element type");
+      wrong = ": dtype must be AF2_F32, AF2_F16 or AF2_BF16";
+    else if (t[i].count < 0 || t[i].count > (int64_t(1) << 44))
+      wrong = " has " + std::to_string(t[i].count) + " elements";
+    else if (t[i].count > 0 && !t[i].data)
+      wrong = " is NULL";
+    else if (reinterpret_cast<uintptr_t>(t[i].data) % element_bytes(t[i].dtype) != 0)
+      wrong = " is not aligned to its element type";
+    if (!wrong.empty())
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, std::string(what) + " " + std::to_string(i) + wrong);
   }
   return AF2_OK;
 }
