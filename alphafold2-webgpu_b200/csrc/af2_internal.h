@@ -117,8 +117,8 @@ struct af2_ctx {
   // af2_set_weight_cache: prepared weights kept per weights pointer and shape, made once
   bool weight_cache = false;
   std::vector<af2::CachedWeights> cached_weights;
-  // scratch of the layers with learned weights: `layer_done` is recorded after each call that
-  // uses it, and a call on another stream waits for it first
+  // scratch of the layers with learned weights, the stream of its last use, and an event behind
+  // that use (LayerScratch)
   af2::DeviceBuffer layer_scratch;
   cudaEvent_t layer_done = nullptr;
   cudaStream_t layer_stream = nullptr;
@@ -430,6 +430,8 @@ class LayerScratch {
   uint8_t *base() const { return base_; }
 
  private:
+  bool lasting(cudaStream_t s) const;
+
   af2_ctx *ctx_;
   cudaStream_t stream_;
   uint8_t *base_ = nullptr;

@@ -58,6 +58,7 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
   constexpr int DEEP = 32 / LANES; // weight rows of one read of a warp (= V)
   __shared__ float work[CHUNK * R];  // x, then the warps' sums
   __shared__ float total[SETS * R * COLS];
+  __shared__ float others[7 * SETS * R * COLS];  // the cluster's other blocks' sums, in rank 0's memory
   static_assert(CHUNK >= WARPS * COLS, "the warps' sums fit where x was");
   float *const xs = work, *const part = work;
   using P = Piece<T, V>;
@@ -89,10 +90,10 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
   for (int c0 = k0; c0 < k1; c0 += CHUNK) {
     const int end = min(k1, c0 + CHUNK);
     if (c0 != k0) __syncthreads();
-    for (int i = threadIdx.x; i < (end - c0) * R; i += THREADS) {
-      const int r = i / (end - c0), k = i - r * (end - c0);
-      xs[k * R + r] = r < p.rows ? to_f32<T>(x[r * p.x_stride + c0 + k]) : 0.f;
-    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      for (int k = threadIdx.x; k < end - c0; k += THREADS)
+        xs[k * R + r] = r < p.rows ? to_f32<T>(x[r * p.x_stride + c0 + k]) : 0.f;
     __syncthreads();
     for (int k = first + (c0 - k0); k < end; k += FLIGHT * STEP) {
       if (k != first) fetch(k, end);
@@ -135,29 +136,26 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < SET_WARPS; ++j) sum += part[(s * SET_WARPS + j) * R * COLS + at];
-    total[i] = sum;
+    if (rank == 0) {
+      total[i] = sum;
+    } else {
+      uint32_t there;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, 0;"
+                   : "=r"(there)
+                   : "r"(smem_u32(&others[(rank - 1) * SETS * R * COLS + i])));
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(sum) : "memory");
+    }
   }
   if (p.splits > 1) {
-    cluster_sync_all();
-    if (rank == 0) {
-      for (int i = threadIdx.x; i < SETS * R * COLS; i += THREADS) {
-        const uint32_t here = smem_u32(&total[i]);
-        float sum = total[i];
-        for (int s = 1; s < p.splits; ++s) {
-          uint32_t there;
-          float v;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(s));
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-          sum += v;
-        }
-        total[i] = sum;
-      }
-    }
-    cluster_sync_all();  // the other blocks' sums have been read before they leave
+    cluster_sync_all();  // the others' sums have arrived
     if (rank != 0) return;
-  } else {
-    __syncthreads();
+    for (int i = threadIdx.x; i < SETS * R * COLS; i += THREADS) {
+      float sum = total[i];  // (written by this thread)
+      for (int s = 1; s < p.splits; ++s) sum += others[(s - 1) * SETS * R * COLS + i];
+      total[i] = sum;
+    }
   }
+  __syncthreads();
   for (int i = threadIdx.x; i < R * COLS; i += THREADS) {
     const int r = i / COLS, c = c_block + (i - r * COLS);
     if (r >= p.rows || c >= p.columns) continue;

@@ -14,6 +14,11 @@
 
 namespace af2 {
 
+// Calls on one stream need no order among themselves.  A call on another stream waits for an event
+// after the last use: recorded then and there if that use was on a stream that lives as long as the
+// context (its own and the legacy default stream, which nothing captures either), else after each use.
+bool LayerScratch::lasting(cudaStream_t s) const { return s == ctx_->stream || s == cudaStreamLegacy; }
+
 af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
   if (workspace) {
     base_ = static_cast<uint8_t *>(workspace);
@@ -28,23 +33,29 @@ af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
     }
   }
   // inside a stream capture the order between streams is the graph's, not this context's
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (cudaError_t e = cudaStreamIsCapturing(stream_, &capture); e != cudaSuccess)
-    return cuda_fail(ctx_, e, "query the stream's capture");
-  capturing_ = capture != cudaStreamCaptureStatusNone;
-  if (ctx_->layer_scratch.bytes < bytes) {
-    if (capturing_)
-      return fail(ctx_, AF2_ERR_UNSUPPORTED, "the context's scratch cannot grow inside a stream capture; pass a "
-                                             "workspace, or make the same call once before the capture");
-    // earlier calls on any stream may still use the buffer that is about to be freed
-    if (ctx_->layer_scratch.ptr)
-      if (cudaError_t e = cudaEventSynchronize(ctx_->layer_done); e != cudaSuccess)
-        return cuda_fail(ctx_, e, "wait for the layer scratch");
-    if (af2_status st = ensure(ctx_, ctx_->layer_scratch, bytes, "layer scratch"); st != AF2_OK) return st;
-  } else if (!capturing_ && ctx_->layer_stream != stream_) {
-    if (cudaError_t e = cudaStreamWaitEvent(stream_, ctx_->layer_done, 0); e != cudaSuccess)
+  if (!lasting(stream_)) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaError_t e = cudaStreamIsCapturing(stream_, &capture); e != cudaSuccess)
+      return cuda_fail(ctx_, e, "query the stream's capture");
+    capturing_ = capture != cudaStreamCaptureStatusNone;
+  }
+  const bool grow = ctx_->layer_scratch.bytes < bytes;
+  if (grow && capturing_)
+    return fail(ctx_, AF2_ERR_UNSUPPORTED, "the context's scratch cannot grow inside a stream capture; pass a "
+                                           "workspace, or make the same call once before the capture");
+  const cudaStream_t last = ctx_->layer_stream;
+  if (!capturing_ && last && (grow || last != stream_)) {
+    if (lasting(last))
+      if (cudaError_t e = cudaEventRecord(ctx_->layer_done, last); e != cudaSuccess)
+        return cuda_fail(ctx_, e, "record the layer scratch's use");
+    // earlier calls may still use the buffer: this one follows them, or the host does before it is freed
+    if (cudaError_t e = grow ? cudaEventSynchronize(ctx_->layer_done)
+                             : cudaStreamWaitEvent(stream_, ctx_->layer_done, 0);
+        e != cudaSuccess)
       return cuda_fail(ctx_, e, "order the layer scratch between streams");
   }
+  if (grow)
+    if (af2_status st = ensure(ctx_, ctx_->layer_scratch, bytes, "layer scratch"); st != AF2_OK) return st;
   base_ = static_cast<uint8_t *>(ctx_->layer_scratch.ptr);
   owned_ = true;
   return AF2_OK;
@@ -53,6 +64,7 @@ af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
 af2_status LayerScratch::release() {
   if (!owned_ || capturing_) return AF2_OK;
   ctx_->layer_stream = stream_;
+  if (lasting(stream_)) return AF2_OK;
   if (cudaError_t e = cudaEventRecord(ctx_->layer_done, stream_); e != cudaSuccess)
     return cuda_fail(ctx_, e, "record the layer scratch's use");
   return AF2_OK;
