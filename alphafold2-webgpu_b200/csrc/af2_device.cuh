@@ -135,6 +135,16 @@ __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// ---- launches that overlap -----------------------------------------------------
+
+// Waits until the kernels before this one on its stream have completed and their writes are visible
+// (at once, when this one was launched in the ordinary way), then lets the next one be set up.  That
+// one waits in turn, so nothing of it but what stands before its wait runs beside this kernel.
+__device__ __forceinline__ void dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---- TMA -------------------------------------------------------------------
 
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {

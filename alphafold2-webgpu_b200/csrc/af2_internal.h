@@ -159,6 +159,25 @@ bool encode_map_3d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base
 bool encode_map_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base, const uint64_t (&dims)[4],
                    const uint64_t (&strides_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle);
 
+// Launches a kernel that may start while the one before it on the stream still runs: it calls
+// dependency_wait() (af2_device.cuh) before it touches memory, so only its launch and its set-up
+// overlap.  (Some 2 us of each launch of a chain of short kernels.)
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                         A &&...args) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // Brackets one kernel launch with CUDA events on its stream while the

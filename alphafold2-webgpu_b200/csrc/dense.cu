@@ -99,6 +99,7 @@ __device__ __forceinline__ void store_operand8(void *dst, int64_t at, int64_t pi
 
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs p) {
+  dependency_wait();
   for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g < p.groups;
        g += static_cast<int64_t>(gridDim.x) * 256) {
     int j = 0;
@@ -114,18 +115,28 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
 
 // ---- passes over rows, with column sums --------------------------------------------
 
-constexpr int kSumRows = 64;  // rows of a block
+// Rows of a block: 64, fewer where that would leave SMs without one.
+inline int row_group(int64_t rows, int64_t width) {
+  int r = 64;
+  while (r > 8 && ceil_div(rows, r) * ceil_div(width, 256) < 296) r /= 2;
+  return r;
+}
 
-// Block (x, y): columns [256 y, + 256) of rows [64 x, + 64); a thread has eight columns of every
+// Block (x, y): columns [256 y, + 256) of the x'th `group` rows; a thread has eight columns of every
 // eighth row.  body(row, column, sums) for each; then sums[s] over the rows go to
 // partial[x][s][pitch], in a fixed order.
 template <int SETS, typename F>
-__device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, float *partial, int64_t pitch, F &&body) {
+__device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, int group, float *partial, int64_t pitch,
+                                               F &&body) {
+  dependency_wait();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + tx) * 8, r0 = static_cast<int64_t>(blockIdx.x) * kSumRows;
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + tx) * 8, r0 = static_cast<int64_t>(blockIdx.x) * group;
   float sums[SETS][8] = {};
-  if (c < width)
-    for (int64_t r = r0 + ty; r < min(rows, r0 + kSumRows); r += 8) body(r, c, sums);
+  if (c < width) {
+    const int64_t end = min(rows, r0 + group);
+#pragma unroll 2
+    for (int64_t r = r0 + ty; r < end; r += 8) body(r, c, sums);
+  }
   if (!partial) return;
   __shared__ float all[8][32][9];
 #pragma unroll
@@ -145,9 +156,9 @@ __device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, floa
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t stride, int64_t rows, int64_t width,
+__global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t stride, int64_t rows, int64_t width, int group,
                                                          float *partial, int64_t pitch) {
-  for_row_groups<1>(rows, width, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
+  for_row_groups<1>(rows, width, group, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
     float x[8];
     load8<T>(src + r * stride + c, static_cast<int>(min(static_cast<int64_t>(8), width - c)), x);
 #pragma unroll
@@ -166,6 +177,7 @@ struct FinishArgs {
 template <typename T>
 __global__ void __launch_bounds__(1024) column_finish_kernel(const FinishArgs p) {
   __shared__ float all[32][33];
+  dependency_wait();
   T *dst = static_cast<T *>(p.dst[blockIdx.y]);
   if (!dst) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -214,9 +226,9 @@ __device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int
 // dz = dy act'(z), the slope saved, as an operand, with its column sums
 template <typename T>
 __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t dy_stride, const SavedPlanes saved,
-                                                          int64_t rows, int64_t width, void *dz, int64_t dz_pitch,
+                                                          int64_t rows, int64_t width, int group, void *dz, int64_t dz_pitch,
                                                           int64_t dz_piece, float *partial, int64_t pitch) {
-  for_row_groups<1>(rows, width, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
+  for_row_groups<1>(rows, width, group, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
     const int n = static_cast<int>(min(static_cast<int64_t>(8), width - c));
     float d[8], z[8];
     load8<T>(dy + r * dy_stride + c, n, d);
@@ -232,9 +244,9 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
 
 // f32: h = act(g) v as an operand, from the saved planes
 template <int ACT>
-__global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, int64_t rows, int64_t width, void *h,
+__global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, int64_t rows, int64_t width, int group, void *h,
                                                        int64_t h_pitch, int64_t h_piece) {
-  for_row_groups<1>(rows, width, nullptr, 0, [&](int64_t r, int64_t c, float (&)[1][8]) {
+  for_row_groups<1>(rows, width, group, nullptr, 0, [&](int64_t r, int64_t c, float (&)[1][8]) {
     float g[8], v[8];
     load_saved8<float>(saved, 0, r, c, g);
     load_saved8<float>(saved, 1, r, c, v);
@@ -251,10 +263,10 @@ __global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, 
 // f32: dg and dv as operands, `dgv_set` elements apart, from dh [rows][saved.pitch] and the saved planes
 template <int ACT>
 __global__ void __launch_bounds__(256) gate_backward_f32_kernel(const float *dh, const SavedPlanes saved, int64_t rows,
-                                                                int64_t width, uint16_t *dgv, int64_t dgv_pitch,
+                                                                int64_t width, int group, uint16_t *dgv, int64_t dgv_pitch,
                                                                 int64_t dgv_piece, int64_t dgv_set, float *partial,
                                                                 int64_t pitch) {
-  for_row_groups<2>(rows, width, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[2][8]) {
+  for_row_groups<2>(rows, width, group, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[2][8]) {
     float d[8], g[8], v[8];
     load8<float>(dh + r * saved.pitch + c, 8, d);
     load_saved8<float>(saved, 0, r, c, g);
@@ -321,9 +333,9 @@ class Pass {
       const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(jobs_.groups, 256), 16 * ctx_->sm_count));
       LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
       with_element(dtype_, [&](auto *tag) {
-        pack_kernel<std::remove_pointer_t<decltype(tag)>><<<blocks, 256, 0, stream_>>>(jobs_);
+        check(launch_early(pack_kernel<std::remove_pointer_t<decltype(tag)>>, dim3(blocks), 256, 0, stream_, jobs_),
+              "layer operand copies");
       });
-      check("layer operand copies");
     }
     jobs_ = PackArgs{};
   }
@@ -366,17 +378,19 @@ class Pass {
     return s;
   }
 
+  // launch(grid, rows of a block) for a kernel of for_row_groups
   template <typename F>
   void rows_kernel(int64_t rows, int64_t width, F &&launch) {
     if (!live()) return;
+    const int group = row_group(rows, width);
     LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
-    const dim3 grid(static_cast<unsigned>(ceil_div(rows, kSumRows)), static_cast<unsigned>(ceil_div(width, 256)));
-    launch(grid);
-    check("layer row pass");
+    const dim3 grid(static_cast<unsigned>(ceil_div(rows, group)), static_cast<unsigned>(ceil_div(width, 256)));
+    check(launch(grid, group), "layer row pass");
   }
-  // The column sums of a tensor, or of partial sums (`sets` sets of `chunks` rows).
+  // The column sums of a tensor: the blocks' sums, `sets` of them, and how many blocks there are.
+  static int64_t sum_chunks(int64_t rows, int64_t width) { return ceil_div(rows, row_group(rows, width)); }
   float *sum_room(int64_t rows, int64_t width, int sets) {
-    return reinterpret_cast<float *>(take(4ull * sets * ceil_div(rows, kSumRows) * saved_pitch(width)));
+    return reinterpret_cast<float *>(take(4ull * sets * sum_chunks(rows, width) * saved_pitch(width)));
   }
   void finish_sums(const float *partial, int64_t chunks, int64_t width, void *dst, int sets = 1,
                    void *second = nullptr) {
@@ -385,29 +399,31 @@ class Pass {
     LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
     const dim3 grid(static_cast<unsigned>(ceil_div(width, 32)), sets);
     with_element(dtype_, [&](auto *tag) {
-      column_finish_kernel<std::remove_pointer_t<decltype(tag)>><<<grid, 1024, 0, stream_>>>(f);
+      check(launch_early(column_finish_kernel<std::remove_pointer_t<decltype(tag)>>, grid, 1024, 0, stream_, f),
+            "layer column sums");
     });
-    check("layer column sums");
   }
   void column_sums(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst) {
     if (!dst) return;
     float *partial = sum_room(rows, width, 1);
-    rows_kernel(rows, width, [&](dim3 grid) {
+    rows_kernel(rows, width, [&](dim3 grid, int group) {
+      cudaError_t e = cudaSuccess;
       with_element(dtype_, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        column_sum_kernel<T><<<grid, 256, 0, stream_>>>(static_cast<const T *>(src), stride, rows, width, partial,
-                                                        saved_pitch(width));
+        e = launch_early(column_sum_kernel<T>, grid, 256, 0, stream_, static_cast<const T *>(src), stride, rows, width,
+                         group, partial, saved_pitch(width));
       });
+      return e;
     });
-    finish_sums(partial, ceil_div(rows, kSumRows), width, dst);
+    finish_sums(partial, sum_chunks(rows, width), width, dst);
   }
   void zero(void *ptr, size_t bytes) {
     if (!ptr || !live()) return;
     if (cudaError_t e = cudaMemsetAsync(ptr, 0, bytes, stream_); e != cudaSuccess)
       status = cuda_fail(ctx_, e, "zero a gradient");
   }
-  void check(const char *what) {
-    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess && status == AF2_OK) status = cuda_fail(ctx_, e, what);
+  void check(cudaError_t e, const char *what) {
+    if (e != cudaSuccess && status == AF2_OK) status = cuda_fail(ctx_, e, what);
   }
   cudaStream_t stream() const { return stream_; }
 
@@ -440,7 +456,7 @@ uint64_t gated_saved_bytes(int64_t rows, int64_t hidden, int dtype) {
 
 af2_status dense_forward(af2_ctx *ctx, const DenseForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
   Pass l(ctx, p.dtype, scratch, stream);
-  if (p.rows <= kFewRows && !(p.saved && p.activation != AF2_ACTIVATION_NONE)) {
+  if (few_rows(p.rows, p.inner, p.columns, p.dtype) && !(p.saved && p.activation != AF2_ACTIVATION_NONE)) {
     *bytes = 0;
     if (!ctx) return AF2_OK;
     FewRows f;
@@ -489,15 +505,17 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
     dz = l.make_operand(p.rows, p.columns);
     const SavedPlanes saved = l.planes(const_cast<void *>(p.saved), p.rows, p.columns, 1);
     float *partial = p.d_bias ? l.sum_room(p.rows, p.columns, 1) : nullptr;
-    l.rows_kernel(p.rows, p.columns, [&](dim3 grid) {
+    l.rows_kernel(p.rows, p.columns, [&](dim3 grid, int group) {
+      cudaError_t e = cudaSuccess;
       with_element(p.dtype, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        dense_slope_kernel<T><<<grid, 256, 0, stream>>>(static_cast<const T *>(p.d_out), p.d_out_stride, saved, p.rows,
-                                                        p.columns, const_cast<void *>(dz.ptr), dz.pitch,
-                                                        dz.piece_stride, partial, saved_pitch(p.columns));
+        e = launch_early(dense_slope_kernel<T>, grid, 256, 0, stream, static_cast<const T *>(p.d_out), p.d_out_stride,
+                         saved, p.rows, p.columns, group, const_cast<void *>(dz.ptr), dz.pitch, dz.piece_stride,
+                         partial, saved_pitch(p.columns));
       });
+      return e;
     });
-    l.finish_sums(partial, ceil_div(p.rows, kSumRows), p.columns, p.d_bias);
+    l.finish_sums(partial, Pass::sum_chunks(p.rows, p.columns), p.columns, p.d_bias);
   }
   if (p.d_x) {
     LayerGemm g = l.product(p.rows, p.inner, p.columns);
@@ -521,7 +539,7 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
 
 af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
   Pass l(ctx, p.dtype, scratch, stream);
-  if (p.rows <= kFewRows && !p.saved) {
+  if (few_rows(p.rows, p.channels, p.hidden, p.dtype) && !p.saved) {
     void *h = l.take(element_size(p.dtype) * p.rows * p.hidden);
     *bytes = l.total();
     if (!ctx) return AF2_OK;
@@ -572,11 +590,13 @@ af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uin
     g.out[1] = s.f32 + s.stride;
     g.out_stride = s.pitch;
     l.run(g);
-    l.rows_kernel(p.rows, p.hidden, [&](dim3 grid) {
+    l.rows_kernel(p.rows, p.hidden, [&](dim3 grid, int group) {
+      cudaError_t e = cudaSuccess;
       with_activation(p.activation, [&](auto act) {
-        gate_f32_kernel<decltype(act)::value><<<grid, 256, 0, stream>>>(s, p.rows, p.hidden, const_cast<void *>(h.ptr),
-                                                                        h.pitch, h.piece_stride);
+        e = launch_early(gate_f32_kernel<decltype(act)::value>, grid, 256, 0, stream, s, p.rows, p.hidden, group,
+                         const_cast<void *>(h.ptr), h.pitch, h.piece_stride);
       });
+      return e;
     });
   } else {
     g.epilogue = kEpilogueGate;
@@ -638,20 +658,22 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     float *partial = nullptr;
     int64_t chunks = 0;
     if (l.f32()) {
-      chunks = ceil_div(p.rows, kSumRows);
+      chunks = Pass::sum_chunks(p.rows, hid);
       if (sums) partial = l.sum_room(p.rows, hid, 2);
       float *dh = reinterpret_cast<float *>(l.take(4ull * p.rows * saved.pitch));
       g.out[0] = dh;
       g.out_stride = saved.pitch;
       l.run(g);
-      l.rows_kernel(p.rows, hid, [&](dim3 grid) {
+      l.rows_kernel(p.rows, hid, [&](dim3 grid, int group) {
+        cudaError_t e = cudaSuccess;
         with_activation(p.activation, [&](auto act) {
-          gate_backward_f32_kernel<decltype(act)::value><<<grid, 256, 0, stream>>>(
-              dh, saved, p.rows, hid, static_cast<uint16_t *>(const_cast<void *>(dgv[0].ptr)), dgv[0].pitch,
-              dgv[0].piece_stride,
-              static_cast<const uint16_t *>(dgv[1].ptr) - static_cast<const uint16_t *>(dgv[0].ptr), partial,
-              saved.pitch);
+          e = launch_early(gate_backward_f32_kernel<decltype(act)::value>, grid, 256, 0, stream, dh, saved, p.rows,
+                           hid, group, static_cast<uint16_t *>(const_cast<void *>(dgv[0].ptr)), dgv[0].pitch,
+                           dgv[0].piece_stride,
+                           static_cast<const uint16_t *>(dgv[1].ptr) - static_cast<const uint16_t *>(dgv[0].ptr),
+                           partial, saved.pitch);
         });
+        return e;
       });
     } else {
       chunks = ceil_div(p.rows, 32);

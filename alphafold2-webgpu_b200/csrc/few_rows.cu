@@ -1,10 +1,11 @@
-// few_rows.cu -- y = act(x W + b) (+ r), or act(x Wg + bg) (x Wv + bv), for up
-// to eight rows: one token, or one position of a small batch.
+// few_rows.cu -- y = act(x W + b) (+ r), or act(x Wg + bg) (x Wv + bv), for a
+// few rows: one token, or one position of a small batch.
 //
-// Each weight is read once and used for all rows, so the read bounds it: 25 MB
-// of a 1024 -> 4096 -> 1024 transition take 3.9 us at the copy rate.  A block
+// Each weight is read once for four rows, so the read bounds it: 25 MB of a
+// 1024 -> 4096 -> 1024 transition take 3.9 us at the copy rate.  More rows are
+// further groups of four beside the first, whose reads find the weights in L2.  A block
 // has 32 columns and sixteen warps over the depth; a lane reads 16 bytes of a
-// weight row and keeps eight such reads in flight.  With few columns a cluster
+// weight row and keeps several such reads in flight.  With few columns a cluster
 // of blocks shares the depth and adds up through distributed shared memory, in
 // rank order.  The launch that follows another (the transition's second
 // product) reads its first weights before it waits for the one before it.
@@ -48,14 +49,17 @@ struct Piece {
   }
 };
 
-// R rows (those past p.rows are zero in x), V weights per read; GATE: warps 0-7 have the gate, 8-15 the value.
-// Registers bound the reads in flight: eight a lane, four beside the sums of eight rows.
-template <typename T, int V, int R, bool GATE>
-__global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const Args p) {
-  constexpr int FLIGHT = R <= 4 ? 8 : 4;
+// A group of R rows per blockIdx.y (those past p.rows are zero in x), V weights per read; GATE: warps 0-7 have the gate, 8-15 the value.
+// Two blocks fit an SM, so the second product's blocks stand ready, their reads issued, while the
+// first's still run; that leaves a lane 64 registers: eight reads in flight, or four beside four rows'
+// sums.  DEEP: one block, and eight reads with four rows too, which large weights need more (four rows
+// of 512 -> 2048 -> 512: two blocks 9.9 us, one 13.2; of 1024 -> 4096 -> 1024: 19.3 and 13.4).
+template <typename T, int V, int R, bool GATE, bool DEEP>
+__global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) few_rows_kernel(const Args p) {
+  constexpr int FLIGHT = R <= 2 || DEEP ? 8 : 4;
   constexpr int SETS = GATE ? 2 : 1, SET_WARPS = WARPS / SETS;
   constexpr int LANES = COLS / V;  // lanes on one weight row
-  constexpr int DEEP = 32 / LANES; // weight rows of one read of a warp (= V)
+  constexpr int DEPTH = 32 / LANES;  // weight rows of one read of a warp (= V)
   __shared__ float work[CHUNK * R];  // x, then the warps' sums
   __shared__ float total[SETS * R * COLS];
   __shared__ float others[7 * SETS * R * COLS];  // the cluster's other blocks' sums, in rank 0's memory
@@ -64,6 +68,7 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
   using P = Piece<T, V>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = p.splits > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int row0 = static_cast<int>(blockIdx.y) * R, rows = min(R, p.rows - row0);
   const int c_block = static_cast<int>(blockIdx.x) / p.splits * COLS;
   const int k0 = static_cast<int>(static_cast<int64_t>(p.inner) * rank / p.splits);
   const int k1 = static_cast<int>(static_cast<int64_t>(p.inner) * (rank + 1) / p.splits);
@@ -71,8 +76,8 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
   const int col = c_block + (lane % LANES) * V;
   const bool in = col < p.columns;  // V > 1: the columns are a multiple of V
   const T *weight = static_cast<const T *>(set ? p.weight[1] : p.weight[0]) + col;
-  const int first = k0 + w * DEEP + lane / LANES;
-  constexpr int STEP = SET_WARPS * DEEP;  // from one read of a lane to its next
+  const int first = k0 + w * DEPTH + lane / LANES;
+  constexpr int STEP = SET_WARPS * DEPTH;  // from one read of a lane to its next
 
   typename P::Word buf[FLIGHT];
   auto fetch = [&](int k, int end) {
@@ -81,19 +86,24 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
       if (in && k + i * STEP < end) buf[i] = P::load(weight + static_cast<int64_t>(k + i * STEP) * p.columns);
   };
   // chunks are CHUNK deep and the first read of each warp starts at its own place in the chunk
-  fetch(first, min(k1, k0 + CHUNK));
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (p.follows) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.follows) {
+    // the launch before this one writes no weight, and waited itself for those before it
+    fetch(first, min(k1, k0 + CHUNK));
+    dependency_wait();
+  } else {
+    dependency_wait();
+    fetch(first, min(k1, k0 + CHUNK));
+  }
 
   float acc[R][V] = {};
-  const T *x = static_cast<const T *>(p.x);
+  const T *x = static_cast<const T *>(p.x) + static_cast<int64_t>(row0) * p.x_stride;
   for (int c0 = k0; c0 < k1; c0 += CHUNK) {
     const int end = min(k1, c0 + CHUNK);
     if (c0 != k0) __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r)
       for (int k = threadIdx.x; k < end - c0; k += THREADS)
-        xs[k * R + r] = r < p.rows ? to_f32<T>(x[r * p.x_stride + c0 + k]) : 0.f;
+        xs[k * R + r] = r < rows ? to_f32<T>(x[r * p.x_stride + c0 + k]) : 0.f;
     __syncthreads();
     for (int k = first + (c0 - k0); k < end; k += FLIGHT * STEP) {
       if (k != first) fetch(k, end);
@@ -158,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
   __syncthreads();
   for (int i = threadIdx.x; i < R * COLS; i += THREADS) {
     const int r = i / COLS, c = c_block + (i - r * COLS);
-    if (r >= p.rows || c >= p.columns) continue;
+    if (r >= rows || c >= p.columns) continue;
     float y = total[i];
     if (p.bias[0]) y += to_f32<T>(static_cast<const T *>(p.bias[0])[c]);
     with_activation(p.activation, [&](auto act) { y = activate2<decltype(act)::value, sizeof(T) == 2>(f2(y)).x; });
@@ -167,15 +177,16 @@ __global__ void __launch_bounds__(THREADS, R <= 2 ? 2 : 1) few_rows_kernel(const
       if (p.bias[1]) v += to_f32<T>(static_cast<const T *>(p.bias[1])[c]);
       y *= v;
     }
-    if (p.residual) y += to_f32<T>(static_cast<const T *>(p.residual)[r * p.residual_stride + c]);
-    static_cast<T *>(p.out)[r * p.out_stride + c] = from_f32<T>(y);
+    const int64_t row = row0 + r;
+    if (p.residual) y += to_f32<T>(static_cast<const T *>(p.residual)[row * p.residual_stride + c]);
+    static_cast<T *>(p.out)[row * p.out_stride + c] = from_f32<T>(y);
   }
 }
 
-template <typename T, int V, int R, bool GATE>
+template <typename T, int V, int R, bool GATE, bool DEEP = false>
 cudaError_t launch(const Args &p, int blocks, cudaStream_t stream) {
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(blocks * p.splits));
+  config.gridDim = dim3(static_cast<unsigned>(blocks * p.splits), static_cast<unsigned>((p.rows + R - 1) / R));
   config.blockDim = dim3(THREADS);
   config.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -184,16 +195,16 @@ cudaError_t launch(const Args &p, int blocks, cudaStream_t stream) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attr;
-  config.numAttrs = p.follows ? 2 : 1;
-  return cudaLaunchKernelEx(&config, few_rows_kernel<T, V, R, GATE>, p);
+  config.numAttrs = 2;
+  return cudaLaunchKernelEx(&config, few_rows_kernel<T, V, R, GATE, DEEP>, p);
 }
 
 template <typename T, int V, bool GATE>
 cudaError_t launch_rows(const Args &p, int blocks, cudaStream_t stream) {
   if (p.rows == 1) return launch<T, V, 1, GATE>(p, blocks, stream);
   if (p.rows == 2) return launch<T, V, 2, GATE>(p, blocks, stream);
-  if (p.rows <= 4) return launch<T, V, 4, GATE>(p, blocks, stream);
-  return launch<T, V, 8, GATE>(p, blocks, stream);
+  if (static_cast<int64_t>(p.inner) * p.columns >= 1 << 21) return launch<T, V, 4, GATE, true>(p, blocks, stream);
+  return launch<T, V, 4, GATE>(p, blocks, stream);
 }
 
 }  // namespace
@@ -205,7 +216,8 @@ af2_status few_rows_launch(af2_ctx *ctx, const FewRows &f, cudaStream_t stream) 
          f.follows};
   const int blocks = (p.columns + COLS - 1) / COLS;
   // the depth over more blocks while the SMs are not all busy and each keeps 128 weight rows
-  while (p.splits < 8 && blocks * p.splits * 2 <= ctx->sm_count && p.inner / (p.splits * 2) >= 128) p.splits *= 2;
+  const int groups = static_cast<int>((f.rows + 3) / 4);
+  while (p.splits < 8 && blocks * groups * p.splits * 2 <= ctx->sm_count && p.inner / (p.splits * 2) >= 128) p.splits *= 2;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
   cudaError_t e = cudaSuccess;
   with_element(f.dtype, [&](auto *tag) {

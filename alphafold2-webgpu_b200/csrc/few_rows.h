@@ -5,9 +5,14 @@
 
 namespace af2 {
 
-// Up to this many rows the layers are bound by the read of the weights and by latency, and the
-// CUDA-core kernel is used.
-constexpr int kFewRows = 8;
+// Whether a product is small enough for the CUDA-core kernel, which starts and ends sooner than the
+// tensor-core one and reads f32 as it is.  Measured on whole transitions, us (few rows | tensor cores):
+// bf16, 512 -> 2048: 8 rows 9.8 | 15, 16 rows 15.0 | 15.1; 1024 -> 4096: 4 rows 13 | 20, 8 rows 25 | 20;
+// f32, 512 -> 2048: 48 rows 39.1 | 39.0; 1024 -> 4096: 16 rows 46 | 80, 24 rows 70 | 72.
+inline bool few_rows(int64_t rows, int64_t inner, int64_t columns, int dtype) {
+  const int64_t most = dtype == AF2_F32 ? 3 << 24 : 1 << 24;  // products of two elements
+  return rows <= 256 && rows * inner * columns <= most;
+}
 
 struct FewRows {
   int64_t rows = 0, inner = 0, columns = 0;

@@ -234,6 +234,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   cluster_sync_all();  // both CTAs' barriers exist before any arrival crosses the pair
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  dependency_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -697,6 +698,7 @@ struct ReduceArgs {
 
 template <typename OT>
 __global__ void __launch_bounds__(256) reduce_kernel(const ReduceArgs p) {
+  dependency_wait();
   const int64_t quads = p.pitch / 4, total = p.batch * p.m * quads;
   const int64_t split_stride = p.batch * p.m * quads;  // float4s
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
@@ -769,8 +771,8 @@ af2_status launch(af2_ctx *ctx, const Maps &maps, Args p, cudaStream_t stream) {
   const int pairs = std::min(p.total_tiles, std::max(1, ctx->sm_count / 2));
   p.alternate = p.total_tiles > pairs;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
-  kernel<<<2 * pairs, THREADS, smem, stream>>>(maps, p);
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cuda_fail(ctx, e, "layer product");
+  if (cudaError_t e = launch_early(kernel, dim3(2 * pairs), THREADS, smem, stream, maps, p); e != cudaSuccess)
+    return cuda_fail(ctx, e, "layer product");
   return AF2_OK;
 }
 
@@ -926,11 +928,11 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
   r.saved_pitch = g.saved.pitch;
   const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(g.batch * g.m * pitch / 4, 256), 8 * ctx->sm_count));
   LaunchScope scope(ctx, stream, kProfLayerElementwise);
+  cudaError_t e = cudaSuccess;
   with_element(g.out_dtype, [&](auto *tag) {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    reduce_kernel<T><<<blocks, 256, 0, stream>>>(r);
+    e = launch_early(reduce_kernel<std::remove_pointer_t<decltype(tag)>>, dim3(blocks), 256, 0, stream, r);
   });
-  if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return cuda_fail(ctx, e, "layer split sums");
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "layer split sums");
   return AF2_OK;
 }
 
