@@ -21,7 +21,11 @@
 // f32 tensors are multiplied as three bf16 terms each, x = x0 + x1 + x2, and
 // the six products whose weight is at least 2^-16 of the largest are summed,
 // the small ones first: what is left out is below 2^-24 of |x||y|, f32's own
-// rounding.  (An infinite f32 element makes its sums NaN or infinite.)
+// rounding.  The tensor core cuts its sums where f32 rounds them (some 2^-27
+// of the sum lost at each step of 16: sums of one sign over a depth of 4096 came
+// out 2e-6 low), so an f32 tile is summed over 256 of the depth at a time and
+// these sums are added in registers.  (An infinite f32 element makes its sums
+// NaN or infinite.)
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -116,6 +120,8 @@ __device__ __forceinline__ Tile tile_at(const Args &p, int t) {
   r.split = t;
   return r;
 }
+constexpr int kPromote = 4;  // K steps of an f32 tile before its sums go to registers
+
 // The tile's range of K steps.
 __device__ __forceinline__ int k_begin(const Args &p, int split) {
   return static_cast<int>(static_cast<int64_t>(p.k_blocks) * split / p.splits);
@@ -249,35 +255,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int kb1 = p.splits > 1 ? k_begin(p, tile.split + 1) : p.k_blocks;
         const int arow = tile.mi * PAIR_M + rank * BM;
         const int brow = GATE ? tile.ni * (BN / 2) : tile.ni * BN + rank * (BN / 2);
-        for (int c = 0; c < p.combos && ok; ++c) {
-          const int ta = p.combos > 1 ? kTermA[c] : 0, tb = p.combos > 1 ? kTermB[c] : 0;
-          for (int seg = 0; seg < p.segments && ok; ++seg) {
-            const CUtensorMap *am = &maps.a[seg];
-            const CUtensorMap *bm = &maps.b[GATE ? rank : seg + tile.z];
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-              // the stage is free in this CTA once the pair's MMAs have read it (multicast commit)
-              if (!mbar_wait(empty(s), ph, abort_flag, p.err, kErrWaitProducer)) {
-                ok = false;
-                break;
-              }
-              const uint32_t dst = sbase + s * S::STAGE_BYTES;
-              if (leader) mbar_arrive_expect_tx(full(s), 2 * S::STAGE_BYTES);
-              if (p.a_mn) {
-                tma_load_3d_pair(dst, am, full(s), arow, kb * BK, ta);
-                tma_load_3d_pair(dst + 8192, am, full(s), arow + 64, kb * BK, ta);
-              } else {
-                tma_load_3d_pair(dst, am, full(s), kb * BK, arow, ta);
-              }
-              if (p.b_mn) {
+        const int part = p.combos > 1 ? kPromote : kb1 - kb0;
+        for (int from = kb0; from < kb1 && ok; from += part) {
+          for (int c = 0; c < p.combos && ok; ++c) {
+            const int ta = p.combos > 1 ? kTermA[c] : 0, tb = p.combos > 1 ? kTermB[c] : 0;
+            for (int seg = 0; seg < p.segments && ok; ++seg) {
+              const CUtensorMap *am = &maps.a[seg];
+              const CUtensorMap *bm = &maps.b[GATE ? rank : seg + tile.z];
+              for (int kb = from; kb < min(from + part, kb1); ++kb, ++it) {
+                // the stage is free in this CTA once the pair's MMAs have read it (multicast commit)
+                if (!mbar_wait(empty(s), ph, abort_flag, p.err, kErrWaitProducer)) {
+                  ok = false;
+                  break;
+                }
+                const uint32_t dst = sbase + s * S::STAGE_BYTES;
+                if (leader) mbar_arrive_expect_tx(full(s), 2 * S::STAGE_BYTES);
+                if (p.a_mn) {
+                  tma_load_3d_pair(dst, am, full(s), arow, kb * BK, ta);
+                  tma_load_3d_pair(dst + 8192, am, full(s), arow + 64, kb * BK, ta);
+                } else {
+                  tma_load_3d_pair(dst, am, full(s), kb * BK, arow, ta);
+                }
+                if (p.b_mn) {
 #pragma unroll
-                for (int j = 0; j < BN / 128; ++j)
-                  tma_load_3d_pair(dst + A_BYTES + j * 8192, bm, full(s), brow + 64 * j, kb * BK, tb);
-              } else {
-                tma_load_3d_pair(dst + A_BYTES, bm, full(s), kb * BK, brow, tb);
-              }
-              if (++s == STAGES) {
-                s = 0;
-                ph ^= 1;
+                  for (int j = 0; j < BN / 128; ++j)
+                    tma_load_3d_pair(dst + A_BYTES + j * 8192, bm, full(s), brow + 64 * j, kb * BK, tb);
+                } else {
+                  tma_load_3d_pair(dst + A_BYTES, bm, full(s), kb * BK, brow, tb);
+                }
+                if (++s == STAGES) {
+                  s = 0;
+                  ph ^= 1;
+                }
               }
             }
           }
@@ -308,33 +317,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const int split = tile_at(p, t).split;
           steps = k_begin(p, split + 1) - k_begin(p, split);
         }
-        const int iters = steps * p.segments * p.combos;
-        if (!warp_wait(acc_empty(buf), bph ^ 1, abort_flag, p.err, kErrWaitMma)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + buf * 256;
-        for (int i = 0; i < iters; ++i) {
-          if (!warp_wait(full(s), ph, abort_flag, p.err, kErrWaitMma)) {
+        const int part = p.combos > 1 ? kPromote : steps;
+        for (int from = 0; from < steps && ok; from += part) {
+          const int iters = min(part, steps - from) * p.segments * p.combos;
+          if (!warp_wait(acc_empty(buf), bph ^ 1, abort_flag, p.err, kErrWaitMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
+          const uint32_t d = tmem + buf * 256;
+          for (int i = 0; i < iters; ++i) {
+            if (!warp_wait(full(s), ph, abort_flag, p.err, kErrWaitMma)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < BK / 16; ++ks)
-            umma_pair(d, ad + ks * a_step, bd + ks * b_step, idesc, (i | ks) != 0);
-          umma_commit_pair_both(empty(s));
-          ad += S::STAGE_BYTES >> 4;
-          bd += S::STAGE_BYTES >> 4;
-          if (++s == STAGES) {
-            s = 0;
-            ph ^= 1;
-            ad = a_base;
-            bd = b_base;
+            for (int ks = 0; ks < BK / 16; ++ks)
+              umma_pair(d, ad + ks * a_step, bd + ks * b_step, idesc, (i | ks) != 0);
+            umma_commit_pair_both(empty(s));
+            ad += S::STAGE_BYTES >> 4;
+            bd += S::STAGE_BYTES >> 4;
+            if (++s == STAGES) {
+              s = 0;
+              ph ^= 1;
+              ad = a_base;
+              bd = b_base;
+            }
           }
+          if (!ok) break;
+          umma_commit_pair_both(acc_full(buf));
+          buf ^= 1;
+          if (buf == 0) bph ^= 1;
         }
-        if (!ok) break;
-        umma_commit_pair_both(acc_full(buf));
-        buf ^= 1;
-        if (buf == 0) bph ^= 1;
       }
       // Every MMA has completed before TMEM is freed, whether or not a consumer gave up.
       umma_commit_pair(drain);
@@ -348,19 +363,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     constexpr int WIDTH = GATE ? BN / 2 : BN;  // output columns of a tile
     uint8_t *const block = smem + S::OFF_STAGE + ew * S::SLOT_BYTES;
     const uint32_t block_addr = sbase + S::OFF_STAGE + ew * S::SLOT_BYTES;
-    int tile_it = 0, stores = 0, loads = 0;  // stores, loads: through the two blocks in turn
-    for (int t = pair; t < p.total_tiles; t += npairs, ++tile_it) {
-      const int buf = tile_it & 1;
-      if (p.alternate && buf != group) continue;
+    int acc_it = 0, stores = 0, loads = 0;  // stores, loads: through the two blocks in turn
+    for (int t = pair; t < p.total_tiles; t += npairs, ++acc_it) {
+      if (p.alternate && (acc_it & 1) != group) continue;
       const Tile tile = tile_at(p, t);
       const int r0 = tile.mi * PAIR_M + rank * BM + q * 32;  // the warp's first row
       const int64_t m = static_cast<int64_t>(r0) + lane;
       const int n0 = tile.ni * WIDTH;
       // this warp's blocks of the tile: first, first + step, ... below `end`
       const int end = r0 < p.m ? min(WIDTH / 32, (p.n - n0 + 31) >> 5) : 0;
-      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
-      const uint32_t acc_phase = (tile_it >> 1) & 1;
       bool ok = true;
+      // f32: all but the last part of the depth, into registers (each warp has one block: BN is 128)
+      [[maybe_unused]] float sums[32];
+      if constexpr (KIND == kOut && sizeof(OT) == 4) {
+        if (p.combos > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sums[i] = 0.f;
+          int steps = p.k_blocks;
+          if (p.splits > 1) steps = k_begin(p, tile.split + 1) - k_begin(p, tile.split);
+          for (int from = kPromote; from < steps; from += kPromote, ++acc_it) {
+            const int buf = acc_it & 1;
+            ok = warp_wait(acc_full(buf), (acc_it >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
+            if (!ok) break;
+            tc_fence_after();
+            if (first < end) {
+              uint32_t r[32];
+              tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256 + first * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sums[i] += __uint_as_float(r[i]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_leader_relaxed(acc_empty(buf));
+          }
+          if (!ok) break;
+        }
+      }
+      const int buf = acc_it & 1;
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
+      const uint32_t acc_phase = (acc_it >> 1) & 1;
 
       if constexpr (KIND == kGateBackward) {
         // dg = dh p and dv = dh a with the saved factors p = v act'(g) and a = act(g).  A block's
@@ -538,6 +580,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
           } else {
             tmem_ld_wait();
+            if (p.combos > 1) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] += sums[i];
+            }
             if (bias) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) y[i] += i < cols ? bias[c0 + i] : 0.f;
@@ -769,7 +815,7 @@ af2_status launch(af2_ctx *ctx, const Maps &maps, Args p, cudaStream_t stream) {
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const int pairs = std::min(p.total_tiles, std::max(1, ctx->sm_count / 2));
-  p.alternate = p.total_tiles > pairs;
+  p.alternate = p.total_tiles > pairs && p.combos == 1;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
   if (cudaError_t e = launch_early(kernel, dim3(2 * pairs), THREADS, smem, stream, maps, p); e != cudaSuccess)
     return cuda_fail(ctx, e, "layer product");
@@ -805,6 +851,7 @@ void layer_gemm_plan(LayerGemm *g) {
   const bool gate = g->epilogue == kEpilogueGate;
   for (int bn : {256, 128}) {
     if (g->epilogue == kEpilogueGateBackward && bn == 128) continue;
+    if (g->pieces > 1 && bn == 256) continue;
     const int64_t tiles = g->batch * ceil_div(g->m, PAIR_M) * ceil_div(g->n, gate ? bn / 2 : bn);
     for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
       if (s > 1 && (g->epilogue != kEpilogueOut || s * 4 > k_blocks || tiles * (s - 1) >= 2 * kPairs)) break;
