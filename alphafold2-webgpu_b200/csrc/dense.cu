@@ -354,11 +354,14 @@ class Pass {
     o.mn_major = true;
     return o;
   }
-  void run(LayerGemm g) {
+  void run(LayerGemm g) { run(&g, 1); }
+  // Independent products in one launch: their tiles fill the SMs together.
+  void run(LayerGemm *g, int count) {
+    if (count == 0) return;
     const uint64_t mark = used;
-    layer_gemm_plan(&g);
-    g.scratch = take(g.scratch_bytes);
-    if (live()) status = layer_gemm_launch(ctx_, g, stream_);
+    layer_gemm_plan(g, count);
+    for (int i = 0; i < count; ++i) g[i].scratch = take(g[i].scratch_bytes);
+    if (live()) status = layer_gemm_launch(ctx_, g, count, stream_);
     peak_ = std::max(peak_, used);
     used = mark;  // launches follow one another on the stream: the next may use the same place
   }
@@ -517,22 +520,23 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
     });
     l.finish_sums(partial, Pass::sum_chunks(p.rows, p.columns), p.columns, p.d_bias);
   }
+  LayerGemm products[2];
+  int count = 0;
   if (p.d_x) {
-    LayerGemm g = l.product(p.rows, p.inner, p.columns);
+    LayerGemm &g = products[count++] = l.product(p.rows, p.inner, p.columns);
     g.a[0] = dz;
     g.b[0] = w;
     g.out[0] = p.d_x;
     g.out_stride = p.d_x_stride;
-    l.run(g);
   }
   if (p.d_weight) {
-    LayerGemm g = l.product(p.inner, p.columns, p.rows);
+    LayerGemm &g = products[count++] = l.product(p.inner, p.columns, p.rows);
     g.a[0] = Pass::mn(x);
     g.b[0] = Pass::mn(dz);
     g.out[0] = p.d_weight;
     g.out_stride = p.columns;
-    l.run(g);
   }
+  l.run(products, count);
   *bytes = l.total();
   return l.status;
 }
@@ -689,8 +693,10 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     }
     l.finish_sums(partial, chunks, hid, p.g.gate_bias, 2, p.g.value_bias);
   }
+  LayerGemm products[3];
+  int count = 0;
   if (p.g.x) {
-    LayerGemm g = l.product(p.rows, c, hid);
+    LayerGemm &g = products[count++] = l.product(p.rows, c, hid);
     g.segments = 2;
     g.a[0] = dgv[0];
     g.a[1] = dgv[1];
@@ -698,26 +704,24 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     g.b[1] = wv;
     g.out[0] = p.g.x;
     g.out_stride = p.d_x_stride;
-    l.run(g);
   }
   if (p.g.gate_weight || p.g.value_weight) {
-    LayerGemm g = l.product(c, hid, p.rows);
+    LayerGemm &g = products[count++] = l.product(c, hid, p.rows);
     g.a[0] = Pass::mn(x);
     int n = 0;
     if (p.g.gate_weight) g.b[n] = Pass::mn(dgv[0]), g.out[n++] = p.g.gate_weight;
     if (p.g.value_weight) g.b[n] = Pass::mn(dgv[1]), g.out[n++] = p.g.value_weight;
     g.batch = n;
     g.out_stride = hid;
-    l.run(g);
   }
   if (p.g.output_weight) {
-    LayerGemm g = l.product(hid, c, p.rows);
+    LayerGemm &g = products[count++] = l.product(hid, c, p.rows);
     g.a[0] = Pass::mn(h);
     g.b[0] = Pass::mn(dy);
     g.out[0] = p.g.output_weight;
     g.out_stride = c;
-    l.run(g);
   }
+  l.run(products, count);
   *bytes = l.total();
   return l.status;
 }

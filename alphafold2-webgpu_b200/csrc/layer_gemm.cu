@@ -42,8 +42,10 @@ constexpr int EPI_WARPS = 16, THREADS = 64 + 32 * EPI_WARPS;
 constexpr uint32_t A_BYTES = BM * 128;
 constexpr int kPairs = 74;  // CTA pairs of a B200; only the choice of tiles and splits depends on it
 
-// The kernels behind the epilogues: Gate with and without what the backward pass needs.
-enum Kind { kOut, kGate, kGateSave, kGateBackward };
+// The kernels behind the epilogues: Out, the same for several products with nothing but their sums
+// (whose arguments are no longer operands from the constant bank but loads), and Gate with and
+// without what the backward pass needs.
+enum Kind { kOut, kProducts, kGate, kGateSave, kGateBackward };
 
 // Stages of the operand ring and bytes of one epilogue warp's staging: 32 x 32 blocks of 16 bits
 // (2 KB), two of them (GateBackward: one of each factor); three where h and two factors leave
@@ -94,16 +96,34 @@ struct Args {
   int64_t m;
   int n, k_blocks, splits, combos, segments;
   Divisor tiles_m, tiles_n, batches;
-  int total_tiles;
   int a_mn, b_mn, bf16, activation;
   int tma_out;       // out rows are 16-byte aligned: whole blocks leave by TMA
   int tma_residual;  // the residual's blocks come by TMA
   int vector_bias;   // 16-byte aligned
   int save;          // Out: the slopes are kept
-  int alternate;     // the two groups of epilogue warps take tiles in turn
-  int partial;     // out[0] is [split][batch][m][n] of f32 sums (no bias, activation or residual)
+  int partial;       // out[0] is [split][batch][m][n] of f32 sums (no bias, activation or residual)
+  int first_tile;    // the tiles of the products before this one
+};
+
+// What a launch computes: up to three products, whose tiles follow one another.
+struct Product {
+  Maps maps;
+  Args args;
+};
+template <int N>
+struct Launch {
+  Product product[N];
+  int products, total_tiles;
+  int alternate;  // the two groups of epilogue warps take tiles in turn
   unsigned int *err;
 };
+template <int N>
+__device__ __forceinline__ const Product &product_of(const Launch<N> &l, int t) {
+  int i = 0;
+  if constexpr (N > 1)
+    while (i + 1 < l.products && t >= l.product[i + 1].args.first_tile) ++i;
+  return l.product[i];
+}
 
 // The terms (of A, of B) of the six products of an f32 operand pair, small ones first.
 __constant__ const int8_t kTermA[6] = {2, 0, 1, 1, 0, 0};
@@ -114,6 +134,7 @@ struct Tile {
 };
 __device__ __forceinline__ Tile tile_at(const Args &p, int t) {
   Tile r;
+  t -= p.first_tile;
   r.ni = p.tiles_n.split(t);
   r.mi = p.tiles_m.split(t);
   r.z = p.batches.split(t);
@@ -193,7 +214,7 @@ __device__ __forceinline__ float lane_sums(float (&x)[32], int lane) {
 
 template <int KIND, typename OT, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-    layer_gemm_kernel(const __grid_constant__ Maps maps, const Args p) {
+    layer_gemm_kernel(const __grid_constant__ Launch<KIND == kProducts ? kMaxProducts : 1> launch) {
   using S = Shape<KIND, BN>;
   constexpr bool GATE = KIND == kGate || KIND == kGateSave;
   constexpr int STAGES = S::STAGES;
@@ -224,7 +245,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), p.alternate ? EPI_WARPS : 2 * EPI_WARPS);  // both CTAs' warps on a tile
+      mbar_init(acc_empty(b), launch.alternate ? EPI_WARPS : 2 * EPI_WARPS);  // both CTAs' warps on a tile
     }
     mbar_init(drain, 1);
     for (int w = 0; w < EPI_WARPS; ++w)
@@ -244,39 +265,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_map(&maps.a[0]);
-      tma_prefetch_map(&maps.b[0]);
+      tma_prefetch_map(&launch.product[0].maps.a[0]);
+      tma_prefetch_map(&launch.product[0].maps.b[0]);
       int it = 0, s = 0;
       uint32_t ph = 1;
       bool ok = true;
-      for (int t = pair; t < p.total_tiles && ok; t += npairs) {
+      for (int t = pair; t < launch.total_tiles && ok; t += npairs) {
+        const Product &product = product_of(launch, t);
+        const Maps &maps = product.maps;
+        const Args &p = product.args;
         const Tile tile = tile_at(p, t);
         const int kb0 = p.splits > 1 ? k_begin(p, tile.split) : 0;
         const int kb1 = p.splits > 1 ? k_begin(p, tile.split + 1) : p.k_blocks;
         const int arow = tile.mi * PAIR_M + rank * BM;
         const int brow = GATE ? tile.ni * (BN / 2) : tile.ni * BN + rank * (BN / 2);
-        const int part = p.combos > 1 ? kPromote : kb1 - kb0;
+        const int combos = p.combos, segments = p.segments, a_mn = p.a_mn, b_mn = p.b_mn;
+        const int part = combos > 1 ? kPromote : kb1 - kb0;
         for (int from = kb0; from < kb1 && ok; from += part) {
-          for (int c = 0; c < p.combos && ok; ++c) {
-            const int ta = p.combos > 1 ? kTermA[c] : 0, tb = p.combos > 1 ? kTermB[c] : 0;
-            for (int seg = 0; seg < p.segments && ok; ++seg) {
+          for (int c = 0; c < combos && ok; ++c) {
+            const int ta = combos > 1 ? kTermA[c] : 0, tb = combos > 1 ? kTermB[c] : 0;
+            for (int seg = 0; seg < segments && ok; ++seg) {
               const CUtensorMap *am = &maps.a[seg];
               const CUtensorMap *bm = &maps.b[GATE ? rank : seg + tile.z];
               for (int kb = from; kb < min(from + part, kb1); ++kb, ++it) {
                 // the stage is free in this CTA once the pair's MMAs have read it (multicast commit)
-                if (!mbar_wait(empty(s), ph, abort_flag, p.err, kErrWaitProducer)) {
+                if (!mbar_wait(empty(s), ph, abort_flag, launch.err, kErrWaitProducer)) {
                   ok = false;
                   break;
                 }
                 const uint32_t dst = sbase + s * S::STAGE_BYTES;
                 if (leader) mbar_arrive_expect_tx(full(s), 2 * S::STAGE_BYTES);
-                if (p.a_mn) {
+                if (a_mn) {
                   tma_load_3d_pair(dst, am, full(s), arow, kb * BK, ta);
                   tma_load_3d_pair(dst + 8192, am, full(s), arow + 64, kb * BK, ta);
                 } else {
                   tma_load_3d_pair(dst, am, full(s), kb * BK, arow, ta);
                 }
-                if (p.b_mn) {
+                if (b_mn) {
 #pragma unroll
                   for (int j = 0; j < BN / 128; ++j)
                     tma_load_3d_pair(dst + A_BYTES + j * 8192, bm, full(s), brow + 64 * j, kb * BK, tb);
@@ -296,22 +321,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       // both CTAs' bytes; the peer waits for the leader at the final cluster barrier)
       if (leader)
         for (int j = it > STAGES ? it - STAGES : 0; j < it; ++j)
-          mbar_wait_drain(full(j % STAGES), (j / STAGES) & 1, p.err);
+          mbar_wait_drain(full(j % STAGES), (j / STAGES) & 1, launch.err);
     }
   } else if (warp == 1) {
     if (leader) {
       // the whole warp runs the issue loop (uniform waits, running descriptors); one elected lane issues
-      const uint32_t idesc = idesc_16_f32(PAIR_M, BN, p.bf16, p.a_mn, p.b_mn);
-      const uint64_t a_base = p.a_mn ? sdesc_mn_sw128(sbase, 8192, 1024) : sdesc_k_sw128(sbase);
-      const uint64_t b_base =
-          p.b_mn ? sdesc_mn_sw128(sbase + A_BYTES, 8192, 1024) : sdesc_k_sw128(sbase + A_BYTES);
-      // bytes >> 4 from one K step of 16 to the next
-      const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
-      uint64_t ad = a_base, bd = b_base;
       int s = 0, buf = 0;
       uint32_t ph = 0, bph = 0;
       bool ok = true;
-      for (int t = pair; t < p.total_tiles && ok; t += npairs) {
+      for (int t = pair; t < launch.total_tiles && ok; t += npairs) {
+        const Args &p = product_of(launch, t).args;
+        const uint32_t idesc = idesc_16_f32(PAIR_M, BN, p.bf16, p.a_mn, p.b_mn);
+        const uint64_t a_base = p.a_mn ? sdesc_mn_sw128(sbase, 8192, 1024) : sdesc_k_sw128(sbase);
+        const uint64_t b_base =
+            p.b_mn ? sdesc_mn_sw128(sbase + A_BYTES, 8192, 1024) : sdesc_k_sw128(sbase + A_BYTES);
+        // bytes >> 4 from one K step of 16 to the next
+        const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
+        uint64_t ad = desc_add(a_base, s * S::STAGE_BYTES), bd = desc_add(b_base, s * S::STAGE_BYTES);
         int steps = p.k_blocks;
         if (p.splits > 1) {
           const int split = tile_at(p, t).split;
@@ -320,14 +346,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int part = p.combos > 1 ? kPromote : steps;
         for (int from = 0; from < steps && ok; from += part) {
           const int iters = min(part, steps - from) * p.segments * p.combos;
-          if (!warp_wait(acc_empty(buf), bph ^ 1, abort_flag, p.err, kErrWaitMma)) {
+          if (!warp_wait(acc_empty(buf), bph ^ 1, abort_flag, launch.err, kErrWaitMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint32_t d = tmem + buf * 256;
           for (int i = 0; i < iters; ++i) {
-            if (!warp_wait(full(s), ph, abort_flag, p.err, kErrWaitMma)) {
+            if (!warp_wait(full(s), ph, abort_flag, launch.err, kErrWaitMma)) {
               ok = false;
               break;
             }
@@ -353,19 +379,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       }
       // Every MMA has completed before TMEM is freed, whether or not a consumer gave up.
       umma_commit_pair(drain);
-      mbar_wait_drain(drain, 0, p.err);
+      mbar_wait_drain(drain, 0, launch.err);
     }
   } else {
     // Each warp: its lane quarter's 32 rows, every second (one of the two warps of its group and
     // quarter) or fourth block of 32 columns.
     const int q = warp & 3, ew = warp - 2, group = ew >> 3;
-    const int first = p.alternate ? (ew >> 2) & 1 : ew >> 2, step = p.alternate ? 2 : 4;
+    const int first = launch.alternate ? (ew >> 2) & 1 : ew >> 2, step = launch.alternate ? 2 : 4;
     constexpr int WIDTH = GATE ? BN / 2 : BN;  // output columns of a tile
     uint8_t *const block = smem + S::OFF_STAGE + ew * S::SLOT_BYTES;
     const uint32_t block_addr = sbase + S::OFF_STAGE + ew * S::SLOT_BYTES;
     int acc_it = 0, stores = 0, loads = 0;  // stores, loads: through the two blocks in turn
-    for (int t = pair; t < p.total_tiles; t += npairs, ++acc_it) {
-      if (p.alternate && (acc_it & 1) != group) continue;
+    for (int t = pair; t < launch.total_tiles; t += npairs, ++acc_it) {
+      if (launch.alternate && (acc_it & 1) != group) continue;
+      const Product &product = product_of(launch, t);
+      const Maps &maps = product.maps;
+      const Args &p = product.args;
       const Tile tile = tile_at(p, t);
       const int r0 = tile.mi * PAIR_M + rank * BM + q * 32;  // the warp's first row
       const int64_t m = static_cast<int64_t>(r0) + lane;
@@ -375,7 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       bool ok = true;
       // f32: all but the last part of the depth, into registers (each warp has one block: BN is 128)
       [[maybe_unused]] float sums[32];
-      if constexpr (KIND == kOut && sizeof(OT) == 4) {
+      if constexpr ((KIND == kOut || KIND == kProducts) && sizeof(OT) == 4) {
         if (p.combos > 1) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) sums[i] = 0.f;
@@ -383,7 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (p.splits > 1) steps = k_begin(p, tile.split + 1) - k_begin(p, tile.split);
           for (int from = kPromote; from < steps; from += kPromote, ++acc_it) {
             const int buf = acc_it & 1;
-            ok = warp_wait(acc_full(buf), (acc_it >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
+            ok = warp_wait(acc_full(buf), (acc_it >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
             if (!ok) break;
             tc_fence_after();
             if (first < end) {
@@ -416,8 +445,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           }
         };
         if (first < end) fetch(first);
-        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) {
-          if (first < end && lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, p.err);
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) {
+          if (first < end && lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, launch.err);
           break;
         }
         tc_fence_after();
@@ -428,7 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           uint32_t v[32];
           tmem_ld32(taddr + b * 32, v);
           const uint32_t scales = p.saved_scale[(c0 >> 5) * p.scale_rows + m];
-          ok = warp_wait(load(ew, 0), loads++ & 1, abort_flag, p.err, kErrWaitEpilogue);
+          ok = warp_wait(load(ew, 0), loads++ & 1, abort_flag, launch.err, kErrWaitEpilogue);
           tmem_ld_wait();
           if (!ok) break;
 #pragma unroll
@@ -467,7 +496,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (!ok) break;
       } else if constexpr (GATE) {
         // h = act(g) v; columns [0, BN / 2) of the accumulator are g, the others v
-        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) break;
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) break;
         tc_fence_after();
 #pragma unroll 1
         for (int b = first; b < end; b += step) {
@@ -538,8 +567,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       } else {
         // out = act(acc + bias) (+ residual)
-        const int z = p.partial ? tile.split * static_cast<int>(p.batches.d) + tile.z : 0;
-        const CUtensorMap *omap = &maps.out[p.partial ? 0 : tile.z];
+        constexpr bool PLAIN = KIND == kProducts;
+        const int partial = p.partial;
+        const bool tma_residual = !PLAIN && p.tma_residual;
+        const OT *residual = PLAIN ? nullptr : static_cast<const OT *>(p.residual);
+        const int z = partial ? tile.split * static_cast<int>(p.batches.d) + tile.z : 0;
+        const CUtensorMap *omap = &maps.out[partial ? 0 : tile.z];
         // the residual's blocks come ahead, each into the block that its result leaves from
         auto fetch = [&](int b, int at) {
           if (lane == 0) {
@@ -548,9 +581,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tma_load_3d(block_addr + (at & 1) * 2048, &maps.residual, load(ew, at & 1), n0 + b * 32, r0, 0);
           }
         };
-        if (p.tma_residual && first < end) fetch(first, loads);
-        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, p.err, kErrWaitEpilogue)) {
-          if (p.tma_residual && first < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, p.err);
+        if (tma_residual && first < end) fetch(first, loads);
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) {
+          if (tma_residual && first < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
           break;
         }
         tc_fence_after();
@@ -559,10 +592,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const int c0 = n0 + b * 32;
           uint32_t r[32];
           tmem_ld32(taddr + b * 32, r);
-          if (p.tma_residual && b + step < end) fetch(b + step, loads + 1);
+          if (tma_residual && b + step < end) fetch(b + step, loads + 1);
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
           const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0)), cols = min(32, p.n - c0);
-          const OT *bias = p.partial ? nullptr : static_cast<const OT *>(p.bias[tile.z]);
+          const OT *bias = PLAIN || partial ? nullptr : static_cast<const OT *>(p.bias[tile.z]);
           if constexpr (sizeof(OT) == 2) {
             uint32_t bw[2][8] = {};
             if (bias) {
@@ -589,7 +622,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               for (int i = 0; i < 32; ++i) y[i] += i < cols ? bias[c0 + i] : 0.f;
             }
           }
-          if (!p.partial && p.activation != AF2_ACTIVATION_NONE) {
+          if (!PLAIN && !partial && p.activation != AF2_ACTIVATION_NONE) {
             if (p.save) {  // the slopes, through the first block (16 bits) or directly (f32)
               if (lane == 0) bulk_wait_read_all();
               __syncwarp();
@@ -637,31 +670,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               });
             }
           }
+          if constexpr (sizeof(OT) == 2) {
+            if (partial) {  // the f32 sums, through both blocks
+              if (lane == 0) bulk_wait_read_all();
+              __syncwarp();
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *piece32(block, lane, c) = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_3d(omap, block_addr, c0, r0, z);
+                bulk_commit();
+              }
+              continue;
+            }
+          }
           // the block that the result leaves from (f32: both), with the residual in it where there is one
           uint32_t at = 0;
           if constexpr (sizeof(OT) == 2)
-            at = 2048u * (p.tma_residual ? loads & 1
-                          : p.save       ? 1  // the first block may still hold slopes
+            at = 2048u * (tma_residual ? loads & 1
+                          : !PLAIN && p.save ? 1  // the first block may still hold slopes
                                          : stores++ & 1);
           uint8_t *const dst = block + at;
-          if (p.tma_residual) {
-            ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
+          if (tma_residual) {
+            ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
             ++loads;
             if (!ok) {
-              if (b + step < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, p.err);
+              if (b + step < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
               break;
             }
           } else {
             if (lane == 0) {
-              if (sizeof(OT) == 4)
-                bulk_wait_read_all();
+              if (sizeof(OT) == 4 || PLAIN)
+                bulk_wait_read_all();  // (f32 sums of another product may be leaving both blocks)
               else
                 bulk_wait_read_but_one();
             }
             __syncwarp();
-            if (p.residual) {
-              move_rows<OT, true>(dst, const_cast<OT *>(static_cast<const OT *>(p.residual)) +
-                                           static_cast<int64_t>(r0) * p.residual_stride + c0,
+            if (residual) {
+              move_rows<OT, true>(dst, const_cast<OT *>(residual) + static_cast<int64_t>(r0) * p.residual_stride + c0,
                                   p.residual_stride, rows, cols, lane);
               __syncwarp();
             }
@@ -671,7 +719,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             for (int c = 0; c < 8; ++c) {
               float4 o = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
               float4 *piece = piece32(dst, lane, c);
-              if (p.residual) {
+              if (residual) {
                 const float4 res = *piece;
                 o.x += res.x, o.y += res.y, o.z += res.z, o.w += res.w;
               }
@@ -682,14 +730,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             for (int c = 0; c < 4; ++c) {
               uint4 *piece = piece16(dst, lane, c);
               uint32_t w[4];
-              if (p.residual) {
+              if (residual) {
                 const uint4 u = *piece;
                 w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
               }
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 float2 o = make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]);
-                if (p.residual) o = f2add(o, unpack2<OT>(w[i]));
+                if (residual) o = f2add(o, unpack2<OT>(w[i]));
                 w[i] = pack2_t<OT>(o.x, o.y);
               }
               *piece = make_uint4(w[0], w[1], w[2], w[3]);
@@ -742,8 +790,13 @@ struct ReduceArgs {
   int64_t saved_pitch;
 };
 
+struct ReduceLaunch {
+  ReduceArgs product[kMaxProducts];  // blockIdx.y
+};
+
 template <typename OT>
-__global__ void __launch_bounds__(256) reduce_kernel(const ReduceArgs p) {
+__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ ReduceLaunch launch) {
+  const ReduceArgs &p = launch.product[blockIdx.y];
   dependency_wait();
   const int64_t quads = p.pitch / 4, total = p.batch * p.m * quads;
   const int64_t split_stride = p.batch * p.m * quads;  // float4s
@@ -803,7 +856,7 @@ bool operand_map(CUtensorMap *map, const GemmOperand &o, int64_t outer, int64_t 
 }
 
 template <int KIND, typename OT, int BN>
-af2_status launch(af2_ctx *ctx, const Maps &maps, Args p, cudaStream_t stream) {
+af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l, cudaStream_t stream) {
   constexpr uint32_t smem = Shape<KIND, BN>::BYTES;
   auto kernel = layer_gemm_kernel<KIND, OT, BN>;
   static std::atomic<uint64_t> allowed{0};  // devices on which this kernel has its shared memory
@@ -814,24 +867,26 @@ af2_status launch(af2_ctx *ctx, const Maps &maps, Args p, cudaStream_t stream) {
       return cuda_fail(ctx, e, "layer product shared memory");
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int pairs = std::min(p.total_tiles, std::max(1, ctx->sm_count / 2));
-  p.alternate = p.total_tiles > pairs && p.combos == 1;
+  const int pairs = std::min(l.total_tiles, std::max(1, ctx->sm_count / 2));
+  l.alternate = l.total_tiles > pairs && l.product[0].args.combos == 1;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
-  if (cudaError_t e = launch_early(kernel, dim3(2 * pairs), THREADS, smem, stream, maps, p); e != cudaSuccess)
+  if (cudaError_t e = launch_early(kernel, dim3(2 * pairs), THREADS, smem, stream, l); e != cudaSuccess)
     return cuda_fail(ctx, e, "layer product");
   return AF2_OK;
 }
 
-template <int KIND, typename OT>
-af2_status launch_bn(af2_ctx *ctx, int bn, const Maps &maps, const Args &p, cudaStream_t stream) {
-  if constexpr (KIND == kGateBackward) return launch<KIND, OT, 256>(ctx, maps, p, stream);
-  return bn == 256 ? launch<KIND, OT, 256>(ctx, maps, p, stream) : launch<KIND, OT, 128>(ctx, maps, p, stream);
+template <int KIND, typename OT, int N>
+af2_status launch_bn(af2_ctx *ctx, int bn, Launch<N> &l, cudaStream_t stream) {
+  if constexpr (KIND == kGateBackward) return launch<KIND, OT, 256>(ctx, l, stream);
+  // f32 tiles are 128 wide: a warp holds the sums of one block of 32 columns
+  if constexpr (sizeof(OT) == 4) return launch<KIND, OT, 128>(ctx, l, stream);
+  return bn == 256 ? launch<KIND, OT, 256>(ctx, l, stream) : launch<KIND, OT, 128>(ctx, l, stream);
 }
 // A 16-bit output type.
-template <int KIND>
-af2_status launch_16(af2_ctx *ctx, int dtype, int bn, const Maps &maps, const Args &p, cudaStream_t stream) {
-  return dtype == AF2_F16 ? launch_bn<KIND, __half>(ctx, bn, maps, p, stream)
-                          : launch_bn<KIND, __nv_bfloat16>(ctx, bn, maps, p, stream);
+template <int KIND, int N>
+af2_status launch_16(af2_ctx *ctx, int dtype, int bn, Launch<N> &l, cudaStream_t stream) {
+  return dtype == AF2_F16 ? launch_bn<KIND, __half>(ctx, bn, l, stream)
+                          : launch_bn<KIND, __nv_bfloat16>(ctx, bn, l, stream);
 }
 
 CUtensorMapDataType map_type(int dtype) {
@@ -842,37 +897,69 @@ CUtensorMapDataType map_type(int dtype) {
 
 }  // namespace
 
-// Tile width and number of splits of the depth, from what a launch costs in SM clocks: a K step of
-// 64 takes 512 (BN = 256) or about 300 (BN = 128) clocks, a tile's start and its last epilogue about
-// 2500, and split sums are written, read and reduced by another kernel.
-void layer_gemm_plan(LayerGemm *g) {
+// Tile width and the parts that each depth is cut into, from what a launch costs in SM clocks.  A pair
+// takes tiles pair, pair + 74, ...; with the products in order of their tiles' cost the first pair
+// has the most.  A K step of 64 takes 512 (BN = 256) or 420 (BN = 128; the ring's latency) clocks, a
+// tile's hand-over 800, and split sums are written, read and reduced by another launch.
+void layer_gemm_plan(LayerGemm *g, int count) {
+  const int64_t combos = g[0].pieces > 1 ? 6 : 1;
+  const bool gate = g[0].epilogue == kEpilogueGate;
   double best = 0;
-  const int64_t k_blocks = ceil_div(g->k, BK), combos = g->pieces > 1 ? 6 : 1;
-  const bool gate = g->epilogue == kEpilogueGate;
   for (int bn : {256, 128}) {
-    if (g->epilogue == kEpilogueGateBackward && bn == 128) continue;
-    if (g->pieces > 1 && bn == 256) continue;
-    const int64_t tiles = g->batch * ceil_div(g->m, PAIR_M) * ceil_div(g->n, gate ? bn / 2 : bn);
-    for (int s : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64}) {
-      if (s > 1 && (g->epilogue != kEpilogueOut || s * 4 > k_blocks || tiles * (s - 1) >= 2 * kPairs)) break;
-      const double waves = static_cast<double>(ceil_div(tiles * s, kPairs));
-      const double steps = static_cast<double>(ceil_div(k_blocks, s) * g->segments * combos);
-      double cost = waves * steps * (bn == 256 ? 512 : 300) + waves * 800 + 2500;
-      if (s > 1) cost += 5000 + 8.0 * s * g->batch * g->m * align_up(g->n, 4) / 2500;
-      if (best == 0 || cost < best) {
-        best = cost;
-        g->tile_n = bn;
-        g->splits = s;
+    if (g[0].epilogue == kEpilogueGateBackward && bn == 128) continue;
+    if (g[0].pieces > 1 && bn == 256) continue;
+    // `most`: K steps that a tile may have before its depth is cut
+    for (int64_t most : {int64_t(1) << 40, int64_t(512), int64_t(384), int64_t(256), int64_t(192), int64_t(128),
+                         int64_t(96), int64_t(64), int64_t(48), int64_t(32), int64_t(24), int64_t(16), int64_t(12),
+                         int64_t(8), int64_t(6)}) {
+      if (most < int64_t(1) << 40 && g[0].epilogue != kEpilogueOut) break;
+      struct { int64_t tiles, steps; } part[kMaxProducts];
+      int splits[kMaxProducts], order[kMaxProducts];
+      double bytes = 0;
+      bool split = false;
+      for (int i = 0; i < count; ++i) {
+        const int64_t k_blocks = ceil_div(g[i].k, BK), all = k_blocks * g[i].segments * combos;
+        splits[i] = static_cast<int>(std::max<int64_t>(1, std::min({ceil_div(all, most), (k_blocks + 1) / 2, int64_t(64)})));
+        part[i].tiles = splits[i] * g[i].batch * ceil_div(g[i].m, PAIR_M) * ceil_div(g[i].n, gate ? bn / 2 : bn);
+        part[i].steps = ceil_div(k_blocks, splits[i]) * g[i].segments * combos;
+        order[i] = i;
+        if (splits[i] > 1) {
+          split = true;
+          bytes += 8.0 * splits[i] * g[i].batch * g[i].m * align_up(g[i].n, 4);
+        }
+      }
+      std::sort(order, order + count, [&](int a, int b) { return part[a].steps > part[b].steps; });
+      double clocks = 2500 + (split ? 4000 + bytes / 2500 : 0);
+      int64_t before = 0;  // tiles of the products before, in order
+      for (int j = 0; j < count; ++j) {
+        const int i = order[j];
+        // of the first pair's tiles 0, kPairs, 2 kPairs, ... those in this product
+        const int64_t turns = ceil_div(before + part[i].tiles, kPairs) - ceil_div(before, kPairs);
+        clocks += turns * (part[i].steps * (bn == 256 ? 512.0 : 420.0) + 800);
+        before += part[i].tiles;
+      }
+      if (best == 0 || clocks < best) {
+        best = clocks;
+        for (int i = 0; i < count; ++i) {
+          g[i].tile_n = bn;
+          g[i].splits = splits[i];
+          g[i].order = order[i];
+        }
       }
     }
   }
-  g->scratch_bytes = g->splits > 1 ? align_up(4ull * g->splits * g->batch * g->m * align_up(g->n, 4), 256) : 0;
+  for (int i = 0; i < count; ++i)
+    g[i].scratch_bytes =
+        g[i].splits > 1 ? align_up(4ull * g[i].splits * g[i].batch * g[i].m * align_up(g[i].n, 4), 256) : 0;
 }
 
-af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stream) {
+namespace {
+
+// One product's maps and arguments; its tiles follow `first_tile`.
+af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Product *product, int64_t *tiles) {
   const bool gate = g.epilogue == kEpilogueGate;
-  Maps maps{};
-  Args p{};
+  Maps &maps = product->maps;
+  Args &p = product->args;
   p.m = g.m;
   p.n = static_cast<int>(g.n);
   p.k_blocks = static_cast<int>(ceil_div(g.k, BK));
@@ -882,13 +969,12 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
   p.batches = Divisor(g.batch);
   p.tiles_m = Divisor(static_cast<uint32_t>(ceil_div(g.m, PAIR_M)));
   p.tiles_n = Divisor(static_cast<uint32_t>(ceil_div(g.n, gate ? g.tile_n / 2 : g.tile_n)));
-  const int64_t total = static_cast<int64_t>(p.splits) * g.batch * p.tiles_m.d * p.tiles_n.d;
-  if (total > 0x3fffffff) return fail(ctx, AF2_ERR_UNSUPPORTED, "the product has too many tiles");
-  p.total_tiles = static_cast<int>(total);
+  *tiles = static_cast<int64_t>(p.splits) * g.batch * p.tiles_m.d * p.tiles_n.d;
+  if (first_tile + *tiles > 0x3fffffff) return fail(ctx, AF2_ERR_UNSUPPORTED, "the product has too many tiles");
+  p.first_tile = static_cast<int>(first_tile);
   p.a_mn = g.a[0].mn_major;
   p.b_mn = g.b[0].mn_major;
   p.bf16 = g.bf16;
-  p.err = ctx->err_word;
   const int bsets = gate ? 2 : std::max(g.segments, g.batch);
   bool maps_ok = true;
   for (int i = 0; i < g.segments; ++i)
@@ -902,9 +988,8 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
   if (g.splits > 1) {
     p.partial = 1;
     p.tma_out = 1;
-    maps_ok &= encode_map_3d(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.scratch, g.n, g.m,
-                             g.splits * g.batch, pitch * 4, g.m * pitch * 4, 32, 32, 1,
-                             CU_TENSOR_MAP_SWIZZLE_128B);
+    maps_ok &= encode_map_3d(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.scratch, g.n, g.m, g.splits * g.batch,
+                             pitch * 4, g.m * pitch * 4, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_128B);
   } else {
     p.activation = g.activation;
     p.residual = g.residual;
@@ -928,7 +1013,6 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
         maps_ok &= encode_map_3d(&maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
                                  g.out_stride * out_bytes, 32, 32, 1,
                                  out_bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-    p.saved_f32 = g.saved.f32;
     p.save = g.saved.half || g.saved.f32;
     p.saved_f32 = g.saved.f32;
     p.saved_scale = g.saved.scale;
@@ -941,43 +1025,81 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm &g, cudaStream_t stre
     p.column_partial = g.column_partial;
   }
   if (!maps_ok) return fail(ctx, AF2_ERR_CUDA, "cannot describe the layer's tensors to the TMA unit");
+  return AF2_OK;
+}
 
-  af2_status st = AF2_OK;
-  if (g.epilogue == kEpilogueGateBackward)
-    st = launch_16<kGateBackward>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
-  else if (gate && g.saved.half)
-    st = launch_16<kGateSave>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
-  else if (gate)
-    st = launch_16<kGate>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
-  else if (p.partial || g.out_dtype == AF2_F32)
-    st = launch_bn<kOut, float>(ctx, g.tile_n, maps, p, stream);
-  else
-    st = launch_16<kOut>(ctx, g.out_dtype, g.tile_n, maps, p, stream);
-  if (st != AF2_OK || g.splits == 1) return st;
+}  // namespace
 
-  ReduceArgs r{};
-  r.partial = reinterpret_cast<const float *>(g.scratch);
-  r.splits = g.splits;
-  r.batch = g.batch;
-  r.activation = g.activation;
-  r.m = g.m;
-  r.n = g.n;
-  r.pitch = pitch;
-  for (int i = 0; i < 2; ++i) {
-    r.out[i] = g.out[i];
-    r.bias[i] = g.bias[i];
+namespace {
+
+// Describes and launches the products; run(launch) picks the kernel.
+template <int N, typename F>
+af2_status describe_and_run(af2_ctx *ctx, const LayerGemm *g, int count, F &&run) {
+  Launch<N> l{};
+  l.products = count;
+  l.err = ctx->err_word;
+  int64_t total = 0;
+  for (int j = 0; j < count; ++j) {
+    int64_t tiles = 0;
+    if (af2_status st = describe(ctx, g[g[j].order], total, &l.product[j], &tiles); st != AF2_OK) return st;
+    total += tiles;
   }
-  r.out_stride = g.out_stride;
-  r.residual = g.residual;
-  r.residual_stride = g.residual_stride;
-  r.saved_half = g.saved.half;
-  r.saved_f32 = g.saved.f32;
-  r.saved_pitch = g.saved.pitch;
-  const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(g.batch * g.m * pitch / 4, 256), 8 * ctx->sm_count));
+  l.total_tiles = static_cast<int>(total);
+  return run(l);
+}
+
+}  // namespace
+
+af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaStream_t stream) {
+  const int bn = g[0].tile_n, dtype = g[0].out_dtype;
+  af2_status st;
+  if (count > 1)
+    st = describe_and_run<kMaxProducts>(ctx, g, count, [&](auto &l) {
+      return dtype == AF2_F32 ? launch_bn<kProducts, float>(ctx, bn, l, stream)
+                              : launch_16<kProducts>(ctx, dtype, bn, l, stream);
+    });
+  else
+    st = describe_and_run<1>(ctx, g, 1, [&](auto &l) {
+      if (g->epilogue == kEpilogueGateBackward) return launch_16<kGateBackward>(ctx, dtype, bn, l, stream);
+      if (g->epilogue == kEpilogueGate)
+        return g->saved.half ? launch_16<kGateSave>(ctx, dtype, bn, l, stream)
+                             : launch_16<kGate>(ctx, dtype, bn, l, stream);
+      return dtype == AF2_F32 ? launch_bn<kOut, float>(ctx, bn, l, stream) : launch_16<kOut>(ctx, dtype, bn, l, stream);
+    });
+  if (st != AF2_OK) return st;
+
+  ReduceLaunch reduce{};
+  int split = 0;
+  int64_t most = 0;
+  for (int j = 0; j < count; ++j) {
+    const LayerGemm &q = g[j];
+    if (q.splits == 1) continue;
+    ReduceArgs &r = reduce.product[split++];
+    r.partial = reinterpret_cast<const float *>(q.scratch);
+    r.splits = q.splits;
+    r.batch = q.batch;
+    r.activation = q.activation;
+    r.m = q.m;
+    r.n = q.n;
+    r.pitch = align_up(q.n, 4);
+    for (int i = 0; i < 2; ++i) {
+      r.out[i] = q.out[i];
+      r.bias[i] = q.bias[i];
+    }
+    r.out_stride = q.out_stride;
+    r.residual = q.residual;
+    r.residual_stride = q.residual_stride;
+    r.saved_half = q.saved.half;
+    r.saved_f32 = q.saved.f32;
+    r.saved_pitch = q.saved.pitch;
+    most = std::max<int64_t>(most, q.batch * q.m * r.pitch / 4);
+  }
+  if (!split) return AF2_OK;
+  const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(most, 256), 8 * ctx->sm_count));
   LaunchScope scope(ctx, stream, kProfLayerElementwise);
   cudaError_t e = cudaSuccess;
-  with_element(g.out_dtype, [&](auto *tag) {
-    e = launch_early(reduce_kernel<std::remove_pointer_t<decltype(tag)>>, dim3(blocks), 256, 0, stream, r);
+  with_element(g[0].out_dtype, [&](auto *tag) {
+    e = launch_early(reduce_kernel<std::remove_pointer_t<decltype(tag)>>, dim3(blocks, split), 256, 0, stream, reduce);
   });
   if (e != cudaSuccess) return cuda_fail(ctx, e, "layer split sums");
   return AF2_OK;
