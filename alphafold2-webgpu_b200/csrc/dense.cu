@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "few_rows.h"
+#include "gated_fused.h"
 #include "layer_factor.cuh"
 #include "layer_gemm.h"
 #include "layer_math.cuh"
@@ -570,6 +571,17 @@ af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uin
   const GemmOperand wv = l.operand(p.w.value_weight, p.hidden, p.channels, p.hidden);
   const GemmOperand wo = l.operand(p.w.output_weight, p.channels, p.hidden, p.channels);
   l.pack();
+  GatedFused fused;
+  fused.rows = p.rows, fused.channels = p.channels, fused.hidden = p.hidden;
+  fused.dtype = p.dtype, fused.activation = p.activation;
+  fused.x = x, fused.gate = wg, fused.value = wv, fused.output = wo;
+  fused.gate_bias = p.w.gate_bias, fused.value_bias = p.w.value_bias, fused.output_bias = p.w.output_bias;
+  fused.residual = p.residual, fused.residual_stride = p.residual_stride;
+  fused.out = p.out, fused.out_stride = p.out_stride;
+  if (!p.saved && gated_fused_covers(fused)) {
+    *bytes = l.total();
+    return l.live() ? gated_fused_launch(ctx, fused, stream) : l.status;
+  }
   GemmOperand h;
   if (p.saved) {
     h.ptr = p.saved;

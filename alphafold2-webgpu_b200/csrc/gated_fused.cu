@@ -1,0 +1,495 @@
+// gated_fused.cu -- the gated transition in one kernel, for up to 128 channels:
+// y = (act(x Wg + bg) (x Wv + bv)) Wo + bo (+ r), the hidden activations never
+// leaving the chip.
+//
+// A CTA takes 128 rows at a time and the hidden channels in chunks of 64: the
+// first product's N = 128 accumulator holds a chunk's gate and value side by
+// side, sixteen warps (two groups of eight, chunks in turn) make h of it and
+// write it to TMEM as the second product's A operand, and that product sums all
+// chunks of the row tile in its own accumulator, drained by four warps.  x is
+// read once, y written once; the weights stream from L2 through two rings, read
+// as they are stored (MN-major).
+//
+// What bounds it.  Per chunk and SM the tensor core takes 768 clocks (512 + 256)
+// and the activations 8192 values: with one exponential and half a reciprocal
+// each the multi-function unit would take 768 clocks too, so every second pair's
+// exponential is computed on the FMA pipe instead (512 clocks there).
+#include <algorithm>
+#include <type_traits>
+
+#include "gated_fused.h"
+#include "layer_math.cuh"
+
+namespace af2 {
+namespace {
+
+constexpr int TILE = 128, HC = 64;             // rows of a tile, hidden channels of a chunk
+constexpr int X_BUFS = 2, W_STAGES = 3, D1_BUFS = 2, H_BUFS = 3;
+constexpr int LAG = 2;                         // chunks by which the second product trails the first
+constexpr int GATE_WARPS = 16, OUT_WARPS = 4;  // warps 2-17 and 18-21
+constexpr int THREADS = 32 * (2 + GATE_WARPS + OUT_WARPS);
+// TMEM columns: D1 2 x 128, D2 128, H 3 x 32 (64 16-bit values each)
+constexpr uint32_t COL_D2 = D1_BUFS * 128, COL_H = COL_D2 + 128;
+
+template <int KB>
+struct Layout {
+  static constexpr uint32_t X = KB * 16384u;   // [KB][128 rows][128 B]
+  static constexpr uint32_t W1 = KB * 16384u;  // [KB][gate, value][64 k][128 B]
+  static constexpr uint32_t W2 = KB * 8192u;   // [KB][64 k][128 B]
+  static constexpr uint32_t OFF_W1 = X_BUFS * X, OFF_W2 = OFF_W1 + W_STAGES * W1;
+  static constexpr uint32_t OFF_OUT = OFF_W2 + W_STAGES * W2;  // per out warp two 2 KB blocks
+  static constexpr uint32_t OFF_BAR = OFF_OUT + OUT_WARPS * 4096;
+  static constexpr uint32_t BYTES = OFF_BAR + 512 + 1024;
+};
+
+struct Maps {
+  CUtensorMap x, gate, value, output, out, residual;
+};
+struct Args {
+  const void *gate_bias, *value_bias, *output_bias;
+  int64_t rows;
+  int channels, hidden, chunks, tiles, activation, vector_hidden, vector_out, has_residual;
+  unsigned int *err;
+};
+
+// 2^x for x in [-126, 60] without the multi-function unit: x = n + f, |f| <= 1/2, 2^f by the
+// polynomial of degree 4 with the least largest relative error there (2.6e-6), n added to its exponent.
+__device__ __forceinline__ float2 ex2_poly2(float2 x) {
+  const float2 magic = f2(12582912.f);  // 1.5 * 2^23: the sum's low bits are the rounded integer
+  const float2 t = f2add(x, magic);
+  const float2 f = f2fma(f2add(t, f2(-12582912.f)), f2(-1.f), x);
+  float2 p = f2fma(f2(0.009570102207362652f), f, f2(0.05591786280274391f));
+  p = f2fma(p, f, f2(0.240247443318367f));
+  p = f2fma(p, f, f2(0.6931217908859253f));
+  p = f2fma(p, f, f2(0.9999992847442627f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// silu of two values, sigmoid2_fast with the exponential on the FMA pipe
+__device__ __forceinline__ float2 silu2_poly(float2 z) {
+  const float2 x = f2mul(z, f2(-1.4426950408889634f));
+  const float2 e = ex2_poly2(make_float2(fmaxf(fminf(x.x, 60.f), -126.f), fmaxf(fminf(x.y, 60.f), -126.f)));
+  const float2 d = f2add(e, f2(1.f));
+  const float r = rcp_approx(d.x * d.y);
+  return f2mul(z, f2mul(f2(r), make_float2(d.y, d.x)));
+}
+
+// 16 values of a bias row from c0 on as raw pairs; zeros past `cols`.
+template <typename T>
+__device__ __forceinline__ void bias16(const T *row, int c0, int cols, bool vector, uint32_t (&w)[8]) {
+  if (vector && c0 + 16 <= cols) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(row + c0)), x = __ldg(reinterpret_cast<const uint4 *>(row + c0) + 1);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w, w[4] = x.x, w[5] = x.y, w[6] = x.z, w[7] = x.w;
+  } else {
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      w[i] = (c0 + 2 * i < cols ? p[c0 + 2 * i] : 0u) | (c0 + 2 * i + 1 < cols ? static_cast<uint32_t>(p[c0 + 2 * i + 1]) << 16 : 0u);
+  }
+}
+
+// The chunks of a CTA's tiles in order; a tile starts at chunk (tile mod chunks), so that the CTAs do
+// not all read the same weights at once.
+struct Cursor {
+  int it = 0, step = 0, chunk;
+  __device__ __forceinline__ explicit Cursor(int chunks) : chunk(static_cast<int>(blockIdx.x) % chunks) {}
+  __device__ __forceinline__ void advance(int chunks) {
+    if (++step == chunks) {
+      step = 0;
+      ++it;
+      chunk = static_cast<int>(blockIdx.x + it * gridDim.x) % chunks;
+    } else if (++chunk == chunks) {
+      chunk = 0;
+    }
+  }
+};
+
+template <typename T, int KB>
+__global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_constant__ Maps maps, const Args p) {
+  using L = Layout<KB>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = align1024(smem_raw);
+  const uint32_t sbase = smem_u32(smem), bar0 = sbase + L::OFF_BAR;
+  auto x_full = [&](int b) { return bar0 + 8u * b; };
+  auto x_empty = [&](int b) { return bar0 + 8u * (2 + b); };
+  auto w1_full = [&](int s) { return bar0 + 8u * (4 + s); };
+  auto w1_empty = [&](int s) { return bar0 + 8u * (7 + s); };
+  auto w2_full = [&](int s) { return bar0 + 8u * (10 + s); };
+  auto w2_empty = [&](int s) { return bar0 + 8u * (13 + s); };
+  auto d1_full = [&](int b) { return bar0 + 8u * (16 + b); };
+  auto d1_empty = [&](int b) { return bar0 + 8u * (18 + b); };
+  auto h_full = [&](int b) { return bar0 + 8u * (20 + b); };
+  auto h_empty = [&](int b) { return bar0 + 8u * (23 + b); };
+  const uint32_t d2_full = bar0 + 8u * 26, d2_empty = bar0 + 8u * 27, drain = bar0 + 8u * 28;
+  auto load = [&](int w, int b) { return bar0 + 8u * (29 + 2 * w + b); };
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_BAR + 480);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_BAR + 488);
+  const int warp = warp_index_uniform(), lane = threadIdx.x & 31;
+  const int my_tiles = (p.tiles - 1 - static_cast<int>(blockIdx.x)) / static_cast<int>(gridDim.x) + 1;
+  const int total = my_tiles * p.chunks;  // chunks of this CTA
+
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < X_BUFS; ++b) {
+      mbar_init(x_full(b), 1);
+      mbar_init(x_empty(b), 1);
+    }
+    for (int s = 0; s < W_STAGES; ++s) {
+      mbar_init(w1_full(s), 1);
+      mbar_init(w1_empty(s), 1);
+      mbar_init(w2_full(s), 1);
+      mbar_init(w2_empty(s), 1);
+    }
+    for (int b = 0; b < D1_BUFS; ++b) {
+      mbar_init(d1_full(b), 1);
+      mbar_init(d1_empty(b), GATE_WARPS / 2);
+    }
+    for (int b = 0; b < H_BUFS; ++b) {
+      mbar_init(h_full(b), GATE_WARPS / 2);
+      mbar_init(h_empty(b), 1);
+    }
+    mbar_init(d2_full, 1);
+    mbar_init(d2_empty, OUT_WARPS);
+    mbar_init(drain, 1);
+    for (int w = 0; w < OUT_WARPS; ++w)
+      for (int b = 0; b < 2; ++b) mbar_init(load(w, b), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  dependency_wait();
+
+  if (warp == 0) {
+    // ---- TMA producer, in the order of the MMAs ----
+    if (lane == 0) {
+      tma_prefetch_map(&maps.x);
+      tma_prefetch_map(&maps.gate);
+      tma_prefetch_map(&maps.value);
+      tma_prefetch_map(&maps.output);
+      int x_issued = 0, n1 = 0, n2 = 0;
+      auto issue_x = [&]() {
+        const int b = x_issued % X_BUFS;
+        if (!mbar_wait(x_empty(b), ((x_issued / X_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer)) return false;
+        mbar_arrive_expect_tx(x_full(b), L::X);
+        const int row0 = static_cast<int>(blockIdx.x + x_issued * gridDim.x) * TILE;
+#pragma unroll
+        for (int k = 0; k < KB; ++k) tma_load_3d(sbase + b * L::X + k * 16384, &maps.x, x_full(b), k * 64, row0, 0);
+        ++x_issued;
+        return true;
+      };
+      bool ok = issue_x();
+      const int early = p.chunks > 1 ? 1 : 0;  // the next tile's x follows this step's weights
+      Cursor c1(p.chunks), c2(p.chunks);
+      for (int j = 0; ok && j < total + LAG; ++j) {
+        if (j < total) {
+          const int s = n1 % W_STAGES;
+          ok = mbar_wait(w1_empty(s), ((n1 / W_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
+          if (!ok) break;
+          mbar_arrive_expect_tx(w1_full(s), L::W1);
+#pragma unroll
+          for (int k = 0; k < KB; ++k) {
+            const uint32_t dst = sbase + L::OFF_W1 + s * L::W1 + k * 16384;
+            tma_load_3d(dst, &maps.gate, w1_full(s), c1.chunk * HC, k * 64, 0);
+            tma_load_3d(dst + 8192, &maps.value, w1_full(s), c1.chunk * HC, k * 64, 0);
+          }
+          ++n1;
+          if (c1.step == early && c1.it + 1 < my_tiles) ok = issue_x();
+          c1.advance(p.chunks);
+        }
+        if (ok && j >= LAG) {
+          const int s = n2 % W_STAGES;
+          ok = mbar_wait(w2_empty(s), ((n2 / W_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
+          if (!ok) break;
+          mbar_arrive_expect_tx(w2_full(s), L::W2);
+#pragma unroll
+          for (int k = 0; k < KB; ++k)
+            tma_load_3d(sbase + L::OFF_W2 + s * L::W2 + k * 8192, &maps.output, w2_full(s), k * 64, c2.chunk * HC, 0);
+          ++n2;
+          c2.advance(p.chunks);
+        }
+      }
+      // every load issued has landed before the CTA exits
+      for (int i = std::max(0, n1 - W_STAGES); i < n1; ++i)
+        mbar_wait_drain(w1_full(i % W_STAGES), (i / W_STAGES) & 1, p.err);
+      for (int i = std::max(0, n2 - W_STAGES); i < n2; ++i)
+        mbar_wait_drain(w2_full(i % W_STAGES), (i / W_STAGES) & 1, p.err);
+      for (int i = std::max(0, x_issued - X_BUFS); i < x_issued; ++i)
+        mbar_wait_drain(x_full(i % X_BUFS), (i / X_BUFS) & 1, p.err);
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer.  MMAs of one thread execute in order, so D1 and D2 need no wait for the MMAs
+    //      before, only for the warps that read them ----
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr uint32_t idesc1 = idesc_16_f32(TILE, 2 * HC, BF16, false, true);
+    constexpr uint32_t idesc2 = idesc_16_f32(TILE, KB * 64, BF16, false, true);
+    const uint64_t x_desc = sdesc_k_sw128(sbase);
+    const uint64_t w1_desc = sdesc_mn_sw128(sbase + L::OFF_W1, 8192, 1024);
+    const uint64_t w2_desc = sdesc_mn_sw128(sbase + L::OFF_W2, 8192, 1024);
+    int it1 = 0, step1 = 0, it2 = 0, step2 = 0;
+    for (int j = 0; j < total + LAG; ++j) {
+      if (j < total) {  // D1[j % 2] = x [Wg, Wv] of chunk j
+        const int xb = it1 % X_BUFS, s = j % W_STAGES, b = j % D1_BUFS;
+        if ((step1 == 0 && !warp_wait(x_full(xb), (it1 / X_BUFS) & 1, abort_flag, p.err, kErrWaitMma)) ||
+            !warp_wait(d1_empty(b), ((j / D1_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitMma) ||
+            !warp_wait(w1_full(s), (j / W_STAGES) & 1, abort_flag, p.err, kErrWaitMma))
+          break;
+        tc_fence_after();
+        const uint64_t xd = desc_add(x_desc, xb * L::X), wd = desc_add(w1_desc, s * L::W1);
+        const uint32_t d = tmem + b * 128;
+        umma_first(d, xd, wd, idesc1);
+#pragma unroll
+        for (int ks = 1; ks < 4 * KB; ++ks)
+          umma_acc(d, desc_add(xd, (ks >> 2) * 16384 + (ks & 3) * 32), desc_add(wd, (ks >> 2) * 16384 + (ks & 3) * 2048),
+                   idesc1);
+        umma_commit(w1_empty(s));
+        umma_commit(d1_full(b));
+        if (step1 == p.chunks - 1) umma_commit(x_empty(xb));
+        if (++step1 == p.chunks) {
+          step1 = 0;
+          ++it1;
+        }
+      }
+      if (j >= LAG) {  // D2 += h Wo of chunk i
+        const int i = j - LAG, s = i % W_STAGES, hb = i % H_BUFS;
+        if (!warp_wait(h_full(hb), (i / H_BUFS) & 1, abort_flag, p.err, kErrWaitMma) ||
+            !warp_wait(w2_full(s), (i / W_STAGES) & 1, abort_flag, p.err, kErrWaitMma) ||
+            (step2 == 0 && !warp_wait(d2_empty, (it2 & 1) ^ 1, abort_flag, p.err, kErrWaitMma)))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem + COL_D2, h = tmem + COL_H + hb * 32;
+        const uint64_t wd = desc_add(w2_desc, s * L::W2);
+        if (step2 == 0)
+          umma_ts_first(d, h, wd, idesc2);
+        else
+          umma_ts_acc(d, h, wd, idesc2);
+#pragma unroll
+        for (int ks = 1; ks < HC / 16; ++ks) umma_ts_acc(d, h + ks * 8, desc_add(wd, ks * 2048), idesc2);
+        umma_commit(w2_empty(s));
+        umma_commit(h_empty(hb));
+        if (step2 == p.chunks - 1) umma_commit(d2_full);
+        if (++step2 == p.chunks) {
+          step2 = 0;
+          ++it2;
+        }
+      }
+    }
+    // Every MMA has completed before TMEM is freed, whether or not a consumer gave up.
+    umma_commit(drain);
+    mbar_wait_drain(drain, 0, p.err);
+  } else if (warp < 2 + GATE_WARPS) {
+    // ---- h = act(g) v: group (warp - 2) / 8 takes every second chunk; a warp 32 rows and 32 of the
+    //      chunk's 64 hidden channels ----
+    const int group = (warp - 2) >> 3, q = warp & 3, half = ((warp - 2) >> 2) & 1;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    Cursor c(p.chunks);
+    for (int j = 0; j < total; ++j, c.advance(p.chunks)) {
+      if ((j & 1) != group) continue;
+      const int b = j % D1_BUFS, hb = j % H_BUFS, c0 = c.chunk * HC + half * 32;
+      if (!warp_wait(d1_full(b), (j / D1_BUFS) & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
+      tc_fence_after();
+      bool ok = true;
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {  // 16 columns each
+        uint32_t g[16], v[16], bg[8] = {}, bv[8] = {};
+        tmem_ld16(lanes + b * 128 + half * 32 + part * 16, g);
+        tmem_ld16(lanes + b * 128 + HC + half * 32 + part * 16, v);
+        if (p.gate_bias) bias16(static_cast<const T *>(p.gate_bias), c0 + part * 16, p.hidden, p.vector_hidden, bg);
+        if (p.value_bias) bias16(static_cast<const T *>(p.value_bias), c0 + part * 16, p.hidden, p.vector_hidden, bv);
+        tmem_ld_wait();
+        if (part == 1) {  // the accumulator is in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(d1_empty(b));
+        }
+        uint32_t h[8];
+        with_activation(p.activation, [&](auto act) {
+          constexpr int ACT = decltype(act)::value;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 gz =
+                f2add(make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])), unpack2<T>(bg[i]));
+            const float2 vz =
+                f2add(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), unpack2<T>(bv[i]));
+            float2 a;
+            if constexpr (ACT == AF2_ACTIVATION_SILU)
+              a = (i & 1) ? silu2_poly(gz) : activate2<ACT, true>(gz);
+            else
+              a = activate2<ACT, true>(gz);
+            a = f2mul(a, vz);
+            h[i] = pack2_t<T>(a.x, a.y);
+          }
+        });
+        if (part == 0) {
+          // the second product is done with what this buffer held
+          ok = warp_wait(h_empty(hb), ((j / H_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitEpilogue);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        tmem_st8(lanes + COL_H + hb * 32 + half * 16 + part * 8, h);
+      }
+      if (!ok) break;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(h_full(hb));
+    }
+  } else {
+    // ---- y = D2 + bo (+ r): a warp 32 rows, 32 columns at a time through two blocks ----
+    const int q = warp & 3, ow = warp - 2 - GATE_WARPS;
+    uint8_t *const block = smem + L::OFF_OUT + ow * 4096;
+    const uint32_t block_addr = sbase + L::OFF_OUT + ow * 4096;
+    const int blocks = (p.channels + 31) / 32;
+    int n = 0;  // blocks so far: through the two in turn
+    for (int it = 0; it < my_tiles; ++it) {
+      const int r0 = static_cast<int>(blockIdx.x + it * gridDim.x) * TILE + q * 32;
+      const bool rows_ok = r0 < p.rows;
+      // the residual's block comes ahead, into the block that the result leaves from
+      auto fetch = [&](int c, int at) {
+        if (lane == 0) {
+          bulk_wait_read_all();
+          mbar_arrive_expect_tx(load(ow, at & 1), 2048);
+          tma_load_3d(block_addr + (at & 1) * 2048, &maps.residual, load(ow, at & 1), c * 32, r0, 0);
+        }
+      };
+      const bool res = p.has_residual && rows_ok;
+      if (res) fetch(0, n);
+      if (!warp_wait(d2_full, it & 1, abort_flag, p.err, kErrWaitEpilogue)) {
+        if (res && lane == 0) mbar_wait_drain(load(ow, n & 1), (n >> 1) & 1, p.err);
+        break;
+      }
+      tc_fence_after();
+      bool ok = true;
+#pragma unroll 1
+      for (int c = 0; c < blocks; ++c) {
+        uint32_t v[32], bw[2][8] = {};
+        tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + COL_D2 + c * 32, v);
+        if (res && c + 1 < blocks) fetch(c + 1, n + 1);
+        if (p.output_bias) {
+          bias16(static_cast<const T *>(p.output_bias), c * 32, p.channels, p.vector_out, bw[0]);
+          bias16(static_cast<const T *>(p.output_bias), c * 32 + 16, p.channels, p.vector_out, bw[1]);
+        }
+        tmem_ld_wait();
+        if (c + 1 == blocks) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(d2_empty);
+        }
+        if (!rows_ok) continue;
+        const int at = n & 1;
+        if (res) {
+          ok = warp_wait(load(ow, at), (n >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
+          if (!ok) {
+            if (c + 1 < blocks && lane == 0) mbar_wait_drain(load(ow, at ^ 1), ((n + 1) >> 1) & 1, p.err);
+            break;
+          }
+        } else {
+          if (lane == 0) bulk_wait_read_but_one();
+          __syncwarp();
+        }
+        ++n;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint4 *piece = reinterpret_cast<uint4 *>(block + at * 2048 + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4));
+          uint32_t w[4] = {};
+          if (res) {
+            const uint4 u = *piece;
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float2 y = f2add(make_float2(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1])),
+                             unpack2<T>(bw[k >> 1][(k & 1) * 4 + i]));
+            if (res) y = f2add(y, unpack2<T>(w[i]));
+            w[i] = pack2_t<T>(y.x, y.y);
+          }
+          *piece = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_3d(&maps.out, block_addr + at * 2048, c * 32, r0, 0);
+          bulk_commit();
+        }
+      }
+      if (!ok) break;
+    }
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+bool addressable(const void *ptr, int64_t stride) {
+  return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && stride % 8 == 0 && stride < (int64_t(1) << 38);
+}
+
+template <typename T, int KB>
+af2_status launch(af2_ctx *ctx, const Maps &maps, const Args &p, cudaStream_t stream) {
+  auto kernel = gated_fused_kernel<T, KB>;
+  constexpr uint32_t smem = Layout<KB>::BYTES;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      e != cudaSuccess)
+    return cuda_fail(ctx, e, "gated transition shared memory");
+  LaunchScope scope(ctx, stream, kProfLayerGemm);
+  const dim3 grid(static_cast<unsigned>(std::min(p.tiles, ctx->sm_count)));
+  if (cudaError_t e = launch_early(kernel, grid, THREADS, smem, stream, maps, p); e != cudaSuccess)
+    return cuda_fail(ctx, e, "gated transition");
+  return AF2_OK;
+}
+
+}  // namespace
+
+bool gated_fused_covers(const GatedFused &f) {
+  if (f.dtype == AF2_F32 || f.channels > 128) return false;
+  return addressable(f.out, f.out_stride) && (!f.residual || addressable(f.residual, f.residual_stride));
+}
+
+af2_status gated_fused_launch(af2_ctx *ctx, const GatedFused &f, cudaStream_t stream) {
+  const bool bf16 = f.dtype == AF2_BF16;
+  const CUtensorMapDataType t = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapSwizzle wide = CU_TENSOR_MAP_SWIZZLE_128B, narrow = CU_TENSOR_MAP_SWIZZLE_64B;
+  Maps maps{};
+  auto map = [&](CUtensorMap *m, const void *ptr, int64_t width, int64_t rows, int64_t pitch, int box_rows, int box_cols,
+                 CUtensorMapSwizzle swizzle) {
+    return encode_map_3d(m, t, ptr, width, rows, 1, pitch * 2, pitch * 2, box_cols, box_rows, 1, swizzle);
+  };
+  bool ok = map(&maps.x, f.x.ptr, f.channels, f.rows, f.x.pitch, TILE, 64, wide) &&
+            map(&maps.gate, f.gate.ptr, f.hidden, f.channels, f.gate.pitch, 64, 64, wide) &&
+            map(&maps.value, f.value.ptr, f.hidden, f.channels, f.value.pitch, 64, 64, wide) &&
+            map(&maps.output, f.output.ptr, f.channels, f.hidden, f.output.pitch, 64, 64, wide) &&
+            map(&maps.out, f.out, f.channels, f.rows, f.out_stride, 32, 32, narrow);
+  if (f.residual) ok = ok && map(&maps.residual, f.residual, f.channels, f.rows, f.residual_stride, 32, 32, narrow);
+  if (!ok) return fail(ctx, AF2_ERR_CUDA, "cannot describe the transition's tensors to the TMA unit");
+  Args p{};
+  p.gate_bias = f.gate_bias;
+  p.value_bias = f.value_bias;
+  p.output_bias = f.output_bias;
+  p.rows = f.rows;
+  p.channels = static_cast<int>(f.channels);
+  p.hidden = static_cast<int>(f.hidden);
+  p.chunks = static_cast<int>((f.hidden + HC - 1) / HC);
+  p.tiles = static_cast<int>((f.rows + TILE - 1) / TILE);
+  p.activation = f.activation;
+  p.vector_hidden =
+      reinterpret_cast<uintptr_t>(f.gate_bias) % 16 == 0 && reinterpret_cast<uintptr_t>(f.value_bias) % 16 == 0;
+  p.vector_out = reinterpret_cast<uintptr_t>(f.output_bias) % 16 == 0;
+  p.has_residual = f.residual != nullptr;
+  p.err = ctx->err_word;
+  if (f.channels <= 64)
+    return bf16 ? launch<__nv_bfloat16, 1>(ctx, maps, p, stream) : launch<__half, 1>(ctx, maps, p, stream);
+  return bf16 ? launch<__nv_bfloat16, 2>(ctx, maps, p, stream) : launch<__half, 2>(ctx, maps, p, stream);
+}
+
+}  // namespace af2

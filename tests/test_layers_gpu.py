@@ -371,3 +371,31 @@ def test_refusals(device):
         gated(device, s["x"], {**s["weights"], "outputWeight": s["weights"]["gateWeight"]})
     with pytest.raises(af2cuda.RangeError, match="workspace"):
         gated(device, s["x"], s["weights"], workspace=torch.empty(0, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("rows,c,h", [(257, 128, 512), (300, 8, 24), (1000, 72, 200), (5000, 64, 64), (20000, 128, 136),
+                                      (40001, 104, 1000), (513, 40, 2056), (700, 100, 300)])
+def test_forward_of_narrow_transitions(device, rows, c, h, act, dtype):
+    """Inference with up to 128 channels, past the few-row sizes: one tile to several per SM, hidden
+    widths inside a chunk and past many, with and without the residual and the biases."""
+    s = gated_case(rows, c, h, dtype, seed=200)
+    y = af2cuda.encode_gated_transition_tensors(device, s["x"], s["weights"], residual=s["residual"], activation=act)
+    close("y", y, ref.gated(s["x"], s["weights"], s["residual"], act)["y"], dtype)
+    bare = {k: v for k, v in s["weights"].items() if k.endswith("Weight")}
+    y = af2cuda.encode_gated_transition_tensors(device, s["x"], bare, activation=act)
+    close("y", y, ref.gated(s["x"], bare, None, act)["y"], dtype)
+    device.sync(1)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_saturated_gates(device, dtype):
+    """Pre-activations far out on both sides: no overflow in the gate's exponentials."""
+    s = gated_case(600, 64, 128, dtype, seed=210)
+    s["x"].mul_(30)
+    for act in ACTS:
+        y = af2cuda.encode_gated_transition_tensors(device, s["x"], s["weights"], activation=act)
+        want = ref.gated(s["x"], s["weights"], None, act)["y"]
+        if dtype == BF16 or want.abs().max() < 6e4:
+            close(act, y, want, dtype)
