@@ -12,8 +12,8 @@
 //
 // What bounds it.  Per chunk and SM the tensor core takes 768 clocks (512 + 256)
 // and the activations 8192 values: with one exponential and half a reciprocal
-// each the multi-function unit would take 768 clocks too, so every second pair's
-// exponential is computed on the FMA pipe instead (512 clocks there).
+// each the multi-function unit would take 768 clocks too: bf16 takes one tanh a
+// value (512), f16 every second pair's exponential on the FMA pipe (512 and that).
 #include <algorithm>
 #include <type_traits>
 
@@ -24,11 +24,11 @@ namespace af2 {
 namespace {
 
 constexpr int TILE = 128, HC = 64;             // rows of a tile, hidden channels of a chunk
-constexpr int X_BUFS = 2, W_STAGES = 3, D1_BUFS = 2, H_BUFS = 3;
-constexpr int LAG = 2;                         // chunks by which the second product trails the first
+constexpr int X_BUFS = 2, W1_STAGES = 3, W2_STAGES = 2, D1_BUFS = 2, H_BUFS = 4;
+constexpr int LAG = 3;                         // chunks by which the second product trails the first
 constexpr int GATE_WARPS = 16, OUT_WARPS = 4;  // warps 2-17 and 18-21
 constexpr int THREADS = 32 * (2 + GATE_WARPS + OUT_WARPS);
-// TMEM columns: D1 2 x 128, D2 128, H 3 x 32 (64 16-bit values each)
+// TMEM columns: D1 2 x 128, D2 128, H 4 x 32 (64 16-bit values each)
 constexpr uint32_t COL_D2 = D1_BUFS * 128, COL_H = COL_D2 + 128;
 
 template <int KB>
@@ -36,9 +36,10 @@ struct Layout {
   static constexpr uint32_t X = KB * 16384u;   // [KB][128 rows][128 B]
   static constexpr uint32_t W1 = KB * 16384u;  // [KB][gate, value][64 k][128 B]
   static constexpr uint32_t W2 = KB * 8192u;   // [KB][64 k][128 B]
-  static constexpr uint32_t OFF_W1 = X_BUFS * X, OFF_W2 = OFF_W1 + W_STAGES * W1;
-  static constexpr uint32_t OFF_OUT = OFF_W2 + W_STAGES * W2;  // per out warp two 2 KB blocks
-  static constexpr uint32_t OFF_BAR = OFF_OUT + OUT_WARPS * 4096;
+  static constexpr uint32_t OFF_W1 = X_BUFS * X, OFF_W2 = OFF_W1 + W1_STAGES * W1;
+  static constexpr uint32_t OUT = KB * 2 * 2048u;  // per out warp a 2 KB block for every 32 columns
+  static constexpr uint32_t OFF_OUT = OFF_W2 + W2_STAGES * W2;
+  static constexpr uint32_t OFF_BAR = OFF_OUT + OUT_WARPS * OUT;
   static constexpr uint32_t BYTES = OFF_BAR + 512 + 1024;
 };
 
@@ -73,6 +74,15 @@ __device__ __forceinline__ float2 silu2_poly(float2 z) {
   const float2 d = f2add(e, f2(1.f));
   const float r = rcp_approx(d.x * d.y);
   return f2mul(z, f2mul(f2(r), make_float2(d.y, d.x)));
+}
+
+// silu of two values for bf16, one instruction of the multi-function unit each: z / 2 (1 + tanh(z / 2)).
+// tanh.approx is within 2^-11 of itself, so the result is within 2^-11 of |z| / 2: below a third of a
+// bf16 rounding where z > 0, and beside values of that size where z < 0 (at z = -4 1 % of a value
+// that is 2 % of |z|).
+__device__ __forceinline__ float2 silu2_tanh(float2 z) {
+  const float2 half = f2mul(z, f2(0.5f));
+  return f2fma(half, make_float2(tanhf_approx(half.x), tanhf_approx(half.y)), half);
 }
 
 // 16 values of a bias row from c0 on as raw pairs; zeros past `cols`.
@@ -116,13 +126,13 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
   auto w1_full = [&](int s) { return bar0 + 8u * (4 + s); };
   auto w1_empty = [&](int s) { return bar0 + 8u * (7 + s); };
   auto w2_full = [&](int s) { return bar0 + 8u * (10 + s); };
-  auto w2_empty = [&](int s) { return bar0 + 8u * (13 + s); };
-  auto d1_full = [&](int b) { return bar0 + 8u * (16 + b); };
-  auto d1_empty = [&](int b) { return bar0 + 8u * (18 + b); };
-  auto h_full = [&](int b) { return bar0 + 8u * (20 + b); };
-  auto h_empty = [&](int b) { return bar0 + 8u * (23 + b); };
+  auto w2_empty = [&](int s) { return bar0 + 8u * (12 + s); };
+  auto d1_full = [&](int b) { return bar0 + 8u * (14 + b); };
+  auto d1_empty = [&](int b) { return bar0 + 8u * (16 + b); };
+  auto h_full = [&](int b) { return bar0 + 8u * (18 + b); };
+  auto h_empty = [&](int b) { return bar0 + 8u * (22 + b); };
   const uint32_t d2_full = bar0 + 8u * 26, d2_empty = bar0 + 8u * 27, drain = bar0 + 8u * 28;
-  auto load = [&](int w, int b) { return bar0 + 8u * (29 + 2 * w + b); };
+  auto load = [&](int w) { return bar0 + 8u * (29 + w); };  // an out warp's residual
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_BAR + 480);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_BAR + 488);
   const int warp = warp_index_uniform(), lane = threadIdx.x & 31;
@@ -134,9 +144,11 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       mbar_init(x_full(b), 1);
       mbar_init(x_empty(b), 1);
     }
-    for (int s = 0; s < W_STAGES; ++s) {
+    for (int s = 0; s < W1_STAGES; ++s) {
       mbar_init(w1_full(s), 1);
       mbar_init(w1_empty(s), 1);
+    }
+    for (int s = 0; s < W2_STAGES; ++s) {
       mbar_init(w2_full(s), 1);
       mbar_init(w2_empty(s), 1);
     }
@@ -151,8 +163,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
     mbar_init(d2_full, 1);
     mbar_init(d2_empty, OUT_WARPS);
     mbar_init(drain, 1);
-    for (int w = 0; w < OUT_WARPS; ++w)
-      for (int b = 0; b < 2; ++b) mbar_init(load(w, b), 1);
+    for (int w = 0; w < OUT_WARPS; ++w) mbar_init(load(w), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -189,8 +200,8 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       Cursor c1(p.chunks), c2(p.chunks);
       for (int j = 0; ok && j < total + LAG; ++j) {
         if (j < total) {
-          const int s = n1 % W_STAGES;
-          ok = mbar_wait(w1_empty(s), ((n1 / W_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
+          const int s = n1 % W1_STAGES;
+          ok = mbar_wait(w1_empty(s), ((n1 / W1_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
           if (!ok) break;
           mbar_arrive_expect_tx(w1_full(s), L::W1);
 #pragma unroll
@@ -204,8 +215,8 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
           c1.advance(p.chunks);
         }
         if (ok && j >= LAG) {
-          const int s = n2 % W_STAGES;
-          ok = mbar_wait(w2_empty(s), ((n2 / W_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
+          const int s = n2 % W2_STAGES;
+          ok = mbar_wait(w2_empty(s), ((n2 / W2_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
           if (!ok) break;
           mbar_arrive_expect_tx(w2_full(s), L::W2);
 #pragma unroll
@@ -216,10 +227,10 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
         }
       }
       // every load issued has landed before the CTA exits
-      for (int i = std::max(0, n1 - W_STAGES); i < n1; ++i)
-        mbar_wait_drain(w1_full(i % W_STAGES), (i / W_STAGES) & 1, p.err);
-      for (int i = std::max(0, n2 - W_STAGES); i < n2; ++i)
-        mbar_wait_drain(w2_full(i % W_STAGES), (i / W_STAGES) & 1, p.err);
+      for (int i = std::max(0, n1 - W1_STAGES); i < n1; ++i)
+        mbar_wait_drain(w1_full(i % W1_STAGES), (i / W1_STAGES) & 1, p.err);
+      for (int i = std::max(0, n2 - W2_STAGES); i < n2; ++i)
+        mbar_wait_drain(w2_full(i % W2_STAGES), (i / W2_STAGES) & 1, p.err);
       for (int i = std::max(0, x_issued - X_BUFS); i < x_issued; ++i)
         mbar_wait_drain(x_full(i % X_BUFS), (i / X_BUFS) & 1, p.err);
     }
@@ -235,10 +246,10 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
     int it1 = 0, step1 = 0, it2 = 0, step2 = 0;
     for (int j = 0; j < total + LAG; ++j) {
       if (j < total) {  // D1[j % 2] = x [Wg, Wv] of chunk j
-        const int xb = it1 % X_BUFS, s = j % W_STAGES, b = j % D1_BUFS;
+        const int xb = it1 % X_BUFS, s = j % W1_STAGES, b = j % D1_BUFS;
         if ((step1 == 0 && !warp_wait(x_full(xb), (it1 / X_BUFS) & 1, abort_flag, p.err, kErrWaitMma)) ||
             !warp_wait(d1_empty(b), ((j / D1_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitMma) ||
-            !warp_wait(w1_full(s), (j / W_STAGES) & 1, abort_flag, p.err, kErrWaitMma))
+            !warp_wait(w1_full(s), (j / W1_STAGES) & 1, abort_flag, p.err, kErrWaitMma))
           break;
         tc_fence_after();
         const uint64_t xd = desc_add(x_desc, xb * L::X), wd = desc_add(w1_desc, s * L::W1);
@@ -257,9 +268,9 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
         }
       }
       if (j >= LAG) {  // D2 += h Wo of chunk i
-        const int i = j - LAG, s = i % W_STAGES, hb = i % H_BUFS;
+        const int i = j - LAG, s = i % W2_STAGES, hb = i % H_BUFS;
         if (!warp_wait(h_full(hb), (i / H_BUFS) & 1, abort_flag, p.err, kErrWaitMma) ||
-            !warp_wait(w2_full(s), (i / W_STAGES) & 1, abort_flag, p.err, kErrWaitMma) ||
+            !warp_wait(w2_full(s), (i / W2_STAGES) & 1, abort_flag, p.err, kErrWaitMma) ||
             (step2 == 0 && !warp_wait(d2_empty, (it2 & 1) ^ 1, abort_flag, p.err, kErrWaitMma)))
           break;
         tc_fence_after();
@@ -318,7 +329,9 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
             const float2 vz =
                 f2add(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), unpack2<T>(bv[i]));
             float2 a;
-            if constexpr (ACT == AF2_ACTIVATION_SILU)
+            if constexpr (ACT == AF2_ACTIVATION_SILU && std::is_same<T, __nv_bfloat16>::value)
+              a = silu2_tanh(gz);
+            else if constexpr (ACT == AF2_ACTIVATION_SILU)
               a = (i & 1) ? silu2_poly(gz) : activate2<ACT, true>(gz);
             else
               a = activate2<ACT, true>(gz);
@@ -343,60 +356,46 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
   } else {
     // ---- y = D2 + bo (+ r): a warp 32 rows, 32 columns at a time through two blocks ----
     const int q = warp & 3, ow = warp - 2 - GATE_WARPS;
-    uint8_t *const block = smem + L::OFF_OUT + ow * 4096;
-    const uint32_t block_addr = sbase + L::OFF_OUT + ow * 4096;
+    uint8_t *const block = smem + L::OFF_OUT + ow * L::OUT;
+    const uint32_t block_addr = sbase + L::OFF_OUT + ow * L::OUT;
     const int blocks = (p.channels + 31) / 32;
-    int n = 0;  // blocks so far: through the two in turn
-    for (int it = 0; it < my_tiles; ++it) {
+    for (int it = 0, loads = 0; it < my_tiles; ++it) {
       const int r0 = static_cast<int>(blockIdx.x + it * gridDim.x) * TILE + q * 32;
-      const bool rows_ok = r0 < p.rows;
-      // the residual's block comes ahead, into the block that the result leaves from
-      auto fetch = [&](int c, int at) {
-        if (lane == 0) {
-          bulk_wait_read_all();
-          mbar_arrive_expect_tx(load(ow, at & 1), 2048);
-          tma_load_3d(block_addr + (at & 1) * 2048, &maps.residual, load(ow, at & 1), c * 32, r0, 0);
+      const bool rows_ok = r0 < p.rows, res = p.has_residual && rows_ok;
+      // the blocks are free once the last tile's results have left them; the residual's come ahead,
+      // each into the block that its result leaves from
+      if (lane == 0) {
+        bulk_wait_read_all();
+        if (res) {
+          mbar_arrive_expect_tx(load(ow), blocks * 2048);
+          for (int c = 0; c < blocks; ++c) tma_load_3d(block_addr + c * 2048, &maps.residual, load(ow), c * 32, r0, 0);
         }
-      };
-      const bool res = p.has_residual && rows_ok;
-      if (res) fetch(0, n);
+      }
+      __syncwarp();
       if (!warp_wait(d2_full, it & 1, abort_flag, p.err, kErrWaitEpilogue)) {
-        if (res && lane == 0) mbar_wait_drain(load(ow, n & 1), (n >> 1) & 1, p.err);
+        if (res && lane == 0) mbar_wait_drain(load(ow), loads & 1, p.err);
         break;
       }
       tc_fence_after();
-      bool ok = true;
+      if (res && !warp_wait(load(ow), loads++ & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
 #pragma unroll 1
       for (int c = 0; c < blocks; ++c) {
         uint32_t v[32], bw[2][8] = {};
         tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + COL_D2 + c * 32, v);
-        if (res && c + 1 < blocks) fetch(c + 1, n + 1);
         if (p.output_bias) {
           bias16(static_cast<const T *>(p.output_bias), c * 32, p.channels, p.vector_out, bw[0]);
           bias16(static_cast<const T *>(p.output_bias), c * 32 + 16, p.channels, p.vector_out, bw[1]);
         }
         tmem_ld_wait();
-        if (c + 1 == blocks) {
+        if (c + 1 == blocks) {  // the accumulator is read: the next tile's products may start
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(d2_empty);
         }
         if (!rows_ok) continue;
-        const int at = n & 1;
-        if (res) {
-          ok = warp_wait(load(ow, at), (n >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
-          if (!ok) {
-            if (c + 1 < blocks && lane == 0) mbar_wait_drain(load(ow, at ^ 1), ((n + 1) >> 1) & 1, p.err);
-            break;
-          }
-        } else {
-          if (lane == 0) bulk_wait_read_but_one();
-          __syncwarp();
-        }
-        ++n;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint4 *piece = reinterpret_cast<uint4 *>(block + at * 2048 + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4));
+          uint4 *piece = reinterpret_cast<uint4 *>(block + c * 2048 + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4));
           uint32_t w[4] = {};
           if (res) {
             const uint4 u = *piece;
@@ -414,11 +413,10 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_3d(&maps.out, block_addr + at * 2048, c * 32, r0, 0);
+          tma_store_3d(&maps.out, block_addr + c * 2048, c * 32, r0, 0);
           bulk_commit();
         }
       }
-      if (!ok) break;
     }
     if (lane == 0) bulk_wait_all();
   }
