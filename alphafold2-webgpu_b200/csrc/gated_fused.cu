@@ -378,24 +378,28 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       }
       tc_fence_after();
       if (res && !warp_wait(load(ow), loads++ & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
-#pragma unroll 1
-      for (int c = 0; c < blocks; ++c) {
-        uint32_t v[32], bw[2][8] = {};
-        tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + COL_D2 + c * 32, v);
-        if (p.output_bias) {
-          bias16(static_cast<const T *>(p.output_bias), c * 32, p.channels, p.vector_out, bw[0]);
-          bias16(static_cast<const T *>(p.output_bias), c * 32 + 16, p.channels, p.vector_out, bw[1]);
-        }
+      // the next tile's second products wait for this read: all blocks first, then the stores
+      const uint32_t d2 = tmem + (static_cast<uint32_t>(q * 32) << 16) + COL_D2;
+      uint32_t v[2][16];
+      tmem_ld16(d2, v[0]);
+#pragma unroll
+      for (int h = 0; h < KB * 4; ++h) {  // 16 columns each
+        if (h >= 2 * blocks) break;
         tmem_ld_wait();
-        if (c + 1 == blocks) {  // the accumulator is read: the next tile's products may start
+        if (h + 1 < 2 * blocks) {
+          tmem_ld16(d2 + (h + 1) * 16, v[(h + 1) & 1]);
+        } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(d2_empty);
         }
-        if (!rows_ok) continue;
+        uint32_t bw[8] = {};
+        if (p.output_bias)
+          bias16(static_cast<const T *>(p.output_bias), h * 16, p.channels, p.vector_out, bw);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint4 *piece = reinterpret_cast<uint4 *>(block + c * 2048 + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4));
+        for (int k = 0; k < 2; ++k) {
+          uint4 *piece = reinterpret_cast<uint4 *>(block + (h >> 1) * 2048 + lane * 64 +
+                                                   ((((h & 1) * 2 + k) ^ ((lane >> 1) & 3)) << 4));
           uint32_t w[4] = {};
           if (res) {
             const uint4 u = *piece;
@@ -403,19 +407,20 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float2 y = f2add(make_float2(__uint_as_float(v[8 * k + 2 * i]), __uint_as_float(v[8 * k + 2 * i + 1])),
-                             unpack2<T>(bw[k >> 1][(k & 1) * 4 + i]));
+            float2 y = f2add(make_float2(__uint_as_float(v[h & 1][8 * k + 2 * i]),
+                                         __uint_as_float(v[h & 1][8 * k + 2 * i + 1])),
+                             unpack2<T>(bw[k * 4 + i]));
             if (res) y = f2add(y, unpack2<T>(w[i]));
             w[i] = pack2_t<T>(y.x, y.y);
           }
           *piece = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_3d(&maps.out, block_addr + c * 2048, c * 32, r0, 0);
-          bulk_commit();
-        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0 && rows_ok) {
+        for (int c = 0; c < blocks; ++c) tma_store_3d(&maps.out, block_addr + c * 2048, c * 32, r0, 0);
+        bulk_commit();
       }
     }
     if (lane == 0) bulk_wait_all();
