@@ -26,7 +26,7 @@ namespace {
 constexpr int TILE = 128, HC = 64;             // rows of a tile, hidden channels of a chunk
 constexpr int X_BUFS = 2, W1_STAGES = 3, W2_STAGES = 2, D1_BUFS = 2, H_BUFS = 4;
 constexpr int LAG = 3;                         // chunks by which the second product trails the first
-constexpr int GATE_WARPS = 16, OUT_WARPS = 4;  // warps 2-17 and 18-21
+constexpr int GATE_WARPS = 16, OUT_WARPS = 8;  // warps 2-17 and 18-25
 constexpr int THREADS = 32 * (2 + GATE_WARPS + OUT_WARPS);
 // TMEM columns: D1 2 x 128, D2 128, H 4 x 32 (64 16-bit values each)
 constexpr uint32_t COL_D2 = D1_BUFS * 128, COL_H = COL_D2 + 128;
@@ -37,9 +37,10 @@ struct Layout {
   static constexpr uint32_t W1 = KB * 16384u;  // [KB][gate, value][64 k][128 B]
   static constexpr uint32_t W2 = KB * 8192u;   // [KB][64 k][128 B]
   static constexpr uint32_t OFF_W1 = X_BUFS * X, OFF_W2 = OFF_W1 + W1_STAGES * W1;
-  static constexpr uint32_t OUT = KB * 2 * 2048u;  // per out warp a 2 KB block for every 32 columns
+  static constexpr uint32_t OUT = KB * 2048u;  // per out warp a 2 KB block for every 32 of its columns
   static constexpr uint32_t OFF_OUT = OFF_W2 + W2_STAGES * W2;
-  static constexpr uint32_t OFF_BAR = OFF_OUT + OUT_WARPS * OUT;
+  static constexpr uint32_t OFF_BIAS = OFF_OUT + OUT_WARPS * OUT;  // the output bias in f32
+  static constexpr uint32_t OFF_BAR = OFF_BIAS + KB * 256u;
   static constexpr uint32_t BYTES = OFF_BAR + 512 + 1024;
 };
 
@@ -49,7 +50,7 @@ struct Maps {
 struct Args {
   const void *gate_bias, *value_bias, *output_bias;
   int64_t rows;
-  int channels, hidden, chunks, tiles, activation, vector_hidden, vector_out, has_residual;
+  int channels, hidden, chunks, tiles, activation, vector_hidden, has_residual;
   unsigned int *err;
 };
 
@@ -115,7 +116,7 @@ struct Cursor {
   }
 };
 
-template <typename T, int KB>
+template <typename T, int KB, int ACT>
 __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_constant__ Maps maps, const Args p) {
   using L = Layout<KB>;
   extern __shared__ uint8_t smem_raw[];
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
   auto h_full = [&](int b) { return bar0 + 8u * (18 + b); };
   auto h_empty = [&](int b) { return bar0 + 8u * (22 + b); };
   const uint32_t d2_full = bar0 + 8u * 26, d2_empty = bar0 + 8u * 27, drain = bar0 + 8u * 28;
-  auto load = [&](int w) { return bar0 + 8u * (29 + w); };  // an out warp's residual
+  auto load = [&](int w) { return bar0 + 8u * (29 + w); };  // an out warp's residual (8 of them)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_BAR + 480);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_BAR + 488);
   const int warp = warp_index_uniform(), lane = threadIdx.x & 31;
@@ -176,6 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   dependency_wait();
+  float *const bias_out = reinterpret_cast<float *>(smem + L::OFF_BIAS);
 
   if (warp == 0) {
     // ---- TMA producer, in the order of the MMAs ----
@@ -299,6 +301,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
     //      chunk's 64 hidden channels ----
     const int group = (warp - 2) >> 3, q = warp & 3, half = ((warp - 2) >> 2) & 1;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    const bool biased = p.gate_bias || p.value_bias;
     Cursor c(p.chunks);
     for (int j = 0; j < total; ++j, c.advance(p.chunks)) {
       if ((j & 1) != group) continue;
@@ -311,8 +314,8 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
         uint32_t g[16], v[16], bg[8] = {}, bv[8] = {};
         tmem_ld16(lanes + b * 128 + half * 32 + part * 16, g);
         tmem_ld16(lanes + b * 128 + HC + half * 32 + part * 16, v);
-        if (p.gate_bias) bias16(static_cast<const T *>(p.gate_bias), c0 + part * 16, p.hidden, p.vector_hidden, bg);
-        if (p.value_bias) bias16(static_cast<const T *>(p.value_bias), c0 + part * 16, p.hidden, p.vector_hidden, bv);
+        if (biased && p.gate_bias) bias16(static_cast<const T *>(p.gate_bias), c0 + part * 16, p.hidden, p.vector_hidden, bg);
+        if (biased && p.value_bias) bias16(static_cast<const T *>(p.value_bias), c0 + part * 16, p.hidden, p.vector_hidden, bv);
         tmem_ld_wait();
         if (part == 1) {  // the accumulator is in registers
           tc_fence_before();
@@ -320,25 +323,24 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
           if (lane == 0) mbar_arrive(d1_empty(b));
         }
         uint32_t h[8];
-        with_activation(p.activation, [&](auto act) {
-          constexpr int ACT = decltype(act)::value;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 gz =
-                f2add(make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1])), unpack2<T>(bg[i]));
-            const float2 vz =
-                f2add(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), unpack2<T>(bv[i]));
-            float2 a;
-            if constexpr (ACT == AF2_ACTIVATION_SILU && std::is_same<T, __nv_bfloat16>::value)
-              a = silu2_tanh(gz);
-            else if constexpr (ACT == AF2_ACTIVATION_SILU)
-              a = (i & 1) ? silu2_poly(gz) : activate2<ACT, true>(gz);
-            else
-              a = activate2<ACT, true>(gz);
-            a = f2mul(a, vz);
-            h[i] = pack2_t<T>(a.x, a.y);
+        for (int i = 0; i < 8; ++i) {
+          float2 gz = make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
+          float2 vz = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          if (biased) {
+            gz = f2add(gz, unpack2<T>(bg[i]));
+            vz = f2add(vz, unpack2<T>(bv[i]));
           }
-        });
+          float2 a;
+          if constexpr (ACT == AF2_ACTIVATION_SILU && std::is_same<T, __nv_bfloat16>::value)
+            a = silu2_tanh(gz);
+          else if constexpr (ACT == AF2_ACTIVATION_SILU)
+            a = (i & 1) ? silu2_poly(gz) : activate2<ACT, true>(gz);
+          else
+            a = activate2<ACT, true>(gz);
+          a = f2mul(a, vz);
+          h[i] = pack2_t<T>(a.x, a.y);
+        }
         if (part == 0) {
           // the second product is done with what this buffer held
           ok = warp_wait(h_empty(hb), ((j / H_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitEpilogue);
@@ -354,21 +356,25 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       if (lane == 0) mbar_arrive(h_full(hb));
     }
   } else {
-    // ---- y = D2 + bo (+ r): a warp 32 rows, 32 columns at a time through two blocks ----
-    const int q = warp & 3, ow = warp - 2 - GATE_WARPS;
+    // ---- y = D2 + bo (+ r): two warps per lane quarter, each half of the columns ----
+    const int q = warp & 3, ow = warp - 2 - GATE_WARPS, col0 = (ow >> 2) * KB * 32;
     uint8_t *const block = smem + L::OFF_OUT + ow * L::OUT;
     const uint32_t block_addr = sbase + L::OFF_OUT + ow * L::OUT;
-    const int blocks = (p.channels + 31) / 32;
+    const int blocks = max(0, min(KB, (p.channels - col0 + 31) / 32));
+    for (int i = threadIdx.x - 32 * (2 + GATE_WARPS); i < KB * 64; i += 32 * OUT_WARPS)
+      bias_out[i] =
+          p.output_bias && i < p.channels ? to_f32<T>(static_cast<const T *>(p.output_bias)[i]) : 0.f;
+    named_barrier(1, 32 * OUT_WARPS);  // the out warps only
     for (int it = 0, loads = 0; it < my_tiles; ++it) {
       const int r0 = static_cast<int>(blockIdx.x + it * gridDim.x) * TILE + q * 32;
-      const bool rows_ok = r0 < p.rows, res = p.has_residual && rows_ok;
+      const bool rows_ok = r0 < p.rows, res = p.has_residual && rows_ok && blocks > 0;
       // the blocks are free once the last tile's results have left them; the residual's come ahead,
       // each into the block that its result leaves from
       if (lane == 0) {
         bulk_wait_read_all();
         if (res) {
           mbar_arrive_expect_tx(load(ow), blocks * 2048);
-          for (int c = 0; c < blocks; ++c) tma_load_3d(block_addr + c * 2048, &maps.residual, load(ow), c * 32, r0, 0);
+          for (int c = 0; c < blocks; ++c) tma_load_3d(block_addr + c * 2048, &maps.residual, load(ow), col0 + c * 32, r0, 0);
         }
       }
       __syncwarp();
@@ -379,23 +385,19 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       tc_fence_after();
       if (res && !warp_wait(load(ow), loads++ & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
       // the next tile's second products wait for this read: all blocks first, then the stores
-      const uint32_t d2 = tmem + (static_cast<uint32_t>(q * 32) << 16) + COL_D2;
+      const uint32_t d2 = tmem + (static_cast<uint32_t>(q * 32) << 16) + COL_D2 + col0;
       uint32_t v[2][16];
       tmem_ld16(d2, v[0]);
 #pragma unroll
-      for (int h = 0; h < KB * 4; ++h) {  // 16 columns each
-        if (h >= 2 * blocks) break;
+      for (int h = 0; h < KB * 2; ++h) {  // 16 columns each
         tmem_ld_wait();
-        if (h + 1 < 2 * blocks) {
+        if (h + 1 < KB * 2) {
           tmem_ld16(d2 + (h + 1) * 16, v[(h + 1) & 1]);
         } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(d2_empty);
         }
-        uint32_t bw[8] = {};
-        if (p.output_bias)
-          bias16(static_cast<const T *>(p.output_bias), h * 16, p.channels, p.vector_out, bw);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           uint4 *piece = reinterpret_cast<uint4 *>(block + (h >> 1) * 2048 + lane * 64 +
@@ -405,11 +407,12 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
             const uint4 u = *piece;
             w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
           }
+          const float2 *bias = reinterpret_cast<const float2 *>(bias_out + col0 + h * 16 + k * 8);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float2 y = f2add(make_float2(__uint_as_float(v[h & 1][8 * k + 2 * i]),
                                          __uint_as_float(v[h & 1][8 * k + 2 * i + 1])),
-                             unpack2<T>(bw[k * 4 + i]));
+                             bias[i]);
             if (res) y = f2add(y, unpack2<T>(w[i]));
             w[i] = pack2_t<T>(y.x, y.y);
           }
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       fence_async_smem();
       __syncwarp();
       if (lane == 0 && rows_ok) {
-        for (int c = 0; c < blocks; ++c) tma_store_3d(&maps.out, block_addr + c * 2048, c * 32, r0, 0);
+        for (int c = 0; c < blocks; ++c) tma_store_3d(&maps.out, block_addr + c * 2048, col0 + c * 32, r0, 0);
         bulk_commit();
       }
     }
@@ -440,15 +443,16 @@ bool addressable(const void *ptr, int64_t stride) {
 
 template <typename T, int KB>
 af2_status launch(af2_ctx *ctx, const Maps &maps, const Args &p, cudaStream_t stream) {
-  auto kernel = gated_fused_kernel<T, KB>;
   constexpr uint32_t smem = Layout<KB>::BYTES;
-  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      e != cudaSuccess)
-    return cuda_fail(ctx, e, "gated transition shared memory");
-  LaunchScope scope(ctx, stream, kProfLayerGemm);
   const dim3 grid(static_cast<unsigned>(std::min(p.tiles, ctx->sm_count)));
-  if (cudaError_t e = launch_early(kernel, grid, THREADS, smem, stream, maps, p); e != cudaSuccess)
-    return cuda_fail(ctx, e, "gated transition");
+  LaunchScope scope(ctx, stream, kProfLayerGemm);
+  cudaError_t e = cudaSuccess;
+  with_activation(p.activation, [&](auto act) {
+    auto kernel = gated_fused_kernel<T, KB, decltype(act)::value>;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = launch_early(kernel, grid, THREADS, smem, stream, maps, p);
+  });
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "gated transition");
   return AF2_OK;
 }
 
@@ -487,7 +491,6 @@ af2_status gated_fused_launch(af2_ctx *ctx, const GatedFused &f, cudaStream_t st
   p.activation = f.activation;
   p.vector_hidden =
       reinterpret_cast<uintptr_t>(f.gate_bias) % 16 == 0 && reinterpret_cast<uintptr_t>(f.value_bias) % 16 == 0;
-  p.vector_out = reinterpret_cast<uintptr_t>(f.output_bias) % 16 == 0;
   p.has_residual = f.residual != nullptr;
   p.err = ctx->err_word;
   if (f.channels <= 64)
