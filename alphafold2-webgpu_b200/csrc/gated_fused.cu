@@ -25,9 +25,10 @@ namespace {
 
 constexpr int TILE = 128, HC = 64;             // rows of a tile, hidden channels of a chunk
 constexpr int X_BUFS = 2, W1_STAGES = 3, W2_STAGES = 2, D1_BUFS = 2, H_BUFS = 4;
-constexpr int LAG = 3;                         // chunks by which the second product trails the first
+constexpr int LAG = 3;                         // chunks by which the second product's loads trail the first's
 constexpr int GATE_WARPS = 16, OUT_WARPS = 8;  // warps 2-17 and 18-25
-constexpr int THREADS = 32 * (2 + GATE_WARPS + OUT_WARPS);
+constexpr int SECOND_WARP = 2 + GATE_WARPS + OUT_WARPS;  // issues the second products
+constexpr int THREADS = 32 * (SECOND_WARP + 1);
 // TMEM columns: D1 2 x 128, D2 128, H 4 x 32 (64 16-bit values each)
 constexpr uint32_t COL_D2 = D1_BUFS * 128, COL_H = COL_D2 + 128;
 
@@ -50,7 +51,7 @@ struct Maps {
 struct Args {
   const void *gate_bias, *value_bias, *output_bias;
   int64_t rows;
-  int channels, hidden, chunks, tiles, activation, vector_hidden, has_residual;
+  int channels, hidden, chunks, tiles, activation, pairs, has_residual;
   unsigned int *err;
 };
 
@@ -86,18 +87,12 @@ __device__ __forceinline__ float2 silu2_tanh(float2 z) {
   return f2fma(half, make_float2(tanhf_approx(half.x), tanhf_approx(half.y)), half);
 }
 
-// 16 values of a bias row from c0 on as raw pairs; zeros past `cols`.
+// Two values of a bias row from (even) c on; zeros past `cols`.  `pairs`: the row is 4-byte aligned.
 template <typename T>
-__device__ __forceinline__ void bias16(const T *row, int c0, int cols, bool vector, uint32_t (&w)[8]) {
-  if (vector && c0 + 16 <= cols) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(row + c0)), x = __ldg(reinterpret_cast<const uint4 *>(row + c0) + 1);
-    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w, w[4] = x.x, w[5] = x.y, w[6] = x.z, w[7] = x.w;
-  } else {
-    const uint16_t *p = reinterpret_cast<const uint16_t *>(row);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      w[i] = (c0 + 2 * i < cols ? p[c0 + 2 * i] : 0u) | (c0 + 2 * i + 1 < cols ? static_cast<uint32_t>(p[c0 + 2 * i + 1]) << 16 : 0u);
-  }
+__device__ __forceinline__ float2 bias2(const T *row, int c, int cols, bool pairs) {
+  if (!row) return f2(0.f);
+  if (pairs && c + 1 < cols) return unpack2<T>(__ldg(reinterpret_cast<const uint32_t *>(row + c)));
+  return make_float2(c < cols ? to_f32<T>(row[c]) : 0.f, c + 1 < cols ? to_f32<T>(row[c + 1]) : 0.f);
 }
 
 // The chunks of a CTA's tiles in order; a tile starts at chunk (tile mod chunks), so that the CTAs do
@@ -119,6 +114,7 @@ struct Cursor {
 template <typename T, int KB, int ACT>
 __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_constant__ Maps maps, const Args p) {
   using L = Layout<KB>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
   const uint32_t sbase = smem_u32(smem), bar0 = sbase + L::OFF_BAR;
@@ -132,7 +128,8 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
   auto d1_empty = [&](int b) { return bar0 + 8u * (16 + b); };
   auto h_full = [&](int b) { return bar0 + 8u * (18 + b); };
   auto h_empty = [&](int b) { return bar0 + 8u * (22 + b); };
-  const uint32_t d2_full = bar0 + 8u * 26, d2_empty = bar0 + 8u * 27, drain = bar0 + 8u * 28;
+  const uint32_t d2_full = bar0 + 8u * 26, d2_empty = bar0 + 8u * 27;
+  auto drain = [&](int i) { return bar0 + 8u * (37 + i); };
   auto load = [&](int w) { return bar0 + 8u * (29 + w); };  // an out warp's residual (8 of them)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_BAR + 480);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_BAR + 488);
@@ -163,7 +160,8 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
     }
     mbar_init(d2_full, 1);
     mbar_init(d2_empty, OUT_WARPS);
-    mbar_init(drain, 1);
+    mbar_init(drain(0), 1);
+    mbar_init(drain(1), 1);
     for (int w = 0; w < OUT_WARPS; ++w) mbar_init(load(w), 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -237,65 +235,66 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
         mbar_wait_drain(x_full(i % X_BUFS), (i / X_BUFS) & 1, p.err);
     }
   } else if (warp == 1) {
-    // ---- MMA issuer.  MMAs of one thread execute in order, so D1 and D2 need no wait for the MMAs
-    //      before, only for the warps that read them ----
-    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-    constexpr uint32_t idesc1 = idesc_16_f32(TILE, 2 * HC, BF16, false, true);
-    constexpr uint32_t idesc2 = idesc_16_f32(TILE, KB * 64, BF16, false, true);
+    // ---- first products: D1[j % 2] = x [Wg, Wv] of chunk j.  The second products have a warp of
+    //      their own: with one warp for both, the tensor core ran dry while it waited for either ----
+    constexpr uint32_t idesc = idesc_16_f32(TILE, 2 * HC, BF16, false, true);
     const uint64_t x_desc = sdesc_k_sw128(sbase);
-    const uint64_t w1_desc = sdesc_mn_sw128(sbase + L::OFF_W1, 8192, 1024);
-    const uint64_t w2_desc = sdesc_mn_sw128(sbase + L::OFF_W2, 8192, 1024);
-    int it1 = 0, step1 = 0, it2 = 0, step2 = 0;
-    for (int j = 0; j < total + LAG; ++j) {
-      if (j < total) {  // D1[j % 2] = x [Wg, Wv] of chunk j
-        const int xb = it1 % X_BUFS, s = j % W1_STAGES, b = j % D1_BUFS;
-        if ((step1 == 0 && !warp_wait(x_full(xb), (it1 / X_BUFS) & 1, abort_flag, p.err, kErrWaitMma)) ||
-            !warp_wait(d1_empty(b), ((j / D1_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitMma) ||
-            !warp_wait(w1_full(s), (j / W1_STAGES) & 1, abort_flag, p.err, kErrWaitMma))
-          break;
-        tc_fence_after();
-        const uint64_t xd = desc_add(x_desc, xb * L::X), wd = desc_add(w1_desc, s * L::W1);
-        const uint32_t d = tmem + b * 128;
-        umma_first(d, xd, wd, idesc1);
+    const uint64_t w_desc = sdesc_mn_sw128(sbase + L::OFF_W1, 8192, 1024);
+    for (int j = 0, it = 0, step = 0; j < total; ++j) {
+      const int xb = it % X_BUFS, s = j % W1_STAGES, b = j % D1_BUFS;
+      if ((step == 0 && !warp_wait(x_full(xb), (it / X_BUFS) & 1, abort_flag, p.err, kErrWaitMma)) ||
+          !warp_wait(w1_full(s), (j / W1_STAGES) & 1, abort_flag, p.err, kErrWaitMma) ||
+          !warp_wait(d1_empty(b), ((j / D1_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitMma))
+        break;
+      tc_fence_after();
+      const uint64_t xd = desc_add(x_desc, xb * L::X), wd = desc_add(w_desc, s * L::W1);
+      const uint32_t d = tmem + b * 128;
+      umma_first(d, xd, wd, idesc);
 #pragma unroll
-        for (int ks = 1; ks < 4 * KB; ++ks)
-          umma_acc(d, desc_add(xd, (ks >> 2) * 16384 + (ks & 3) * 32), desc_add(wd, (ks >> 2) * 16384 + (ks & 3) * 2048),
-                   idesc1);
-        umma_commit(w1_empty(s));
-        umma_commit(d1_full(b));
-        if (step1 == p.chunks - 1) umma_commit(x_empty(xb));
-        if (++step1 == p.chunks) {
-          step1 = 0;
-          ++it1;
-        }
-      }
-      if (j >= LAG) {  // D2 += h Wo of chunk i
-        const int i = j - LAG, s = i % W2_STAGES, hb = i % H_BUFS;
-        if (!warp_wait(h_full(hb), (i / H_BUFS) & 1, abort_flag, p.err, kErrWaitMma) ||
-            !warp_wait(w2_full(s), (i / W2_STAGES) & 1, abort_flag, p.err, kErrWaitMma) ||
-            (step2 == 0 && !warp_wait(d2_empty, (it2 & 1) ^ 1, abort_flag, p.err, kErrWaitMma)))
-          break;
-        tc_fence_after();
-        const uint32_t d = tmem + COL_D2, h = tmem + COL_H + hb * 32;
-        const uint64_t wd = desc_add(w2_desc, s * L::W2);
-        if (step2 == 0)
-          umma_ts_first(d, h, wd, idesc2);
-        else
-          umma_ts_acc(d, h, wd, idesc2);
-#pragma unroll
-        for (int ks = 1; ks < HC / 16; ++ks) umma_ts_acc(d, h + ks * 8, desc_add(wd, ks * 2048), idesc2);
-        umma_commit(w2_empty(s));
-        umma_commit(h_empty(hb));
-        if (step2 == p.chunks - 1) umma_commit(d2_full);
-        if (++step2 == p.chunks) {
-          step2 = 0;
-          ++it2;
-        }
+      for (int ks = 1; ks < 4 * KB; ++ks)
+        umma_acc(d, desc_add(xd, (ks >> 2) * 16384 + (ks & 3) * 32), desc_add(wd, (ks >> 2) * 16384 + (ks & 3) * 2048),
+                 idesc);
+      umma_commit(w1_empty(s));
+      umma_commit(d1_full(b));
+      if (step == p.chunks - 1) umma_commit(x_empty(xb));
+      if (++step == p.chunks) {
+        step = 0;
+        ++it;
       }
     }
     // Every MMA has completed before TMEM is freed, whether or not a consumer gave up.
-    umma_commit(drain);
-    mbar_wait_drain(drain, 0, p.err);
+    umma_commit(drain(0));
+    mbar_wait_drain(drain(0), 0, p.err);
+  } else if (warp == SECOND_WARP) {
+    // ---- second products: D2 += h Wo of chunk j ----
+    constexpr uint32_t idesc = idesc_16_f32(TILE, KB * 64, BF16, false, true);
+    const uint64_t w_desc = sdesc_mn_sw128(sbase + L::OFF_W2, 8192, 1024);
+    const uint32_t d = tmem + COL_D2;
+    for (int j = 0, it = 0, step = 0; j < total; ++j) {
+      const int s = j % W2_STAGES, hb = j % H_BUFS;
+      if ((step == 0 && !warp_wait(d2_empty, (it & 1) ^ 1, abort_flag, p.err, kErrWaitMma)) ||
+          !warp_wait(w2_full(s), (j / W2_STAGES) & 1, abort_flag, p.err, kErrWaitMma) ||
+          !warp_wait(h_full(hb), (j / H_BUFS) & 1, abort_flag, p.err, kErrWaitMma))
+        break;
+      tc_fence_after();
+      const uint32_t h = tmem + COL_H + hb * 32;
+      const uint64_t wd = desc_add(w_desc, s * L::W2);
+      if (step == 0)
+        umma_ts_first(d, h, wd, idesc);
+      else
+        umma_ts_acc(d, h, wd, idesc);
+#pragma unroll
+      for (int ks = 1; ks < HC / 16; ++ks) umma_ts_acc(d, h + ks * 8, desc_add(wd, ks * 2048), idesc);
+      umma_commit(w2_empty(s));
+      umma_commit(h_empty(hb));
+      if (step == p.chunks - 1) umma_commit(d2_full);
+      if (++step == p.chunks) {
+        step = 0;
+        ++it;
+      }
+    }
+    umma_commit(drain(1));
+    mbar_wait_drain(drain(1), 0, p.err);
   } else if (warp < 2 + GATE_WARPS) {
     // ---- h = act(g) v: group (warp - 2) / 8 takes every second chunk; a warp 32 rows and 32 of the
     //      chunk's 64 hidden channels ----
@@ -308,31 +307,40 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       const int b = j % D1_BUFS, hb = j % H_BUFS, c0 = c.chunk * HC + half * 32;
       if (!warp_wait(d1_full(b), (j / D1_BUFS) & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
       tc_fence_after();
+      // The 16x256b shape: a thread has columns 8 k + 2 (lane % 4), + 1 of four rows, so it needs the
+      // biases of eight columns only.
+      float2 bg[4], bv[4];
+      if (biased) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int col = c0 + 8 * k + 2 * (lane & 3);
+          bg[k] = bias2(static_cast<const T *>(p.gate_bias), col, p.hidden, p.pairs);
+          bv[k] = bias2(static_cast<const T *>(p.value_bias), col, p.hidden, p.pairs);
+        }
+      }
       bool ok = true;
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {  // 16 columns each
-        uint32_t g[16], v[16], bg[8] = {}, bv[8] = {};
-        tmem_ld16(lanes + b * 128 + half * 32 + part * 16, g);
-        tmem_ld16(lanes + b * 128 + HC + half * 32 + part * 16, v);
-        if (biased && p.gate_bias) bias16(static_cast<const T *>(p.gate_bias), c0 + part * 16, p.hidden, p.vector_hidden, bg);
-        if (biased && p.value_bias) bias16(static_cast<const T *>(p.value_bias), c0 + part * 16, p.hidden, p.vector_hidden, bv);
+      for (int part = 0; part < 2; ++part) {  // 16 rows each
+        const uint32_t rows = lanes + (static_cast<uint32_t>(16 * part) << 16);
+        uint32_t g[16], v[16], h[8];
+        tmem_ld_16x256b_x4(rows + b * 128 + half * 32, g);
+        tmem_ld_16x256b_x4(rows + b * 128 + HC + half * 32, v);
         tmem_ld_wait();
         if (part == 1) {  // the accumulator is in registers
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(d1_empty(b));
         }
-        uint32_t h[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float2 gz = make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
           float2 vz = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
           if (biased) {
-            gz = f2add(gz, unpack2<T>(bg[i]));
-            vz = f2add(vz, unpack2<T>(bv[i]));
+            gz = f2add(gz, bg[i >> 1]);
+            vz = f2add(vz, bv[i >> 1]);
           }
           float2 a;
-          if constexpr (ACT == AF2_ACTIVATION_SILU && std::is_same<T, __nv_bfloat16>::value)
+          if constexpr (ACT == AF2_ACTIVATION_SILU && BF16)
             a = silu2_tanh(gz);
           else if constexpr (ACT == AF2_ACTIVATION_SILU)
             a = (i & 1) ? silu2_poly(gz) : activate2<ACT, true>(gz);
@@ -347,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
           if (!ok) break;
           tc_fence_after();
         }
-        tmem_st8(lanes + COL_H + hb * 32 + half * 16 + part * 8, h);
+        tmem_st_16x128b_x4(rows + COL_H + hb * 32 + half * 16, h);
       }
       if (!ok) break;
       tmem_st_wait();
@@ -489,8 +497,7 @@ af2_status gated_fused_launch(af2_ctx *ctx, const GatedFused &f, cudaStream_t st
   p.chunks = static_cast<int>((f.hidden + HC - 1) / HC);
   p.tiles = static_cast<int>((f.rows + TILE - 1) / TILE);
   p.activation = f.activation;
-  p.vector_hidden =
-      reinterpret_cast<uintptr_t>(f.gate_bias) % 16 == 0 && reinterpret_cast<uintptr_t>(f.value_bias) % 16 == 0;
+  p.pairs = reinterpret_cast<uintptr_t>(f.gate_bias) % 4 == 0 && reinterpret_cast<uintptr_t>(f.value_bias) % 4 == 0;
   p.has_residual = f.residual != nullptr;
   p.err = ctx->err_word;
   if (f.channels <= 64)
