@@ -24,24 +24,26 @@ namespace af2 {
 namespace {
 
 constexpr int TILE = 128, HC = 64;             // rows of a tile, hidden channels of a chunk
-constexpr int X_BUFS = 2, W1_STAGES = 3, W2_STAGES = 2, D1_BUFS = 2, H_BUFS = 4;
-constexpr int LAG = 3;                         // chunks by which the second product's loads trail the first's
+constexpr int X_BUFS = 2, W1_STAGES = 5, W2_STAGES = 2, D1_BUFS = 2, H_BUFS = 4;
+constexpr int MOST_HIDDEN = 2048;              // the gate's and the value's biases in shared memory
 constexpr int GATE_WARPS = 16, OUT_WARPS = 8;  // warps 2-17 and 18-25
 constexpr int SECOND_WARP = 2 + GATE_WARPS + OUT_WARPS;  // issues the second products
-constexpr int THREADS = 32 * (SECOND_WARP + 1);
+constexpr int W2_WARP = SECOND_WARP + 1;                // loads their weights
+constexpr int THREADS = 32 * (W2_WARP + 1);
 // TMEM columns: D1 2 x 128, D2 128, H 4 x 32 (64 16-bit values each)
 constexpr uint32_t COL_D2 = D1_BUFS * 128, COL_H = COL_D2 + 128;
 
 template <int KB>
 struct Layout {
   static constexpr uint32_t X = KB * 16384u;   // [KB][128 rows][128 B]
-  static constexpr uint32_t W1 = KB * 16384u;  // [KB][gate, value][64 k][128 B]
+  static constexpr uint32_t W1 = 16384u;       // a stage holds one of a chunk's KB parts: [gate, value][64 k][128 B]
   static constexpr uint32_t W2 = KB * 8192u;   // [KB][64 k][128 B]
   static constexpr uint32_t OFF_W1 = X_BUFS * X, OFF_W2 = OFF_W1 + W1_STAGES * W1;
   static constexpr uint32_t OUT = KB * 2048u;  // per out warp a 2 KB block for every 32 of its columns
   static constexpr uint32_t OFF_OUT = OFF_W2 + W2_STAGES * W2;
   static constexpr uint32_t OFF_BIAS = OFF_OUT + OUT_WARPS * OUT;  // the output bias in f32
-  static constexpr uint32_t OFF_BAR = OFF_BIAS + KB * 256u;
+  static constexpr uint32_t OFF_GATE_BIAS = OFF_BIAS + KB * 256u;  // gate and value biases in f32
+  static constexpr uint32_t OFF_BAR = OFF_GATE_BIAS + 2 * 4 * MOST_HIDDEN;
   static constexpr uint32_t BYTES = OFF_BAR + 512 + 1024;
 };
 
@@ -51,7 +53,7 @@ struct Maps {
 struct Args {
   const void *gate_bias, *value_bias, *output_bias;
   int64_t rows;
-  int channels, hidden, chunks, tiles, activation, pairs, has_residual;
+  int channels, hidden, chunks, tiles, activation, has_residual;
   unsigned int *err;
 };
 
@@ -87,14 +89,6 @@ __device__ __forceinline__ float2 silu2_tanh(float2 z) {
   return f2fma(half, make_float2(tanhf_approx(half.x), tanhf_approx(half.y)), half);
 }
 
-// Two values of a bias row from (even) c on; zeros past `cols`.  `pairs`: the row is 4-byte aligned.
-template <typename T>
-__device__ __forceinline__ float2 bias2(const T *row, int c, int cols, bool pairs) {
-  if (!row) return f2(0.f);
-  if (pairs && c + 1 < cols) return unpack2<T>(__ldg(reinterpret_cast<const uint32_t *>(row + c)));
-  return make_float2(c < cols ? to_f32<T>(row[c]) : 0.f, c + 1 < cols ? to_f32<T>(row[c + 1]) : 0.f);
-}
-
 // The chunks of a CTA's tiles in order; a tile starts at chunk (tile mod chunks), so that the CTAs do
 // not all read the same weights at once.
 struct Cursor {
@@ -121,16 +115,16 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
   auto x_full = [&](int b) { return bar0 + 8u * b; };
   auto x_empty = [&](int b) { return bar0 + 8u * (2 + b); };
   auto w1_full = [&](int s) { return bar0 + 8u * (4 + s); };
-  auto w1_empty = [&](int s) { return bar0 + 8u * (7 + s); };
-  auto w2_full = [&](int s) { return bar0 + 8u * (10 + s); };
-  auto w2_empty = [&](int s) { return bar0 + 8u * (12 + s); };
-  auto d1_full = [&](int b) { return bar0 + 8u * (14 + b); };
-  auto d1_empty = [&](int b) { return bar0 + 8u * (16 + b); };
-  auto h_full = [&](int b) { return bar0 + 8u * (18 + b); };
-  auto h_empty = [&](int b) { return bar0 + 8u * (22 + b); };
-  const uint32_t d2_full = bar0 + 8u * 26, d2_empty = bar0 + 8u * 27;
-  auto drain = [&](int i) { return bar0 + 8u * (37 + i); };
-  auto load = [&](int w) { return bar0 + 8u * (29 + w); };  // an out warp's residual (8 of them)
+  auto w1_empty = [&](int s) { return bar0 + 8u * (9 + s); };
+  auto w2_full = [&](int s) { return bar0 + 8u * (14 + s); };
+  auto w2_empty = [&](int s) { return bar0 + 8u * (16 + s); };
+  auto d1_full = [&](int b) { return bar0 + 8u * (18 + b); };
+  auto d1_empty = [&](int b) { return bar0 + 8u * (20 + b); };
+  auto h_full = [&](int b) { return bar0 + 8u * (22 + b); };
+  auto h_empty = [&](int b) { return bar0 + 8u * (26 + b); };
+  const uint32_t d2_full = bar0 + 8u * 30, d2_empty = bar0 + 8u * 31;
+  auto load = [&](int w) { return bar0 + 8u * (32 + w); };  // an out warp's residual (8 of them)
+  auto drain = [&](int i) { return bar0 + 8u * (40 + i); };
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::OFF_BAR + 480);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::OFF_BAR + 488);
   const int warp = warp_index_uniform(), lane = threadIdx.x & 31;
@@ -178,13 +172,12 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
   float *const bias_out = reinterpret_cast<float *>(smem + L::OFF_BIAS);
 
   if (warp == 0) {
-    // ---- TMA producer, in the order of the MMAs ----
+    // ---- loads of x and of the first products' weights, in their order ----
     if (lane == 0) {
       tma_prefetch_map(&maps.x);
       tma_prefetch_map(&maps.gate);
       tma_prefetch_map(&maps.value);
-      tma_prefetch_map(&maps.output);
-      int x_issued = 0, n1 = 0, n2 = 0;
+      int x_issued = 0, n = 0;
       auto issue_x = [&]() {
         const int b = x_issued % X_BUFS;
         if (!mbar_wait(x_empty(b), ((x_issued / X_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer)) return false;
@@ -197,42 +190,42 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
       };
       bool ok = issue_x();
       const int early = p.chunks > 1 ? 1 : 0;  // the next tile's x follows this step's weights
-      Cursor c1(p.chunks), c2(p.chunks);
-      for (int j = 0; ok && j < total + LAG; ++j) {
-        if (j < total) {
-          const int s = n1 % W1_STAGES;
-          ok = mbar_wait(w1_empty(s), ((n1 / W1_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
+      Cursor c(p.chunks);
+      for (int j = 0; ok && j < total; ++j) {
+        for (int k = 0; k < KB; ++k, ++n) {
+          const int s = n % W1_STAGES;
+          ok = mbar_wait(w1_empty(s), ((n / W1_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
           if (!ok) break;
           mbar_arrive_expect_tx(w1_full(s), L::W1);
-#pragma unroll
-          for (int k = 0; k < KB; ++k) {
-            const uint32_t dst = sbase + L::OFF_W1 + s * L::W1 + k * 16384;
-            tma_load_3d(dst, &maps.gate, w1_full(s), c1.chunk * HC, k * 64, 0);
-            tma_load_3d(dst + 8192, &maps.value, w1_full(s), c1.chunk * HC, k * 64, 0);
-          }
-          ++n1;
-          if (c1.step == early && c1.it + 1 < my_tiles) ok = issue_x();
-          c1.advance(p.chunks);
+          const uint32_t dst = sbase + L::OFF_W1 + s * L::W1;
+          tma_load_3d(dst, &maps.gate, w1_full(s), c.chunk * HC, k * 64, 0);
+          tma_load_3d(dst + 8192, &maps.value, w1_full(s), c.chunk * HC, k * 64, 0);
         }
-        if (ok && j >= LAG) {
-          const int s = n2 % W2_STAGES;
-          ok = mbar_wait(w2_empty(s), ((n2 / W2_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer);
-          if (!ok) break;
-          mbar_arrive_expect_tx(w2_full(s), L::W2);
-#pragma unroll
-          for (int k = 0; k < KB; ++k)
-            tma_load_3d(sbase + L::OFF_W2 + s * L::W2 + k * 8192, &maps.output, w2_full(s), k * 64, c2.chunk * HC, 0);
-          ++n2;
-          c2.advance(p.chunks);
-        }
+        if (ok && c.step == early && c.it + 1 < my_tiles) ok = issue_x();
+        c.advance(p.chunks);
       }
       // every load issued has landed before the CTA exits
-      for (int i = std::max(0, n1 - W1_STAGES); i < n1; ++i)
+      for (int i = std::max(0, n - W1_STAGES); i < n; ++i)
         mbar_wait_drain(w1_full(i % W1_STAGES), (i / W1_STAGES) & 1, p.err);
-      for (int i = std::max(0, n2 - W2_STAGES); i < n2; ++i)
-        mbar_wait_drain(w2_full(i % W2_STAGES), (i / W2_STAGES) & 1, p.err);
       for (int i = std::max(0, x_issued - X_BUFS); i < x_issued; ++i)
         mbar_wait_drain(x_full(i % X_BUFS), (i / X_BUFS) & 1, p.err);
+    }
+  } else if (warp == W2_WARP) {
+    // ---- loads of the second products' weights (in one thread with the others they came late) ----
+    if (lane == 0) {
+      tma_prefetch_map(&maps.output);
+      int n = 0;
+      Cursor c(p.chunks);
+      for (; n < total; ++n, c.advance(p.chunks)) {
+        const int s = n % W2_STAGES;
+        if (!mbar_wait(w2_empty(s), ((n / W2_STAGES) & 1) ^ 1, abort_flag, p.err, kErrWaitProducer)) break;
+        mbar_arrive_expect_tx(w2_full(s), L::W2);
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+          tma_load_3d(sbase + L::OFF_W2 + s * L::W2 + k * 8192, &maps.output, w2_full(s), k * 64, c.chunk * HC, 0);
+      }
+      for (int i = std::max(0, n - W2_STAGES); i < n; ++i)
+        mbar_wait_drain(w2_full(i % W2_STAGES), (i / W2_STAGES) & 1, p.err);
     }
   } else if (warp == 1) {
     // ---- first products: D1[j % 2] = x [Wg, Wv] of chunk j.  The second products have a warp of
@@ -240,21 +233,29 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
     constexpr uint32_t idesc = idesc_16_f32(TILE, 2 * HC, BF16, false, true);
     const uint64_t x_desc = sdesc_k_sw128(sbase);
     const uint64_t w_desc = sdesc_mn_sw128(sbase + L::OFF_W1, 8192, 1024);
-    for (int j = 0, it = 0, step = 0; j < total; ++j) {
-      const int xb = it % X_BUFS, s = j % W1_STAGES, b = j % D1_BUFS;
+    for (int j = 0, it = 0, step = 0, n = 0; j < total; ++j) {
+      const int xb = it % X_BUFS, b = j % D1_BUFS;
       if ((step == 0 && !warp_wait(x_full(xb), (it / X_BUFS) & 1, abort_flag, p.err, kErrWaitMma)) ||
-          !warp_wait(w1_full(s), (j / W1_STAGES) & 1, abort_flag, p.err, kErrWaitMma) ||
           !warp_wait(d1_empty(b), ((j / D1_BUFS) & 1) ^ 1, abort_flag, p.err, kErrWaitMma))
         break;
-      tc_fence_after();
-      const uint64_t xd = desc_add(x_desc, xb * L::X), wd = desc_add(w_desc, s * L::W1);
       const uint32_t d = tmem + b * 128;
-      umma_first(d, xd, wd, idesc);
+      bool ok = true;
 #pragma unroll
-      for (int ks = 1; ks < 4 * KB; ++ks)
-        umma_acc(d, desc_add(xd, (ks >> 2) * 16384 + (ks & 3) * 32), desc_add(wd, (ks >> 2) * 16384 + (ks & 3) * 2048),
-                 idesc);
-      umma_commit(w1_empty(s));
+      for (int k = 0; k < KB; ++k, ++n) {
+        const int s = n % W1_STAGES;
+        ok = warp_wait(w1_full(s), (n / W1_STAGES) & 1, abort_flag, p.err, kErrWaitMma);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t xd = desc_add(x_desc, xb * L::X + k * 16384), wd = desc_add(w_desc, s * L::W1);
+        if (k == 0)
+          umma_first(d, xd, wd, idesc);
+        else
+          umma_acc(d, xd, wd, idesc);
+#pragma unroll
+        for (int ks = 1; ks < 4; ++ks) umma_acc(d, desc_add(xd, ks * 32), desc_add(wd, ks * 2048), idesc);
+        umma_commit(w1_empty(s));
+      }
+      if (!ok) break;
       umma_commit(d1_full(b));
       if (step == p.chunks - 1) umma_commit(x_empty(xb));
       if (++step == p.chunks) {
@@ -301,53 +302,63 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
     const int group = (warp - 2) >> 3, q = warp & 3, half = ((warp - 2) >> 2) & 1;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
     const bool biased = p.gate_bias || p.value_bias;
+    float *const gate_bias = reinterpret_cast<float *>(smem + L::OFF_GATE_BIAS);
+    if (biased) {
+      for (int i = threadIdx.x - 64; i < p.chunks * HC; i += 32 * GATE_WARPS) {
+        gate_bias[i] = p.gate_bias && i < p.hidden ? to_f32<T>(static_cast<const T *>(p.gate_bias)[i]) : 0.f;
+        gate_bias[MOST_HIDDEN + i] =
+            p.value_bias && i < p.hidden ? to_f32<T>(static_cast<const T *>(p.value_bias)[i]) : 0.f;
+      }
+      named_barrier(2, 32 * GATE_WARPS);  // the gate warps only
+    }
     Cursor c(p.chunks);
     for (int j = 0; j < total; ++j, c.advance(p.chunks)) {
       if ((j & 1) != group) continue;
       const int b = j % D1_BUFS, hb = j % H_BUFS, c0 = c.chunk * HC + half * 32;
       if (!warp_wait(d1_full(b), (j / D1_BUFS) & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
       tc_fence_after();
-      // The 16x256b shape: a thread has columns 8 k + 2 (lane % 4), + 1 of four rows, so it needs the
-      // biases of eight columns only.
-      float2 bg[4], bv[4];
-      if (biased) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int col = c0 + 8 * k + 2 * (lane & 3);
-          bg[k] = bias2(static_cast<const T *>(p.gate_bias), col, p.hidden, p.pairs);
-          bv[k] = bias2(static_cast<const T *>(p.value_bias), col, p.hidden, p.pairs);
-        }
-      }
       bool ok = true;
 #pragma unroll
-      for (int part = 0; part < 2; ++part) {  // 16 rows each
-        const uint32_t rows = lanes + (static_cast<uint32_t>(16 * part) << 16);
+      for (int part = 0; part < 2; ++part) {  // 16 columns each
         uint32_t g[16], v[16], h[8];
-        tmem_ld_16x256b_x4(rows + b * 128 + half * 32, g);
-        tmem_ld_16x256b_x4(rows + b * 128 + HC + half * 32, v);
+        tmem_ld16(lanes + b * 128 + half * 32 + part * 16, g);
+        tmem_ld16(lanes + b * 128 + HC + half * 32 + part * 16, v);
         tmem_ld_wait();
         if (part == 1) {  // the accumulator is in registers
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(d1_empty(b));
         }
+        const float4 *bg = reinterpret_cast<const float4 *>(gate_bias + c0 + part * 16);
+        const float4 *bv = reinterpret_cast<const float4 *>(gate_bias + MOST_HIDDEN + c0 + part * 16);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float2 gz = make_float2(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]));
-          float2 vz = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-          if (biased) {
-            gz = f2add(gz, bg[i >> 1]);
-            vz = f2add(vz, bv[i >> 1]);
+        for (int i4 = 0; i4 < 4; ++i4) {
+          float2 gz[2], vz[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int at = 4 * i4 + 2 * i;
+            gz[i] = make_float2(__uint_as_float(g[at]), __uint_as_float(g[at + 1]));
+            vz[i] = make_float2(__uint_as_float(v[at]), __uint_as_float(v[at + 1]));
           }
-          float2 a;
-          if constexpr (ACT == AF2_ACTIVATION_SILU && BF16)
-            a = silu2_tanh(gz);
-          else if constexpr (ACT == AF2_ACTIVATION_SILU)
-            a = (i & 1) ? silu2_poly(gz) : activate2<ACT, true>(gz);
-          else
-            a = activate2<ACT, true>(gz);
-          a = f2mul(a, vz);
-          h[i] = pack2_t<T>(a.x, a.y);
+          if (biased) {
+            const float4 g4 = bg[i4], v4 = bv[i4];
+            gz[0] = f2add(gz[0], make_float2(g4.x, g4.y));
+            gz[1] = f2add(gz[1], make_float2(g4.z, g4.w));
+            vz[0] = f2add(vz[0], make_float2(v4.x, v4.y));
+            vz[1] = f2add(vz[1], make_float2(v4.z, v4.w));
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float2 a;
+            if constexpr (ACT == AF2_ACTIVATION_SILU && BF16)
+              a = silu2_tanh(gz[i]);
+            else if constexpr (ACT == AF2_ACTIVATION_SILU)
+              a = i ? silu2_poly(gz[i]) : activate2<ACT, true>(gz[i]);
+            else
+              a = activate2<ACT, true>(gz[i]);
+            a = f2mul(a, vz[i]);
+            h[2 * i4 + i] = pack2_t<T>(a.x, a.y);
+          }
         }
         if (part == 0) {
           // the second product is done with what this buffer held
@@ -355,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
           if (!ok) break;
           tc_fence_after();
         }
-        tmem_st_16x128b_x4(rows + COL_H + hb * 32 + half * 16, h);
+        tmem_st8(lanes + COL_H + hb * 32 + half * 16 + part * 8, h);
       }
       if (!ok) break;
       tmem_st_wait();
@@ -467,7 +478,7 @@ af2_status launch(af2_ctx *ctx, const Maps &maps, const Args &p, cudaStream_t st
 }  // namespace
 
 bool gated_fused_covers(const GatedFused &f) {
-  if (f.dtype == AF2_F32 || f.channels > 128) return false;
+  if (f.dtype == AF2_F32 || f.channels > 128 || f.hidden > MOST_HIDDEN) return false;
   return addressable(f.out, f.out_stride) && (!f.residual || addressable(f.residual, f.residual_stride));
 }
 
@@ -497,7 +508,6 @@ af2_status gated_fused_launch(af2_ctx *ctx, const GatedFused &f, cudaStream_t st
   p.chunks = static_cast<int>((f.hidden + HC - 1) / HC);
   p.tiles = static_cast<int>((f.rows + TILE - 1) / TILE);
   p.activation = f.activation;
-  p.pairs = reinterpret_cast<uintptr_t>(f.gate_bias) % 4 == 0 && reinterpret_cast<uintptr_t>(f.value_bias) % 4 == 0;
   p.has_residual = f.residual != nullptr;
   p.err = ctx->err_word;
   if (f.channels <= 64)
