@@ -19,13 +19,16 @@
 // result leaves from.
 //
 // f32 tensors are multiplied as three bf16 terms each, x = x0 + x1 + x2, and
-// the six products whose weight is at least 2^-16 of the largest are summed,
-// the small ones first: what is left out is below 2^-24 of |x||y|, f32's own
-// rounding.  The tensor core cuts its sums where f32 rounds them (some 2^-27
-// of the sum lost at each step of 16: sums of one sign over a depth of 4096 came
-// out 2e-6 low), so an f32 tile is summed over 256 of the depth at a time and
-// these sums are added in registers.  (An infinite f32 element makes its sums
-// NaN or infinite.)
+// the six products whose weight is at least 2^-16 of the largest are summed:
+// what is left out is below 2^-24 of |x||y|, f32's own rounding.  A K step's
+// three terms of both operands are in shared memory together, so each is read
+// once for its products (one read for each product was bound by L2: 900 SM
+// clocks a product and step of a 256 x 128 tile against 256 of work).  The
+// tensor core cuts its sums where f32 rounds them (some 2^-27 of the sum lost
+// at each step of 16: sums of one sign over a depth of 4096 came out 2e-6 low),
+// so the five small products have an accumulator of their own, and a tile is
+// summed over 256 of the depth at a time and these sums are added in registers.
+// (An infinite f32 element makes its sums NaN or infinite.)
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -94,7 +97,7 @@ struct Args {
   int64_t saved_pitch, scale_rows;
   float *column_partial;
   int64_t m;
-  int n, k_blocks, splits, combos, segments;
+  int n, k_blocks, splits, segments;
   Divisor tiles_m, tiles_n, batches;
   int a_mn, b_mn, bf16, activation;
   int tma_out;       // out rows are 16-byte aligned: whole blocks leave by TMA
@@ -125,9 +128,10 @@ __device__ __forceinline__ const Product &product_of(const Launch<N> &l, int t) 
   return l.product[i];
 }
 
-// The terms (of A, of B) of the six products of an f32 operand pair, small ones first.
-__constant__ const int8_t kTermA[6] = {2, 0, 1, 1, 0, 0};
-__constant__ const int8_t kTermB[6] = {0, 2, 1, 0, 1, 0};
+// The terms (of A, of B) of the six products of an f32 operand pair, the largest last.
+constexpr int kProductsF32 = 6;
+__device__ constexpr int term_a(int c) { return c == 0 ? 2 : c == 2 || c == 3 ? 1 : 0; }
+__device__ constexpr int term_b(int c) { return c == 1 ? 2 : c == 2 || c == 4 ? 1 : 0; }
 
 struct Tile {
   int split, z, mi, ni;
@@ -141,7 +145,7 @@ __device__ __forceinline__ Tile tile_at(const Args &p, int t) {
   r.split = t;
   return r;
 }
-constexpr int kPromote = 4;  // K steps of an f32 tile before its sums go to registers
+constexpr int kPromote = 4;  // K steps of an f32 tile (and segment) before its sums go to registers
 
 // The tile's range of K steps.
 __device__ __forceinline__ int k_begin(const Args &p, int split) {
@@ -217,6 +221,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     layer_gemm_kernel(const __grid_constant__ Launch<KIND == kProducts ? kMaxProducts : 1> launch) {
   using S = Shape<KIND, BN>;
   constexpr bool GATE = KIND == kGate || KIND == kGateSave;
+  constexpr bool F32 = sizeof(OT) == 4;
   constexpr int STAGES = S::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = align1024(smem_raw);
@@ -279,15 +284,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int kb1 = p.splits > 1 ? k_begin(p, tile.split + 1) : p.k_blocks;
         const int arow = tile.mi * PAIR_M + rank * BM;
         const int brow = GATE ? tile.ni * (BN / 2) : tile.ni * BN + rank * (BN / 2);
-        const int combos = p.combos, segments = p.segments, a_mn = p.a_mn, b_mn = p.b_mn;
-        const int part = combos > 1 ? kPromote : kb1 - kb0;
+        const int segments = p.segments, a_mn = p.a_mn, b_mn = p.b_mn, part = F32 ? kPromote : kb1 - kb0;
+        // K steps of a part, segment by segment; f32: a stage for each of a step's three terms
         for (int from = kb0; from < kb1 && ok; from += part) {
-          for (int c = 0; c < combos && ok; ++c) {
-            const int ta = combos > 1 ? kTermA[c] : 0, tb = combos > 1 ? kTermB[c] : 0;
-            for (int seg = 0; seg < segments && ok; ++seg) {
-              const CUtensorMap *am = &maps.a[seg];
-              const CUtensorMap *bm = &maps.b[GATE ? rank : seg + tile.z];
-              for (int kb = from; kb < min(from + part, kb1); ++kb, ++it) {
+          for (int seg = 0; seg < segments && ok; ++seg) {
+            const CUtensorMap *am = &maps.a[seg];
+            const CUtensorMap *bm = &maps.b[GATE ? rank : seg + tile.z];
+            for (int kb = from; kb < min(from + part, kb1) && ok; ++kb) {
+              for (int term = 0; term < (F32 ? 3 : 1); ++term, ++it) {
                 // the stage is free in this CTA once the pair's MMAs have read it (multicast commit)
                 if (!mbar_wait(empty(s), ph, abort_flag, launch.err, kErrWaitProducer)) {
                   ok = false;
@@ -296,17 +300,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 const uint32_t dst = sbase + s * S::STAGE_BYTES;
                 if (leader) mbar_arrive_expect_tx(full(s), 2 * S::STAGE_BYTES);
                 if (a_mn) {
-                  tma_load_3d_pair(dst, am, full(s), arow, kb * BK, ta);
-                  tma_load_3d_pair(dst + 8192, am, full(s), arow + 64, kb * BK, ta);
+                  tma_load_3d_pair(dst, am, full(s), arow, kb * BK, term);
+                  tma_load_3d_pair(dst + 8192, am, full(s), arow + 64, kb * BK, term);
                 } else {
-                  tma_load_3d_pair(dst, am, full(s), kb * BK, arow, ta);
+                  tma_load_3d_pair(dst, am, full(s), kb * BK, arow, term);
                 }
                 if (b_mn) {
 #pragma unroll
                   for (int j = 0; j < BN / 128; ++j)
-                    tma_load_3d_pair(dst + A_BYTES + j * 8192, bm, full(s), brow + 64 * j, kb * BK, tb);
+                    tma_load_3d_pair(dst + A_BYTES + j * 8192, bm, full(s), brow + 64 * j, kb * BK, term);
                 } else {
-                  tma_load_3d_pair(dst + A_BYTES, bm, full(s), kb * BK, brow, tb);
+                  tma_load_3d_pair(dst + A_BYTES, bm, full(s), kb * BK, brow, term);
                 }
                 if (++s == STAGES) {
                   s = 0;
@@ -343,9 +347,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const int split = tile_at(p, t).split;
           steps = k_begin(p, split + 1) - k_begin(p, split);
         }
-        const int part = p.combos > 1 ? kPromote : steps;
+        const int part = F32 ? kPromote : steps;
         for (int from = 0; from < steps && ok; from += part) {
-          const int iters = min(part, steps - from) * p.segments * p.combos;
+          const int iters = min(part, steps - from) * p.segments;
           if (!warp_wait(acc_empty(buf), bph ^ 1, abort_flag, launch.err, kErrWaitMma)) {
             ok = false;
             break;
@@ -353,18 +357,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           tc_fence_after();
           const uint32_t d = tmem + buf * 256;
           for (int i = 0; i < iters; ++i) {
-            if (!warp_wait(full(s), ph, abort_flag, launch.err, kErrWaitMma)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+            if constexpr (F32) {
+              static_assert(STAGES % 3 == 0, "a step's three stages do not wrap");
 #pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks)
-              umma_pair(d, ad + ks * a_step, bd + ks * b_step, idesc, (i | ks) != 0);
-            umma_commit_pair_both(empty(s));
-            ad += S::STAGE_BYTES >> 4;
-            bd += S::STAGE_BYTES >> 4;
-            if (++s == STAGES) {
+              for (int term = 0; term < 3; ++term) ok = ok && warp_wait(full(s + term), ph, abort_flag, launch.err, kErrWaitMma);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < kProductsF32; ++c)
+#pragma unroll
+                for (int ks = 0; ks < BK / 16; ++ks)
+                  umma_pair(d + (c < kProductsF32 - 1 ? 128 : 0), desc_add(ad, term_a(c) * S::STAGE_BYTES) + ks * a_step,
+                            desc_add(bd, term_b(c) * S::STAGE_BYTES) + ks * b_step, idesc,
+                            (i | ks | (c < kProductsF32 - 1 ? c : 0)) != 0);
+            } else {
+              if (!warp_wait(full(s), ph, abort_flag, launch.err, kErrWaitMma)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+#pragma unroll
+              for (int ks = 0; ks < BK / 16; ++ks)
+                umma_pair(d, ad + ks * a_step, bd + ks * b_step, idesc, (i | ks) != 0);
+            }
+            constexpr int TAKEN = F32 ? 3 : 1;
+#pragma unroll
+            for (int term = 0; term < TAKEN; ++term) umma_commit_pair_both(empty(s + term));
+            ad += TAKEN * S::STAGE_BYTES >> 4;
+            bd += TAKEN * S::STAGE_BYTES >> 4;
+            s += TAKEN;
+            if (s == STAGES) {
               s = 0;
               ph ^= 1;
               ad = a_base;
@@ -402,32 +424,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       // this warp's blocks of the tile: first, first + step, ... below `end`
       const int end = r0 < p.m ? min(WIDTH / 32, (p.n - n0 + 31) >> 5) : 0;
       bool ok = true;
-      // f32: all but the last part of the depth, into registers (each warp has one block: BN is 128)
+      // f32: the sums of each part of the depth, into registers (each warp has one block: BN is 128)
       [[maybe_unused]] float sums[32];
-      if constexpr ((KIND == kOut || KIND == kProducts) && sizeof(OT) == 4) {
-        if (p.combos > 1) {
+      auto add_part = [&](int b) {
+        uint32_t r[32], small[32];
+        const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + first * 32;
+        tmem_ld32(at, r);
+        tmem_ld32(at + 128, small);
+        tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sums[i] = 0.f;
-          int steps = p.k_blocks;
-          if (p.splits > 1) steps = k_begin(p, tile.split + 1) - k_begin(p, tile.split);
-          for (int from = kPromote; from < steps; from += kPromote, ++acc_it) {
-            const int buf = acc_it & 1;
-            ok = warp_wait(acc_full(buf), (acc_it >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
-            if (!ok) break;
-            tc_fence_after();
-            if (first < end) {
-              uint32_t r[32];
-              tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256 + first * 32, r);
-              tmem_ld_wait();
+        for (int i = 0; i < 32; ++i) sums[i] += __uint_as_float(r[i]) + __uint_as_float(small[i]);
+      };
+      if constexpr (F32) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) sums[i] += __uint_as_float(r[i]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_leader_relaxed(acc_empty(buf));
-          }
+        for (int i = 0; i < 32; ++i) sums[i] = 0.f;
+        int steps = p.k_blocks;
+        if (p.splits > 1) steps = k_begin(p, tile.split + 1) - k_begin(p, tile.split);
+        for (int from = kPromote; from < steps; from += kPromote, ++acc_it) {  // (the last part below)
+          const int b = acc_it & 1;
+          ok = warp_wait(acc_full(b), (acc_it >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
           if (!ok) break;
+          tc_fence_after();
+          if (first < end) add_part(b);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_leader_relaxed(acc_empty(b));
         }
+        if (!ok) break;
       }
       const int buf = acc_it & 1;
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
@@ -591,7 +614,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         for (int b = first; b < end; b += step) {
           const int c0 = n0 + b * 32;
           uint32_t r[32];
-          tmem_ld32(taddr + b * 32, r);
+          if constexpr (F32) {
+            add_part(buf);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sums[i]);
+          } else {
+            tmem_ld32(taddr + b * 32, r);
+          }
           if (tma_residual && b + step < end) fetch(b + step, loads + 1);
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
           const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0)), cols = min(32, p.n - c0);
@@ -612,11 +641,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               }
             }
           } else {
-            tmem_ld_wait();
-            if (p.combos > 1) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] += sums[i];
-            }
             if (bias) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) y[i] += i < cols ? bias[c0 + i] : 0.f;
@@ -868,7 +892,7 @@ af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l,
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const int pairs = std::min(l.total_tiles, std::max(1, ctx->sm_count / 2));
-  l.alternate = l.total_tiles > pairs && l.product[0].args.combos == 1;
+  l.alternate = l.total_tiles > pairs && sizeof(OT) == 2;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
   if (cudaError_t e = launch_early(kernel, dim3(2 * pairs), THREADS, smem, stream, l); e != cudaSuccess)
     return cuda_fail(ctx, e, "layer product");
@@ -877,10 +901,13 @@ af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l,
 
 template <int KIND, typename OT, int N>
 af2_status launch_bn(af2_ctx *ctx, int bn, Launch<N> &l, cudaStream_t stream) {
-  if constexpr (KIND == kGateBackward) return launch<KIND, OT, 256>(ctx, l, stream);
   // f32 tiles are 128 wide: a warp holds the sums of one block of 32 columns
-  if constexpr (sizeof(OT) == 4) return launch<KIND, OT, 128>(ctx, l, stream);
-  return bn == 256 ? launch<KIND, OT, 256>(ctx, l, stream) : launch<KIND, OT, 128>(ctx, l, stream);
+  if constexpr (sizeof(OT) == 4)
+    return launch<KIND, OT, 128>(ctx, l, stream);
+  else if constexpr (KIND == kGateBackward)
+    return launch<KIND, OT, 256>(ctx, l, stream);
+  else
+    return bn == 256 ? launch<KIND, OT, 256>(ctx, l, stream) : launch<KIND, OT, 128>(ctx, l, stream);
 }
 // A 16-bit output type.
 template <int KIND, int N>
@@ -899,29 +926,30 @@ CUtensorMapDataType map_type(int dtype) {
 
 // Tile width and the parts that each depth is cut into, from what a launch costs in SM clocks.  A pair
 // takes tiles pair, pair + 74, ...; with the products in order of their tiles' cost the first pair
-// has the most.  A K step of 64 takes 512 (BN = 256) or 420 (BN = 128; the ring's latency) clocks, a
-// tile's hand-over 800, and split sums are written, read and reduced by another launch.
+// has the most.  A K step of 64 takes 512 (BN = 256) or 420 (BN = 128; the ring's latency) clocks, in
+// f32 1800, a tile's hand-over 800, and split sums are written, read and reduced by another launch.
 void layer_gemm_plan(LayerGemm *g, int count) {
-  const int64_t combos = g[0].pieces > 1 ? 6 : 1;
+  const bool f32 = g[0].pieces > 1;
   const bool gate = g[0].epilogue == kEpilogueGate;
   double best = 0;
   for (int bn : {256, 128}) {
     if (g[0].epilogue == kEpilogueGateBackward && bn == 128) continue;
-    if (g[0].pieces > 1 && bn == 256) continue;
+    if (f32 && bn == 256) continue;
+    const double step_clocks = f32 ? 1800 : bn == 256 ? 512 : 420;
     // `most`: K steps that a tile may have before its depth is cut
     for (int64_t most : {int64_t(1) << 40, int64_t(512), int64_t(384), int64_t(256), int64_t(192), int64_t(128),
                          int64_t(96), int64_t(64), int64_t(48), int64_t(32), int64_t(24), int64_t(16), int64_t(12),
-                         int64_t(8), int64_t(6)}) {
+                         int64_t(8), int64_t(6), int64_t(4), int64_t(2)}) {
       if (most < int64_t(1) << 40 && g[0].epilogue != kEpilogueOut) break;
       struct { int64_t tiles, steps; } part[kMaxProducts];
       int splits[kMaxProducts], order[kMaxProducts];
       double bytes = 0;
       bool split = false;
       for (int i = 0; i < count; ++i) {
-        const int64_t k_blocks = ceil_div(g[i].k, BK), all = k_blocks * g[i].segments * combos;
+        const int64_t k_blocks = ceil_div(g[i].k, BK), all = k_blocks * g[i].segments;
         splits[i] = static_cast<int>(std::max<int64_t>(1, std::min({ceil_div(all, most), (k_blocks + 1) / 2, int64_t(64)})));
         part[i].tiles = splits[i] * g[i].batch * ceil_div(g[i].m, PAIR_M) * ceil_div(g[i].n, gate ? bn / 2 : bn);
-        part[i].steps = ceil_div(k_blocks, splits[i]) * g[i].segments * combos;
+        part[i].steps = ceil_div(k_blocks, splits[i]) * g[i].segments;
         order[i] = i;
         if (splits[i] > 1) {
           split = true;
@@ -935,7 +963,7 @@ void layer_gemm_plan(LayerGemm *g, int count) {
         const int i = order[j];
         // of the first pair's tiles 0, kPairs, 2 kPairs, ... those in this product
         const int64_t turns = ceil_div(before + part[i].tiles, kPairs) - ceil_div(before, kPairs);
-        clocks += turns * (part[i].steps * (bn == 256 ? 512.0 : 420.0) + 800);
+        clocks += turns * (part[i].steps * step_clocks + 800);
         before += part[i].tiles;
       }
       if (best == 0 || clocks < best) {
@@ -964,7 +992,6 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
   p.n = static_cast<int>(g.n);
   p.k_blocks = static_cast<int>(ceil_div(g.k, BK));
   p.splits = g.splits;
-  p.combos = g.pieces > 1 ? 6 : 1;
   p.segments = g.segments;
   p.batches = Divisor(g.batch);
   p.tiles_m = Divisor(static_cast<uint32_t>(ceil_div(g.m, PAIR_M)));
