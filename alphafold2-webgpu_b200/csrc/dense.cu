@@ -47,21 +47,21 @@ struct PackArgs {
   int64_t groups;
 };
 
-// The three bf16 terms of eight f32: x = t0 + t1 + t2 up to 2^-24 of |x|.  A finite x whose rounding
-// to bf16 would overflow takes the largest bf16 first; an infinite or NaN x is whole in t0.
+// The three bf16 terms of eight f32, x = t0 + t1 + t2 exactly (but for what is below f32's smallest
+// normal number): the upper 16 bits of x, of what that leaves, and of what is then left.  Cutting
+// instead of rounding costs an and and a subtraction a term, and no finite x can overflow.
 __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&t)[3]) {
   uint32_t w[3][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float a = x[2 * i], b = x[2 * i + 1];
+    uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      constexpr float kMost = 0x1.fep127f;
-      w[k][i] = pack2_t<__nv_bfloat16>(isfinite(a) ? fminf(fmaxf(a, -kMost), kMost) : a,
-                                       isfinite(b) ? fminf(fmaxf(b, -kMost), kMost) : b);
-      const float2 r = unpack2<__nv_bfloat16>(w[k][i]);
-      a = isfinite(r.x) ? a - r.x : 0.f;
-      b = isfinite(r.y) ? b - r.y : 0.f;
+      w[k][i] = __byte_perm(a, b, 0x7632);
+      if (k < 2) {
+        a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
+        b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
+      }
     }
   }
 #pragma unroll

@@ -6,20 +6,19 @@
 //   silu:    z s;        s (1 + z (1 - s))
 //   gelu:    z Phi(z);   Phi(z) + z phi(z)    Phi, phi of the standard normal
 //
-// Two forms.  FAST = false, for f32 tensors: sigmoidf (a few ulp) and CUDA's
-// erff.  FAST = true, for 16-bit tensors, relative error below 2^-16 where the
-// value matters to them, on two elements at a time, because the epilogues that
-// call it are bound by the multi-function unit and by issue slots:
-//   - two sigmoids share one reciprocal: with d = 1 + e^-z, 1 / d0 = d1 / (d0 d1).
-//     The exponent is held below 2^60 so that the product cannot overflow; a
-//     sigmoid below 2^-60 (z < -41) is 2^-60.
-//   - Phi(-u) = e^(-u^2 / 2) t Q(t), t = 1 / (1 + 0.31 u), u >= 0: the form of
-//     Hastings' approximations with a polynomial of degree 5 fitted to
-//     Phi(-u) e^(u^2 / 2) / t on u in [0, 14] for the least largest relative
-//     error, 4.7e-6; the exponential serves the slope too.
+// Two elements at a time, because the epilogues that call it are bound by the
+// multi-function unit and by issue slots.  Two forms: FAST = false, for f32
+// tensors, within a few units of f32's last place; FAST = true, for 16-bit ones,
+// relative error below 2^-16 where the value matters to them.
+//   - FAST: two sigmoids share one reciprocal: with d = 1 + e^-z, 1 / d0 =
+//     d1 / (d0 d1).  The exponent is held below 2^60 so that the product cannot
+//     overflow; a sigmoid below 2^-60 (z < -41) is 2^-60.
+//   - Phi(-u) = e^(-u^2 / 2) t Q(t), t = 1 / (1 + c u), u >= 0: the form of
+//     Hastings' approximations, Q fitted to Phi(-u) e^(u^2 / 2) / t on u in [0, 14]
+//     for the least largest relative error (degree 5, c = 0.31: 4.7e-6; degree 8,
+//     c = 0.265: 1.2e-8).  No cancellation for z < 0, and the exponential serves
+//     the slope too.
 #pragma once
-
-#include <math.h>
 
 #include "../../include/af2cuda.h"
 #include "af2_device.cuh"
@@ -46,16 +45,29 @@ __device__ __forceinline__ float2 sigmoid2_fast(float2 z) {
 }
 
 // Phi and, for the slope, e^(-z^2 / 2).
-__device__ __forceinline__ float2 normal_cdf2_fast(float2 z, float2 &e) {
+template <bool FAST>
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2 &e) {
   const float2 arg = f2mul(f2mul(z, z), f2(-0.72134752044448170f));
   e = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
-  const float2 d = f2fma(make_float2(fabsf(z.x), fabsf(z.y)), f2(0.31f), f2(1.f));
+  const float2 d = f2fma(make_float2(fabsf(z.x), fabsf(z.y)), f2(FAST ? 0.31f : 0.265f), f2(1.f));
   const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
-  float2 q = f2fma(f2(-0.07392890751361847f), t, f2(0.1804496943950653f));
-  q = f2fma(q, t, f2(0.015745392069220543f));
-  q = f2fma(q, t, f2(0.13342945277690887f));
-  q = f2fma(q, t, f2(0.12044135481119156f));
-  q = f2fma(q, t, f2(0.12386069446802139f));
+  float2 q;
+  if constexpr (FAST) {
+    q = f2fma(f2(-0.07392890751361847f), t, f2(0.1804496943950653f));
+    q = f2fma(q, t, f2(0.015745392069220543f));
+    q = f2fma(q, t, f2(0.13342945277690887f));
+    q = f2fma(q, t, f2(0.12044135481119156f));
+    q = f2fma(q, t, f2(0.12386069446802139f));
+  } else {
+    q = f2fma(f2(0.030820608139038086f), t, f2(-0.14422746002674103f));
+    q = f2fma(q, t, f2(0.21781262755393982f));
+    q = f2fma(q, t, f2(-0.11636003851890564f));
+    q = f2fma(q, t, f2(0.13795138895511627f));
+    q = f2fma(q, t, f2(0.06031380966305733f));
+    q = f2fma(q, t, f2(0.10270080715417862f));
+    q = f2fma(q, t, f2(0.10524668544530869f));
+    q = f2fma(q, t, f2(0.10574156045913696f));
+  }
   const float2 w = f2mul(f2mul(q, t), e);
   return make_float2(z.x < 0.f ? w.x : 1.f - w.x, z.y < 0.f ? w.y : 1.f - w.y);
 }
@@ -70,12 +82,8 @@ __device__ __forceinline__ float2 activate2(float2 z) {
   if constexpr (ACT == AF2_ACTIVATION_SILU)
     return f2mul(z, FAST ? sigmoid2_fast(z) : make_float2(sigmoidf(z.x), sigmoidf(z.y)));
   if constexpr (ACT == AF2_ACTIVATION_GELU) {
-    if constexpr (FAST) {
-      float2 e;
-      return f2mul(z, normal_cdf2_fast(z, e));
-    }
-    return make_float2(z.x * fmaf(0.5f, erff(z.x * 0.70710678118654752f), 0.5f),
-                       z.y * fmaf(0.5f, erff(z.y * 0.70710678118654752f), 0.5f));
+    float2 e;
+    return f2mul(z, normal_cdf2<FAST>(z, e));
   }
   return z;
 }
@@ -90,14 +98,8 @@ __device__ __forceinline__ void activate_slope2(float2 z, float2 &value, float2 
     value = make_float2(relu(z.x), relu(z.y));
     slope = make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
   } else if constexpr (ACT == AF2_ACTIVATION_GELU) {
-    float2 cdf, e;
-    if constexpr (FAST) {
-      cdf = normal_cdf2_fast(z, e);
-    } else {
-      cdf = make_float2(fmaf(0.5f, erff(z.x * 0.70710678118654752f), 0.5f),
-                        fmaf(0.5f, erff(z.y * 0.70710678118654752f), 0.5f));
-      e = make_float2(exp2f(z.x * z.x * -0.72134752044448170f), exp2f(z.y * z.y * -0.72134752044448170f));
-    }
+    float2 e;
+    const float2 cdf = normal_cdf2<FAST>(z, e);
     value = f2mul(z, cdf);
     slope = f2fma(f2mul(z, f2(0.39894228040143268f)), e, cdf);
   } else {
