@@ -22,8 +22,9 @@
 // the six products whose weight is at least 2^-16 of the largest are summed:
 // what is left out is below 2^-24 of |x||y|, f32's own rounding.  A K step's
 // three terms of both operands are in shared memory together, so each is read
-// once for its products (one read for each product was bound by L2: 900 SM
-// clocks a product and step of a 256 x 128 tile against 256 of work).  The
+// once for its products (one read for each product took 900 SM clocks a product
+// and step of 64 against 256 of work), and a step is 32 deep, so that the ring
+// holds four (with 64 it held two, and waited for each load).  The
 // tensor core cuts its sums where f32 rounds them (some 2^-27 of the sum lost
 // at each step of 16: sums of one sign over a depth of 4096 came out 2e-6 low),
 // so the five small products have an accumulator of their own, and a tile is
@@ -42,7 +43,6 @@ namespace {
 
 constexpr int BM = 128, PAIR_M = 256, BK = 64;
 constexpr int EPI_WARPS = 16, THREADS = 64 + 32 * EPI_WARPS;
-constexpr uint32_t A_BYTES = BM * 128;
 constexpr int kPairs = 74;  // CTA pairs of a B200; only the choice of tiles and splits depends on it
 
 // The kernels behind the epilogues: Out, the same for several products with nothing but their sums
@@ -53,10 +53,14 @@ enum Kind { kOut, kProducts, kGate, kGateSave, kGateBackward };
 // Stages of the operand ring and bytes of one epilogue warp's staging: 32 x 32 blocks of 16 bits
 // (2 KB), two of them (GateBackward: one of each factor); three where h and two factors leave
 // together, paid for with a stage.
-template <int KIND, int BN>
+// f32: a stage has a step's three terms, A's [3][128 x 32] and B's behind them; the staged blocks
+// are 32 x 16.
+template <int KIND, int BN, bool F32>
 struct Shape {
-  static constexpr uint32_t B_BYTES = (BN / 2) * 128;
-  static constexpr uint32_t STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STEP = F32 ? 32 : BK;
+  static constexpr uint32_t A_TERM = BM * STEP * 2, B_TERM = (BN / 2) * STEP * 2;
+  static constexpr uint32_t OFF_B = (F32 ? 3 : 1) * A_TERM;
+  static constexpr uint32_t STAGE_BYTES = OFF_B + (F32 ? 3 : 1) * B_TERM;
   static constexpr uint32_t SLOT_BYTES = KIND == kGateSave ? 6144 : 4096;
   static constexpr int STAGES = (229376 - EPI_WARPS * SLOT_BYTES) / STAGE_BYTES;
   static constexpr uint32_t OFF_STAGE = STAGES * STAGE_BYTES;
@@ -145,7 +149,7 @@ __device__ __forceinline__ Tile tile_at(const Args &p, int t) {
   r.split = t;
   return r;
 }
-constexpr int kPromote = 4;  // K steps of an f32 tile (and segment) before its sums go to registers
+constexpr int kPromote = 8;  // K steps (of 32) of an f32 tile, and segment, before its sums go to registers
 
 // The tile's range of K steps.
 __device__ __forceinline__ int k_begin(const Args &p, int split) {
@@ -176,30 +180,59 @@ __device__ __forceinline__ uint4 *piece16(uint8_t *block, int row, int c) {
 __device__ __forceinline__ uint16_t *element16(uint8_t *block, int row, int col) {
   return reinterpret_cast<uint16_t *>(piece16(block, row, col >> 3)) + (col & 7);
 }
-// The same of a block of f32 (128B-swizzled, 4 KB).
+// 16-byte piece c of a 32 x 32 block of f32 (128B-swizzled, 4 KB).
 __device__ __forceinline__ float4 *piece32(uint8_t *block, int row, int c) {
   return reinterpret_cast<float4 *>(block + sw128_offset(row, c));
 }
-__device__ __forceinline__ float *element32(uint8_t *block, int row, int col) {
-  return reinterpret_cast<float *>(piece32(block, row, col >> 2)) + (col & 3);
-}
 
-// Rows that TMA cannot address, moved between memory and a block with the lanes along each row.
+// Rows that TMA cannot address, moved between memory and a block with the lanes along each row:
+// eight loads, then eight stores (one after the other each waits for its load: a residual in f32
+// took 25,000 clocks a tile).
 template <typename T, bool IN>
 __device__ __forceinline__ void move_rows(uint8_t *block, T *at, int64_t stride, int rows, int cols, int lane) {
-  if (lane < cols)
-    for (int r = 0; r < rows; ++r) {
-      T *s;
-      if constexpr (sizeof(T) == 4)
-        s = element32(block, r, lane);
-      else
-        s = reinterpret_cast<T *>(element16(block, r, lane));
-      T *g = at + r * stride + lane;
-      if constexpr (IN)
-        *s = *g;
-      else
-        *g = *s;
+  if (lane >= cols) return;
+  T *g = at + lane;
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (r0 + i < rows) v[i] = IN ? g[(r0 + i) * stride] : *reinterpret_cast<T *>(element16(block, r0 + i, lane));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (r0 + i < rows) {
+        if constexpr (IN)
+          *reinterpret_cast<T *>(element16(block, r0 + i, lane)) = v[i];
+        else
+          g[(r0 + i) * stride] = v[i];
+      }
+  }
+}
+// The same of 16 columns of f32, two rows at a time.
+template <bool IN>
+__device__ __forceinline__ void move_rows_f32(uint8_t *block, float *at, int64_t stride, int rows, int cols, int lane) {
+  const int c = lane & 15;
+  if (c >= cols) return;
+  float *g = at + c;
+  auto s = [&](int r) { return reinterpret_cast<float *>(piece16(block, r, c >> 2)) + (c & 3); };
+#pragma unroll
+  for (int r0 = 0; r0 < 32; r0 += 16) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 2 * i + (lane >> 4);
+      if (r < rows) v[i] = IN ? g[r * stride] : *s(r);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 2 * i + (lane >> 4);
+      if (r < rows) {
+        if constexpr (IN)
+          *s(r) = v[i];
+        else
+          g[r * stride] = v[i];
+      }
+    }
+  }
 }
 
 // x[i] of lane l becomes, in x[0] of lane i, the sum over the lanes: 31 exchanges for 32 columns.
@@ -219,7 +252,7 @@ __device__ __forceinline__ float lane_sums(float (&x)[32], int lane) {
 template <int KIND, typename OT, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     layer_gemm_kernel(const __grid_constant__ Launch<KIND == kProducts ? kMaxProducts : 1> launch) {
-  using S = Shape<KIND, BN>;
+  using S = Shape<KIND, BN, sizeof(OT) == 4>;
   constexpr bool GATE = KIND == kGate || KIND == kGateSave;
   constexpr bool F32 = sizeof(OT) == 4;
   constexpr int STAGES = S::STAGES;
@@ -285,37 +318,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int arow = tile.mi * PAIR_M + rank * BM;
         const int brow = GATE ? tile.ni * (BN / 2) : tile.ni * BN + rank * (BN / 2);
         const int segments = p.segments, a_mn = p.a_mn, b_mn = p.b_mn, part = F32 ? kPromote : kb1 - kb0;
-        // K steps of a part, segment by segment; f32: a stage for each of a step's three terms
+        // K steps of a part, segment by segment
         for (int from = kb0; from < kb1 && ok; from += part) {
           for (int seg = 0; seg < segments && ok; ++seg) {
             const CUtensorMap *am = &maps.a[seg];
             const CUtensorMap *bm = &maps.b[GATE ? rank : seg + tile.z];
             for (int kb = from; kb < min(from + part, kb1) && ok; ++kb) {
-              for (int term = 0; term < (F32 ? 3 : 1); ++term, ++it) {
-                // the stage is free in this CTA once the pair's MMAs have read it (multicast commit)
-                if (!mbar_wait(empty(s), ph, abort_flag, launch.err, kErrWaitProducer)) {
-                  ok = false;
-                  break;
-                }
-                const uint32_t dst = sbase + s * S::STAGE_BYTES;
-                if (leader) mbar_arrive_expect_tx(full(s), 2 * S::STAGE_BYTES);
+              // the stage is free in this CTA once the pair's MMAs have read it (multicast commit)
+              if (!mbar_wait(empty(s), ph, abort_flag, launch.err, kErrWaitProducer)) {
+                ok = false;
+                break;
+              }
+              const uint32_t stage = sbase + s * S::STAGE_BYTES;
+              if (leader) mbar_arrive_expect_tx(full(s), 2 * S::STAGE_BYTES);
+#pragma unroll
+              for (int term = 0; term < (F32 ? 3 : 1); ++term) {
+                const uint32_t dst = stage + term * S::A_TERM, dst_b = stage + S::OFF_B + term * S::B_TERM;
                 if (a_mn) {
-                  tma_load_3d_pair(dst, am, full(s), arow, kb * BK, term);
-                  tma_load_3d_pair(dst + 8192, am, full(s), arow + 64, kb * BK, term);
+                  tma_load_3d_pair(dst, am, full(s), arow, kb * S::STEP, term);
+                  tma_load_3d_pair(dst + S::STEP * 128, am, full(s), arow + 64, kb * S::STEP, term);
                 } else {
-                  tma_load_3d_pair(dst, am, full(s), kb * BK, arow, term);
+                  tma_load_3d_pair(dst, am, full(s), kb * S::STEP, arow, term);
                 }
                 if (b_mn) {
 #pragma unroll
                   for (int j = 0; j < BN / 128; ++j)
-                    tma_load_3d_pair(dst + A_BYTES + j * 8192, bm, full(s), brow + 64 * j, kb * BK, term);
+                    tma_load_3d_pair(dst_b + j * S::STEP * 128, bm, full(s), brow + 64 * j, kb * S::STEP, term);
                 } else {
-                  tma_load_3d_pair(dst + A_BYTES, bm, full(s), kb * BK, brow, term);
+                  tma_load_3d_pair(dst_b, bm, full(s), kb * S::STEP, brow, term);
                 }
-                if (++s == STAGES) {
-                  s = 0;
-                  ph ^= 1;
-                }
+              }
+              ++it;
+              if (++s == STAGES) {
+                s = 0;
+                ph ^= 1;
               }
             }
           }
@@ -336,9 +372,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       for (int t = pair; t < launch.total_tiles && ok; t += npairs) {
         const Args &p = product_of(launch, t).args;
         const uint32_t idesc = idesc_16_f32(PAIR_M, BN, p.bf16, p.a_mn, p.b_mn);
-        const uint64_t a_base = p.a_mn ? sdesc_mn_sw128(sbase, 8192, 1024) : sdesc_k_sw128(sbase);
-        const uint64_t b_base =
-            p.b_mn ? sdesc_mn_sw128(sbase + A_BYTES, 8192, 1024) : sdesc_k_sw128(sbase + A_BYTES);
+        auto k_major = [](uint32_t at) { return F32 ? sdesc_k_sw64(at) : sdesc_k_sw128(at); };
+        const uint64_t a_base = p.a_mn ? sdesc_mn_sw128(sbase, S::STEP * 128, 1024) : k_major(sbase);
+        const uint64_t b_base = p.b_mn ? sdesc_mn_sw128(sbase + S::OFF_B, S::STEP * 128, 1024) : k_major(sbase + S::OFF_B);
         // bytes >> 4 from one K step of 16 to the next
         const uint32_t a_step = p.a_mn ? 2048 >> 4 : 32 >> 4, b_step = p.b_mn ? 2048 >> 4 : 32 >> 4;
         uint64_t ad = desc_add(a_base, s * S::STAGE_BYTES), bd = desc_add(b_base, s * S::STAGE_BYTES);
@@ -357,36 +393,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           tc_fence_after();
           const uint32_t d = tmem + buf * 256;
           for (int i = 0; i < iters; ++i) {
+            if (!warp_wait(full(s), ph, abort_flag, launch.err, kErrWaitMma)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
             if constexpr (F32) {
-              static_assert(STAGES % 3 == 0, "a step's three stages do not wrap");
-#pragma unroll
-              for (int term = 0; term < 3; ++term) ok = ok && warp_wait(full(s + term), ph, abort_flag, launch.err, kErrWaitMma);
-              if (!ok) break;
-              tc_fence_after();
 #pragma unroll
               for (int c = 0; c < kProductsF32; ++c)
 #pragma unroll
-                for (int ks = 0; ks < BK / 16; ++ks)
-                  umma_pair(d + (c < kProductsF32 - 1 ? 128 : 0), desc_add(ad, term_a(c) * S::STAGE_BYTES) + ks * a_step,
-                            desc_add(bd, term_b(c) * S::STAGE_BYTES) + ks * b_step, idesc,
+                for (int ks = 0; ks < S::STEP / 16; ++ks)
+                  umma_pair(d + (c < kProductsF32 - 1 ? 128 : 0), desc_add(ad, term_a(c) * S::A_TERM) + ks * a_step,
+                            desc_add(bd, term_b(c) * S::B_TERM) + ks * b_step, idesc,
                             (i | ks | (c < kProductsF32 - 1 ? c : 0)) != 0);
             } else {
-              if (!warp_wait(full(s), ph, abort_flag, launch.err, kErrWaitMma)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
 #pragma unroll
               for (int ks = 0; ks < BK / 16; ++ks)
                 umma_pair(d, ad + ks * a_step, bd + ks * b_step, idesc, (i | ks) != 0);
             }
-            constexpr int TAKEN = F32 ? 3 : 1;
-#pragma unroll
-            for (int term = 0; term < TAKEN; ++term) umma_commit_pair_both(empty(s + term));
-            ad += TAKEN * S::STAGE_BYTES >> 4;
-            bd += TAKEN * S::STAGE_BYTES >> 4;
-            s += TAKEN;
-            if (s == STAGES) {
+            umma_commit_pair_both(empty(s));
+            ad += S::STAGE_BYTES >> 4;
+            bd += S::STAGE_BYTES >> 4;
+            if (++s == STAGES) {
               s = 0;
               ph ^= 1;
               ad = a_base;
@@ -426,14 +454,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       bool ok = true;
       // f32: the sums of each part of the depth, into registers (each warp has one block: BN is 128)
       [[maybe_unused]] float sums[32];
-      auto add_part = [&](int b) {
-        uint32_t r[32], small[32];
+      auto add_part = [&](int b, int from, int to) {
         const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + first * 32;
-        tmem_ld32(at, r);
-        tmem_ld32(at + 128, small);
-        tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) sums[i] += __uint_as_float(r[i]) + __uint_as_float(small[i]);
+        for (int c = 0; c < 32; c += 16) {  // (all at once takes more registers than there are)
+          if (c < from || c >= to) continue;
+          uint32_t r[16], small[16];
+          tmem_ld16(at + c, r);
+          tmem_ld16(at + 128 + c, small);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sums[c + i] += __uint_as_float(r[i]) + __uint_as_float(small[i]);
+        }
       };
       if constexpr (F32) {
 #pragma unroll
@@ -445,7 +477,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           ok = warp_wait(acc_full(b), (acc_it >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
           if (!ok) break;
           tc_fence_after();
-          if (first < end) add_part(b);
+          if (first < end) add_part(b, 0, 32);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_leader_relaxed(acc_empty(b));
@@ -597,57 +629,144 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int z = partial ? tile.split * static_cast<int>(p.batches.d) + tile.z : 0;
         const CUtensorMap *omap = &maps.out[partial ? 0 : tile.z];
         // the residual's blocks come ahead, each into the block that its result leaves from
+        // (f32: the two halves of the warp's only block of columns)
         auto fetch = [&](int b, int at) {
           if (lane == 0) {
             bulk_wait_read_all();
-            mbar_arrive_expect_tx(load(ew, at & 1), 2048);
-            tma_load_3d(block_addr + (at & 1) * 2048, &maps.residual, load(ew, at & 1), n0 + b * 32, r0, 0);
+            mbar_arrive_expect_tx(load(ew, at & 1), F32 ? 4096 : 2048);
+            tma_load_3d(block_addr + (at & 1) * (F32 ? 0 : 2048), &maps.residual, load(ew, at & 1), n0 + b * 32, r0, 0);
+            if (F32) tma_load_3d(block_addr + 2048, &maps.residual, load(ew, at & 1), n0 + b * 32 + 16, r0, 0);
           }
         };
+        const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0));
         if (tma_residual && first < end) fetch(first, loads);
+        if constexpr (F32) {
+          if (residual && !tma_residual && first < end) {
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              const int c = n0 + first * 32 + 16 * h;
+              move_rows_f32<true>(block + 2048 * h, const_cast<float *>(residual) + static_cast<int64_t>(r0) * p.residual_stride + c,
+                                  p.residual_stride, rows, min(16, p.n - c), lane);
+            }
+            __syncwarp();
+          }
+        }
         if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) {
           if (tma_residual && first < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
           break;
         }
         tc_fence_after();
+        if constexpr (F32) {
+          if (first < end) {
+            if (tma_residual) {
+              ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
+              ++loads;
+              if (!ok) break;
+            }
+            const float *bias = PLAIN || partial ? nullptr : static_cast<const float *>(p.bias[tile.z]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              add_part(buf, 16 * h, 16 * h + 16);
+              const int c0 = n0 + first * 32 + 16 * h;
+              if (c0 >= p.n) break;
+              float *y = sums + 16 * h;
+              const int cols = min(16, p.n - c0);
+              if (bias) {
+                if (p.vector_bias && cols == 16) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const float4 u = __ldg(reinterpret_cast<const float4 *>(bias + c0) + i);
+                    y[4 * i] += u.x, y[4 * i + 1] += u.y, y[4 * i + 2] += u.z, y[4 * i + 3] += u.w;
+                  }
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) y[i] += i < cols ? __ldg(bias + c0 + i) : 0.f;
+                }
+              }
+              if (!PLAIN && !partial && p.activation != AF2_ACTIVATION_NONE)
+                with_activation(p.activation, [&](auto act) {
+                  constexpr int ACT = decltype(act)::value;
+                  if (p.save) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                      float2 value[2], s[2];
+#pragma unroll
+                      for (int i = 0; i < 2; ++i)
+                        activate_slope2<ACT, false>(make_float2(y[4 * c + 2 * i], y[4 * c + 2 * i + 1]), value[i], s[i]);
+                      y[4 * c] = value[0].x, y[4 * c + 1] = value[0].y, y[4 * c + 2] = value[1].x, y[4 * c + 3] = value[1].y;
+                      if (m < p.m)
+                        *reinterpret_cast<float4 *>(p.saved_f32 + m * p.saved_pitch + c0 + 4 * c) =
+                            make_float4(s[0].x, s[0].y, s[1].x, s[1].y);
+                    }
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                      const float2 v2 = activate2<ACT, false>(make_float2(y[2 * i], y[2 * i + 1]));
+                      y[2 * i] = v2.x;
+                      y[2 * i + 1] = v2.y;
+                    }
+                  }
+                });
+              // out of the half's own block where the residual is in it, else of the two in turn
+              const uint32_t at = 2048u * (residual ? h : stores++ & 1);
+              uint8_t *const dst = block + at;
+              if (!residual) {
+                if (lane == 0) bulk_wait_read_but_one();
+                __syncwarp();
+              }
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float4 o = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+                float4 *piece = reinterpret_cast<float4 *>(piece16(dst, lane, c));
+                if (residual) {
+                  const float4 res = *piece;
+                  o.x += res.x, o.y += res.y, o.z += res.z, o.w += res.w;
+                }
+                *piece = o;
+              }
+              if (p.tma_out) {
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_3d(omap, block_addr + at, c0, r0, z);
+                  bulk_commit();
+                }
+              } else {
+                __syncwarp();
+                move_rows_f32<false>(dst, static_cast<float *>(p.out[tile.z]) + static_cast<int64_t>(r0) * p.out_stride + c0,
+                                     p.out_stride, rows, cols, lane);
+                __syncwarp();
+              }
+            }
+          }
+        } else {
 #pragma unroll 1
         for (int b = first; b < end; b += step) {
           const int c0 = n0 + b * 32;
           uint32_t r[32];
-          if constexpr (F32) {
-            add_part(buf);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(sums[i]);
-          } else {
-            tmem_ld32(taddr + b * 32, r);
-          }
+          tmem_ld32(taddr + b * 32, r);
           if (tma_residual && b + step < end) fetch(b + step, loads + 1);
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
-          const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0)), cols = min(32, p.n - c0);
+          const int cols = min(32, p.n - c0);
           const OT *bias = PLAIN || partial ? nullptr : static_cast<const OT *>(p.bias[tile.z]);
-          if constexpr (sizeof(OT) == 2) {
-            uint32_t bw[2][8] = {};
-            if (bias) {
-              load_raw16(bias, c0, p.n, p.vector_bias, bw[0]);
-              load_raw16(bias, c0 + 16, p.n, p.vector_bias, bw[1]);
-            }
-            tmem_ld_wait();
-            if (bias) {
+          uint32_t bw[2][8] = {};
+          if (bias) {
+            load_raw16(bias, c0, p.n, p.vector_bias, bw[0]);
+            load_raw16(bias, c0 + 16, p.n, p.vector_bias, bw[1]);
+          }
+          tmem_ld_wait();
+          if (bias) {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float2 s2 = f2add(make_float2(y[2 * i], y[2 * i + 1]), unpack2<OT>(bw[i >> 3][i & 7]));
-                y[2 * i] = s2.x;
-                y[2 * i + 1] = s2.y;
-              }
-            }
-          } else {
-            if (bias) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] += i < cols ? bias[c0 + i] : 0.f;
+            for (int i = 0; i < 16; ++i) {
+              const float2 s2 = f2add(make_float2(y[2 * i], y[2 * i + 1]), unpack2<OT>(bw[i >> 3][i & 7]));
+              y[2 * i] = s2.x;
+              y[2 * i + 1] = s2.y;
             }
           }
           if (!PLAIN && !partial && p.activation != AF2_ACTIVATION_NONE) {
-            if (p.save) {  // the slopes, through the first block (16 bits) or directly (f32)
+            if (p.save) {  // the slopes, through the first block
               if (lane == 0) bulk_wait_read_all();
               __syncwarp();
               with_activation(p.activation, [&](auto act) {
@@ -658,64 +777,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
                     float2 v2;
-                    activate_slope2<ACT, sizeof(OT) == 2>(make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]), v2, s[i]);
+                    activate_slope2<ACT, true>(make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]), v2, s[i]);
                     y[8 * c + 2 * i] = v2.x;
                     y[8 * c + 2 * i + 1] = v2.y;
                   }
-                  if constexpr (sizeof(OT) == 4) {
-                    if (m < p.m) {
-                      float4 *dst = reinterpret_cast<float4 *>(p.saved_f32 + m * p.saved_pitch + c0 + 8 * c);
-                      dst[0] = make_float4(s[0].x, s[0].y, s[1].x, s[1].y);
-                      dst[1] = make_float4(s[2].x, s[2].y, s[3].x, s[3].y);
-                    }
-                  } else {
-                    *piece16(block, lane, c) =
-                        make_uint4(Factor<OT>::slope(s[0]), Factor<OT>::slope(s[1]), Factor<OT>::slope(s[2]),
-                                   Factor<OT>::slope(s[3]));
-                  }
+                  *piece16(block, lane, c) = make_uint4(Factor<OT>::slope(s[0]), Factor<OT>::slope(s[1]),
+                                                        Factor<OT>::slope(s[2]), Factor<OT>::slope(s[3]));
                 }
               });
-              if constexpr (sizeof(OT) == 2) {
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                  tma_store_3d(&maps.half, block_addr, c0, r0, 0);
-                  bulk_commit();
-                }
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_3d(&maps.half, block_addr, c0, r0, 0);
+                bulk_commit();
               }
             } else {
               with_activation(p.activation, [&](auto act) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                  const float2 v2 = activate2<decltype(act)::value, sizeof(OT) == 2>(make_float2(y[2 * i], y[2 * i + 1]));
+                  const float2 v2 = activate2<decltype(act)::value, true>(make_float2(y[2 * i], y[2 * i + 1]));
                   y[2 * i] = v2.x;
                   y[2 * i + 1] = v2.y;
                 }
               });
             }
           }
-          if constexpr (sizeof(OT) == 2) {
-            if (partial) {  // the f32 sums, through both blocks
-              if (lane == 0) bulk_wait_read_all();
-              __syncwarp();
+          if (partial) {  // the f32 sums, through both blocks
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *piece32(block, lane, c) = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
-              fence_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_3d(omap, block_addr, c0, r0, z);
-                bulk_commit();
-              }
-              continue;
+            for (int c = 0; c < 8; ++c)
+              *piece32(block, lane, c) = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(omap, block_addr, c0, r0, z);
+              bulk_commit();
             }
+            continue;
           }
-          // the block that the result leaves from (f32: both), with the residual in it where there is one
-          uint32_t at = 0;
-          if constexpr (sizeof(OT) == 2)
-            at = 2048u * (tma_residual ? loads & 1
-                          : !PLAIN && p.save ? 1  // the first block may still hold slopes
-                                         : stores++ & 1);
+          // the block that the result leaves from, with the residual in it where there is one
+          const uint32_t at = 2048u * (tma_residual       ? loads & 1
+                                       : !PLAIN && p.save ? 1  // the first block may still hold slopes
+                                                          : stores++ & 1);
           uint8_t *const dst = block + at;
           if (tma_residual) {
             ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
@@ -726,7 +830,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
           } else {
             if (lane == 0) {
-              if (sizeof(OT) == 4 || PLAIN)
+              if (PLAIN)
                 bulk_wait_read_all();  // (f32 sums of another product may be leaving both blocks)
               else
                 bulk_wait_read_but_one();
@@ -738,34 +842,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               __syncwarp();
             }
           }
-          if constexpr (sizeof(OT) == 4) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              float4 o = make_float4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
-              float4 *piece = piece32(dst, lane, c);
-              if (residual) {
-                const float4 res = *piece;
-                o.x += res.x, o.y += res.y, o.z += res.z, o.w += res.w;
-              }
-              *piece = o;
+          for (int c = 0; c < 4; ++c) {
+            uint4 *piece = piece16(dst, lane, c);
+            uint32_t w[4];
+            if (residual) {
+              const uint4 u = *piece;
+              w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
             }
-          } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint4 *piece = piece16(dst, lane, c);
-              uint32_t w[4];
-              if (residual) {
-                const uint4 u = *piece;
-                w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float2 o = make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]);
-                if (residual) o = f2add(o, unpack2<OT>(w[i]));
-                w[i] = pack2_t<OT>(o.x, o.y);
-              }
-              *piece = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int i = 0; i < 4; ++i) {
+              float2 o = make_float2(y[8 * c + 2 * i], y[8 * c + 2 * i + 1]);
+              if (residual) o = f2add(o, unpack2<OT>(w[i]));
+              w[i] = pack2_t<OT>(o.x, o.y);
             }
+            *piece = make_uint4(w[0], w[1], w[2], w[3]);
           }
           if (p.tma_out) {
             fence_async_smem();
@@ -780,6 +871,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                  p.out_stride, rows, cols, lane);
             __syncwarp();
           }
+        }
         }
         if (!ok) break;
       }
@@ -874,14 +966,16 @@ bool operand_map(CUtensorMap *map, const GemmOperand &o, int64_t outer, int64_t 
                  int box_outer) {
   const CUtensorMapDataType t = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint64_t row = o.pitch * 2, piece = pieces > 1 ? o.piece_stride * 2 : row;  // (one piece: no step)
+  const int step = pieces > 1 ? 32 : BK;
   if (o.mn_major)
-    return encode_map_3d(map, t, o.ptr, outer, k, pieces, row, piece, 64, BK, 1, CU_TENSOR_MAP_SWIZZLE_128B);
-  return encode_map_3d(map, t, o.ptr, k, outer, pieces, row, piece, BK, box_outer, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+    return encode_map_3d(map, t, o.ptr, outer, k, pieces, row, piece, 64, step, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+  return encode_map_3d(map, t, o.ptr, k, outer, pieces, row, piece, step, box_outer, 1,
+                       pieces > 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int KIND, typename OT, int BN>
 af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l, cudaStream_t stream) {
-  constexpr uint32_t smem = Shape<KIND, BN>::BYTES;
+  constexpr uint32_t smem = Shape<KIND, BN, sizeof(OT) == 4>::BYTES;
   auto kernel = layer_gemm_kernel<KIND, OT, BN>;
   static std::atomic<uint64_t> allowed{0};  // devices on which this kernel has its shared memory
   const uint64_t bit = uint64_t(1) << (ctx->device & 63);
@@ -927,7 +1021,7 @@ CUtensorMapDataType map_type(int dtype) {
 // Tile width and the parts that each depth is cut into, from what a launch costs in SM clocks.  A pair
 // takes tiles pair, pair + 74, ...; with the products in order of their tiles' cost the first pair
 // has the most.  A K step of 64 takes 512 (BN = 256) or 420 (BN = 128; the ring's latency) clocks, in
-// f32 1800, a tile's hand-over 800, and split sums are written, read and reduced by another launch.
+// f32 900 for 32, a tile's hand-over 800, and split sums are written, read and reduced by another launch.
 void layer_gemm_plan(LayerGemm *g, int count) {
   const bool f32 = g[0].pieces > 1;
   const bool gate = g[0].epilogue == kEpilogueGate;
@@ -935,7 +1029,7 @@ void layer_gemm_plan(LayerGemm *g, int count) {
   for (int bn : {256, 128}) {
     if (g[0].epilogue == kEpilogueGateBackward && bn == 128) continue;
     if (f32 && bn == 256) continue;
-    const double step_clocks = f32 ? 1800 : bn == 256 ? 512 : 420;
+    const double step_clocks = f32 ? 900 : bn == 256 ? 512 : 420;  // (a step of 32 in f32)
     // `most`: K steps that a tile may have before its depth is cut
     for (int64_t most : {int64_t(1) << 40, int64_t(512), int64_t(384), int64_t(256), int64_t(192), int64_t(128),
                          int64_t(96), int64_t(64), int64_t(48), int64_t(32), int64_t(24), int64_t(16), int64_t(12),
@@ -946,7 +1040,7 @@ void layer_gemm_plan(LayerGemm *g, int count) {
       double bytes = 0;
       bool split = false;
       for (int i = 0; i < count; ++i) {
-        const int64_t k_blocks = ceil_div(g[i].k, BK), all = k_blocks * g[i].segments;
+        const int64_t k_blocks = ceil_div(g[i].k, f32 ? 32 : BK), all = k_blocks * g[i].segments;
         splits[i] = static_cast<int>(std::max<int64_t>(1, std::min({ceil_div(all, most), (k_blocks + 1) / 2, int64_t(64)})));
         part[i].tiles = splits[i] * g[i].batch * ceil_div(g[i].m, PAIR_M) * ceil_div(g[i].n, gate ? bn / 2 : bn);
         part[i].steps = ceil_div(k_blocks, splits[i]) * g[i].segments;
@@ -990,7 +1084,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
   Args &p = product->args;
   p.m = g.m;
   p.n = static_cast<int>(g.n);
-  p.k_blocks = static_cast<int>(ceil_div(g.k, BK));
+  p.k_blocks = static_cast<int>(ceil_div(g.k, g.pieces > 1 ? 32 : BK));
   p.splits = g.splits;
   p.segments = g.segments;
   p.batches = Divisor(g.batch);
@@ -1016,15 +1110,17 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
     p.partial = 1;
     p.tma_out = 1;
     maps_ok &= encode_map_3d(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.scratch, g.n, g.m, g.splits * g.batch,
-                             pitch * 4, g.m * pitch * 4, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+                             pitch * 4, g.m * pitch * 4, g.pieces > 1 ? 16 : 32, 32, 1,
+                             g.pieces > 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
   } else {
     p.activation = g.activation;
     p.residual = g.residual;
     p.residual_stride = g.residual_stride;
-    if (g.residual && !g.saved.half && out_bytes == 2 && aligned16(g.residual, g.residual_stride, 2)) {
+    if (g.residual && !g.saved.half && aligned16(g.residual, g.residual_stride, out_bytes)) {
       p.tma_residual = 1;
-      maps_ok &= encode_map_3d(&maps.residual, map_type(g.out_dtype), g.residual, g.n, g.m, 1, g.residual_stride * 2,
-                               g.residual_stride * 2, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
+      const int64_t row = g.residual_stride * out_bytes;
+      maps_ok &= encode_map_3d(&maps.residual, map_type(g.out_dtype), g.residual, g.n, g.m, 1, row, row,
+                               out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     }
     p.out_stride = g.out_stride;
     p.vector_bias = 1;
@@ -1038,8 +1134,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
     if (p.tma_out)
       for (int i = 0; i < outs; ++i)
         maps_ok &= encode_map_3d(&maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
-                                 g.out_stride * out_bytes, 32, 32, 1,
-                                 out_bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                                 g.out_stride * out_bytes, out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     p.save = g.saved.half || g.saved.f32;
     p.saved_f32 = g.saved.f32;
     p.saved_scale = g.saved.scale;
