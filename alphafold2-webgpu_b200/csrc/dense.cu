@@ -68,18 +68,56 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&t)[3]) {
   for (int k = 0; k < 3; ++k) t[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
 }
 
+// Eight values of a row as they are in memory (nothing is computed from them yet, so that a thread's
+// loads need not wait for one another), and as f32; zeros past the first n.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, int n, float (&x)[8]) {
+struct Raw8 {
+  uint32_t w[2 * sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ void load_raw8(const T *p, int n, Raw8<T> &x) {
+  constexpr int WORDS = 2 * sizeof(T);
   if (n >= 8 && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-      unpack8<T>(*reinterpret_cast<const uint4 *>(p), x);
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 u = reinterpret_cast<const uint4 *>(p)[i / 4];
+      x.w[i] = u.x, x.w[i + 1] = u.y, x.w[i + 2] = u.z, x.w[i + 3] = u.w;
+    }
+  } else if (n >= 8 && reinterpret_cast<uintptr_t>(p) % (2 * sizeof(T)) == 0) {  // rows of an even length
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        const uint2 u = reinterpret_cast<const uint2 *>(p)[i];
+        x.w[2 * i] = u.x, x.w[2 * i + 1] = u.y;
+      } else {
+        x.w[i] = reinterpret_cast<const uint32_t *>(p)[i];
+      }
     }
   } else {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < n ? to_f32<T>(p[i]) : 0.f;
+      for (int i = 0; i < 8; ++i) x.w[i] = i < n ? reinterpret_cast<const uint32_t *>(p)[i] : 0u;
+    } else {
+      const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = 2 * i < n ? q[2 * i] : 0u, hi = 2 * i + 1 < n ? q[2 * i + 1] : 0u;
+        x.w[i] = lo | (hi << 16);
+      }
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void values8(const Raw8<T> &r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 v;
+    if constexpr (sizeof(T) == 4)
+      v = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    else
+      v = unpack2<T>(r.w[i]);
+    x[2 * i] = v.x;
+    x[2 * i + 1] = v.y;
   }
 }
 
@@ -107,64 +145,104 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
     while (j + 1 < p.count && g >= p.job[j + 1].first) ++j;
     const PackJob &job = p.job[j];
     const int64_t per_row = job.pitch / 8, at = g - job.first, r = at / per_row, c = (at - r * per_row) * 8;
+    Raw8<T> raw;
+    load_raw8<T>(static_cast<const T *>(job.src) + r * job.stride + c,
+                 static_cast<int>(min(static_cast<int64_t>(8), job.width - c)), raw);
     float x[8];
-    load8<T>(static_cast<const T *>(job.src) + r * job.stride + c,
-             static_cast<int>(min(static_cast<int64_t>(8), job.width - c)), x);
+    values8<T>(raw, x);
     store_operand8<T>(job.dst, r * job.pitch + c, job.piece_stride, x);
   }
 }
 
 // ---- passes over rows, with column sums --------------------------------------------
 
-// Rows of a block: 64, fewer where that would leave SMs without one.
-inline int row_group(int64_t rows, int64_t width) {
-  int r = 64;
-  while (r > 8 && ceil_div(rows, r) * ceil_div(width, 256) < 296) r /= 2;
-  return r;
+// How a pass covers its rows: `lanes` threads of eight columns each along a row and `at_once` rows side
+// by side in a block of 256 threads, `group` rows a block, `across` blocks along the width.  Few threads
+// are left without work (at a width of 320, 40 lanes and six rows instead of 64 lanes of which 24 would
+// idle), and among the splits of the width that are within 1/16 of the best the narrowest is taken:
+// blocks of more rows have fewer sums to write and to join (16384 x 4096 bf16 in two blocks of 256 lanes
+// took 117 us, in 16 of 32 lanes 80).  A thread has eight rows, fewer where that would leave SMs without
+// a block.
+struct RowGrid {
+  int lanes, at_once, group;
+  unsigned across;
+};
+inline RowGrid row_grid(int64_t rows, int64_t width) {
+  const int64_t pieces = ceil_div(width, 8), least = ceil_div(pieces, 256);
+  RowGrid g{};
+  int64_t best = 0;
+  for (int pass = 0; pass < 2; ++pass)
+    for (int64_t n = least; n < least + 16; ++n) {
+      const int64_t lanes = ceil_div(pieces, n), at_once = 256 / lanes;
+      if (n > least && lanes < 32) break;
+      const int64_t use = (pieces * at_once << 16) / n;  // threads with work of each block
+      if (pass == 0)
+        best = std::max(best, use);
+      else if (use >= best - best / 16)
+        g = {static_cast<int>(lanes), static_cast<int>(at_once), 0, static_cast<unsigned>(n)};
+    }
+  int each = 8;
+  while (each > 1 && ceil_div(rows, g.at_once * each) * g.across < 296) each /= 2;
+  g.group = g.at_once * each;
+  return g;
 }
 
-// Block (x, y): columns [256 y, + 256) of the x'th `group` rows; a thread has eight columns of every
-// eighth row.  body(row, column, sums) for each; then sums[s] over the rows go to
-// partial[x][s][pitch], in a fixed order.
-template <int SETS, typename F>
-__device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, int group, float *partial, int64_t pitch,
-                                               F &&body) {
+// load(row, column, in) for DEPTH rows a thread, then use(row, column, in, sums) for them: the loads of
+// one are held up neither by the other's stores nor by its arithmetic.  Then sums[s] over the block's rows
+// go to partial[x][s][pitch], in a fixed order.
+template <typename T, int SETS, int DEPTH, int STREAMS, typename Load, typename Use>
+__device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, const RowGrid &grid, float *partial,
+                                               int64_t pitch, Load &&load, Use &&use) {
   dependency_wait();
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + tx) * 8, r0 = static_cast<int64_t>(blockIdx.x) * group;
+  const int ty = threadIdx.x / grid.lanes, tx = threadIdx.x - ty * grid.lanes;
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * grid.lanes + tx) * 8;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * grid.group;
   float sums[SETS][8] = {};
-  if (c < width) {
-    const int64_t end = min(rows, r0 + group);
-#pragma unroll 2
-    for (int64_t r = r0 + ty; r < end; r += 8) body(r, c, sums);
+  if (c < width && ty < grid.at_once) {
+    const int end = static_cast<int>(min(rows - r0, static_cast<int64_t>(grid.group)));
+    for (int r = ty; r < end; r += DEPTH * grid.at_once) {
+      Raw8<T> in[DEPTH][STREAMS];
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i)
+        if (r + i * grid.at_once < end) load(r0 + r + i * grid.at_once, c, in[i]);
+#pragma unroll
+      for (int i = 0; i < DEPTH; ++i)
+        if (r + i * grid.at_once < end) use(r0 + r + i * grid.at_once, c, in[i], sums);
+    }
   }
   if (!partial) return;
-  __shared__ float all[8][32][9];
+  __shared__ float all[256][9];
 #pragma unroll
   for (int s = 0; s < SETS; ++s) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) all[ty][tx][i] = sums[s][i];
+    for (int i = 0; i < 8; ++i) all[threadIdx.x][i] = sums[s][i];
     __syncthreads();
-    // thread t sums column t of the block's 256
-    const int cx = threadIdx.x >> 3, ci = threadIdx.x & 7;
-    float total = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) total += all[w][cx][ci];
-    const int64_t col = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x;
-    if (col < pitch) partial[(static_cast<int64_t>(blockIdx.x) * SETS + s) * pitch + col] = total;
+    for (int k = threadIdx.x; k < grid.lanes * 8; k += 256) {
+      float total = 0.f;
+      for (int w = 0; w < grid.at_once; ++w) total += all[w * grid.lanes + (k >> 3)][k & 7];
+      const int64_t col = static_cast<int64_t>(blockIdx.y) * grid.lanes * 8 + k;
+      if (col < pitch) partial[(static_cast<int64_t>(blockIdx.x) * SETS + s) * pitch + col] = total;
+    }
   }
 }
 
+__device__ __forceinline__ int columns_of(int64_t width, int64_t c) {
+  return static_cast<int>(min(static_cast<int64_t>(8), width - c));
+}
+
 template <typename T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t stride, int64_t rows, int64_t width, int group,
-                                                         float *partial, int64_t pitch) {
-  for_row_groups<1>(rows, width, group, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
-    float x[8];
-    load8<T>(src + r * stride + c, static_cast<int>(min(static_cast<int64_t>(8), width - c)), x);
+__global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t stride, int64_t rows, int64_t width,
+                                                         const RowGrid grid, float *partial, int64_t pitch) {
+  for_row_groups<T, 1, 4, 1>(
+      rows, width, grid, partial, pitch,
+      [&](int64_t r, int64_t c, Raw8<T>(&in)[1]) { load_raw8<T>(src + r * stride + c, columns_of(width, c), in[0]); },
+      [&](int64_t, int64_t, const Raw8<T>(&in)[1], float (&sums)[1][8]) {
+        float x[8];
+        values8<T>(in[0], x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[0][i] += x[i];
-  });
+        for (int i = 0; i < 8; ++i) sums[0][i] += x[i];
+      });
 }
 
 // dst[set][c] = the sum over `chunks` of partial[chunk][set][pitch] at c.  Block (x, y): 32 columns of
@@ -208,83 +286,115 @@ __global__ void __launch_bounds__(1024) column_finish_kernel(const FinishArgs p)
 
 // Eight saved values (16-bit types: slopes).
 template <typename T>
-__device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int64_t r, int64_t c, float (&z)[8]) {
+__device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int64_t r, int64_t c, Raw8<T> &x) {
   const int64_t at = plane * s.stride + r * s.pitch + c;
+  if constexpr (sizeof(T) == 4)
+    load_raw8<float>(s.f32 + at, 8, x);
+  else
+    load_raw8<T>(reinterpret_cast<const T *>(s.half + at), 8, x);
+}
+template <typename T>
+__device__ __forceinline__ void slopes8(const Raw8<T> &r, float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
-    load8<float>(s.f32 + at, 8, z);
+    values8<T>(r, x);
   } else {
-    const uint4 u = *reinterpret_cast<const uint4 *>(s.half + at);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 v = Factor<T>::slope_value(w[i]);
-      z[2 * i] = v.x;
-      z[2 * i + 1] = v.y;
+      const float2 v = Factor<T>::slope_value(r.w[i]);
+      x[2 * i] = v.x;
+      x[2 * i + 1] = v.y;
     }
   }
 }
 
-// dz = dy act'(z), the slope saved, as an operand, with its column sums
-template <typename T>
+// dz = dy act'(z), the slope saved (without SLOPE dy itself), as an operand, with its column sums
+template <typename T, bool SLOPE>
 __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t dy_stride, const SavedPlanes saved,
-                                                          int64_t rows, int64_t width, int group, void *dz, int64_t dz_pitch,
-                                                          int64_t dz_piece, float *partial, int64_t pitch) {
-  for_row_groups<1>(rows, width, group, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[1][8]) {
-    const int n = static_cast<int>(min(static_cast<int64_t>(8), width - c));
-    float d[8], z[8];
-    load8<T>(dy + r * dy_stride + c, n, d);
-    load_saved8<T>(saved, 0, r, c, z);
+                                                          int64_t rows, int64_t width, const RowGrid grid, void *dz,
+                                                          int64_t dz_pitch, int64_t dz_piece, float *partial,
+                                                          int64_t pitch) {
+  constexpr int STREAMS = SLOPE ? 2 : 1, DEPTH = sizeof(T) == 4 ? 2 : 4;
+  for_row_groups<T, 1, DEPTH, STREAMS>(
+      rows, width, grid, partial, pitch,
+      [&](int64_t r, int64_t c, Raw8<T>(&in)[STREAMS]) {
+        load_raw8<T>(dy + r * dy_stride + c, columns_of(width, c), in[0]);
+        if constexpr (SLOPE) load_saved8<T>(saved, 0, r, c, in[1]);
+      },
+      [&](int64_t r, int64_t c, const Raw8<T>(&in)[STREAMS], float (&sums)[1][8]) {
+        float d[8];
+        values8<T>(in[0], d);
+        if constexpr (SLOPE) {
+          float z[8];
+          slopes8<T>(in[1], z);
+          const int n = columns_of(width, c);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      d[i] = i < n ? d[i] * z[i] : 0.f;
-      sums[0][i] += d[i];
-    }
-    store_operand8<T>(dz, r * dz_pitch + c, dz_piece, d);
-  });
+          for (int i = 0; i < 8; ++i) d[i] = i < n ? d[i] * z[i] : 0.f;  // (past the width nothing was saved)
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[0][i] += d[i];
+        store_operand8<T>(dz, r * dz_pitch + c, dz_piece, d);
+      });
 }
 
 // f32: h = act(g) v as an operand, from the saved planes
 template <int ACT>
-__global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, int64_t rows, int64_t width, int group, void *h,
-                                                       int64_t h_pitch, int64_t h_piece) {
-  for_row_groups<1>(rows, width, group, nullptr, 0, [&](int64_t r, int64_t c, float (&)[1][8]) {
-    float g[8], v[8];
-    load_saved8<float>(saved, 0, r, c, g);
-    load_saved8<float>(saved, 1, r, c, v);
+__global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, int64_t rows, int64_t width,
+                                                       const RowGrid grid, void *h, int64_t h_pitch, int64_t h_piece) {
+  for_row_groups<float, 1, 2, 2>(
+      rows, width, grid, nullptr, 0,
+      [&](int64_t r, int64_t c, Raw8<float>(&in)[2]) {
+        load_saved8<float>(saved, 0, r, c, in[0]);
+        load_saved8<float>(saved, 1, r, c, in[1]);
+      },
+      [&](int64_t r, int64_t c, const Raw8<float>(&in)[2], float (&)[1][8]) {
+        float g[8], v[8];
+        values8<float>(in[0], g);
+        values8<float>(in[1], v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 a = activate2<ACT, false>(make_float2(g[2 * i], g[2 * i + 1]));
-      g[2 * i] = a.x * v[2 * i];
-      g[2 * i + 1] = a.y * v[2 * i + 1];
-    }
-    store_operand8<float>(h, r * h_pitch + c, h_piece, g);
-  });
+        for (int i = 0; i < 4; ++i) {
+          const float2 a = activate2<ACT, false>(make_float2(g[2 * i], g[2 * i + 1]));
+          g[2 * i] = a.x * v[2 * i];
+          g[2 * i + 1] = a.y * v[2 * i + 1];
+        }
+        store_operand8<float>(h, r * h_pitch + c, h_piece, g);
+      });
 }
 
 // f32: dg and dv as operands, `dgv_set` elements apart, from dh [rows][saved.pitch] and the saved planes
 template <int ACT>
 __global__ void __launch_bounds__(256) gate_backward_f32_kernel(const float *dh, const SavedPlanes saved, int64_t rows,
-                                                                int64_t width, int group, uint16_t *dgv, int64_t dgv_pitch,
-                                                                int64_t dgv_piece, int64_t dgv_set, float *partial,
-                                                                int64_t pitch) {
-  for_row_groups<2>(rows, width, group, partial, pitch, [&](int64_t r, int64_t c, float (&sums)[2][8]) {
-    float d[8], g[8], v[8];
-    load8<float>(dh + r * saved.pitch + c, 8, d);
-    load_saved8<float>(saved, 0, r, c, g);
-    load_saved8<float>(saved, 1, r, c, v);
+                                                                int64_t width, const RowGrid grid, uint16_t *dgv,
+                                                                int64_t dgv_pitch, int64_t dgv_piece, int64_t dgv_set,
+                                                                float *partial, int64_t pitch) {
+  for_row_groups<float, 2, 2, 3>(
+      rows, width, grid, partial, pitch,
+      [&](int64_t r, int64_t c, Raw8<float>(&in)[3]) {
+        load_raw8<float>(dh + r * saved.pitch + c, 8, in[0]);
+        load_saved8<float>(saved, 0, r, c, in[1]);
+        load_saved8<float>(saved, 1, r, c, in[2]);
+      },
+      [&](int64_t r, int64_t c, const Raw8<float>(&in)[3], float (&sums)[2][8]) {
+        float d[8], g[8], v[8];
+        values8<float>(in[0], d);
+        values8<float>(in[1], g);
+        values8<float>(in[2], v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float2 value, slope;
-      activate_slope2<ACT, false>(f2(g[i]), value, slope);
-      const bool in = c + i < width;  // past the width nothing was written
-      g[i] = in ? d[i] * v[i] * slope.x : 0.f;
-      v[i] = in ? d[i] * value.x : 0.f;
-      sums[0][i] += g[i];
-      sums[1][i] += v[i];
-    }
-    store_operand8<float>(dgv, r * dgv_pitch + c, dgv_piece, g);
-    store_operand8<float>(dgv + dgv_set, r * dgv_pitch + c, dgv_piece, v);
-  });
+        for (int i = 0; i < 4; ++i) {
+          float2 value, slope;
+          activate_slope2<ACT, false>(make_float2(g[2 * i], g[2 * i + 1]), value, slope);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int j = 2 * i + k;
+            const bool in_row = c + j < width;  // past the width nothing was written
+            g[j] = in_row ? d[j] * v[j] * (k ? slope.y : slope.x) : 0.f;
+            v[j] = in_row ? d[j] * (k ? value.y : value.x) : 0.f;
+            sums[0][j] += g[j];
+            sums[1][j] += v[j];
+          }
+        }
+        store_operand8<float>(dgv, r * dgv_pitch + c, dgv_piece, g);
+        store_operand8<float>(dgv + dgv_set, r * dgv_pitch + c, dgv_piece, v);
+      });
 }
 
 // ---- one pass of a layer --------------------------------------------------------------
@@ -315,9 +425,13 @@ class Pass {
     o.ptr = take(2ull * pieces() * rows * o.pitch);
     return o;
   }
-  // A tensor of the call's type as an operand: itself, or a copy (pack() launches the copies).
+  // Whether a tensor of the call's type is an operand as it is.
+  bool in_place(const void *src, int64_t stride) const {
+    return !f32() && reinterpret_cast<uintptr_t>(src) % 16 == 0 && stride % 8 == 0 && stride < (int64_t(1) << 38);
+  }
+  // The tensor as an operand: itself, or a copy (pack() launches the copies).
   GemmOperand operand(const void *src, int64_t stride, int64_t rows, int64_t width) {
-    if (!f32() && reinterpret_cast<uintptr_t>(src) % 16 == 0 && stride % 8 == 0 && stride < (int64_t(1) << 38)) {
+    if (in_place(src, stride)) {
       GemmOperand o;
       o.ptr = src;
       o.pitch = stride;
@@ -382,17 +496,16 @@ class Pass {
     return s;
   }
 
-  // launch(grid, rows of a block) for a kernel of for_row_groups
+  // launch(blocks, grid) for a kernel of for_row_groups
   template <typename F>
   void rows_kernel(int64_t rows, int64_t width, F &&launch) {
     if (!live()) return;
-    const int group = row_group(rows, width);
+    const RowGrid grid = row_grid(rows, width);
     LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
-    const dim3 grid(static_cast<unsigned>(ceil_div(rows, group)), static_cast<unsigned>(ceil_div(width, 256)));
-    check(launch(grid, group), "layer row pass");
+    check(launch(dim3(static_cast<unsigned>(ceil_div(rows, grid.group)), grid.across), grid), "layer row pass");
   }
   // The column sums of a tensor: the blocks' sums, `sets` of them, and how many blocks there are.
-  static int64_t sum_chunks(int64_t rows, int64_t width) { return ceil_div(rows, row_group(rows, width)); }
+  static int64_t sum_chunks(int64_t rows, int64_t width) { return ceil_div(rows, row_grid(rows, width).group); }
   float *sum_room(int64_t rows, int64_t width, int sets) {
     return reinterpret_cast<float *>(take(4ull * sets * sum_chunks(rows, width) * saved_pitch(width)));
   }
@@ -410,16 +523,47 @@ class Pass {
   void column_sums(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst) {
     if (!dst) return;
     float *partial = sum_room(rows, width, 1);
-    rows_kernel(rows, width, [&](dim3 grid, int group) {
+    rows_kernel(rows, width, [&](dim3 blocks, const RowGrid &grid) {
       cudaError_t e = cudaSuccess;
       with_element(dtype_, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        e = launch_early(column_sum_kernel<T>, grid, 256, 0, stream_, static_cast<const T *>(src), stride, rows, width,
-                         group, partial, saved_pitch(width));
+        e = launch_early(column_sum_kernel<T>, blocks, 256, 0, stream_, static_cast<const T *>(src), stride, rows,
+                         width, grid, partial, saved_pitch(width));
       });
       return e;
     });
     finish_sums(partial, sum_chunks(rows, width), width, dst);
+  }
+  // dz = dy act'(z) (without SLOPE dy) into an operand, and its column sums
+  template <bool SLOPE>
+  void slope(const void *dy, int64_t stride, const SavedPlanes &saved, int64_t rows, int64_t width,
+             const GemmOperand &dz, void *d_bias) {
+    float *partial = d_bias ? sum_room(rows, width, 1) : nullptr;
+    rows_kernel(rows, width, [&](dim3 blocks, const RowGrid &grid) {
+      cudaError_t e = cudaSuccess;
+      with_element(dtype_, [&](auto *tag) {
+        using T = std::remove_pointer_t<decltype(tag)>;
+        e = launch_early(dense_slope_kernel<T, SLOPE>, blocks, 256, 0, stream_, static_cast<const T *>(dy), stride, saved,
+                         rows, width, grid, const_cast<void *>(dz.ptr), dz.pitch, dz.piece_stride, partial,
+                         saved_pitch(width));
+      });
+      return e;
+    });
+    finish_sums(partial, sum_chunks(rows, width), width, d_bias);
+  }
+  // The operands taken so far copied, and a gradient as an operand (where one is wanted) with its
+  // column sums: one pass for both where the operand is a copy.
+  GemmOperand operand_and_sums(const void *dy, int64_t stride, int64_t rows, int64_t width, bool wanted, void *d_bias) {
+    if (wanted && d_bias && !in_place(dy, stride)) {
+      pack();
+      const GemmOperand o = make_operand(rows, width);
+      slope<false>(dy, stride, SavedPlanes{}, rows, width, o, d_bias);
+      return o;
+    }
+    const GemmOperand o = wanted ? operand(dy, stride, rows, width) : GemmOperand{};
+    pack();
+    column_sums(dy, stride, rows, width, d_bias);
+    return o;
   }
   void zero(void *ptr, size_t bytes) {
     if (!ptr || !live()) return;
@@ -501,25 +645,12 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
   if (p.d_weight) x = l.operand(p.x, p.x_stride, p.rows, p.inner);
   if (p.d_x) w = l.operand(p.weight, p.columns, p.inner, p.columns);
   if (p.activation == AF2_ACTIVATION_NONE) {
-    if (p.d_x || p.d_weight) dz = l.operand(p.d_out, p.d_out_stride, p.rows, p.columns);
-    l.pack();
-    l.column_sums(p.d_out, p.d_out_stride, p.rows, p.columns, p.d_bias);
+    dz = l.operand_and_sums(p.d_out, p.d_out_stride, p.rows, p.columns, p.d_x || p.d_weight, p.d_bias);
   } else {
     l.pack();
     dz = l.make_operand(p.rows, p.columns);
     const SavedPlanes saved = l.planes(const_cast<void *>(p.saved), p.rows, p.columns, 1);
-    float *partial = p.d_bias ? l.sum_room(p.rows, p.columns, 1) : nullptr;
-    l.rows_kernel(p.rows, p.columns, [&](dim3 grid, int group) {
-      cudaError_t e = cudaSuccess;
-      with_element(p.dtype, [&](auto *tag) {
-        using T = std::remove_pointer_t<decltype(tag)>;
-        e = launch_early(dense_slope_kernel<T>, grid, 256, 0, stream, static_cast<const T *>(p.d_out), p.d_out_stride,
-                         saved, p.rows, p.columns, group, const_cast<void *>(dz.ptr), dz.pitch, dz.piece_stride,
-                         partial, saved_pitch(p.columns));
-      });
-      return e;
-    });
-    l.finish_sums(partial, Pass::sum_chunks(p.rows, p.columns), p.columns, p.d_bias);
+    l.slope<true>(p.d_out, p.d_out_stride, saved, p.rows, p.columns, dz, p.d_bias);
   }
   LayerGemm products[2];
   int count = 0;
@@ -606,10 +737,10 @@ af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uin
     g.out[1] = s.f32 + s.stride;
     g.out_stride = s.pitch;
     l.run(g);
-    l.rows_kernel(p.rows, p.hidden, [&](dim3 grid, int group) {
+    l.rows_kernel(p.rows, p.hidden, [&](dim3 blocks, const RowGrid &grid) {
       cudaError_t e = cudaSuccess;
       with_activation(p.activation, [&](auto act) {
-        e = launch_early(gate_f32_kernel<decltype(act)::value>, grid, 256, 0, stream, s, p.rows, p.hidden, group,
+        e = launch_early(gate_f32_kernel<decltype(act)::value>, blocks, 256, 0, stream, s, p.rows, p.hidden, grid,
                          const_cast<void *>(h.ptr), h.pitch, h.piece_stride);
       });
       return e;
@@ -647,7 +778,6 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     return l.status;
   }
   const bool gradients_at_hidden = p.g.x || p.g.gate_weight || p.g.gate_bias || p.g.value_weight || p.g.value_bias;
-  const GemmOperand dy = l.operand(p.d_out, p.d_out_stride, p.rows, c);
   GemmOperand x, wg, wv, wo, dgv[2];
   if (p.g.gate_weight || p.g.value_weight) x = l.operand(p.x, p.x_stride, p.rows, c);
   if (p.g.x) {
@@ -655,7 +785,8 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     wv = l.operand(p.w.value_weight, hid, c, hid);
   }
   if (gradients_at_hidden) wo = l.operand(p.w.output_weight, c, hid, c);
-  l.pack();
+  const GemmOperand dy = l.operand_and_sums(p.d_out, p.d_out_stride, p.rows, c,
+                                            gradients_at_hidden || p.g.output_weight, p.g.output_bias);
   GemmOperand h;
   h.ptr = p.saved;
   h.pitch = operand_pitch(hid);
@@ -663,7 +794,6 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
   uint8_t *planes_at = static_cast<uint8_t *>(const_cast<void *>(p.saved)) + hidden_bytes(p.rows, hid, p.dtype);
   const SavedPlanes saved = l.planes(planes_at, p.rows, hid, 2);
 
-  l.column_sums(p.d_out, p.d_out_stride, p.rows, c, p.g.output_bias);
   if (gradients_at_hidden) {
     dgv[0] = l.make_operand(p.rows, hid);
     dgv[1] = l.make_operand(p.rows, hid);
@@ -680,11 +810,11 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
       g.out[0] = dh;
       g.out_stride = saved.pitch;
       l.run(g);
-      l.rows_kernel(p.rows, hid, [&](dim3 grid, int group) {
+      l.rows_kernel(p.rows, hid, [&](dim3 blocks, const RowGrid &grid) {
         cudaError_t e = cudaSuccess;
         with_activation(p.activation, [&](auto act) {
-          e = launch_early(gate_backward_f32_kernel<decltype(act)::value>, grid, 256, 0, stream, dh, saved, p.rows,
-                           hid, group, static_cast<uint16_t *>(const_cast<void *>(dgv[0].ptr)), dgv[0].pitch,
+          e = launch_early(gate_backward_f32_kernel<decltype(act)::value>, blocks, 256, 0, stream, dh, saved, p.rows,
+                           hid, grid, static_cast<uint16_t *>(const_cast<void *>(dgv[0].ptr)), dgv[0].pitch,
                            dgv[0].piece_stride,
                            static_cast<const uint16_t *>(dgv[1].ptr) - static_cast<const uint16_t *>(dgv[0].ptr),
                            partial, saved.pitch);

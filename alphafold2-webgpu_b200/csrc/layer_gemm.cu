@@ -192,13 +192,13 @@ template <typename T, bool IN>
 __device__ __forceinline__ void move_rows(uint8_t *block, T *at, int64_t stride, int rows, int cols, int lane) {
   if (lane >= cols) return;
   T *g = at + lane;
-  for (int r0 = 0; r0 < rows; r0 += 8) {
-    T v[8];
+  for (int r0 = 0; r0 < rows; r0 += 4) {
+    T v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
       if (r0 + i < rows) v[i] = IN ? g[(r0 + i) * stride] : *reinterpret_cast<T *>(element16(block, r0 + i, lane));
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
       if (r0 + i < rows) {
         if constexpr (IN)
           *reinterpret_cast<T *>(element16(block, r0 + i, lane)) = v[i];
@@ -214,16 +214,16 @@ __device__ __forceinline__ void move_rows_f32(uint8_t *block, float *at, int64_t
   if (c >= cols) return;
   float *g = at + c;
   auto s = [&](int r) { return reinterpret_cast<float *>(piece16(block, r, c >> 2)) + (c & 3); };
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += 8) {
+    float v[4];
 #pragma unroll
-  for (int r0 = 0; r0 < 32; r0 += 16) {
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int r = r0 + 2 * i + (lane >> 4);
       if (r < rows) v[i] = IN ? g[r * stride] : *s(r);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int r = r0 + 2 * i + (lane >> 4);
       if (r < rows) {
         if constexpr (IN)
@@ -628,14 +628,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const OT *residual = PLAIN ? nullptr : static_cast<const OT *>(p.residual);
         const int z = partial ? tile.split * static_cast<int>(p.batches.d) + tile.z : 0;
         const CUtensorMap *omap = &maps.out[partial ? 0 : tile.z];
-        // the residual's blocks come ahead, each into the block that its result leaves from
-        // (f32: the two halves of the warp's only block of columns)
+        // The residual's blocks come ahead, each into the block that its result leaves from: the two in
+        // turn, the second where the first holds slopes (f32: the two halves of the warp's only block of
+        // columns).
+        const bool keep = !PLAIN && p.save;
         auto fetch = [&](int b, int at) {
           if (lane == 0) {
             bulk_wait_read_all();
             mbar_arrive_expect_tx(load(ew, at & 1), F32 ? 4096 : 2048);
-            tma_load_3d(block_addr + (at & 1) * (F32 ? 0 : 2048), &maps.residual, load(ew, at & 1), n0 + b * 32, r0, 0);
-            if (F32) tma_load_3d(block_addr + 2048, &maps.residual, load(ew, at & 1), n0 + b * 32 + 16, r0, 0);
+            const uint32_t to = block_addr + (F32 ? 0 : 2048 * (keep ? 1 : at & 1));
+            tma_load_3d(to, &maps.residual, load(ew, at & 1), n0 + b * 32, r0, 0);
+            if (F32) tma_load_3d(to + 2048, &maps.residual, load(ew, at & 1), n0 + b * 32 + 16, r0, 0);
           }
         };
         const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0));
@@ -662,8 +665,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           if (first < end) {
             if (tma_residual) {
               ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
+              if (!ok) {
+                if (lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
+                break;
+              }
               ++loads;
-              if (!ok) break;
             }
             const float *bias = PLAIN || partial ? nullptr : static_cast<const float *>(p.bias[tile.z]);
 #pragma unroll
@@ -747,7 +753,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const int c0 = n0 + b * 32;
           uint32_t r[32];
           tmem_ld32(taddr + b * 32, r);
-          if (tma_residual && b + step < end) fetch(b + step, loads + 1);
+          if (tma_residual && !keep && b + step < end) fetch(b + step, loads + 1);
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
           const int cols = min(32, p.n - c0);
           const OT *bias = PLAIN || partial ? nullptr : static_cast<const OT *>(p.bias[tile.z]);
@@ -817,17 +823,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             continue;
           }
           // the block that the result leaves from, with the residual in it where there is one
-          const uint32_t at = 2048u * (tma_residual       ? loads & 1
-                                       : !PLAIN && p.save ? 1  // the first block may still hold slopes
-                                                          : stores++ & 1);
+          const uint32_t at = 2048u * (keep ? 1 : tma_residual ? loads & 1 : stores++ & 1);
           uint8_t *const dst = block + at;
           if (tma_residual) {
             ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
-            ++loads;
             if (!ok) {
-              if (b + step < end && lane == 0) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
+              if (lane == 0) {
+                mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
+                ++loads;
+                if (!keep && b + step < end) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
+              }
               break;
             }
+            ++loads;
           } else {
             if (lane == 0) {
               if (PLAIN)
@@ -871,6 +879,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                  p.out_stride, rows, cols, lane);
             __syncwarp();
           }
+          if (tma_residual && keep && b + step < end) fetch(b + step, loads);
         }
         }
         if (!ok) break;
@@ -1116,7 +1125,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
     p.activation = g.activation;
     p.residual = g.residual;
     p.residual_stride = g.residual_stride;
-    if (g.residual && !g.saved.half && aligned16(g.residual, g.residual_stride, out_bytes)) {
+    if (g.residual && aligned16(g.residual, g.residual_stride, out_bytes)) {
       p.tma_residual = 1;
       const int64_t row = g.residual_stride * out_bytes;
       maps_ok &= encode_map_3d(&maps.residual, map_type(g.out_dtype), g.residual, g.n, g.m, 1, row, row,
