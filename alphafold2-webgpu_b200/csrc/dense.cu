@@ -469,12 +469,16 @@ class Pass {
     o.mn_major = true;
     return o;
   }
-  void run(LayerGemm g) { run(&g, 1); }
-  // Independent products in one launch: their tiles fill the SMs together.
+  void run(const LayerGemm &g) {
+    LayerGemm one[kMaxProducts];
+    one[0] = g;
+    run(one, 1);
+  }
+  // Independent products in one launch: their tiles fill the SMs together.  g: room for kMaxProducts.
   void run(LayerGemm *g, int count) {
     if (count == 0) return;
     const uint64_t mark = used;
-    layer_gemm_plan(g, count);
+    count = layer_gemm_plan(g, count);
     for (int i = 0; i < count; ++i) g[i].scratch = take(g[i].scratch_bytes);
     if (live()) status = layer_gemm_launch(ctx_, g, count, stream_);
     peak_ = std::max(peak_, used);
@@ -652,7 +656,7 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
     const SavedPlanes saved = l.planes(const_cast<void *>(p.saved), p.rows, p.columns, 1);
     l.slope<true>(p.d_out, p.d_out_stride, saved, p.rows, p.columns, dz, p.d_bias);
   }
-  LayerGemm products[2];
+  LayerGemm products[kMaxProducts];
   int count = 0;
   if (p.d_x) {
     LayerGemm &g = products[count++] = l.product(p.rows, p.inner, p.columns);
@@ -835,7 +839,7 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     }
     l.finish_sums(partial, chunks, hid, p.g.gate_bias, 2, p.g.value_bias);
   }
-  LayerGemm products[3];
+  LayerGemm products[kMaxProducts];
   int count = 0;
   if (p.g.x) {
     LayerGemm &g = products[count++] = l.product(p.rows, c, hid);

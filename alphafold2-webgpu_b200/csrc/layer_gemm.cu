@@ -32,6 +32,7 @@
 // (An infinite f32 element makes its sums NaN or infinite.)
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "layer_factor.cuh"
@@ -112,14 +113,27 @@ struct Args {
   int first_tile;    // the tiles of the products before this one
 };
 
-// What a launch computes: up to three products, whose tiles follow one another.
+// What a launch computes: products whose tiles follow one another.  One product's tiles go to the pairs
+// in turn.  Several products' tiles differ in length, and the pairs that have a long one take fewer of the
+// short: each wave is a run of pairs that take `repeats` tiles each, from `first` on.
 struct Product {
   Maps maps;
   Args args;
 };
+struct Wave {
+  int first, repeats;
+  int at, pairs;
+};
+constexpr int kMaxWaves = 24;
+struct Waves {
+  Wave wave[kMaxWaves];
+  int count;
+};
+struct NoWaves {};
 template <int N>
 struct Launch {
   Product product[N];
+  std::conditional_t<(N > 1), Waves, NoWaves> waves;
   int products, total_tiles;
   int alternate;  // the two groups of epilogue warps take tiles in turn
   unsigned int *err;
@@ -131,6 +145,30 @@ __device__ __forceinline__ const Product &product_of(const Launch<N> &l, int t) 
     while (i + 1 < l.products && t >= l.product[i + 1].args.first_tile) ++i;
   return l.product[i];
 }
+
+// The tiles of a pair, one after the other.
+template <int N>
+struct Walk {
+  const Launch<N> &launch;
+  int pair, pairs;
+  int at = 0, turn = 0;  // one product: turns taken; several: the wave, and the turns in it
+  __device__ __forceinline__ bool next(int &t) {
+    if constexpr (N == 1) {
+      t = pair + turn++ * pairs;
+      return t < launch.total_tiles;
+    } else {
+      for (; at < launch.waves.count; ++at, turn = 0) {
+        const Wave &w = launch.waves.wave[at];
+        const int i = pair - w.at;
+        if (i >= 0 && i < w.pairs && turn < w.repeats) {
+          t = w.first + turn++ * w.pairs + i;
+          return true;
+        }
+      }
+      return false;
+    }
+  }
+};
 
 // The terms (of A, of B) of the six products of an f32 operand pair, the largest last.
 constexpr int kProductsF32 = 6;
@@ -252,6 +290,7 @@ __device__ __forceinline__ float lane_sums(float (&x)[32], int lane) {
 template <int KIND, typename OT, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     layer_gemm_kernel(const __grid_constant__ Launch<KIND == kProducts ? kMaxProducts : 1> launch) {
+  constexpr int LIMIT = KIND == kProducts ? kMaxProducts : 1;
   using S = Shape<KIND, BN, sizeof(OT) == 4>;
   constexpr bool GATE = KIND == kGate || KIND == kGateSave;
   constexpr bool F32 = sizeof(OT) == 4;
@@ -308,7 +347,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       int it = 0, s = 0;
       uint32_t ph = 1;
       bool ok = true;
-      for (int t = pair; t < launch.total_tiles && ok; t += npairs) {
+      Walk<LIMIT> walk{launch, pair, npairs};
+      for (int t; ok && walk.next(t);) {
         const Product &product = product_of(launch, t);
         const Maps &maps = product.maps;
         const Args &p = product.args;
@@ -369,7 +409,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       int s = 0, buf = 0;
       uint32_t ph = 0, bph = 0;
       bool ok = true;
-      for (int t = pair; t < launch.total_tiles && ok; t += npairs) {
+      Walk<LIMIT> walk{launch, pair, npairs};
+      for (int t; ok && walk.next(t);) {
         const Args &p = product_of(launch, t).args;
         const uint32_t idesc = idesc_16_f32(PAIR_M, BN, p.bf16, p.a_mn, p.b_mn);
         auto k_major = [](uint32_t at) { return F32 ? sdesc_k_sw64(at) : sdesc_k_sw128(at); };
@@ -440,7 +481,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint8_t *const block = smem + S::OFF_STAGE + ew * S::SLOT_BYTES;
     const uint32_t block_addr = sbase + S::OFF_STAGE + ew * S::SLOT_BYTES;
     int acc_it = 0, stores = 0, loads = 0;  // stores, loads: through the two blocks in turn
-    for (int t = pair; t < launch.total_tiles; t += npairs, ++acc_it) {
+    Walk<LIMIT> walk{launch, pair, npairs};
+    for (int t; walk.next(t); ++acc_it) {
       if (launch.alternate && (acc_it & 1) != group) continue;
       const Product &product = product_of(launch, t);
       const Maps &maps = product.maps;
@@ -982,6 +1024,8 @@ bool operand_map(CUtensorMap *map, const GemmOperand &o, int64_t outer, int64_t 
                        pieces > 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+int launch_pairs(const af2_ctx *ctx, int tiles) { return std::min(tiles, std::max(1, ctx->sm_count / 2)); }
+
 template <int KIND, typename OT, int BN>
 af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l, cudaStream_t stream) {
   constexpr uint32_t smem = Shape<KIND, BN, sizeof(OT) == 4>::BYTES;
@@ -994,7 +1038,7 @@ af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l,
       return cuda_fail(ctx, e, "layer product shared memory");
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int pairs = std::min(l.total_tiles, std::max(1, ctx->sm_count / 2));
+  const int pairs = launch_pairs(ctx, l.total_tiles);
   l.alternate = l.total_tiles > pairs && sizeof(OT) == 2;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
   if (cudaError_t e = launch_early(kernel, dim3(2 * pairs), THREADS, smem, stream, l); e != cudaSuccess)
@@ -1027,61 +1071,198 @@ CUtensorMapDataType map_type(int dtype) {
 
 }  // namespace
 
-// Tile width and the parts that each depth is cut into, from what a launch costs in SM clocks.  A pair
-// takes tiles pair, pair + 74, ...; with the products in order of their tiles' cost the first pair
-// has the most.  A K step of 64 takes 512 (BN = 256) or 420 (BN = 128; the ring's latency) clocks, in
-// f32 900 for 32, a tile's hand-over 800, and split sums are written, read and reduced by another launch.
-void layer_gemm_plan(LayerGemm *g, int count) {
+namespace {
+
+// Tiles of one length.
+struct TileClass {
+  int64_t tiles;
+  double clocks;  // of each
+};
+
+// Tiles of several lengths, the longest first, dealt out to `pairs`: always to the pairs that have the
+// least to do, neighbours within half a tile of one another together.  Returns the clocks of the pair that
+// has the most; fills in the waves.
+double deal(const TileClass *classes, int count, int pairs, Waves *waves) {
+  struct Run { int at, pairs; double load; } run[kMaxWaves];
+  int runs = 1, n = 0, first = 0;
+  run[0] = {0, pairs, 0};
+  bool fits = true;
+  for (int j = 0; j < count && fits; ++j) {
+    const double cost = classes[j].clocks;
+    for (int64_t left = classes[j].tiles; left > 0 && fits;) {
+      int lo = 0;
+      for (int i = 1; i < runs; ++i)
+        if (run[i].load < run[lo].load) lo = i;
+      const double least = run[lo].load + cost / 2;
+      int hi = lo;
+      while (lo > 0 && run[lo - 1].load <= least) --lo;
+      while (hi + 1 < runs && run[hi + 1].load <= least) ++hi;
+      for (int i = lo + 1; i <= hi; ++i) {
+        run[lo].pairs += run[i].pairs;
+        run[lo].load = std::max(run[lo].load, run[i].load);
+      }
+      std::copy(run + hi + 1, run + runs, run + lo + 1);
+      runs -= hi - lo;
+      Run &r = run[lo];
+      int64_t turns = left / r.pairs;
+      for (int i = 0; i < runs; ++i)
+        if (i != lo) turns = std::min(turns, std::max<int64_t>(1, std::llround((run[i].load - r.load) / cost)));
+      if (n == kMaxWaves || (turns == 0 && runs == kMaxWaves)) {
+        fits = false;
+      } else if (turns > 0) {
+        if (waves) waves->wave[n] = {first, static_cast<int>(turns), r.at, r.pairs};
+        r.load += turns * cost;
+        first += static_cast<int>(turns * r.pairs);
+        left -= turns * r.pairs;
+      } else {  // fewer tiles than pairs
+        std::copy_backward(run + lo + 1, run + runs, run + runs + 1);
+        ++runs;
+        run[lo + 1] = {r.at + static_cast<int>(left), r.pairs - static_cast<int>(left), r.load};
+        if (waves) waves->wave[n] = {first, 1, r.at, static_cast<int>(left)};
+        run[lo].pairs = static_cast<int>(left);
+        run[lo].load += cost;
+        first += static_cast<int>(left);
+        left = 0;
+      }
+      ++n;
+    }
+  }
+  double most = 0;
+  if (fits) {
+    for (int i = 0; i < runs; ++i) most = std::max(most, run[i].load);
+  } else {  // too many waves: every product's tiles to all pairs in turn
+    n = first = 0;
+    for (int j = 0; j < count; ++j) {
+      const int turns = static_cast<int>(classes[j].tiles / pairs), rest = static_cast<int>(classes[j].tiles % pairs);
+      if (waves) {
+        if (turns) waves->wave[n++] = {first, turns, 0, pairs};
+        if (rest) waves->wave[n++] = {first + turns * pairs, 1, 0, rest};
+      }
+      first += static_cast<int>(classes[j].tiles);
+      most += (turns + (rest ? 1 : 0)) * classes[j].clocks;
+    }
+  }
+  if (waves) waves->count = n;
+  return most;
+}
+
+// What a launch costs in SM clocks: a K step of 64 takes 512 (BN = 256) or 420 (BN = 128; the ring's
+// latency) clocks, in f32 900 for 32, a tile's hand-over 800.
+double step_clocks(bool f32, int bn) { return f32 ? 900 : bn == 256 ? 512 : 420; }
+TileClass tile_class(const LayerGemm &g, int bn, int splits) {
+  const bool f32 = g.pieces > 1;
+  const int64_t k_blocks = ceil_div(g.k, f32 ? 32 : BK);
+  const int width = g.epilogue == kEpilogueGate ? bn / 2 : bn;
+  return {splits * g.batch * ceil_div(g.m, PAIR_M) * ceil_div(g.n, width),
+          ceil_div(k_blocks, splits) * g.segments * step_clocks(f32, bn) + 800};
+}
+int split_limit(const LayerGemm &g) {
+  return static_cast<int>(std::min<int64_t>((ceil_div(g.k, g.pieces > 1 ? 32 : BK) + 1) / 2, 64));
+}
+// Split sums are written, read and reduced by another launch.
+double split_clocks(double bytes) { return bytes > 0 ? 4000 + bytes / 2500 : 0; }
+double split_bytes(const LayerGemm &g, int splits) {
+  return splits > 1 ? 8.0 * splits * g.batch * g.m * align_up(g.n, 4) : 0;
+}
+double launch_clocks(TileClass *classes, int count, double bytes) {
+  std::sort(classes, classes + count, [](const TileClass &a, const TileClass &b) { return a.clocks > b.clocks; });
+  return 2500 + split_clocks(bytes) + deal(classes, count, kPairs, nullptr);
+}
+
+// The rows of g from `row` on (a multiple of 8) as a product of their own; g keeps those before.
+LayerGemm cut_rows(LayerGemm &g, int64_t row) {
+  LayerGemm tail = g;
+  auto past = [&](const void *p, int64_t elements, int size) {
+    return static_cast<const uint8_t *>(p) + elements * size;
+  };
+  for (int i = 0; i < g.segments; ++i)
+    tail.a[i].ptr = past(g.a[i].ptr, g.a[i].mn_major ? row : row * g.a[i].pitch, 2);
+  for (int i = 0; i < g.batch; ++i)
+    tail.out[i] = const_cast<uint8_t *>(past(g.out[i], row * g.out_stride, g.out_dtype == AF2_F32 ? 4 : 2));
+  tail.m = g.m - row;
+  g.m = row;
+  return tail;
+}
+
+// Launches this long (SM clocks) are worth the host's search for a cut, some 20 us.
+constexpr double kCutFrom = 200000;
+
+}  // namespace
+
+// Tile width and the parts that each depth is cut into, by the clocks that the launch costs.  Where the
+// tiles of long products leave pairs without work at the end, the last rows of one become a product of its
+// own whose depth is cut: at 8192 x 1024 -> 4096 the gradients' 320 tiles fill 74 pairs 4.3 times, and
+// 24 of them cut in three end all pairs together.
+int layer_gemm_plan(LayerGemm *g, int count) {
   const bool f32 = g[0].pieces > 1;
-  const bool gate = g[0].epilogue == kEpilogueGate;
+  TileClass classes[kMaxProducts];
   double best = 0;
+  int64_t longest = 0;
+  for (int i = 0; i < count; ++i) longest = std::max(longest, ceil_div(g[i].k, f32 ? 32 : BK) * g[i].segments);
   for (int bn : {256, 128}) {
     if (g[0].epilogue == kEpilogueGateBackward && bn == 128) continue;
     if (f32 && bn == 256) continue;
-    const double step_clocks = f32 ? 900 : bn == 256 ? 512 : 420;  // (a step of 32 in f32)
     // `most`: K steps that a tile may have before its depth is cut
     for (int64_t most : {int64_t(1) << 40, int64_t(512), int64_t(384), int64_t(256), int64_t(192), int64_t(128),
                          int64_t(96), int64_t(64), int64_t(48), int64_t(32), int64_t(24), int64_t(16), int64_t(12),
                          int64_t(8), int64_t(6), int64_t(4), int64_t(2)}) {
-      if (most < int64_t(1) << 40 && g[0].epilogue != kEpilogueOut) break;
-      struct { int64_t tiles, steps; } part[kMaxProducts];
-      int splits[kMaxProducts], order[kMaxProducts];
+      if (most < int64_t(1) << 40 && (most >= longest || g[0].epilogue != kEpilogueOut)) continue;
+      int splits[kMaxProducts];
       double bytes = 0;
-      bool split = false;
       for (int i = 0; i < count; ++i) {
-        const int64_t k_blocks = ceil_div(g[i].k, f32 ? 32 : BK), all = k_blocks * g[i].segments;
-        splits[i] = static_cast<int>(std::max<int64_t>(1, std::min({ceil_div(all, most), (k_blocks + 1) / 2, int64_t(64)})));
-        part[i].tiles = splits[i] * g[i].batch * ceil_div(g[i].m, PAIR_M) * ceil_div(g[i].n, gate ? bn / 2 : bn);
-        part[i].steps = ceil_div(k_blocks, splits[i]) * g[i].segments;
-        order[i] = i;
-        if (splits[i] > 1) {
-          split = true;
-          bytes += 8.0 * splits[i] * g[i].batch * g[i].m * align_up(g[i].n, 4);
-        }
+        const int64_t all = ceil_div(g[i].k, f32 ? 32 : BK) * g[i].segments;
+        splits[i] = std::max(1, static_cast<int>(std::min<int64_t>(ceil_div(all, most), split_limit(g[i]))));
+        classes[i] = tile_class(g[i], bn, splits[i]);
+        bytes += split_bytes(g[i], splits[i]);
       }
-      std::sort(order, order + count, [&](int a, int b) { return part[a].steps > part[b].steps; });
-      double clocks = 2500 + (split ? 4000 + bytes / 2500 : 0);
-      int64_t before = 0;  // tiles of the products before, in order
-      for (int j = 0; j < count; ++j) {
-        const int i = order[j];
-        // of the first pair's tiles 0, kPairs, 2 kPairs, ... those in this product
-        const int64_t turns = ceil_div(before + part[i].tiles, kPairs) - ceil_div(before, kPairs);
-        clocks += turns * (part[i].steps * step_clocks + 800);
-        before += part[i].tiles;
-      }
+      const double clocks = launch_clocks(classes, count, bytes);
       if (best == 0 || clocks < best) {
         best = clocks;
         for (int i = 0; i < count; ++i) {
           g[i].tile_n = bn;
           g[i].splits = splits[i];
-          g[i].order = order[i];
         }
       }
+    }
+  }
+  if (count > 1 && count < kMaxProducts && best > kCutFrom) {
+    const int bn = g[0].tile_n;
+    double whole = 0;
+    for (int i = 0; i < count; ++i) whole += split_bytes(g[i], g[i].splits);
+    int cut = -1, cut_splits = 0;
+    int64_t cut_row = 0;
+    for (int i = 0; i < count; ++i) {
+      const int64_t tile_rows = ceil_div(g[i].m, PAIR_M), in_row = g[i].batch * ceil_div(g[i].n, bn);
+      if (g[i].splits > 1) continue;
+      for (int64_t rows = 1; rows < tile_rows && rows * in_row <= kPairs; ++rows)
+        for (int splits = 2; splits <= std::min(8, split_limit(g[i])); ++splits) {
+          LayerGemm head = g[i];
+          const int64_t row = (tile_rows - rows) * PAIR_M;
+          const LayerGemm tail = cut_rows(head, row);
+          for (int j = 0; j < count; ++j) classes[j] = tile_class(j == i ? head : g[j], bn, g[j].splits);
+          classes[count] = tile_class(tail, bn, splits);
+          const double clocks = launch_clocks(classes, count + 1, whole + split_bytes(tail, splits));
+          if (clocks < best) {
+            best = clocks;
+            cut = i;
+            cut_splits = splits;
+            cut_row = row;
+          }
+        }
+    }
+    if (cut >= 0) {
+      g[count] = cut_rows(g[cut], cut_row);
+      g[count++].splits = cut_splits;
     }
   }
   for (int i = 0; i < count; ++i)
     g[i].scratch_bytes =
         g[i].splits > 1 ? align_up(4ull * g[i].splits * g[i].batch * g[i].m * align_up(g[i].n, 4), 256) : 0;
+  if (count > 1)  // (the waves take the longest tiles first)
+    std::stable_sort(g, g + count, [&](const LayerGemm &a, const LayerGemm &b) {
+      return tile_class(a, a.tile_n, a.splits).clocks > tile_class(b, b.tile_n, b.splits).clocks;
+    });
+  return count;
 }
 
 namespace {
@@ -1172,10 +1353,15 @@ af2_status describe_and_run(af2_ctx *ctx, const LayerGemm *g, int count, F &&run
   int64_t total = 0;
   for (int j = 0; j < count; ++j) {
     int64_t tiles = 0;
-    if (af2_status st = describe(ctx, g[g[j].order], total, &l.product[j], &tiles); st != AF2_OK) return st;
+    if (af2_status st = describe(ctx, g[j], total, &l.product[j], &tiles); st != AF2_OK) return st;
     total += tiles;
   }
   l.total_tiles = static_cast<int>(total);
+  if constexpr (N > 1) {
+    TileClass classes[N];
+    for (int j = 0; j < count; ++j) classes[j] = tile_class(g[j], g[j].tile_n, g[j].splits);
+    deal(classes, count, launch_pairs(ctx, l.total_tiles), &l.waves);
+  }
   return run(l);
 }
 

@@ -54,7 +54,6 @@ struct LayerGemm {
   float *column_partial = nullptr;           // GateBackward: [ceil(m / 32)][2 * saved.pitch] column sums, or NULL
   // layer_gemm_plan: the tile's width, the parts the depth is cut into and the split sums' bytes
   int tile_n = 0, splits = 0;
-  int order = 0;  // g[i].order: the product whose tiles come i'th
   uint64_t scratch_bytes = 0;
   uint8_t *scratch = nullptr;
 };
@@ -63,10 +62,12 @@ struct LayerGemm {
 inline int64_t operand_pitch(int64_t width) { return align_up(width, 8); }
 inline int64_t saved_pitch(int64_t width) { return align_up(width, 32); }
 
-// Up to this many products of one type in a launch (more than one: kEpilogueOut only).
-constexpr int kMaxProducts = 3;
-// Fills in the plan; then each product with scratch_bytes needs scratch.
-void layer_gemm_plan(LayerGemm *g, int count);
+// Up to this many products of one type in a launch (more than one: kEpilogueOut with no bias, activation
+// or residual).
+constexpr int kMaxProducts = 4;
+// Fills in the plan, in which a product may have become two, in another order: g has room for
+// kMaxProducts; returns how many there are.  Then each product with scratch_bytes needs scratch.
+int layer_gemm_plan(LayerGemm *g, int count);
 af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaStream_t stream);
 
 }  // namespace af2
