@@ -245,45 +245,6 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t s
       });
 }
 
-// dst[set][c] = the sum over `chunks` of partial[chunk][set][pitch] at c.  Block (x, y): 32 columns of
-// set y, 32 warps with eight loads in flight each (two rows of blocks are few: latency bounds them).
-struct FinishArgs {
-  const float *partial;
-  int64_t chunks, pitch, cols;
-  int sets;
-  void *dst[2];
-};
-template <typename T>
-__global__ void __launch_bounds__(1024) column_finish_kernel(const FinishArgs p) {
-  __shared__ float all[32][33];
-  dependency_wait();
-  T *dst = static_cast<T *>(p.dst[blockIdx.y]);
-  if (!dst) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane, row = p.sets * p.pitch;
-  const float *src = p.partial + blockIdx.y * p.pitch + c;
-  float sum = 0.f;
-  if (c < p.cols) {
-    int64_t k = warp;
-    for (; k + 7 * 32 < p.chunks; k += 8 * 32) {
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = src[(k + 32 * i) * row];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum += x[i];
-    }
-    for (; k < p.chunks; k += 32) sum += src[k * row];
-  }
-  all[warp][lane] = sum;
-  __syncthreads();
-  if (warp == 0 && c < p.cols) {
-    float total = 0.f;
-#pragma unroll
-    for (int w = 0; w < 32; ++w) total += all[w][lane];
-    dst[c] = from_f32<T>(total);
-  }
-}
-
 // Eight saved values (16-bit types: slopes).
 template <typename T>
 __device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int64_t r, int64_t c, Raw8<T> &x) {
@@ -475,12 +436,13 @@ class Pass {
     run(one, 1);
   }
   // Independent products in one launch: their tiles fill the SMs together.  g: room for kMaxProducts.
-  void run(LayerGemm *g, int count) {
-    if (count == 0) return;
+  // With the last ones go the column sums asked for so far.
+  void run(LayerGemm *g, int count, bool last = false) {
     const uint64_t mark = used;
-    count = layer_gemm_plan(g, count);
+    if (count) count = layer_gemm_plan(g, count);
     for (int i = 0; i < count; ++i) g[i].scratch = take(g[i].scratch_bytes);
-    if (live()) status = layer_gemm_launch(ctx_, g, count, stream_);
+    if (live() && count) status = layer_gemm_launch(ctx_, g, count, stream_);
+    if (live()) status = layer_finish_launch(ctx_, dtype_, g, count, sums_, last ? sum_count_ : 0, stream_);
     peak_ = std::max(peak_, used);
     used = mark;  // launches follow one another on the stream: the next may use the same place
   }
@@ -513,16 +475,11 @@ class Pass {
   float *sum_room(int64_t rows, int64_t width, int sets) {
     return reinterpret_cast<float *>(take(4ull * sets * sum_chunks(rows, width) * saved_pitch(width)));
   }
-  void finish_sums(const float *partial, int64_t chunks, int64_t width, void *dst, int sets = 1,
-                   void *second = nullptr) {
-    if (!live() || !(dst || second)) return;
-    const FinishArgs f{partial, chunks, saved_pitch(width), width, sets, {dst, second}};
-    LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
-    const dim3 grid(static_cast<unsigned>(ceil_div(width, 32)), sets);
-    with_element(dtype_, [&](auto *tag) {
-      check(launch_early(column_finish_kernel<std::remove_pointer_t<decltype(tag)>>, grid, 1024, 0, stream_, f),
-            "layer column sums");
-    });
+  // Sums of chunks, one set of a row of `sets`, to go out with the last products.
+  void finish_sums(const float *partial, int64_t chunks, int64_t width, void *dst, int set = 0, int sets = 1) {
+    if (!dst) return;
+    const int64_t pitch = saved_pitch(width);
+    sums_[sum_count_++] = {partial + set * pitch, chunks, sets * pitch, width, dst};
   }
   void column_sums(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst) {
     if (!dst) return;
@@ -585,6 +542,8 @@ class Pass {
   uint8_t *base_;
   cudaStream_t stream_;
   PackArgs jobs_{};
+  ColumnSums sums_[kMaxSums];
+  int sum_count_ = 0;
   uint64_t peak_ = 0;
 };
 
@@ -672,7 +631,7 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
     g.out[0] = p.d_weight;
     g.out_stride = p.columns;
   }
-  l.run(products, count);
+  l.run(products, count, true);
   *bytes = l.total();
   return l.status;
 }
@@ -837,7 +796,8 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
       g.column_partial = partial;
       l.run(g);
     }
-    l.finish_sums(partial, chunks, hid, p.g.gate_bias, 2, p.g.value_bias);
+    l.finish_sums(partial, chunks, hid, p.g.gate_bias, 0, 2);
+    l.finish_sums(partial, chunks, hid, p.g.value_bias, 1, 2);
   }
   LayerGemm products[kMaxProducts];
   int count = 0;
@@ -867,7 +827,7 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     g.out[0] = p.g.output_weight;
     g.out_stride = c;
   }
-  l.run(products, count);
+  l.run(products, count, true);
   *bytes = l.total();
   return l.status;
 }

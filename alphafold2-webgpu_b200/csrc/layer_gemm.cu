@@ -330,6 +330,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     *abort_flag = 0;
     fence_mbar_init();
   }
+  if (warp == 0 && lane < launch.products) {  // (the maps are the launch's own: nothing to wait for)
+    const Maps &maps = launch.product[lane].maps;
+    tma_prefetch_map(&maps.a[0]);
+    tma_prefetch_map(&maps.b[0]);
+    tma_prefetch_map(&maps.out[0]);
+  }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_slot), 512);
     tmem_relinquish_pair();
@@ -342,8 +348,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      tma_prefetch_map(&launch.product[0].maps.a[0]);
-      tma_prefetch_map(&launch.product[0].maps.b[0]);
       int it = 0, s = 0;
       uint32_t ph = 1;
       bool ok = true;
@@ -941,8 +945,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   }
 }
 
-// out = act(sum of the splits' partial sums + bias) (+ residual), saved = the slope.  One thread per
-// four columns.
+// ---- what follows the products ---------------------------------------------------
+
+// out = act(sum of the splits' partial sums + bias) (+ residual), saved = the slope.
 struct ReduceArgs {
   const float *partial;  // [split][batch][m][pitch]
   int splits, batch, activation;
@@ -957,53 +962,116 @@ struct ReduceArgs {
   int64_t saved_pitch;
 };
 
-struct ReduceLaunch {
-  ReduceArgs product[kMaxProducts];  // blockIdx.y
+// The split products' sums (blockIdx.y below `products`), then the column sums: one launch for both.
+struct FinishLaunch {
+  ReduceArgs product[kMaxProducts];
+  ColumnSums sums[kMaxSums];
+  int products;
 };
 
+// A thread has four columns of a row; latency bounds it, so all that it reads is asked for at once.
 template <typename OT>
-__global__ void __launch_bounds__(256) reduce_kernel(const __grid_constant__ ReduceLaunch launch) {
-  const ReduceArgs &p = launch.product[blockIdx.y];
-  dependency_wait();
-  const int64_t quads = p.pitch / 4, total = p.batch * p.m * quads;
-  const int64_t split_stride = p.batch * p.m * quads;  // float4s
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const float4 *src = reinterpret_cast<const float4 *>(p.partial) + i;
-    float4 a = src[0];
-    for (int s = 1; s < p.splits; ++s) {
-      const float4 b = src[s * split_stride];
-      a.x += b.x;
-      a.y += b.y;
-      a.z += b.z;
-      a.w += b.w;
-    }
-    const int64_t row = i / quads, z = row / p.m, m = row - z * p.m, c0 = (i - row * quads) * 4;
-    float y[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void reduce(const ReduceArgs &p) {
+  // (a product is only split while it has few tiles: its elements count in 32 bits)
+  const uint32_t quads = static_cast<uint32_t>(p.pitch / 4), rows = static_cast<uint32_t>(p.m);
+  const uint32_t total = p.batch * rows * quads;
+  for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
+    const uint32_t row = i / quads, c0 = (i - row * quads) * 4, z = row / rows;
+    const int64_t m = row - z * rows;
+    const int cols = static_cast<int>(min(static_cast<int64_t>(4), p.n - c0));
     const OT *bias = static_cast<const OT *>(p.bias[z]);
-    OT *out = static_cast<OT *>(p.out[z]) + m * p.out_stride;
-    const OT *res = p.residual ? static_cast<const OT *>(p.residual) + m * p.residual_stride : nullptr;
+    OT *out = static_cast<OT *>(p.out[z]) + m * p.out_stride + c0;
+    float b[4] = {}, r[4] = {};
+    if (bias) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cols) b[j] = to_f32<OT>(bias[c0 + j]);
+    }
+    if (p.residual) {
+      const OT *res = static_cast<const OT *>(p.residual) + m * p.residual_stride + c0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < cols) r[j] = to_f32<OT>(res[j]);
+    }
+    const float4 *src = reinterpret_cast<const float4 *>(p.partial) + i;
+    float y[4] = {};
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {
+      float4 part[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s0 + s < p.splits) part[s] = src[static_cast<int64_t>(s0 + s) * total];
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        if (s0 + s < p.splits) {
+          y[0] += part[s].x;
+          y[1] += part[s].y;
+          y[2] += part[s].z;
+          y[3] += part[s].w;
+        }
+    }
+    float slope[4];
+    with_activation(p.activation, [&](auto act) {
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        float2 value, slopes;
+        activate_slope2<decltype(act)::value, sizeof(OT) == 2>(make_float2(y[j] + b[j], y[j + 1] + b[j + 1]), value, slopes);
+        y[j] = value.x, y[j + 1] = value.y;
+        slope[j] = slopes.x, slope[j + 1] = slopes.y;
+      }
+    });
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int64_t c = c0 + j;
-      if (c >= p.n) break;
-      if (bias) y[j] += to_f32<OT>(bias[c]);
-      float slope = 1.f;
-      with_activation(p.activation, [&](auto act) {
-        float2 value, slopes;
-        activate_slope2<decltype(act)::value, sizeof(OT) == 2>(make_float2(y[j], y[j]), value, slopes);
-        y[j] = value.x;
-        slope = slopes.x;
-      });
+      if (j >= cols) break;
       if constexpr (sizeof(OT) == 2) {
         if (p.saved_half)
-          p.saved_half[m * p.saved_pitch + c] = static_cast<uint16_t>(Factor<OT>::slope(f2(slope)));
+          p.saved_half[m * p.saved_pitch + c0 + j] = static_cast<uint16_t>(Factor<OT>::slope(f2(slope[j])));
       }
-      if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c] = slope;
-      if (res) y[j] += to_f32<OT>(res[c]);
-      out[c] = from_f32<OT>(y[j]);
+      if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c0 + j] = slope[j];
+      out[j] = from_f32<OT>(y[j] + r[j]);
     }
   }
+}
+
+// dst[c] = the sum over the chunks of partial[chunk][c]: eight columns a block, 32 threads a column with
+// eight reads in flight each, joined in a fixed order.
+template <typename OT>
+__device__ __forceinline__ void column_sums(const ColumnSums &p) {
+  __shared__ float all[8][8];
+  const int c = threadIdx.x & 7, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int64_t c0 = static_cast<int64_t>(blockIdx.x) * 8; c0 < p.columns; c0 += static_cast<int64_t>(gridDim.x) * 8) {
+    float sum = 0.f;
+    if (c0 + c < p.columns) {
+      const float *src = p.partial + c0 + c;
+      for (int64_t k0 = threadIdx.x >> 3; k0 < p.chunks; k0 += 8 * 32) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = k0 + 32 * i < p.chunks ? src[(k0 + 32 * i) * p.stride] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += x[i];
+      }
+    }
+    sum += __shfl_xor_sync(kFull, sum, 8);
+    sum += __shfl_xor_sync(kFull, sum, 16);
+    if (lane < 8) all[warp][lane] = sum;
+    __syncthreads();
+    if (threadIdx.x < 8 && c0 + c < p.columns) {
+      float total = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) total += all[w][c];
+      static_cast<OT *>(p.out)[c0 + c] = from_f32<OT>(total);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename OT>
+__global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ FinishLaunch launch) {
+  dependency_wait();
+  const int y = blockIdx.y;
+  if (y < launch.products)
+    reduce<OT>(launch.product[y]);
+  else
+    column_sums<OT>(launch.sums[y - launch.products]);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1157,6 +1225,7 @@ TileClass tile_class(const LayerGemm &g, int bn, int splits) {
           ceil_div(k_blocks, splits) * g.segments * step_clocks(f32, bn) + 800};
 }
 int split_limit(const LayerGemm &g) {
+  if (g.batch * g.m * align_up(g.n, 4) >= int64_t(1) << 31) return 1;
   return static_cast<int>(std::min<int64_t>((ceil_div(g.k, g.pieces > 1 ? 32 : BK) + 1) / 2, 64));
 }
 // Split sums are written, read and reduced by another launch.
@@ -1383,15 +1452,17 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaSt
                              : launch_16<kGate>(ctx, dtype, bn, l, stream);
       return dtype == AF2_F32 ? launch_bn<kOut, float>(ctx, bn, l, stream) : launch_16<kOut>(ctx, dtype, bn, l, stream);
     });
-  if (st != AF2_OK) return st;
+  return st;
+}
 
-  ReduceLaunch reduce{};
-  int split = 0;
-  int64_t most = 0;
+af2_status layer_finish_launch(af2_ctx *ctx, int dtype, const LayerGemm *g, int count, const ColumnSums *sums,
+                               int sum_count, cudaStream_t stream) {
+  FinishLaunch l{};
+  int64_t blocks = 0;
   for (int j = 0; j < count; ++j) {
     const LayerGemm &q = g[j];
     if (q.splits == 1) continue;
-    ReduceArgs &r = reduce.product[split++];
+    ReduceArgs &r = l.product[l.products++];
     r.partial = reinterpret_cast<const float *>(q.scratch);
     r.splits = q.splits;
     r.batch = q.batch;
@@ -1409,16 +1480,21 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaSt
     r.saved_half = q.saved.half;
     r.saved_f32 = q.saved.f32;
     r.saved_pitch = q.saved.pitch;
-    most = std::max<int64_t>(most, q.batch * q.m * r.pitch / 4);
+    blocks = std::max(blocks, ceil_div(q.batch * q.m * r.pitch / 4, 256));
   }
-  if (!split) return AF2_OK;
-  const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(most, 256), 8 * ctx->sm_count));
+  for (int j = 0; j < sum_count; ++j) {
+    l.sums[j] = sums[j];
+    blocks = std::max(blocks, ceil_div(sums[j].columns, 8));
+  }
+  if (blocks == 0) return AF2_OK;
+  blocks = std::min<int64_t>(blocks, 8 * ctx->sm_count);
   LaunchScope scope(ctx, stream, kProfLayerElementwise);
   cudaError_t e = cudaSuccess;
-  with_element(g[0].out_dtype, [&](auto *tag) {
-    e = launch_early(reduce_kernel<std::remove_pointer_t<decltype(tag)>>, dim3(blocks, split), 256, 0, stream, reduce);
+  with_element(dtype, [&](auto *tag) {
+    e = launch_early(finish_kernel<std::remove_pointer_t<decltype(tag)>>,
+                     dim3(static_cast<unsigned>(blocks), l.products + sum_count), 256, 0, stream, l);
   });
-  if (e != cudaSuccess) return cuda_fail(ctx, e, "layer split sums");
+  if (e != cudaSuccess) return cuda_fail(ctx, e, "layer sums");
   return AF2_OK;
 }
 

@@ -70,4 +70,16 @@ constexpr int kMaxProducts = 4;
 int layer_gemm_plan(LayerGemm *g, int count);
 af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaStream_t stream);
 
+// out[c] of the call's type = the sum over the chunks of partial[chunk * stride + c].
+struct ColumnSums {
+  const float *partial = nullptr;
+  int64_t chunks = 0, stride = 0, columns = 0;
+  void *out = nullptr;
+};
+constexpr int kMaxSums = 3;
+// What is left after layer_gemm_launch, in one launch (none where there is nothing): the sums of the
+// products that were split, and column sums.
+af2_status layer_finish_launch(af2_ctx *ctx, int dtype, const LayerGemm *g, int count, const ColumnSums *sums,
+                               int sum_count, cudaStream_t stream);
+
 }  // namespace af2
