@@ -744,7 +744,8 @@ AF2_API af2_status af2_gradient_norm_workspace_bytes(int64_t count, uint64_t *by
 /*
  * norm[0] (f32, on the device) = the square root of the sum of the squares of
  * every element of the `count` tensors (a host array of refs, read before the
- * call returns).  Squares are summed in f64, so no finite f32 input overflows,
+ * call returns).  Squares are summed in f64 (eight at a time in f32 where
+ * their sum neither overflows nor is tiny), so no finite f32 input overflows,
  * in an order that depends on the sizes alone; an infinity or a NaN among the
  * elements makes the norm infinite or NaN.  No tensors: 0.
  */
