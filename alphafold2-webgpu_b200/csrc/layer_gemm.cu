@@ -46,10 +46,12 @@ constexpr int BM = 128, PAIR_M = 256, BK = 64;
 constexpr int EPI_WARPS = 16, THREADS = 64 + 32 * EPI_WARPS;
 constexpr int kPairs = 74;  // CTA pairs of a B200; only the choice of tiles and splits depends on it
 
-// The kernels behind the epilogues: Out, the same for several products with nothing but their sums
+// The kernels behind the epilogues: Out, the same with the slopes kept and (with or without them) where
+// TMA cannot address the rows of what is written or of the residual (their code costs Out registers:
+// 163578 x 112 -> 40 took 27 us with both in it, 22 without), Out for several products with nothing but their sums
 // (whose arguments are no longer operands from the constant bank but loads), and Gate with and
 // without what the backward pass needs.
-enum Kind { kOut, kProducts, kGate, kGateSave, kGateBackward };
+enum Kind { kOut, kOutSave, kOutRows, kProducts, kGate, kGateSave, kGateBackward };
 
 // Stages of the operand ring and bytes of one epilogue warp's staging: 32 x 32 blocks of 16 bits
 // (2 KB), two of them (GateBackward: one of each factor); three where h and two factors leave
@@ -211,63 +213,52 @@ __device__ __forceinline__ void load_raw16(const T *row, int c0, int cols, bool 
   }
 }
 
-// 16-byte piece c of row `row` of a 32 x 32 block of 16 bits (64B-swizzled), and one element of it.
+// 16-byte piece c of row `row` of a 32 x 32 block of 16 bits (64B-swizzled).
 __device__ __forceinline__ uint4 *piece16(uint8_t *block, int row, int c) {
   return reinterpret_cast<uint4 *>(block + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
-}
-__device__ __forceinline__ uint16_t *element16(uint8_t *block, int row, int col) {
-  return reinterpret_cast<uint16_t *>(piece16(block, row, col >> 3)) + (col & 7);
 }
 // 16-byte piece c of a 32 x 32 block of f32 (128B-swizzled, 4 KB).
 __device__ __forceinline__ float4 *piece32(uint8_t *block, int row, int c) {
   return reinterpret_cast<float4 *>(block + sw128_offset(row, c));
 }
 
-// Rows that TMA cannot address, moved between memory and a block with the lanes along each row:
-// eight loads, then eight stores (one after the other each waits for its load: a residual in f32
-// took 25,000 clocks a tile).
-template <typename T, bool IN>
+// Rows that TMA cannot address, moved between memory and a block with the lanes along each row (f32: 16
+// lanes, two rows at a time): BATCH loads, then their stores.  (One after the other each store waits for
+// its load; with the block's swizzled addresses worked out for each element instead of four times, 34
+// instructions a row made an unaligned 60690 x 424 -> 737 product 91 us instead of 55.)
+template <typename T, bool IN, int BATCH = 8>
 __device__ __forceinline__ void move_rows(uint8_t *block, T *at, int64_t stride, int rows, int cols, int lane) {
-  if (lane >= cols) return;
-  T *g = at + lane;
-  for (int r0 = 0; r0 < rows; r0 += 4) {
-    T v[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (r0 + i < rows) v[i] = IN ? g[(r0 + i) * stride] : *reinterpret_cast<T *>(element16(block, r0 + i, lane));
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (r0 + i < rows) {
-        if constexpr (IN)
-          *reinterpret_cast<T *>(element16(block, r0 + i, lane)) = v[i];
-        else
-          g[(r0 + i) * stride] = v[i];
-      }
-  }
-}
-// The same of 16 columns of f32, two rows at a time.
-template <bool IN>
-__device__ __forceinline__ void move_rows_f32(uint8_t *block, float *at, int64_t stride, int rows, int cols, int lane) {
-  const int c = lane & 15;
+  constexpr int SIDE = sizeof(T) == 4 ? 2 : 1, EACH = 16 / sizeof(T), SPAN = BATCH * SIDE;  // rows at a time
+  static_assert(SPAN % 8 == 0 && 32 % SPAN == 0);
+  const int c = SIDE == 2 ? lane & 15 : lane, side = SIDE == 2 ? lane >> 4 : 0;
   if (c >= cols) return;
-  float *g = at + c;
-  auto s = [&](int r) { return reinterpret_cast<float *>(piece16(block, r, c >> 2)) + (c & 3); };
+  // where the column lies in a row whose number / 2 leaves k to 4
+  uint8_t *column[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    column[k] = block + side * 64 + (((c / EACH) ^ k) << 4) + (c % EACH) * static_cast<int>(sizeof(T));
+  T *g = at + c;
+  auto element = [&](int r0, int i) { return reinterpret_cast<T *>(column[(SIDE * i >> 1) & 3] + (r0 + SIDE * i) * 64); };
 #pragma unroll 1
-  for (int r0 = 0; r0 < rows; r0 += 8) {
-    float v[4];
+  for (int r0 = 0; r0 < rows; r0 += SPAN) {
+    T v[BATCH];
+    if constexpr (IN) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + 2 * i + (lane >> 4);
-      if (r < rows) v[i] = IN ? g[r * stride] : *s(r);
-    }
+      for (int i = 0; i < BATCH; ++i)  // (the last row again instead of one past it: a condition would part the loads)
+        v[i] = g[min(r0 + SIDE * i + side, rows - 1) * stride];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + 2 * i + (lane >> 4);
-      if (r < rows) {
-        if constexpr (IN)
-          *s(r) = v[i];
-        else
-          g[r * stride] = v[i];
+      for (int i = 0; i < BATCH; ++i) *element(r0, i) = v[i];
+    } else {
+      T *to = g + (r0 + side) * stride;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) v[i] = *element(r0, i);
+      if (r0 + SPAN <= rows) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i, to += SIDE * stride) *to = v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i, to += SIDE * stride)
+          if (r0 + SIDE * i + side < rows) *to = v[i];
       }
     }
   }
@@ -668,7 +659,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       } else {
         // out = act(acc + bias) (+ residual)
-        constexpr bool PLAIN = KIND == kProducts;
+        constexpr bool PLAIN = KIND == kProducts, LANES = KIND == kOutRows || PLAIN;
         const int partial = p.partial;
         const bool tma_residual = !PLAIN && p.tma_residual;
         const OT *residual = PLAIN ? nullptr : static_cast<const OT *>(p.residual);
@@ -677,7 +668,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         // The residual's blocks come ahead, each into the block that its result leaves from: the two in
         // turn, the second where the first holds slopes (f32: the two halves of the warp's only block of
         // columns).
-        const bool keep = !PLAIN && p.save;
+        const bool keep = (KIND == kOutSave || KIND == kOutRows) && p.save;
         auto fetch = [&](int b, int at) {
           if (lane == 0) {
             bulk_wait_read_all();
@@ -689,14 +680,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         };
         const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - r0));
         if (tma_residual && first < end) fetch(first, loads);
-        if constexpr (F32) {
-          if (residual && !tma_residual && first < end) {
+        // ... or by the lanes, into the second block
+        const bool lane_residual = KIND == kOutRows && residual && !tma_residual;
+        [[maybe_unused]] auto bring = [&](int b) {
+          if (lane == 0) bulk_wait_read_all();
+          __syncwarp();
+          const int c = n0 + b * 32;
+          move_rows<OT, true, 16>(block + 2048, const_cast<OT *>(residual) + static_cast<int64_t>(r0) * p.residual_stride + c,
+                                  p.residual_stride, rows, min(32, p.n - c), lane);
+          __syncwarp();
+        };
+        if constexpr (!F32) {
+          if (lane_residual && first < end) bring(first);
+        } else {
+          if (lane_residual && first < end) {
             if (lane == 0) bulk_wait_read_all();
             __syncwarp();
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
               const int c = n0 + first * 32 + 16 * h;
-              move_rows_f32<true>(block + 2048 * h, const_cast<float *>(residual) + static_cast<int64_t>(r0) * p.residual_stride + c,
+              move_rows<OT, true>(block + 2048 * h, const_cast<OT *>(residual) + static_cast<int64_t>(r0) * p.residual_stride + c,
                                   p.residual_stride, rows, min(16, p.n - c), lane);
             }
             __syncwarp();
@@ -740,7 +743,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               if (!PLAIN && !partial && p.activation != AF2_ACTIVATION_NONE)
                 with_activation(p.activation, [&](auto act) {
                   constexpr int ACT = decltype(act)::value;
-                  if (p.save) {
+                  if (keep) {
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                       float2 value[2], s[2];
@@ -778,7 +781,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
                 *piece = o;
               }
-              if (p.tma_out) {
+              if (!LANES || p.tma_out) {
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
@@ -787,7 +790,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
               } else {
                 __syncwarp();
-                move_rows_f32<false>(dst, static_cast<float *>(p.out[tile.z]) + static_cast<int64_t>(r0) * p.out_stride + c0,
+                move_rows<OT, false>(dst, static_cast<OT *>(p.out[tile.z]) + static_cast<int64_t>(r0) * p.out_stride + c0,
                                      p.out_stride, rows, cols, lane);
                 __syncwarp();
               }
@@ -818,7 +821,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
           }
           if (!PLAIN && !partial && p.activation != AF2_ACTIVATION_NONE) {
-            if (p.save) {  // the slopes, through the first block
+            if (keep) {  // the slopes, through the first block
               if (lane == 0) bulk_wait_read_all();
               __syncwarp();
               with_activation(p.activation, [&](auto act) {
@@ -869,7 +872,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             continue;
           }
           // the block that the result leaves from, with the residual in it where there is one
-          const uint32_t at = 2048u * (keep ? 1 : tma_residual ? loads & 1 : stores++ & 1);
+          const uint32_t at = 2048u * (keep || lane_residual ? 1 : tma_residual ? loads & 1 : stores++ & 1);
           uint8_t *const dst = block + at;
           if (tma_residual) {
             ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
@@ -882,7 +885,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               break;
             }
             ++loads;
-          } else {
+          } else if (!lane_residual) {
             if (lane == 0) {
               if (PLAIN)
                 bulk_wait_read_all();  // (f32 sums of another product may be leaving both blocks)
@@ -890,11 +893,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 bulk_wait_read_but_one();
             }
             __syncwarp();
-            if (residual) {
-              move_rows<OT, true>(dst, const_cast<OT *>(residual) + static_cast<int64_t>(r0) * p.residual_stride + c0,
-                                  p.residual_stride, rows, cols, lane);
-              __syncwarp();
-            }
           }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -912,7 +910,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
             *piece = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          if (p.tma_out) {
+          if (!LANES || p.tma_out) {
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -926,6 +924,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             __syncwarp();
           }
           if (tma_residual && keep && b + step < end) fetch(b + step, loads);
+          if (lane_residual && b + step < end) bring(b + step);
         }
         }
         if (!ok) break;
@@ -1107,7 +1106,11 @@ af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l,
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const int pairs = launch_pairs(ctx, l.total_tiles);
-  l.alternate = l.total_tiles > pairs && sizeof(OT) == 2;
+  // Two groups of eight warps take tiles in turn where a tile has at most four blocks of columns, so that
+  // some warps would have none of it; otherwise all take each tile, whose accumulator is then free sooner
+  // (60690 x 424 -> 736: 60.5 us in turn, 54.1 together; 163578 x 112 -> 40: 22.4 and 29.4).
+  const int width = std::min(KIND == kGate || KIND == kGateSave ? BN / 2 : BN, l.product[0].args.n);
+  l.alternate = l.total_tiles > pairs && sizeof(OT) == 2 && width <= 128;
   LaunchScope scope(ctx, stream, kProfLayerGemm);
   if (cudaError_t e = launch_early(kernel, dim3(2 * pairs), THREADS, smem, stream, l); e != cudaSuccess)
     return cuda_fail(ctx, e, "layer product");
@@ -1450,7 +1453,13 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaSt
       if (g->epilogue == kEpilogueGate)
         return g->saved.half ? launch_16<kGateSave>(ctx, dtype, bn, l, stream)
                              : launch_16<kGate>(ctx, dtype, bn, l, stream);
-      return dtype == AF2_F32 ? launch_bn<kOut, float>(ctx, bn, l, stream) : launch_16<kOut>(ctx, dtype, bn, l, stream);
+      const Args &p = l.product[0].args;
+      auto out = [&](auto kind) {
+        constexpr int KIND = decltype(kind)::value;
+        return dtype == AF2_F32 ? launch_bn<KIND, float>(ctx, bn, l, stream) : launch_16<KIND>(ctx, dtype, bn, l, stream);
+      };
+      if (!p.tma_out || (p.residual && !p.tma_residual)) return out(std::integral_constant<int, kOutRows>());
+      return p.save ? out(std::integral_constant<int, kOutSave>()) : out(std::integral_constant<int, kOut>());
     });
   return st;
 }
