@@ -136,11 +136,11 @@ __device__ __forceinline__ void store_operand8(void *dst, int64_t at, int64_t pi
   }
 }
 
+// The copies, by block `block` of `blocks`.
 template <typename T>
-__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs p) {
-  dependency_wait();
-  for (int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; g < p.groups;
-       g += static_cast<int64_t>(gridDim.x) * 256) {
+__device__ __forceinline__ void pack_groups(const PackArgs &p, unsigned block, unsigned blocks) {
+  for (int64_t g = static_cast<int64_t>(block) * 256 + threadIdx.x; g < p.groups;
+       g += static_cast<int64_t>(blocks) * 256) {
     int j = 0;
     while (j + 1 < p.count && g >= p.job[j + 1].first) ++j;
     const PackJob &job = p.job[j];
@@ -152,6 +152,12 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
     values8<T>(raw, x);
     store_operand8<T>(job.dst, r * job.pitch + c, job.piece_stride, x);
   }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs p) {
+  dependency_wait();
+  pack_groups<T>(p, blockIdx.x, gridDim.x);
 }
 
 // ---- passes over rows, with column sums --------------------------------------------
@@ -166,6 +172,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
 struct RowGrid {
   int lanes, at_once, group;
   unsigned across;
+  unsigned down = 0;  // blocks along the rows
 };
 inline RowGrid row_grid(int64_t rows, int64_t width) {
   const int64_t pieces = ceil_div(width, 8), least = ceil_div(pieces, 256);
@@ -179,11 +186,12 @@ inline RowGrid row_grid(int64_t rows, int64_t width) {
       if (pass == 0)
         best = std::max(best, use);
       else if (use >= best - best / 16)
-        g = {static_cast<int>(lanes), static_cast<int>(at_once), 0, static_cast<unsigned>(n)};
+        g = {static_cast<int>(lanes), static_cast<int>(at_once), 0, static_cast<unsigned>(n), 0};
     }
   int each = 8;
   while (each > 1 && ceil_div(rows, g.at_once * each) * g.across < 296) each /= 2;
   g.group = g.at_once * each;
+  g.down = static_cast<unsigned>(ceil_div(rows, g.group));
   return g;
 }
 
@@ -193,10 +201,10 @@ inline RowGrid row_grid(int64_t rows, int64_t width) {
 template <typename T, int SETS, int DEPTH, int STREAMS, typename Load, typename Use>
 __device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, const RowGrid &grid, float *partial,
                                                int64_t pitch, Load &&load, Use &&use) {
-  dependency_wait();
+  const unsigned y = blockIdx.x / grid.down, x = blockIdx.x - y * grid.down;
   const int ty = threadIdx.x / grid.lanes, tx = threadIdx.x - ty * grid.lanes;
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * grid.lanes + tx) * 8;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * grid.group;
+  const int64_t c = (static_cast<int64_t>(y) * grid.lanes + tx) * 8;
+  const int64_t r0 = static_cast<int64_t>(x) * grid.group;
   float sums[SETS][8] = {};
   if (c < width && ty < grid.at_once) {
     const int end = static_cast<int>(min(rows - r0, static_cast<int64_t>(grid.group)));
@@ -221,8 +229,8 @@ __device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, cons
     for (int k = threadIdx.x; k < grid.lanes * 8; k += 256) {
       float total = 0.f;
       for (int w = 0; w < grid.at_once; ++w) total += all[w * grid.lanes + (k >> 3)][k & 7];
-      const int64_t col = static_cast<int64_t>(blockIdx.y) * grid.lanes * 8 + k;
-      if (col < pitch) partial[(static_cast<int64_t>(blockIdx.x) * SETS + s) * pitch + col] = total;
+      const int64_t col = static_cast<int64_t>(y) * grid.lanes * 8 + k;
+      if (col < pitch) partial[(static_cast<int64_t>(x) * SETS + s) * pitch + col] = total;
     }
   }
 }
@@ -234,6 +242,7 @@ __device__ __forceinline__ int columns_of(int64_t width, int64_t c) {
 template <typename T>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t stride, int64_t rows, int64_t width,
                                                          const RowGrid grid, float *partial, int64_t pitch) {
+  dependency_wait();
   for_row_groups<T, 1, 4, 1>(
       rows, width, grid, partial, pitch,
       [&](int64_t r, int64_t c, Raw8<T>(&in)[1]) { load_raw8<T>(src + r * stride + c, columns_of(width, c), in[0]); },
@@ -268,12 +277,16 @@ __device__ __forceinline__ void slopes8(const Raw8<T> &r, float (&x)[8]) {
   }
 }
 
-// dz = dy act'(z), the slope saved (without SLOPE dy itself), as an operand, with its column sums
+// dz = dy act'(z), the slope saved (without SLOPE dy itself), as an operand, with its column sums; the
+// blocks past these make the copies of other operands.
 template <typename T, bool SLOPE>
 __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t dy_stride, const SavedPlanes saved,
                                                           int64_t rows, int64_t width, const RowGrid grid, void *dz,
                                                           int64_t dz_pitch, int64_t dz_piece, float *partial,
-                                                          int64_t pitch) {
+                                                          int64_t pitch, const __grid_constant__ PackArgs copies) {
+  dependency_wait();
+  const unsigned own = grid.down * grid.across;
+  if (blockIdx.x >= own) return pack_groups<T>(copies, blockIdx.x - own, gridDim.x - own);
   constexpr int STREAMS = SLOPE ? 2 : 1, DEPTH = sizeof(T) == 4 ? 2 : 4;
   for_row_groups<T, 1, DEPTH, STREAMS>(
       rows, width, grid, partial, pitch,
@@ -301,6 +314,7 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
 template <int ACT>
 __global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, int64_t rows, int64_t width,
                                                        const RowGrid grid, void *h, int64_t h_pitch, int64_t h_piece) {
+  dependency_wait();
   for_row_groups<float, 1, 2, 2>(
       rows, width, grid, nullptr, 0,
       [&](int64_t r, int64_t c, Raw8<float>(&in)[2]) {
@@ -327,6 +341,7 @@ __global__ void __launch_bounds__(256) gate_backward_f32_kernel(const float *dh,
                                                                 int64_t width, const RowGrid grid, uint16_t *dgv,
                                                                 int64_t dgv_pitch, int64_t dgv_piece, int64_t dgv_set,
                                                                 float *partial, int64_t pitch) {
+  dependency_wait();
   for_row_groups<float, 2, 2, 3>(
       rows, width, grid, partial, pitch,
       [&](int64_t r, int64_t c, Raw8<float>(&in)[3]) {
@@ -404,9 +419,12 @@ class Pass {
     jobs_.groups += rows * (o.pitch / 8);
     return o;
   }
+  unsigned pack_blocks() const {
+    return static_cast<unsigned>(std::min<int64_t>(ceil_div(jobs_.groups, 256), 16 * ctx_->sm_count));
+  }
   void pack() {
     if (live() && jobs_.count) {
-      const int blocks = static_cast<int>(std::min<int64_t>(ceil_div(jobs_.groups, 256), 16 * ctx_->sm_count));
+      const unsigned blocks = pack_blocks();
       LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
       with_element(dtype_, [&](auto *tag) {
         check(launch_early(pack_kernel<std::remove_pointer_t<decltype(tag)>>, dim3(blocks), 256, 0, stream_, jobs_),
@@ -468,7 +486,7 @@ class Pass {
     if (!live()) return;
     const RowGrid grid = row_grid(rows, width);
     LaunchScope scope(ctx_, stream_, kProfLayerElementwise);
-    check(launch(dim3(static_cast<unsigned>(ceil_div(rows, grid.group)), grid.across), grid), "layer row pass");
+    check(launch(dim3(grid.down * grid.across), grid), "layer row pass");
   }
   // The column sums of a tensor: the blocks' sums, `sets` of them, and how many blocks there are.
   static int64_t sum_chunks(int64_t rows, int64_t width) { return ceil_div(rows, row_grid(rows, width).group); }
@@ -495,7 +513,8 @@ class Pass {
     });
     finish_sums(partial, sum_chunks(rows, width), width, dst);
   }
-  // dz = dy act'(z) (without SLOPE dy) into an operand, and its column sums
+  // dz = dy act'(z) (without SLOPE dy) into an operand, and its column sums; with it the operands taken
+  // so far are copied
   template <bool SLOPE>
   void slope(const void *dy, int64_t stride, const SavedPlanes &saved, int64_t rows, int64_t width,
              const GemmOperand &dz, void *d_bias) {
@@ -504,19 +523,19 @@ class Pass {
       cudaError_t e = cudaSuccess;
       with_element(dtype_, [&](auto *tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        e = launch_early(dense_slope_kernel<T, SLOPE>, blocks, 256, 0, stream_, static_cast<const T *>(dy), stride, saved,
-                         rows, width, grid, const_cast<void *>(dz.ptr), dz.pitch, dz.piece_stride, partial,
-                         saved_pitch(width));
+        e = launch_early(dense_slope_kernel<T, SLOPE>, dim3(blocks.x + pack_blocks()), 256, 0, stream_,
+                         static_cast<const T *>(dy), stride, saved, rows, width, grid, const_cast<void *>(dz.ptr),
+                         dz.pitch, dz.piece_stride, partial, saved_pitch(width), jobs_);
       });
       return e;
     });
+    jobs_ = PackArgs{};
     finish_sums(partial, sum_chunks(rows, width), width, d_bias);
   }
   // The operands taken so far copied, and a gradient as an operand (where one is wanted) with its
   // column sums: one pass for both where the operand is a copy.
   GemmOperand operand_and_sums(const void *dy, int64_t stride, int64_t rows, int64_t width, bool wanted, void *d_bias) {
     if (wanted && d_bias && !in_place(dy, stride)) {
-      pack();
       const GemmOperand o = make_operand(rows, width);
       slope<false>(dy, stride, SavedPlanes{}, rows, width, o, d_bias);
       return o;
@@ -610,7 +629,6 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
   if (p.activation == AF2_ACTIVATION_NONE) {
     dz = l.operand_and_sums(p.d_out, p.d_out_stride, p.rows, p.columns, p.d_x || p.d_weight, p.d_bias);
   } else {
-    l.pack();
     dz = l.make_operand(p.rows, p.columns);
     const SavedPlanes saved = l.planes(const_cast<void *>(p.saved), p.rows, p.columns, 1);
     l.slope<true>(p.d_out, p.d_out_stride, saved, p.rows, p.columns, dz, p.d_bias);
