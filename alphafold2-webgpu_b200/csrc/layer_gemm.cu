@@ -6,12 +6,9 @@
 // (cta_group::2): CTA r holds rows 128 r .. of A's tile and half of B's rows,
 // so each SM reads half of the B tile that it multiplies by.  Warp 0 of each
 // CTA issues TMA loads, warp 1 of the even CTA the MMAs, warps 2-17 drain the
-// two accumulators: where a pair has more than one tile, one group of eight
-// warps (two per TMEM lane quarter) each, so that the loads, arithmetic and
-// stores of one group fall between those of the other (all sixteen warps on one
-// tile keep in step, each unit idle while they use the next); else all on the
-// one tile.  One tile's epilogue overlaps the next
-// tile's MMAs.  Operands are taken as they are stored: K-major rows as one
+// two accumulators, together, or in two groups of eight (two per TMEM lane
+// quarter) that take tiles in turn where a tile is too narrow for all.  One
+// tile's epilogue overlaps the next tile's MMAs.  Operands are taken as they are stored: K-major rows as one
 // 128-byte-swizzled block per K step of 64, MN-major ones as 64-wide blocks of
 // 64 k each (the tensor core's transposed order), so no weight and no
 // activation is ever transposed in memory.  What an epilogue reads (residual,
