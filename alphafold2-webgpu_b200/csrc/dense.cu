@@ -47,27 +47,6 @@ struct PackArgs {
   int64_t groups;
 };
 
-// The three bf16 terms of eight f32, x = t0 + t1 + t2 exactly (but for what is below f32's smallest
-// normal number): the upper 16 bits of x, of what that leaves, and of what is then left.  Cutting
-// instead of rounding costs an and and a subtraction a term, and no finite x can overflow.
-__device__ __forceinline__ void split8(const float (&x)[8], uint4 (&t)[3]) {
-  uint32_t w[3][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      w[k][i] = __byte_perm(a, b, 0x7632);
-      if (k < 2) {
-        a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
-        b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
-      }
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < 3; ++k) t[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
-}
-
 // Eight values of a row as they are in memory (nothing is computed from them yet, so that a thread's
 // loads need not wait for one another), and as f32; zeros past the first n.
 template <typename T>
@@ -307,31 +286,6 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
 #pragma unroll
         for (int i = 0; i < 8; ++i) sums[0][i] += d[i];
         store_operand8<T>(dz, r * dz_pitch + c, dz_piece, d);
-      });
-}
-
-// f32: h = act(g) v as an operand, from the saved planes
-template <int ACT>
-__global__ void __launch_bounds__(256) gate_f32_kernel(const SavedPlanes saved, int64_t rows, int64_t width,
-                                                       const RowGrid grid, void *h, int64_t h_pitch, int64_t h_piece) {
-  dependency_wait();
-  for_row_groups<float, 1, 2, 2>(
-      rows, width, grid, nullptr, 0,
-      [&](int64_t r, int64_t c, Raw8<float>(&in)[2]) {
-        load_saved8<float>(saved, 0, r, c, in[0]);
-        load_saved8<float>(saved, 1, r, c, in[1]);
-      },
-      [&](int64_t r, int64_t c, const Raw8<float>(&in)[2], float (&)[1][8]) {
-        float g[8], v[8];
-        values8<float>(in[0], g);
-        values8<float>(in[1], v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 a = activate2<ACT, false>(make_float2(g[2 * i], g[2 * i + 1]));
-          g[2 * i] = a.x * v[2 * i];
-          g[2 * i + 1] = a.y * v[2 * i + 1];
-        }
-        store_operand8<float>(h, r * h_pitch + c, h_piece, g);
       });
 }
 
@@ -702,38 +656,20 @@ af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uin
   } else {
     h = l.make_operand(p.rows, p.hidden);
   }
-  uint8_t *const planes_at =
-      p.saved ? static_cast<uint8_t *>(p.saved) + hidden_bytes(p.rows, p.hidden, p.dtype)
-              : (l.f32() ? l.take(planes_bytes(p.rows, p.hidden, p.dtype, 2)) : nullptr);
   LayerGemm g = l.product(p.rows, p.hidden, p.channels);
   g.a[0] = x;
   g.b[0] = Pass::mn(wg);
   g.b[1] = Pass::mn(wv);
   g.bias[0] = p.w.gate_bias;
   g.bias[1] = p.w.value_bias;
-  if (l.f32()) {
-    const SavedPlanes s = l.planes(planes_at, p.rows, p.hidden, 2);
-    g.batch = 2;
-    g.out[0] = s.f32;
-    g.out[1] = s.f32 + s.stride;
-    g.out_stride = s.pitch;
-    l.run(g);
-    l.rows_kernel(p.rows, p.hidden, [&](dim3 blocks, const RowGrid &grid) {
-      cudaError_t e = cudaSuccess;
-      with_activation(p.activation, [&](auto act) {
-        e = launch_early(gate_f32_kernel<decltype(act)::value>, blocks, 256, 0, stream, s, p.rows, p.hidden, grid,
-                         const_cast<void *>(h.ptr), h.pitch, h.piece_stride);
-      });
-      return e;
-    });
-  } else {
-    g.epilogue = kEpilogueGate;
-    g.activation = p.activation;
-    g.out[0] = const_cast<void *>(h.ptr);
-    g.out_stride = h.pitch;
-    if (p.saved) g.saved = l.planes(planes_at, p.rows, p.hidden, 2);
-    l.run(g);
-  }
+  g.epilogue = kEpilogueGate;
+  g.activation = p.activation;
+  g.out[0] = const_cast<void *>(h.ptr);
+  g.out_stride = h.pitch;
+  g.out_piece_stride = h.piece_stride;
+  if (p.saved)
+    g.saved = l.planes(static_cast<uint8_t *>(p.saved) + hidden_bytes(p.rows, p.hidden, p.dtype), p.rows, p.hidden, 2);
+  l.run(g);
   LayerGemm y = l.product(p.rows, p.channels, p.hidden);
   y.a[0] = h;
   y.b[0] = Pass::mn(wo);

@@ -61,7 +61,7 @@ struct Shape {
   static constexpr uint32_t A_TERM = BM * STEP * 2, B_TERM = (BN / 2) * STEP * 2;
   static constexpr uint32_t OFF_B = (F32 ? 3 : 1) * A_TERM;
   static constexpr uint32_t STAGE_BYTES = OFF_B + (F32 ? 3 : 1) * B_TERM;
-  static constexpr uint32_t SLOT_BYTES = KIND == kGateSave ? 6144 : 4096;
+  static constexpr uint32_t SLOT_BYTES = KIND == kGateSave && !F32 ? 6144 : 4096;
   static constexpr int STAGES = (229376 - EPI_WARPS * SLOT_BYTES) / STAGE_BYTES;
   static constexpr uint32_t OFF_STAGE = STAGES * STAGE_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_STAGE + EPI_WARPS * SLOT_BYTES;
@@ -484,18 +484,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const int64_t m = static_cast<int64_t>(r0) + lane;
       const int n0 = tile.ni * WIDTH;
       // this warp's blocks of the tile: first, first + step, ... below `end`
-      const int end = r0 < p.m ? min(WIDTH / 32, (p.n - n0 + 31) >> 5) : 0;
+      // (the f32 gate's are 16 columns wide: a warp has those of the gate and of the value)
+      constexpr int SHIFT = F32 && GATE ? 4 : 5;
+      const int end = r0 < p.m ? min(WIDTH >> SHIFT, (p.n - n0 + (1 << SHIFT) - 1) >> SHIFT) : 0;
       bool ok = true;
       // f32: the sums of each part of the depth, into registers (each warp has one block: BN is 128)
       [[maybe_unused]] float sums[32];
       auto add_part = [&](int b, int from, int to) {
-        const uint32_t at = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + first * 32;
+        const uint32_t at0 = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + (first << SHIFT);
 #pragma unroll
         for (int c = 0; c < 32; c += 16) {  // (all at once takes more registers than there are)
           if (c < from || c >= to) continue;
           uint32_t r[16], small[16];
-          tmem_ld16(at + c, r);
-          tmem_ld16(at + 128 + c, small);
+          const uint32_t at = at0 + (GATE && c ? WIDTH : c);
+          tmem_ld16(at, r);
+          tmem_ld16(at + 128, small);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; ++i) sums[c + i] += __uint_as_float(r[i]) + __uint_as_float(small[i]);
@@ -587,6 +590,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         // h = act(g) v; columns [0, BN / 2) of the accumulator are g, the others v
         if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) break;
         tc_fence_after();
+        if constexpr (F32) {
+          if (first < end) {
+            add_part(buf, 0, 32);
+            const int c0 = n0 + first * 16, cols = min(16, p.n - c0);
+#pragma unroll
+            for (int set = 0; set < 2; ++set) {
+              const float *bias = static_cast<const float *>(p.bias[set]);
+              float *z = sums + 16 * set;
+              if (bias && p.vector_bias && cols == 16) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float4 u = __ldg(reinterpret_cast<const float4 *>(bias + c0) + i);
+                  z[4 * i] += u.x, z[4 * i + 1] += u.y, z[4 * i + 2] += u.z, z[4 * i + 3] += u.w;
+                }
+              } else if (bias) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] += i < cols ? __ldg(bias + c0 + i) : 0.f;
+              }
+            }
+            // h as three terms [3][32][16], then g and v
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+            with_activation(p.activation, [&](auto act) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                float h[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int j = 8 * half + 2 * i;
+                  const float2 a = activate2<decltype(act)::value, false>(make_float2(sums[j], sums[j + 1]));
+                  h[2 * i] = a.x * sums[16 + j];
+                  h[2 * i + 1] = a.y * sums[16 + j + 1];
+                }
+                uint4 terms[3];
+                split8(h, terms);
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                  *reinterpret_cast<uint4 *>(block + k * 1024 + lane * 32 + half * 16) = terms[k];
+              }
+            });
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&maps.out[0], block_addr, c0, r0, 0);
+              bulk_commit();
+            }
+            if constexpr (KIND == kGateSave) {
+              if (lane == 0) bulk_wait_read_all();
+              __syncwarp();
+#pragma unroll
+              for (int set = 0; set < 2; ++set)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const float *z = sums + 16 * set + 4 * c;
+                  *reinterpret_cast<float4 *>(piece16(block + 2048 * set, lane, c)) = make_float4(z[0], z[1], z[2], z[3]);
+                }
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_3d(&maps.half, block_addr, c0, r0, 0);
+                tma_store_3d(&maps.half, block_addr + 2048, c0, r0, 1);
+                bulk_commit();
+              }
+            }
+          }
+        } else
 #pragma unroll 1
         for (int b = first; b < end; b += step) {
           const int c0 = n0 + b * 32;
@@ -1390,7 +1459,11 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
       if (g.bias[i] && reinterpret_cast<uintptr_t>(g.bias[i]) % 16 != 0) p.vector_bias = 0;
       if (i < outs && !aligned16(g.out[i], g.out_stride, out_bytes)) p.tma_out = 0;
     }
-    if (p.tma_out)
+    const bool terms = gate && out_bytes == 4;
+    if (terms)  // h, and below g and v
+      maps_ok &= encode_map_3d(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.out[0], g.n, g.m, 3, g.out_stride * 2,
+                               g.out_piece_stride * 2, 16, 32, 3, CU_TENSOR_MAP_SWIZZLE_NONE);
+    else if (p.tma_out)
       for (int i = 0; i < outs; ++i)
         maps_ok &= encode_map_3d(&maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
                                  g.out_stride * out_bytes, out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -1403,6 +1476,9 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
       maps_ok &= encode_map_3d(&maps.half, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.saved.half, g.saved.pitch, g.m,
                                g.epilogue == kEpilogueOut ? 1 : 2, g.saved.pitch * 2, g.saved.stride * 2, 32, 32, 1,
                                CU_TENSOR_MAP_SWIZZLE_64B);
+    if (terms && g.saved.f32)
+      maps_ok &= encode_map_3d(&maps.half, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.saved.f32, g.n, g.m, 2, g.saved.pitch * 4,
+                               g.saved.stride * 4, 16, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     p.column_partial = g.column_partial;
   }
   if (!maps_ok) return fail(ctx, AF2_ERR_CUDA, "cannot describe the layer's tensors to the TMA unit");
@@ -1448,7 +1524,9 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaSt
     st = describe_and_run<1>(ctx, g, 1, [&](auto &l) {
       if (g->epilogue == kEpilogueGateBackward) return launch_16<kGateBackward>(ctx, dtype, bn, l, stream);
       if (g->epilogue == kEpilogueGate)
-        return g->saved.half ? launch_16<kGateSave>(ctx, dtype, bn, l, stream)
+        return dtype == AF2_F32 ? (g->saved.f32 ? launch_bn<kGateSave, float>(ctx, bn, l, stream)
+                                                : launch_bn<kGate, float>(ctx, bn, l, stream))
+               : g->saved.half  ? launch_16<kGateSave>(ctx, dtype, bn, l, stream)
                              : launch_16<kGate>(ctx, dtype, bn, l, stream);
       const Args &p = l.product[0].args;
       auto out = [&](auto kind) {

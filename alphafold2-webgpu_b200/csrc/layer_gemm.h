@@ -19,7 +19,7 @@ struct GemmOperand {
 enum GemmEpilogue {
   kEpilogueOut = 0,       // out = act(acc + bias) (+ residual), saved = act'(acc + bias)
   kEpilogueGate = 1,      // b[0], b[1] are the gate's and the value's weights: out = act(g) v,
-                          // saved = v act'(g) and act(g): what the backward pass multiplies dh by
+                          // saved = v act'(g) and act(g): what the backward pass multiplies dh by (f32: g and v)
   kEpilogueGateBackward,  // acc = dh: out = dh times each of the two saved factors (dg and dv)
 };
 
@@ -47,6 +47,7 @@ struct LayerGemm {
   int out_dtype = 0;
   void *out[2] = {nullptr, nullptr};
   int64_t out_stride = 0;
+  int64_t out_piece_stride = 0;              // f32 gate: out[0] is an operand of three terms this far apart
   const void *bias[2] = {nullptr, nullptr};  // of out_dtype, or NULL
   const void *residual = nullptr;            // of out_dtype
   int64_t residual_stride = 0;

@@ -138,4 +138,25 @@ inline void with_element(int dtype, F &&f) {
     f(static_cast<float *>(nullptr));
 }
 
+// The three bf16 terms of eight f32, x = t0 + t1 + t2 exactly (but for what is below f32's smallest
+// normal number): the upper 16 bits of x, of what that leaves, and of what is then left.  Cutting
+// instead of rounding costs an and and a subtraction a term, and no finite x can overflow.
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 (&t)[3]) {
+  uint32_t w[3][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      w[k][i] = __byte_perm(a, b, 0x7632);
+      if (k < 2) {
+        a = __float_as_uint(__uint_as_float(a) - __uint_as_float(a & 0xffff0000u));
+        b = __float_as_uint(__uint_as_float(b) - __uint_as_float(b & 0xffff0000u));
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) t[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+}
+
 }  // namespace af2
