@@ -289,44 +289,6 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
       });
 }
 
-// f32: dg and dv as operands, `dgv_set` elements apart, from dh [rows][saved.pitch] and the saved planes
-template <int ACT>
-__global__ void __launch_bounds__(256) gate_backward_f32_kernel(const float *dh, const SavedPlanes saved, int64_t rows,
-                                                                int64_t width, const RowGrid grid, uint16_t *dgv,
-                                                                int64_t dgv_pitch, int64_t dgv_piece, int64_t dgv_set,
-                                                                float *partial, int64_t pitch) {
-  dependency_wait();
-  for_row_groups<float, 2, 2, 3>(
-      rows, width, grid, partial, pitch,
-      [&](int64_t r, int64_t c, Raw8<float>(&in)[3]) {
-        load_raw8<float>(dh + r * saved.pitch + c, 8, in[0]);
-        load_saved8<float>(saved, 0, r, c, in[1]);
-        load_saved8<float>(saved, 1, r, c, in[2]);
-      },
-      [&](int64_t r, int64_t c, const Raw8<float>(&in)[3], float (&sums)[2][8]) {
-        float d[8], g[8], v[8];
-        values8<float>(in[0], d);
-        values8<float>(in[1], g);
-        values8<float>(in[2], v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float2 value, slope;
-          activate_slope2<ACT, false>(make_float2(g[2 * i], g[2 * i + 1]), value, slope);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int j = 2 * i + k;
-            const bool in_row = c + j < width;  // past the width nothing was written
-            g[j] = in_row ? d[j] * v[j] * (k ? slope.y : slope.x) : 0.f;
-            v[j] = in_row ? d[j] * (k ? value.y : value.x) : 0.f;
-            sums[0][j] += g[j];
-            sums[1][j] += v[j];
-          }
-        }
-        store_operand8<float>(dgv, r * dgv_pitch + c, dgv_piece, g);
-        store_operand8<float>(dgv + dgv_set, r * dgv_pitch + c, dgv_piece, v);
-      });
-}
-
 // ---- one pass of a layer --------------------------------------------------------------
 
 // Lays the scratch out and launches; without a context it only counts the scratch.
@@ -718,38 +680,17 @@ af2_status gated_backward(af2_ctx *ctx, const GatedBackward &p, void *scratch, u
     LayerGemm g = l.product(p.rows, hid, c);
     g.a[0] = dy;
     g.b[0] = wo;
-    float *partial = nullptr;
-    int64_t chunks = 0;
-    if (l.f32()) {
-      chunks = Pass::sum_chunks(p.rows, hid);
-      if (sums) partial = l.sum_room(p.rows, hid, 2);
-      float *dh = reinterpret_cast<float *>(l.take(4ull * p.rows * saved.pitch));
-      g.out[0] = dh;
-      g.out_stride = saved.pitch;
-      l.run(g);
-      l.rows_kernel(p.rows, hid, [&](dim3 blocks, const RowGrid &grid) {
-        cudaError_t e = cudaSuccess;
-        with_activation(p.activation, [&](auto act) {
-          e = launch_early(gate_backward_f32_kernel<decltype(act)::value>, blocks, 256, 0, stream, dh, saved, p.rows,
-                           hid, grid, static_cast<uint16_t *>(const_cast<void *>(dgv[0].ptr)), dgv[0].pitch,
-                           dgv[0].piece_stride,
-                           static_cast<const uint16_t *>(dgv[1].ptr) - static_cast<const uint16_t *>(dgv[0].ptr),
-                           partial, saved.pitch);
-        });
-        return e;
-      });
-    } else {
-      chunks = ceil_div(p.rows, 32);
-      if (sums) partial = reinterpret_cast<float *>(l.take(8ull * chunks * saved.pitch));
-      g.epilogue = kEpilogueGateBackward;
-      g.activation = p.activation;
-      g.saved = saved;
-      g.out[0] = const_cast<void *>(dgv[0].ptr);
-      g.out[1] = const_cast<void *>(dgv[1].ptr);
-      g.out_stride = dgv[0].pitch;
-      g.column_partial = partial;
-      l.run(g);
-    }
+    const int64_t chunks = ceil_div(p.rows, 32);
+    float *partial = sums ? reinterpret_cast<float *>(l.take(8ull * chunks * saved.pitch)) : nullptr;
+    g.epilogue = kEpilogueGateBackward;
+    g.activation = p.activation;
+    g.saved = saved;
+    g.out[0] = const_cast<void *>(dgv[0].ptr);
+    g.out[1] = const_cast<void *>(dgv[1].ptr);
+    g.out_stride = dgv[0].pitch;
+    g.out_piece_stride = dgv[0].piece_stride;
+    g.column_partial = partial;
+    l.run(g);
     l.finish_sums(partial, chunks, hid, p.g.gate_bias, 0, 2);
     l.finish_sums(partial, chunks, hid, p.g.value_bias, 1, 2);
   }

@@ -525,7 +525,83 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256;
       const uint32_t acc_phase = (acc_it >> 1) & 1;
 
-      if constexpr (KIND == kGateBackward) {
+      if constexpr (KIND == kGateBackward && F32) {
+        // dg = dh v act'(g) and dv = dh act(g) from the saved g and v, 16 columns at a time: g and v come
+        // into the warp's blocks, the terms of dg and then of dv leave from them.
+        const int blocks = first < end ? min(2, (p.n - n0 - first * 32 + 15) >> 4) : 0;
+        auto fetch = [&](int c) {
+          if (lane == 0) {
+            bulk_wait_read_all();  // the terms before them have left
+            mbar_arrive_expect_tx(load(ew, 0), 4096);
+            tma_load_3d(block_addr, &maps.half, load(ew, 0), c, r0, 0);
+            tma_load_3d(block_addr + 2048, &maps.half, load(ew, 0), c, r0, 1);
+          }
+        };
+        if (blocks) fetch(n0 + first * 32);
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) {
+          if (blocks && lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, launch.err);
+          break;
+        }
+        tc_fence_after();
+        if (blocks) add_part(buf, 0, 32);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (half >= blocks) break;
+          const int c0 = n0 + first * 32 + 16 * half;
+          if (half) fetch(c0);
+          ok = warp_wait(load(ew, 0), loads & 1, abort_flag, launch.err, kErrWaitEpilogue);
+          if (!ok) {
+            if (lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, launch.err);
+            break;
+          }
+          ++loads;
+          float d[32];  // g and v, then dg and dv
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float4 u = *reinterpret_cast<const float4 *>(piece16(block + (c >> 2) * 2048, lane, c & 3));
+            d[4 * c] = u.x, d[4 * c + 1] = u.y, d[4 * c + 2] = u.z, d[4 * c + 3] = u.w;
+          }
+          with_activation(p.activation, [&](auto act) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float2 dh = make_float2(sums[16 * half + i], sums[16 * half + i + 1]);
+              const float2 v = make_float2(d[16 + i], d[16 + i + 1]);
+              float2 value, slope;
+              activate_slope2<decltype(act)::value, false>(make_float2(d[i], d[i + 1]), value, slope);
+              const float2 dg = f2mul(f2mul(dh, v), slope), dv = f2mul(dh, value);
+              d[i] = dg.x, d[i + 1] = dg.y;
+              d[16 + i] = dv.x, d[16 + i + 1] = dv.y;
+            }
+          });
+          __syncwarp();  // every lane has read g and v
+#pragma unroll
+          for (int set = 0; set < 2; ++set) {
+            if (set) {
+              if (lane == 0) bulk_wait_read_all();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              uint4 terms[3];
+              split8(reinterpret_cast<const float(&)[8]>(d[16 * set + 8 * part]), terms);
+#pragma unroll
+              for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<uint4 *>(block + k * 1024 + lane * 32 + part * 16) = terms[k];
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_3d(&maps.out[set], block_addr, c0, r0, 0);
+              bulk_commit();
+            }
+          }
+          if (p.column_partial) {
+            const float sum = lane_sums(d, lane);
+            p.column_partial[(static_cast<int64_t>(r0 >> 5) * 2 + (lane >> 4)) * p.saved_pitch + c0 + (lane & 15)] = sum;
+          }
+        }
+        if (!ok) break;
+      } else if constexpr (KIND == kGateBackward) {
         // dg = dh p and dv = dh a with the saved factors p = v act'(g) and a = act(g).  A block's
         // factors come into the warp's two blocks and the products leave from the same place.
         auto fetch = [&](int b) {
@@ -1338,7 +1414,7 @@ int layer_gemm_plan(LayerGemm *g, int count) {
   int64_t longest = 0;
   for (int i = 0; i < count; ++i) longest = std::max(longest, ceil_div(g[i].k, f32 ? 32 : BK) * g[i].segments);
   for (int bn : {256, 128}) {
-    if (g[0].epilogue == kEpilogueGateBackward && bn == 128) continue;
+    if (!f32 && g[0].epilogue == kEpilogueGateBackward && bn == 128) continue;
     if (f32 && bn == 256) continue;
     // `most`: K steps that a tile may have before its depth is cut
     for (int64_t most : {int64_t(1) << 40, int64_t(512), int64_t(384), int64_t(256), int64_t(192), int64_t(128),
@@ -1459,10 +1535,11 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
       if (g.bias[i] && reinterpret_cast<uintptr_t>(g.bias[i]) % 16 != 0) p.vector_bias = 0;
       if (i < outs && !aligned16(g.out[i], g.out_stride, out_bytes)) p.tma_out = 0;
     }
-    const bool terms = gate && out_bytes == 4;
-    if (terms)  // h, and below g and v
-      maps_ok &= encode_map_3d(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.out[0], g.n, g.m, 3, g.out_stride * 2,
-                               g.out_piece_stride * 2, 16, 32, 3, CU_TENSOR_MAP_SWIZZLE_NONE);
+    const bool terms = g.epilogue != kEpilogueOut && out_bytes == 4;
+    if (terms)  // h, or dg and dv; below g and v
+      for (int i = 0; i < outs; ++i)
+        maps_ok &= encode_map_3d(&maps.out[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.out[i], g.n, g.m, 3, g.out_stride * 2,
+                                 g.out_piece_stride * 2, 16, 32, 3, CU_TENSOR_MAP_SWIZZLE_NONE);
     else if (p.tma_out)
       for (int i = 0; i < outs; ++i)
         maps_ok &= encode_map_3d(&maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
@@ -1522,7 +1599,9 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaSt
     });
   else
     st = describe_and_run<1>(ctx, g, 1, [&](auto &l) {
-      if (g->epilogue == kEpilogueGateBackward) return launch_16<kGateBackward>(ctx, dtype, bn, l, stream);
+      if (g->epilogue == kEpilogueGateBackward)
+        return dtype == AF2_F32 ? launch_bn<kGateBackward, float>(ctx, bn, l, stream)
+                                : launch_16<kGateBackward>(ctx, dtype, bn, l, stream);
       if (g->epilogue == kEpilogueGate)
         return dtype == AF2_F32 ? (g->saved.f32 ? launch_bn<kGateSave, float>(ctx, bn, l, stream)
                                                 : launch_bn<kGate, float>(ctx, bn, l, stream))
