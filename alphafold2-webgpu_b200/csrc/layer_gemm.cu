@@ -92,13 +92,13 @@ struct Divisor {
 
 struct Args {
   void *out[2];
-  int64_t out_stride;
+  int64_t out_stride, out_piece_stride;
   const void *bias[2];
   const void *residual;
   int64_t residual_stride;
   uint32_t *saved_scale;
   float *saved_f32;
-  int64_t saved_pitch, scale_rows;
+  int64_t saved_pitch, saved_stride, scale_rows;
   float *column_partial;
   int64_t m;
   int n, k_blocks, splits, segments;
@@ -258,6 +258,25 @@ __device__ __forceinline__ void move_rows(uint8_t *block, T *at, int64_t stride,
           if (r0 + SIDE * i + side < rows) *to = v[i];
       }
     }
+  }
+}
+
+// 32 aligned bytes (a sector): a TMA store of 16 columns of terms, rows of 32 bytes, takes two clocks a row,
+// 12,000 for the six that a tile of the f32 gate's backward pass writes.
+__device__ __forceinline__ void store_sector(void *at, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+// The three terms of 16 f32, `piece` elements apart.
+__device__ __forceinline__ void store_terms16(uint16_t *at, int64_t piece, const float (&x)[16]) {
+  uint4 t[2][3];
+  split8(reinterpret_cast<const float(&)[8]>(x[0]), t[0]);
+  split8(reinterpret_cast<const float(&)[8]>(x[8]), t[1]);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const uint32_t w[8] = {t[0][k].x, t[0][k].y, t[0][k].z, t[0][k].w, t[1][k].x, t[1][k].y, t[1][k].z, t[1][k].w};
+    store_sector(at + k * piece, w);
   }
 }
 
@@ -490,11 +509,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       bool ok = true;
       // f32: the sums of each part of the depth, into registers (each warp has one block: BN is 128)
       [[maybe_unused]] float sums[32];
-      auto add_part = [&](int b, int from, int to) {
+      auto add_part = [&](int b) {
         const uint32_t at0 = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * 256 + (first << SHIFT);
 #pragma unroll
         for (int c = 0; c < 32; c += 16) {  // (all at once takes more registers than there are)
-          if (c < from || c >= to) continue;
           uint32_t r[16], small[16];
           const uint32_t at = at0 + (GATE && c ? WIDTH : c);
           tmem_ld16(at, r);
@@ -514,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           ok = warp_wait(acc_full(b), (acc_it >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
           if (!ok) break;
           tc_fence_after();
-          if (first < end) add_part(b, 0, 32);
+          if (first < end) add_part(b);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_leader_relaxed(acc_empty(b));
@@ -527,11 +545,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
       if constexpr (KIND == kGateBackward && F32) {
         // dg = dh v act'(g) and dv = dh act(g) from the saved g and v, 16 columns at a time: g and v come
-        // into the warp's blocks, the terms of dg and then of dv leave from them.
+        // into the warp's blocks, the terms of dg and dv leave from each lane along its row.
         const int blocks = first < end ? min(2, (p.n - n0 - first * 32 + 15) >> 4) : 0;
         auto fetch = [&](int c) {
           if (lane == 0) {
-            bulk_wait_read_all();  // the terms before them have left
             mbar_arrive_expect_tx(load(ew, 0), 4096);
             tma_load_3d(block_addr, &maps.half, load(ew, 0), c, r0, 0);
             tma_load_3d(block_addr + 2048, &maps.half, load(ew, 0), c, r0, 1);
@@ -543,12 +560,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           break;
         }
         tc_fence_after();
-        if (blocks) add_part(buf, 0, 32);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (half >= blocks) break;
+        if (blocks) add_part(buf);
+        // (rolled, the second half's sums moved to the first's place: a small launch runs this code once,
+        // and reading it takes longer than running it)
+#pragma unroll 1
+        for (int half = 0; half < blocks; ++half) {
           const int c0 = n0 + first * 32 + 16 * half;
-          if (half) fetch(c0);
           ok = warp_wait(load(ew, 0), loads & 1, abort_flag, launch.err, kErrWaitEpilogue);
           if (!ok) {
             if (lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, launch.err);
@@ -561,10 +578,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const float4 u = *reinterpret_cast<const float4 *>(piece16(block + (c >> 2) * 2048, lane, c & 3));
             d[4 * c] = u.x, d[4 * c + 1] = u.y, d[4 * c + 2] = u.z, d[4 * c + 3] = u.w;
           }
+          fence_async_smem();
+          __syncwarp();  // every lane has read g and v
+          if (half + 1 < blocks) fetch(c0 + 16);
           with_activation(p.activation, [&](auto act) {
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-              const float2 dh = make_float2(sums[16 * half + i], sums[16 * half + i + 1]);
+              const float2 dh = make_float2(sums[i], sums[i + 1]);
               const float2 v = make_float2(d[16 + i], d[16 + i + 1]);
               float2 value, slope;
               activate_slope2<decltype(act)::value, false>(make_float2(d[i], d[i + 1]), value, slope);
@@ -573,32 +593,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               d[16 + i] = dv.x, d[16 + i + 1] = dv.y;
             }
           });
-          __syncwarp();  // every lane has read g and v
+          if (m < p.m)
 #pragma unroll
-          for (int set = 0; set < 2; ++set) {
-            if (set) {
-              if (lane == 0) bulk_wait_read_all();
-              __syncwarp();
-            }
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              uint4 terms[3];
-              split8(reinterpret_cast<const float(&)[8]>(d[16 * set + 8 * part]), terms);
-#pragma unroll
-              for (int k = 0; k < 3; ++k)
-                *reinterpret_cast<uint4 *>(block + k * 1024 + lane * 32 + part * 16) = terms[k];
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_3d(&maps.out[set], block_addr, c0, r0, 0);
-              bulk_commit();
-            }
-          }
+            for (int set = 0; set < 2; ++set)
+              store_terms16(static_cast<uint16_t *>(p.out[set]) + m * p.out_stride + c0, p.out_piece_stride,
+                            reinterpret_cast<const float(&)[16]>(d[16 * set]));
           if (p.column_partial) {
             const float sum = lane_sums(d, lane);
             p.column_partial[(static_cast<int64_t>(r0 >> 5) * 2 + (lane >> 4)) * p.saved_pitch + c0 + (lane & 15)] = sum;
           }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sums[i] = sums[16 + i];
         }
         if (!ok) break;
       } else if constexpr (KIND == kGateBackward) {
@@ -668,7 +673,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         tc_fence_after();
         if constexpr (F32) {
           if (first < end) {
-            add_part(buf, 0, 32);
+            add_part(buf);
             const int c0 = n0 + first * 16, cols = min(16, p.n - c0);
 #pragma unroll
             for (int set = 0; set < 2; ++set) {
@@ -685,49 +690,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 for (int i = 0; i < 16; ++i) z[i] += i < cols ? __ldg(bias + c0 + i) : 0.f;
               }
             }
-            // h as three terms [3][32][16], then g and v
-            if (lane == 0) bulk_wait_read_all();
-            __syncwarp();
-            with_activation(p.activation, [&](auto act) {
+            // h as three terms, g and v, from each lane along its row
+            if (m < p.m) {
+              with_activation(p.activation, [&](auto act) {
+                float h[16];
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                float h[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int j = 8 * half + 2 * i;
-                  const float2 a = activate2<decltype(act)::value, false>(make_float2(sums[j], sums[j + 1]));
-                  h[2 * i] = a.x * sums[16 + j];
-                  h[2 * i + 1] = a.y * sums[16 + j + 1];
+                for (int i = 0; i < 16; i += 2) {
+                  const float2 a = activate2<decltype(act)::value, false>(make_float2(sums[i], sums[i + 1]));
+                  h[i] = a.x * sums[16 + i];
+                  h[i + 1] = a.y * sums[16 + i + 1];
                 }
-                uint4 terms[3];
-                split8(h, terms);
+                store_terms16(static_cast<uint16_t *>(p.out[0]) + m * p.out_stride + c0, p.out_piece_stride, h);
+              });
+              if constexpr (KIND == kGateSave) {
 #pragma unroll
-                for (int k = 0; k < 3; ++k)
-                  *reinterpret_cast<uint4 *>(block + k * 1024 + lane * 32 + half * 16) = terms[k];
-              }
-            });
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_3d(&maps.out[0], block_addr, c0, r0, 0);
-              bulk_commit();
-            }
-            if constexpr (KIND == kGateSave) {
-              if (lane == 0) bulk_wait_read_all();
-              __syncwarp();
+                for (int set = 0; set < 2; ++set)
 #pragma unroll
-              for (int set = 0; set < 2; ++set)
+                  for (int c = 0; c < 16; c += 8) {
+                    const float *z = sums + 16 * set + c;
+                    uint32_t w[8];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  const float *z = sums + 16 * set + 4 * c;
-                  *reinterpret_cast<float4 *>(piece16(block + 2048 * set, lane, c)) = make_float4(z[0], z[1], z[2], z[3]);
-                }
-              fence_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_3d(&maps.half, block_addr, c0, r0, 0);
-                tma_store_3d(&maps.half, block_addr + 2048, c0, r0, 1);
-                bulk_commit();
+                    for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(z[i]);
+                    store_sector(p.saved_f32 + set * p.saved_stride + m * p.saved_pitch + c0 + c, w);
+                  }
               }
             }
           }
@@ -863,12 +848,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               ++loads;
             }
             const float *bias = PLAIN || partial ? nullptr : static_cast<const float *>(p.bias[tile.z]);
-#pragma unroll
+            add_part(buf);
+            // (rolled, the second half's sums moved to the first's place: a small launch runs this code
+            // once, and reading it takes longer than running it)
+#pragma unroll 1
             for (int h = 0; h < 2; ++h) {
-              add_part(buf, 16 * h, 16 * h + 16);
               const int c0 = n0 + first * 32 + 16 * h;
               if (c0 >= p.n) break;
-              float *y = sums + 16 * h;
+              float *y = sums;
               const int cols = min(16, p.n - c0);
               if (bias) {
                 if (p.vector_bias && cols == 16) {
@@ -936,6 +923,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                      p.out_stride, rows, cols, lane);
                 __syncwarp();
               }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sums[i] = sums[16 + i];
             }
           }
         } else {
@@ -1527,6 +1516,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
                                out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     }
     p.out_stride = g.out_stride;
+    p.out_piece_stride = g.out_piece_stride;
     p.vector_bias = 1;
     p.tma_out = 1;
     for (int i = 0; i < 2; ++i) {
@@ -1535,12 +1525,8 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
       if (g.bias[i] && reinterpret_cast<uintptr_t>(g.bias[i]) % 16 != 0) p.vector_bias = 0;
       if (i < outs && !aligned16(g.out[i], g.out_stride, out_bytes)) p.tma_out = 0;
     }
-    const bool terms = g.epilogue != kEpilogueOut && out_bytes == 4;
-    if (terms)  // h, or dg and dv; below g and v
-      for (int i = 0; i < outs; ++i)
-        maps_ok &= encode_map_3d(&maps.out[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.out[i], g.n, g.m, 3, g.out_stride * 2,
-                                 g.out_piece_stride * 2, 16, 32, 3, CU_TENSOR_MAP_SWIZZLE_NONE);
-    else if (p.tma_out)
+    const bool terms = g.epilogue != kEpilogueOut && out_bytes == 4;  // written by the lanes
+    if (p.tma_out && !terms)
       for (int i = 0; i < outs; ++i)
         maps_ok &= encode_map_3d(&maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
                                  g.out_stride * out_bytes, out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -1548,12 +1534,13 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
     p.saved_f32 = g.saved.f32;
     p.saved_scale = g.saved.scale;
     p.saved_pitch = g.saved.pitch;
+    p.saved_stride = g.saved.stride;
     p.scale_rows = g.saved.scale_rows;
     if (g.saved.half)
       maps_ok &= encode_map_3d(&maps.half, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.saved.half, g.saved.pitch, g.m,
                                g.epilogue == kEpilogueOut ? 1 : 2, g.saved.pitch * 2, g.saved.stride * 2, 32, 32, 1,
                                CU_TENSOR_MAP_SWIZZLE_64B);
-    if (terms && g.saved.f32)
+    if (g.epilogue == kEpilogueGateBackward && out_bytes == 4)
       maps_ok &= encode_map_3d(&maps.half, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.saved.f32, g.n, g.m, 2, g.saved.pitch * 4,
                                g.saved.stride * 4, 16, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     p.column_partial = g.column_partial;

@@ -59,8 +59,8 @@ struct LayerGemm {
   uint8_t *scratch = nullptr;
 };
 
-// Row pitch (elements) of a 16-bit operand of `width`, and of the saved planes.
-inline int64_t operand_pitch(int64_t width) { return align_up(width, 8); }
+// Row pitch (elements) of a 16-bit operand of `width` (rows begin on a 32-byte sector), and of the saved planes.
+inline int64_t operand_pitch(int64_t width) { return align_up(width, 16); }
 inline int64_t saved_pitch(int64_t width) { return align_up(width, 32); }
 
 // Up to this many products of one type in a launch (more than one: kEpilogueOut with no bias, activation
