@@ -77,6 +77,13 @@ struct ProfilePending {
   int id;
   cudaEvent_t start, stop;
 };
+// A tensor map as last encoded for a shape.
+struct LayerMap {
+  static constexpr int kCount = 256;
+  uint64_t shape[7] = {};  // extents, strides, box, type and swizzle: all but the address
+  CUtensorMap map;
+};
+
 }  // namespace af2
 
 struct af2_ctx {
@@ -120,6 +127,7 @@ struct af2_ctx {
   // scratch of the layers with learned weights, the stream of its last use, and an event behind
   // that use (LayerScratch)
   af2::DeviceBuffer layer_scratch;
+  std::vector<af2::LayerMap> layer_maps;  // descriptors by their shapes (layer_map_3d)
   cudaEvent_t layer_done = nullptr;
   cudaStream_t layer_stream = nullptr;
 };
@@ -156,6 +164,11 @@ void clear_weight_cache(af2_ctx *ctx);
 bool encode_map_3d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base, uint64_t d0, uint64_t d1,
                    uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1,
                    uint32_t b2, CUtensorMapSwizzle swizzle);
+// The same for the layers, whose small calls would spend a third of their host time on it: a shape met
+// before keeps everything but the address (0.5 us an encoding; a gated training step has 27).
+bool layer_map_3d(af2_ctx *ctx, CUtensorMap *map, CUtensorMapDataType dtype, const void *base, uint64_t d0, uint64_t d1,
+                  uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1, uint32_t b2,
+                  CUtensorMapSwizzle swizzle);
 bool encode_map_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base, const uint64_t (&dims)[4],
                    const uint64_t (&strides_bytes)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle);
 

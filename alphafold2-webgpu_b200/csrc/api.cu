@@ -150,11 +150,16 @@ LaunchScope::~LaunchScope() {
 
 namespace {
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+PFN_cuTensorMapReplaceAddress_v12000 g_replace = nullptr;
 std::once_flag g_encode_once;
 
 void load_encode() {
   void *fn = nullptr;
   cudaDriverEntryPointQueryResult q{};
+  if (cudaGetDriverEntryPointByVersion("cuTensorMapReplaceAddress", &fn, 12000, cudaEnableDefault, &q) ==
+          cudaSuccess &&
+      q == cudaDriverEntryPointSuccess)
+    g_replace = reinterpret_cast<PFN_cuTensorMapReplaceAddress_v12000>(fn);
   if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) ==
           cudaSuccess &&
       q == cudaDriverEntryPointSuccess)
@@ -173,6 +178,25 @@ bool encode_map_3d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base
   const cuuint32_t estr[3] = {1, 1, 1};
   return g_encode(map, dtype, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool layer_map_3d(af2_ctx *ctx, CUtensorMap *map, CUtensorMapDataType dtype, const void *base, uint64_t d0, uint64_t d1,
+                  uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0, uint32_t b1, uint32_t b2,
+                  CUtensorMapSwizzle swizzle) {
+  const uint64_t shape[7] = {d0, d1, d2, stride1_bytes, stride2_bytes, b0 | static_cast<uint64_t>(b1) << 32,
+                             b2 | static_cast<uint64_t>(dtype) << 32 | static_cast<uint64_t>(swizzle) << 48};
+  uint64_t hash = 0;
+  for (uint64_t v : shape) hash = (hash ^ v) * 0x9e3779b97f4a7c15ull;
+  if (ctx->layer_maps.empty()) ctx->layer_maps.resize(LayerMap::kCount);
+  LayerMap &kept = ctx->layer_maps[hash >> 56];
+  if (g_replace && std::equal(shape, shape + 7, kept.shape)) {
+    *map = kept.map;
+    return g_replace(map, const_cast<void *>(base)) == CUDA_SUCCESS;
+  }
+  if (!encode_map_3d(map, dtype, base, d0, d1, d2, stride1_bytes, stride2_bytes, b0, b1, b2, swizzle)) return false;
+  std::copy(shape, shape + 7, kept.shape);
+  kept.map = *map;
+  return true;
 }
 
 bool encode_map_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base, const uint64_t (&dims)[4],

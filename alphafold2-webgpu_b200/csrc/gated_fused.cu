@@ -491,7 +491,7 @@ af2_status gated_fused_launch(af2_ctx *ctx, const GatedFused &f, cudaStream_t st
   Maps maps{};
   auto map = [&](CUtensorMap *m, const void *ptr, int64_t width, int64_t rows, int64_t pitch, int box_rows, int box_cols,
                  CUtensorMapSwizzle swizzle) {
-    return encode_map_3d(m, t, ptr, width, rows, 1, pitch * 2, pitch * 2, box_cols, box_rows, 1, swizzle);
+    return layer_map_3d(ctx, m, t, ptr, width, rows, 1, pitch * 2, pitch * 2, box_cols, box_rows, 1, swizzle);
   };
   bool ok = map(&maps.x, f.x.ptr, f.channels, f.rows, f.x.pitch, TILE, 64, wide) &&
             map(&maps.gate, f.gate.ptr, f.hidden, f.channels, f.gate.pitch, 64, 64, wide) &&

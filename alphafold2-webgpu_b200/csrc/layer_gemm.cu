@@ -1211,14 +1211,14 @@ bool aligned16(const void *ptr, int64_t stride, int element) {
          stride * element < (int64_t(1) << 40);
 }
 
-bool operand_map(CUtensorMap *map, const GemmOperand &o, int64_t outer, int64_t k, bool bf16, int pieces,
+bool operand_map(af2_ctx *ctx, CUtensorMap *map, const GemmOperand &o, int64_t outer, int64_t k, bool bf16, int pieces,
                  int box_outer) {
   const CUtensorMapDataType t = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint64_t row = o.pitch * 2, piece = pieces > 1 ? o.piece_stride * 2 : row;  // (one piece: no step)
   const int step = pieces > 1 ? 32 : BK;
   if (o.mn_major)
-    return encode_map_3d(map, t, o.ptr, outer, k, pieces, row, piece, 64, step, 1, CU_TENSOR_MAP_SWIZZLE_128B);
-  return encode_map_3d(map, t, o.ptr, k, outer, pieces, row, piece, step, box_outer, 1,
+    return layer_map_3d(ctx, map, t, o.ptr, outer, k, pieces, row, piece, 64, step, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+  return layer_map_3d(ctx, map, t, o.ptr, k, outer, pieces, row, piece, step, box_outer, 1,
                        pieces > 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
@@ -1383,6 +1383,7 @@ LayerGemm cut_rows(LayerGemm &g, int64_t row) {
   for (int i = 0; i < g.batch; ++i)
     tail.out[i] = const_cast<uint8_t *>(past(g.out[i], row * g.out_stride, g.out_dtype == AF2_F32 ? 4 : 2));
   tail.m = g.m - row;
+  tail.first_row = row;
   g.m = row;
   return tail;
 }
@@ -1390,13 +1391,11 @@ LayerGemm cut_rows(LayerGemm &g, int64_t row) {
 // Launches this long (SM clocks) are worth the host's search for a cut, some 20 us.
 constexpr double kCutFrom = 200000;
 
-}  // namespace
-
 // Tile width and the parts that each depth is cut into, by the clocks that the launch costs.  Where the
 // tiles of long products leave pairs without work at the end, the last rows of one become a product of its
 // own whose depth is cut: at 8192 x 1024 -> 4096 the gradients' 320 tiles fill 74 pairs 4.3 times, and
 // 24 of them cut in three end all pairs together.
-int layer_gemm_plan(LayerGemm *g, int count) {
+int search_plan(LayerGemm *g, int count) {
   const bool f32 = g[0].pieces > 1;
   TileClass classes[kMaxProducts];
   double best = 0;
@@ -1458,14 +1457,59 @@ int layer_gemm_plan(LayerGemm *g, int count) {
       g[count++].splits = cut_splits;
     }
   }
-  for (int i = 0; i < count; ++i)
-    g[i].scratch_bytes =
-        g[i].splits > 1 ? align_up(4ull * g[i].splits * g[i].batch * g[i].m * align_up(g[i].n, 4), 256) : 0;
   if (count > 1)  // (the waves take the longest tiles first)
     std::stable_sort(g, g + count, [&](const LayerGemm &a, const LayerGemm &b) {
       return tile_class(a, a.tile_n, a.splits).clocks > tile_class(b, b.tile_n, b.splits).clocks;
     });
   return count;
+}
+
+// A plan by the shapes that it was made for: it is asked for twice a call (to size the scratch, and to
+// launch), and costs 2 us to 50.
+struct KeptPlan {
+  static constexpr int kGiven = kMaxProducts - 1, kWords = 1 + 6 * kGiven;
+  int64_t shapes[kWords];
+  int count;
+  struct { int64_t first_row, m; int given, tile_n, splits; } product[kMaxProducts];
+};
+
+}  // namespace
+
+int layer_gemm_plan(LayerGemm *g, int count) {
+  static thread_local KeptPlan plans[64];
+  int64_t shapes[KeptPlan::kWords] = {count};
+  uint64_t hash = count;
+  for (int i = 0; i < count; ++i) {
+    const int64_t words[6] = {g[i].m, g[i].n, g[i].k, g[i].segments, g[i].batch | static_cast<int64_t>(g[i].pieces) << 32,
+                              g[i].epilogue};
+    for (int w = 0; w < 6; ++w) {
+      shapes[1 + 6 * i + w] = words[w];
+      hash = (hash ^ static_cast<uint64_t>(words[w])) * 0x9e3779b97f4a7c15ull;
+    }
+    g[i].given = i;
+    g[i].first_row = 0;
+  }
+  KeptPlan &kept = plans[hash >> 58];
+  if (!std::equal(shapes, shapes + KeptPlan::kWords, kept.shapes)) {
+    LayerGemm made[kMaxProducts];
+    std::copy(g, g + count, made);
+    kept.count = search_plan(made, count);
+    for (int i = 0; i < kept.count; ++i)
+      kept.product[i] = {made[i].first_row, made[i].m, made[i].given, made[i].tile_n, made[i].splits};
+    std::copy(shapes, shapes + KeptPlan::kWords, kept.shapes);
+  }
+  LayerGemm given[KeptPlan::kGiven];
+  std::copy(g, g + count, given);
+  for (int i = 0; i < kept.count; ++i) {
+    const auto &k = kept.product[i];
+    LayerGemm &q = g[i] = given[k.given];
+    if (k.first_row) q = cut_rows(q, k.first_row);
+    q.m = k.m;
+    q.tile_n = k.tile_n;
+    q.splits = k.splits;
+    q.scratch_bytes = q.splits > 1 ? align_up(4ull * q.splits * q.batch * q.m * align_up(q.n, 4), 256) : 0;
+  }
+  return kept.count;
 }
 
 namespace {
@@ -1492,9 +1536,9 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
   const int bsets = gate ? 2 : std::max(g.segments, g.batch);
   bool maps_ok = true;
   for (int i = 0; i < g.segments; ++i)
-    maps_ok &= operand_map(&maps.a[i], g.a[i], g.m, g.k, g.bf16, g.pieces, BM);
+    maps_ok &= operand_map(ctx, &maps.a[i], g.a[i], g.m, g.k, g.bf16, g.pieces, BM);
   for (int i = 0; i < bsets; ++i)
-    maps_ok &= operand_map(&maps.b[i], g.b[i], g.n, g.k, g.bf16, g.pieces, g.tile_n / 2);
+    maps_ok &= operand_map(ctx, &maps.b[i], g.b[i], g.n, g.k, g.bf16, g.pieces, g.tile_n / 2);
 
   const int out_bytes = g.out_dtype == AF2_F32 ? 4 : 2;
   const int64_t pitch = align_up(g.n, 4);
@@ -1502,7 +1546,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
   if (g.splits > 1) {
     p.partial = 1;
     p.tma_out = 1;
-    maps_ok &= encode_map_3d(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.scratch, g.n, g.m, g.splits * g.batch,
+    maps_ok &= layer_map_3d(ctx, &maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.scratch, g.n, g.m, g.splits * g.batch,
                              pitch * 4, g.m * pitch * 4, g.pieces > 1 ? 16 : 32, 32, 1,
                              g.pieces > 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
   } else {
@@ -1512,7 +1556,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
     if (g.residual && aligned16(g.residual, g.residual_stride, out_bytes)) {
       p.tma_residual = 1;
       const int64_t row = g.residual_stride * out_bytes;
-      maps_ok &= encode_map_3d(&maps.residual, map_type(g.out_dtype), g.residual, g.n, g.m, 1, row, row,
+      maps_ok &= layer_map_3d(ctx, &maps.residual, map_type(g.out_dtype), g.residual, g.n, g.m, 1, row, row,
                                out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     }
     p.out_stride = g.out_stride;
@@ -1528,7 +1572,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
     const bool terms = g.epilogue != kEpilogueOut && out_bytes == 4;  // written by the lanes
     if (p.tma_out && !terms)
       for (int i = 0; i < outs; ++i)
-        maps_ok &= encode_map_3d(&maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
+        maps_ok &= layer_map_3d(ctx, &maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
                                  g.out_stride * out_bytes, out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     p.save = g.saved.half || g.saved.f32;
     p.saved_f32 = g.saved.f32;
@@ -1537,11 +1581,11 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
     p.saved_stride = g.saved.stride;
     p.scale_rows = g.saved.scale_rows;
     if (g.saved.half)
-      maps_ok &= encode_map_3d(&maps.half, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.saved.half, g.saved.pitch, g.m,
+      maps_ok &= layer_map_3d(ctx, &maps.half, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.saved.half, g.saved.pitch, g.m,
                                g.epilogue == kEpilogueOut ? 1 : 2, g.saved.pitch * 2, g.saved.stride * 2, 32, 32, 1,
                                CU_TENSOR_MAP_SWIZZLE_64B);
     if (g.epilogue == kEpilogueGateBackward && out_bytes == 4)
-      maps_ok &= encode_map_3d(&maps.half, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.saved.f32, g.n, g.m, 2, g.saved.pitch * 4,
+      maps_ok &= layer_map_3d(ctx, &maps.half, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.saved.f32, g.n, g.m, 2, g.saved.pitch * 4,
                                g.saved.stride * 4, 16, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     p.column_partial = g.column_partial;
   }

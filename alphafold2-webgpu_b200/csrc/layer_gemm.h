@@ -55,6 +55,8 @@ struct LayerGemm {
   float *column_partial = nullptr;           // GateBackward: [ceil(m / 32)][2 * saved.pitch] column sums, or NULL
   // layer_gemm_plan: the tile's width, the parts the depth is cut into and the split sums' bytes
   int tile_n = 0, splits = 0;
+  int given = 0;  // which of the products given this is, or is rows of, from first_row on
+  int64_t first_row = 0;
   uint64_t scratch_bytes = 0;
   uint8_t *scratch = nullptr;
 };
@@ -65,7 +67,7 @@ inline int64_t saved_pitch(int64_t width) { return align_up(width, 32); }
 
 // Up to this many products of one type in a launch (more than one: kEpilogueOut with no bias, activation
 // or residual).
-constexpr int kMaxProducts = 4;
+constexpr int kMaxProducts = 4;  // three, and what is cut from one
 // Fills in the plan, in which a product may have become two, in another order: g has room for
 // kMaxProducts; returns how many there are.  Then each product with scratch_bytes needs scratch.
 int layer_gemm_plan(LayerGemm *g, int count);
