@@ -413,10 +413,14 @@ class Pass {
   void finish_sums(const float *partial, int64_t chunks, int64_t width, void *dst, int set = 0, int sets = 1) {
     if (!dst) return;
     const int64_t pitch = saved_pitch(width);
-    sums_[sum_count_++] = {partial + set * pitch, chunks, sets * pitch, width, dst};
+    sums_[sum_count_++] = {partial + set * pitch, chunks, sets * pitch, width, dst, false};
   }
   void column_sums(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst) {
     if (!dst) return;
+    if (rows <= 1024) {  // four reads one after the other in the last launch are less than a launch more
+      sums_[sum_count_++] = {src, rows, stride, width, dst, true};
+      return;
+    }
     float *partial = sum_room(rows, width, 1);
     rows_kernel(rows, width, [&](dim3 blocks, const RowGrid &grid) {
       cudaError_t e = cudaSuccess;

@@ -1164,20 +1164,20 @@ __device__ __forceinline__ void reduce(const ReduceArgs &p) {
 
 // dst[c] = the sum over the chunks of partial[chunk][c]: eight columns a block, 32 threads a column with
 // eight reads in flight each, joined in a fixed order.
-template <typename OT>
+template <typename OT, typename ST>
 __device__ __forceinline__ void column_sums(const ColumnSums &p) {
   __shared__ float all[8][8];
   const int c = threadIdx.x & 7, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int64_t c0 = static_cast<int64_t>(blockIdx.x) * 8; c0 < p.columns; c0 += static_cast<int64_t>(gridDim.x) * 8) {
     float sum = 0.f;
     if (c0 + c < p.columns) {
-      const float *src = p.partial + c0 + c;
+      const ST *src = static_cast<const ST *>(p.partial) + c0 + c;
       for (int64_t k0 = threadIdx.x >> 3; k0 < p.chunks; k0 += 8 * 32) {
-        float x[8];
+        ST x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = k0 + 32 * i < p.chunks ? src[(k0 + 32 * i) * p.stride] : 0.f;
+        for (int i = 0; i < 8; ++i) x[i] = src[min(k0 + 32 * i, p.chunks - 1) * p.stride];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += x[i];
+        for (int i = 0; i < 8; ++i) sum += k0 + 32 * i < p.chunks ? to_f32<ST>(x[i]) : 0.f;
       }
     }
     sum += __shfl_xor_sync(kFull, sum, 8);
@@ -1200,8 +1200,10 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Fin
   const int y = blockIdx.y;
   if (y < launch.products)
     reduce<OT>(launch.product[y]);
+  else if (launch.sums[y - launch.products].rows)
+    column_sums<OT, OT>(launch.sums[y - launch.products]);
   else
-    column_sums<OT>(launch.sums[y - launch.products]);
+    column_sums<OT, float>(launch.sums[y - launch.products]);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

@@ -73,11 +73,13 @@ constexpr int kMaxProducts = 4;  // three, and what is cut from one
 int layer_gemm_plan(LayerGemm *g, int count);
 af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaStream_t stream);
 
-// out[c] of the call's type = the sum over the chunks of partial[chunk * stride + c].
+// out[c] of the call's type = the sum over the chunks of partial[chunk * stride + c], f32, or with `rows`
+// the rows of a tensor of the call's type.
 struct ColumnSums {
-  const float *partial = nullptr;
+  const void *partial = nullptr;
   int64_t chunks = 0, stride = 0, columns = 0;
   void *out = nullptr;
+  bool rows = false;
 };
 constexpr int kMaxSums = 3;
 // What is left after layer_gemm_launch, in one launch (none where there is nothing): the sums of the
