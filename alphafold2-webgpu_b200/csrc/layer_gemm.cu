@@ -1255,8 +1255,6 @@ af2_status launch_bn(af2_ctx *ctx, int bn, Launch<N> &l, cudaStream_t stream) {
   // f32 tiles are 128 wide: a warp holds the sums of one block of 32 columns
   if constexpr (sizeof(OT) == 4)
     return launch<KIND, OT, 128>(ctx, l, stream);
-  else if constexpr (KIND == kGateBackward)
-    return launch<KIND, OT, 256>(ctx, l, stream);
   else
     return bn == 256 ? launch<KIND, OT, 256>(ctx, l, stream) : launch<KIND, OT, 128>(ctx, l, stream);
 }
@@ -1404,7 +1402,6 @@ int search_plan(LayerGemm *g, int count) {
   int64_t longest = 0;
   for (int i = 0; i < count; ++i) longest = std::max(longest, ceil_div(g[i].k, f32 ? 32 : BK) * g[i].segments);
   for (int bn : {256, 128}) {
-    if (!f32 && g[0].epilogue == kEpilogueGateBackward && bn == 128) continue;
     if (f32 && bn == 256) continue;
     // `most`: K steps that a tile may have before its depth is cut
     for (int64_t most : {int64_t(1) << 40, int64_t(512), int64_t(384), int64_t(256), int64_t(192), int64_t(128),
