@@ -506,7 +506,7 @@ uint64_t gated_saved_bytes(int64_t rows, int64_t hidden, int dtype) {
 
 af2_status dense_forward(af2_ctx *ctx, const DenseForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
   Pass l(ctx, p.dtype, scratch, stream);
-  if (few_rows(p.rows, p.inner, p.columns, p.dtype) && !(p.saved && p.activation != AF2_ACTIVATION_NONE)) {
+  if (few_rows(p.rows, p.inner, p.columns, p.dtype, false) && !(p.saved && p.activation != AF2_ACTIVATION_NONE)) {
     *bytes = 0;
     if (!ctx) return AF2_OK;
     FewRows f;
@@ -576,7 +576,17 @@ af2_status dense_backward(af2_ctx *ctx, const DenseBackward &p, void *scratch, u
 
 af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uint64_t *bytes, cudaStream_t stream) {
   Pass l(ctx, p.dtype, scratch, stream);
-  if (few_rows(p.rows, p.channels, p.hidden, p.dtype) && !p.saved) {
+  GatedFused fused;
+  fused.rows = p.rows, fused.channels = p.channels, fused.hidden = p.hidden;
+  fused.dtype = p.dtype, fused.activation = p.activation;
+  fused.residual = p.residual, fused.residual_stride = p.residual_stride;
+  fused.out = p.out, fused.out_stride = p.out_stride;
+  const bool one_kernel = !p.saved && gated_fused_covers(fused);
+  const bool few = !p.saved && few_rows(p.rows, p.channels, p.hidden, p.dtype, true);
+  // One kernel for both products takes 8.1 us at 128 -> 512 up to 256 rows, few rows 8.0 at 4 and 19 at 256.
+  // Which of them runs depends on addresses too, so the scratch is counted for both.
+  const bool fits = p.rows > 4 && gated_fused_fits(fused);
+  if (few && (!fits || (ctx && !one_kernel))) {
     void *h = l.take(element_size(p.dtype) * p.rows * p.hidden);
     *bytes = l.total();
     if (!ctx) return AF2_OK;
@@ -598,20 +608,16 @@ af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uin
     y.follows = true;
     return few_rows_launch(ctx, y, stream);
   }
+  const uint64_t few_bytes = few ? part(element_size(p.dtype) * p.rows * p.hidden) : 0;
   const GemmOperand x = l.operand(p.x, p.x_stride, p.rows, p.channels);
   const GemmOperand wg = l.operand(p.w.gate_weight, p.hidden, p.channels, p.hidden);
   const GemmOperand wv = l.operand(p.w.value_weight, p.hidden, p.channels, p.hidden);
   const GemmOperand wo = l.operand(p.w.output_weight, p.channels, p.hidden, p.channels);
   l.pack();
-  GatedFused fused;
-  fused.rows = p.rows, fused.channels = p.channels, fused.hidden = p.hidden;
-  fused.dtype = p.dtype, fused.activation = p.activation;
   fused.x = x, fused.gate = wg, fused.value = wv, fused.output = wo;
   fused.gate_bias = p.w.gate_bias, fused.value_bias = p.w.value_bias, fused.output_bias = p.w.output_bias;
-  fused.residual = p.residual, fused.residual_stride = p.residual_stride;
-  fused.out = p.out, fused.out_stride = p.out_stride;
-  if (!p.saved && gated_fused_covers(fused)) {
-    *bytes = l.total();
+  if (one_kernel) {
+    *bytes = std::max(l.total(), few_bytes);
     return l.live() ? gated_fused_launch(ctx, fused, stream) : l.status;
   }
   GemmOperand h;
@@ -645,7 +651,7 @@ af2_status gated_forward(af2_ctx *ctx, const GatedForward &p, void *scratch, uin
   y.out[0] = p.out;
   y.out_stride = p.out_stride;
   l.run(y);
-  *bytes = l.total();
+  *bytes = std::max(l.total(), few_bytes);
   return l.status;
 }
 

@@ -5,13 +5,21 @@
 
 namespace af2 {
 
-// Whether a product is small enough for the CUDA-core kernel, which starts and ends sooner than the
-// tensor-core one and reads f32 as it is.  Measured on whole transitions, us (few rows | tensor cores):
-// bf16, 512 -> 2048: 8 rows 9.8 | 15, 16 rows 15.0 | 15.1; 1024 -> 4096: 4 rows 13 | 20, 8 rows 25 | 20;
-// f32, 512 -> 2048: 48 rows 39.1 | 39.0; 1024 -> 4096: 16 rows 46 | 80, 24 rows 70 | 72.
-inline bool few_rows(int64_t rows, int64_t inner, int64_t columns, int dtype) {
-  const int64_t most = dtype == AF2_F32 ? 3 << 24 : 1 << 24;  // products of two elements
-  return rows <= 256 && rows * inner * columns <= most;
+// Whether a product (`gated`: the transition's first, of two weights) is small enough for the CUDA-core
+// kernel, which starts and ends sooner than the tensor-core ones and reads f32 as it is.  Its time grows
+// with rows x weight, theirs hardly with the rows: they meet at some rows for any weight and more for
+// small ones.  Measured, us (few rows | tensor cores), whole transitions or one dense layer:
+//   bf16 gated  256 -> 1024: 32 rows 10.4 | 12.9, 48 rows 15.6 | 13.2;  512 -> 2048: 8 rows 11.3 | 14.4,
+//               16 rows 15.2 | 14.6;  1024 -> 4096: 4 rows 12.8 | 19.1, 8 rows 22.3 | 19.1
+//   bf16 dense  512 -> 512: 64 rows 5.1 | 6.2, 96 rows 8.0 | 6.2;  1024 -> 4096: 4 rows 5.0 | 8.7, 8 rows 9.3 | 8.6
+//   f32 gated   256 -> 1024: 96 rows 19.9 | 21.2, 128 rows 23.6 | 22.3;  1024 -> 4096: 16 rows 45 | 64, 24 rows 69 | 55
+//   f32 dense   512 -> 512: 128 rows 9.3 | 11.3, 192 rows 13.0 | 11.7;  1024 -> 4096: 16 rows 17 | 26, 24 rows 24 | 21
+// Weight rows that are not 16-byte pieces are read one element at a time (293 -> 893, gated: bf16 24 rows
+// 13.7 | 15.5, 32 rows 17.5 | 15.7; f32 48 rows 21.3 | 21.7, 96 rows 27.6 | 22.7).
+inline bool few_rows(int64_t rows, int64_t inner, int64_t columns, int dtype, bool gated) {
+  const bool f32 = dtype == AF2_F32, pieces = columns % (f32 ? 4 : 8) == 0;
+  const int64_t always = f32 ? 16 : 4, most = (f32 ? 24 << 20 : gated ? 8 << 20 : 12 << 20) / (pieces ? 3 : 4) * 3;
+  return rows <= 256 && (rows - always) * inner * columns <= most;
 }
 
 struct FewRows {

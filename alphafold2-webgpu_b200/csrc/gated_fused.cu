@@ -479,9 +479,9 @@ af2_status launch(af2_ctx *ctx, const Maps &maps, const Args &p, cudaStream_t st
 
 }  // namespace
 
+bool gated_fused_fits(const GatedFused &f) { return f.dtype != AF2_F32 && f.channels <= 128 && f.hidden <= MOST_HIDDEN; }
 bool gated_fused_covers(const GatedFused &f) {
-  if (f.dtype == AF2_F32 || f.channels > 128 || f.hidden > MOST_HIDDEN) return false;
-  return addressable(f.out, f.out_stride) && (!f.residual || addressable(f.residual, f.residual_stride));
+  return gated_fused_fits(f) && addressable(f.out, f.out_stride) && (!f.residual || addressable(f.residual, f.residual_stride));
 }
 
 af2_status gated_fused_launch(af2_ctx *ctx, const GatedFused &f, cudaStream_t stream) {

@@ -15,7 +15,8 @@ struct GatedFused {
   void *out = nullptr;
 };
 // Whether the kernel covers the call, and is the faster one for it.
-bool gated_fused_covers(const GatedFused &f);
+bool gated_fused_fits(const GatedFused &f);    // its sizes and type
+bool gated_fused_covers(const GatedFused &f);  // and its output and residual
 af2_status gated_fused_launch(af2_ctx *ctx, const GatedFused &f, cudaStream_t stream);
 
 }  // namespace af2
