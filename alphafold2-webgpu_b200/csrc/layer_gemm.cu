@@ -15,6 +15,12 @@
 // saved factors) comes by TMA into the same block of shared memory that its
 // result leaves from.
 //
+// Measured: 16384 x 1024 -> 4096 in bf16 96 us, 1.43 PFLOP/s, bound by the tensor
+// core (with gelu 108, its slopes kept 119); the gate with factors of 32768 x 256
+// -> 1024 55 us for 226 MB, its backward product 61 us for 293 MB: epilogues whose
+// phases overlap in part; the gradients' products of 8192 x 1024 -> 4096 258 us,
+// 0.80 of cuBLAS's rate.  Small products take some 7 us whatever their size.
+//
 // f32 tensors are multiplied as three bf16 terms each, x = x0 + x1 + x2, and
 // the six products whose weight is at least 2^-16 of the largest are summed:
 // what is left out is below 2^-24 of |x||y|, f32's own rounding.  A K step's
@@ -26,7 +32,8 @@
 // at each step of 16: sums of one sign over a depth of 4096 came out 2e-6 low),
 // so the five small products have an accumulator of their own, and a tile is
 // summed over 256 of the depth at a time and these sums are added in registers.
-// (An infinite f32 element makes its sums NaN or infinite.)
+// (An infinite f32 element makes its sums NaN or infinite.)  18944 x 1024 -> 768:
+// 121 us, the depth at 1.69 PFLOP/s of its six products.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -1092,14 +1099,16 @@ struct ReduceArgs {
   int64_t saved_pitch;
 };
 
-// The split products' sums (blockIdx.y below `products`), then the column sums: one launch for both.
+// The column sums (blockIdx.y below `sum_count`), whose few blocks run longest, then the split products'
+// sums: one launch for both.
 struct FinishLaunch {
   ReduceArgs product[kMaxProducts];
   ColumnSums sums[kMaxSums];
-  int products;
+  int products, sum_count;
 };
 
-// A thread has four columns of a row; latency bounds it, so all that it reads is asked for at once.
+// A thread has four columns of a row; latency bounds it, so all that it reads is asked for at once (some
+// 3 us for a small layer's sums).
 template <typename OT>
 __device__ __forceinline__ void reduce(const ReduceArgs &p) {
   // (a product is only split while it has few tiles: its elements count in 32 bits)
@@ -1163,7 +1172,7 @@ __device__ __forceinline__ void reduce(const ReduceArgs &p) {
 }
 
 // dst[c] = the sum over the chunks of partial[chunk][c]: eight columns a block, 32 threads a column with
-// eight reads in flight each, joined in a fixed order.
+// sixteen reads in flight each, joined in a fixed order.
 template <typename OT, typename ST>
 __device__ __forceinline__ void column_sums(const ColumnSums &p) {
   __shared__ float all[8][8];
@@ -1172,12 +1181,12 @@ __device__ __forceinline__ void column_sums(const ColumnSums &p) {
     float sum = 0.f;
     if (c0 + c < p.columns) {
       const ST *src = static_cast<const ST *>(p.partial) + c0 + c;
-      for (int64_t k0 = threadIdx.x >> 3; k0 < p.chunks; k0 += 8 * 32) {
-        ST x[8];
+      for (int64_t k0 = threadIdx.x >> 3; k0 < p.chunks; k0 += 16 * 32) {
+        ST x[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = src[min(k0 + 32 * i, p.chunks - 1) * p.stride];
+        for (int i = 0; i < 16; ++i) x[i] = src[min(k0 + 32 * i, p.chunks - 1) * p.stride];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += k0 + 32 * i < p.chunks ? to_f32<ST>(x[i]) : 0.f;
+        for (int i = 0; i < 16; ++i) sum += k0 + 32 * i < p.chunks ? to_f32<ST>(x[i]) : 0.f;
       }
     }
     sum += __shfl_xor_sync(kFull, sum, 8);
@@ -1198,12 +1207,12 @@ template <typename OT>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ FinishLaunch launch) {
   dependency_wait();
   const int y = blockIdx.y;
-  if (y < launch.products)
-    reduce<OT>(launch.product[y]);
-  else if (launch.sums[y - launch.products].rows)
-    column_sums<OT, OT>(launch.sums[y - launch.products]);
+  if (y >= launch.sum_count)
+    reduce<OT>(launch.product[y - launch.sum_count]);
+  else if (launch.sums[y].rows)
+    column_sums<OT, OT>(launch.sums[y]);
   else
-    column_sums<OT, float>(launch.sums[y - launch.products]);
+    column_sums<OT, float>(launch.sums[y]);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1675,6 +1684,7 @@ af2_status layer_finish_launch(af2_ctx *ctx, int dtype, const LayerGemm *g, int 
     r.saved_pitch = q.saved.pitch;
     blocks = std::max(blocks, ceil_div(q.batch * q.m * r.pitch / 4, 256));
   }
+  l.sum_count = sum_count;
   for (int j = 0; j < sum_count; ++j) {
     l.sums[j] = sums[j];
     blocks = std::max(blocks, ceil_div(sums[j].columns, 8));
