@@ -16,10 +16,17 @@ namespace af2 {
 //   f32 dense   512 -> 512: 128 rows 9.3 | 11.3, 192 rows 13.0 | 11.7;  1024 -> 4096: 16 rows 17 | 26, 24 rows 24 | 21
 // Weight rows that are not 16-byte pieces are read one element at a time (293 -> 893, gated: bf16 24 rows
 // 13.7 | 15.5, 32 rows 17.5 | 15.7; f32 48 rows 21.3 | 21.7, 96 rows 27.6 | 22.7).
+// A dense layer's times part where the kernel's blocks (four rows by 32 columns) are more than the SMs hold
+// at a time, two each, or one where the weight is large; the f32 products take twice and four times that.
 inline bool few_rows(int64_t rows, int64_t inner, int64_t columns, int dtype, bool gated) {
   const bool f32 = dtype == AF2_F32, pieces = columns % (f32 ? 4 : 8) == 0;
-  const int64_t always = f32 ? 16 : 4, most = (f32 ? 24 << 20 : gated ? 8 << 20 : 12 << 20) / (pieces ? 3 : 4) * 3;
-  return rows <= 256 && (rows - always) * inner * columns <= most;
+  if (rows > 256) return false;
+  if (gated) {
+    const int64_t always = f32 ? 16 : 4, most = f32 ? 24 << 20 : 8 << 20;
+    return (rows - always) * inner * columns <= (pieces ? most : most / 4 * 3);
+  }
+  const int64_t held = f32 ? 592 : inner * columns >= 1 << 21 ? 148 : 296;
+  return rows <= 4 || (rows + 3) / 4 * ((columns + 31) / 32) <= (pieces ? held : held / 4 * 3);
 }
 
 struct FewRows {
