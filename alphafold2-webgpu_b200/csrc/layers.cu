@@ -6,6 +6,7 @@
 // No counterpart in the reference, which runs fixed weights forward only; the
 // checks follow its conventions (positive safe integers, a RangeError-class
 // status with the reason in the message).
+#include <algorithm>
 #include <cmath>
 #include <new>
 #include <string>
@@ -176,6 +177,34 @@ af2_status run_pass(af2_ctx *ctx, void *workspace, cudaStream_t stream, const P 
 // Stands for a tensor at an unknown address when scratch is sized: one that TMA cannot read in place.
 void *const kAnywhere = reinterpret_cast<void *>(uintptr_t(4));
 
+// The scratch of a backward pass whichever gradients are wanted.  Fewer products are planned otherwise
+// than all of them -- alone, one has its depth cut further, and more split sums -- so each set of
+// products is counted (everything else only grows with what is wanted): count(set, bytes) for the sets
+// below `sets`.  Kept by shape, since that is up to twelve plans and a call with a caller's workspace asks.
+template <typename F>
+af2_status largest_set(const int64_t (&shape)[6], int sets, uint64_t *bytes, F &&count) {
+  struct Kept {
+    int64_t shape[6];  // [0] is not 0
+    uint64_t bytes;
+  };
+  static thread_local Kept table[64];
+  uint64_t hash = 0;
+  for (int64_t v : shape) hash = (hash ^ static_cast<uint64_t>(v)) * 0x9e3779b97f4a7c15ull;
+  Kept &kept = table[hash >> 58];
+  if (!std::equal(shape, shape + 6, kept.shape)) {
+    uint64_t most = 0;
+    for (int set = 0; set < sets; ++set) {
+      uint64_t n = 0;
+      if (af2_status st = count(set, &n); st != AF2_OK) return st;
+      most = std::max(most, n);
+    }
+    std::copy(shape, shape + 6, kept.shape);
+    kept.bytes = most;
+  }
+  *bytes = kept.bytes;
+  return AF2_OK;
+}
+
 cudaStream_t stream_of(af2_ctx *ctx, void *stream) {
   return stream ? static_cast<cudaStream_t>(stream) : ctx->stream;
 }
@@ -226,8 +255,11 @@ af2_status af2_dense_workspace_bytes(const af2_linear_shape *shape, int dtype, i
     void *const any = kAnywhere;
     const int64_t rows = shape->rows, in = shape->inner, cols = shape->columns;
     if (backward)
-      return dense_backward(nullptr, {rows, in, cols, dtype, activation, any, any, any, any, cols, in, in, any, any, any},
-                            nullptr, bytes, nullptr);
+      return largest_set({1, rows, in, cols, dtype, activation}, 4, bytes, [&](int set, uint64_t *n) {
+        return dense_backward(nullptr, {rows, in, cols, dtype, activation, any, any, any, any, cols, in, in,
+                                        set & 1 ? any : nullptr, set & 2 ? any : nullptr, any},
+                              nullptr, n, nullptr);
+      });
     return dense_forward(nullptr, {rows, in, cols, dtype, activation, any, any, any, any, in, cols, cols, any, any},
                          nullptr, bytes, nullptr);
   });
@@ -313,8 +345,13 @@ af2_status af2_gated_transition_workspace_bytes(const af2_transition_shape *shap
     const int64_t rows = shape->rows, c = shape->channels, h = shape->hidden_channels;
     const af2_gated_weights w{any, any, any, any, any, any};
     if (backward)
-      return gated_backward(nullptr, {rows, c, h, dtype, 0, any, any, any, w, {any, any, any, any, any, any, any}, c, c, c},
-                            nullptr, bytes, nullptr);
+      return largest_set({2, rows, c, h, dtype, 0}, 12, bytes, [&](int set, uint64_t *n) {
+        // x, the output's weight, and none, one or both of the gate's and the value's
+        return gated_backward(nullptr, {rows, c, h, dtype, 0, any, any, any, w,
+                                        {set & 1 ? any : nullptr, set >= 4 ? any : nullptr, any,
+                                         set >= 8 ? any : nullptr, any, set & 2 ? any : nullptr, any}, c, c, c},
+                              nullptr, n, nullptr);
+      });
     uint64_t saving = 0;  // the forward pass that saves nothing needs the most
     if (af2_status st = gated_forward(nullptr, {rows, c, h, dtype, 0, any, any, w, c, c, c, any, any}, nullptr, &saving,
                                       nullptr);

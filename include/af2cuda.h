@@ -664,7 +664,7 @@ typedef struct af2_layer_options {
 /* Bytes of `saved`: what the forward pass leaves for the backward pass (0 for
  * AF2_ACTIVATION_NONE).  Its layout is the library's. */
 AF2_API af2_status af2_dense_saved_bytes(const af2_linear_shape *shape, int dtype, int activation, uint64_t *bytes);
-/* Scratch bytes of the forward (backward = 0) or the backward pass. */
+/* Scratch bytes of the forward (backward = 0) or the backward pass, whichever gradients that one is asked for. */
 AF2_API af2_status af2_dense_workspace_bytes(const af2_linear_shape *shape, int dtype, int activation, int backward,
                                              uint64_t *bytes);
 
