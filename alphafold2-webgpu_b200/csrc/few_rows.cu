@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) few_rows_kernel(const A
   const bool in = col < p.columns;  // V > 1: the columns are a multiple of V
   const T *weight = static_cast<const T *>(set ? p.weight[1] : p.weight[0]) + col;
   const int first = k0 + w * DEPTH + lane / LANES;
+  if (p.splits > 1) cluster_started();
   constexpr int STEP = SET_WARPS * DEPTH;  // from one read of a lane to its next
 
   typename P::Word buf[FLIGHT];
@@ -142,6 +143,8 @@ __global__ void __launch_bounds__(THREADS, DEEP ? 1 : 2) few_rows_kernel(const A
 #pragma unroll
   for (int r = 0; r < R; ++r) part[(warp * R + r) * COLS + mine] = acc[r][0];
   __syncthreads();
+  // blocks of a cluster are scheduled together, but one may be here before rank 0 has begun
+  if (p.splits > 1) cluster_wait_started();
   for (int i = threadIdx.x; i < SETS * R * COLS; i += THREADS) {
     const int s = i / (R * COLS), at = i - s * (R * COLS);
     float sum = 0.f;

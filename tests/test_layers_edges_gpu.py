@@ -54,3 +54,18 @@ def test_gated_backward_in_the_callers_scratch(device, rows, channels, hidden, d
         for k in got:
             close(k, got[k], want[k], dtype)
         assert intact(), need
+
+
+# ---- blocks that add up through one another's shared memory ------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("inner,columns", [(256, 32), (512, 64), (1024, 200), (4096, 96), (4096, 1000)])
+def test_few_rows_whose_depth_is_shared(device, inner, columns, dtype):
+    """Clusters of two to eight blocks, launch upon launch: the same bits each time."""
+    s = dense_case(3, inner, columns, dtype, seed=1020)
+    want = ref.dense(s["x"], s["weight"], s["bias"], s["residual"], "silu")["y"]
+    outs = [af2cuda.encode_dense_tensors(device, s["x"], s["weight"], bias=s["bias"], residual=s["residual"],
+                                         activation="silu") for _ in range(100)]
+    close("y", outs[0], want, dtype)
+    assert all(torch.equal(y, outs[0]) for y in outs)
