@@ -7,6 +7,7 @@
 // The module links nothing of the library: bind() takes the entry points'
 // addresses, so that one loaded libaf2cuda.so serves all of the package.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -123,6 +124,26 @@ struct Call {
     cudaStream_t s = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(ordinal)).stream();
     return s ? static_cast<void *>(s) : reinterpret_cast<void *>(uintptr_t(1));
   }
+  // Scratch: the caller's; else none (the context's is used), but while the stream is being captured a block
+  // from torch's allocator, which keeps it for the graph as it keeps the outputs.  query(bytes) asks for the
+  // size.
+  at::Tensor own_scratch;
+  template <typename F>
+  void *scratch(const at::Tensor *given, void *stream, F &&query) {
+    if (!given && !capturing(stream)) return nullptr;
+    uint64_t need = 0;
+    done(query(&need));
+    if (given) return block(given, need, "workspace", "hold what the call needs");
+    own_scratch = bytes(need);
+    return need ? own_scratch.data_ptr() : nullptr;
+  }
+  static bool capturing(void *stream) {
+    // (no capture takes in the context's own stream or the legacy default one)
+    if (!stream || stream == reinterpret_cast<void *>(uintptr_t(1))) return false;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    C10_CUDA_CHECK(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &status));
+    return status != cudaStreamCaptureStatusNone;
+  }
   void done(af2_status status) const {
     if (status == AF2_OK) return;
     PyObject *r = PyObject_CallFunction(check_status, "iK", static_cast<int>(status),
@@ -184,14 +205,11 @@ PyObject *dense(PyObject *const *a) {
     c.done(entry.dense_saved_bytes(&shape, c.code, act, &bytes));
     saved = c.bytes(bytes);
   }
-  void *ws = nullptr;
-  if (workspace) {
-    uint64_t need = 0;
-    c.done(entry.dense_workspace_bytes(&shape, c.code, act, 0, &need));
-    ws = c.block(workspace, need, "workspace", "hold what the call needs");
-  }
+  void *const stream = c.stream(integer(a[9]));
+  void *const ws = c.scratch(
+      workspace, stream, [&](uint64_t *need) { return entry.dense_workspace_bytes(&shape, c.code, act, 0, need); });
   c.done(entry.dense(c.ctx, &shape, c.code, x.data_ptr(), wp, bp, ptr(residual), &o, y.data_ptr(),
-                     bytes ? saved.data_ptr() : nullptr, ws, c.stream(integer(a[9]))));
+                     bytes ? saved.data_ptr() : nullptr, ws, stream));
   return with_saved(y, saved, save);
 }
 
@@ -208,24 +226,22 @@ PyObject *dense_backward(PyObject *const *a) {
   const int64_t rows = x.size(0);
   const af2_linear_shape shape{rows, inner, columns};
   o.out_stride = c.rows("d_out", dy, rows, columns);
-  void *wp = c.whole("weight", w, {inner, columns}), *kept = nullptr, *ws = nullptr;
+  void *wp = c.whole("weight", w, {inner, columns}), *kept = nullptr;
   if (act != AF2_ACTIVATION_NONE) {
     uint64_t bytes = 0;
     c.done(entry.dense_saved_bytes(&shape, c.code, act, &bytes));
     kept = c.block(saved, bytes, "saved", "be what the forward pass returned");
   }
-  if (workspace) {
-    uint64_t need = 0;
-    c.done(entry.dense_workspace_bytes(&shape, c.code, act, 1, &need));
-    ws = c.block(workspace, need, "workspace", "hold what the call needs");
-  }
+  void *const stream = c.stream(integer(a[10]));
+  void *const ws = c.scratch(
+      workspace, stream, [&](uint64_t *need) { return entry.dense_workspace_bytes(&shape, c.code, act, 1, need); });
   at::Tensor dx, dw, db;
   if (PyObject_IsTrue(a[8])) dx = c.make({rows, inner});
   if (PyObject_IsTrue(a[9])) dw = c.make({inner, columns});
   if (PyObject_IsTrue(a[6])) db = c.make({columns});
   auto at_of = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
   c.done(entry.dense_backward(c.ctx, &shape, c.code, dy.data_ptr(), x.data_ptr(), wp, kept, &o, at_of(dx), at_of(dw),
-                              at_of(db), ws, c.stream(integer(a[10]))));
+                              at_of(db), ws, stream));
   PyObject *d = PyDict_New();
   if (dx.defined()) put(d, "x", dx);
   if (dw.defined()) put(d, "weight", dw);
@@ -292,14 +308,11 @@ PyObject *gated(PyObject *const *a) {
     c.done(entry.gated_saved_bytes(&shape, c.code, &bytes));
     saved = c.bytes(bytes);
   }
-  void *ws = nullptr;
-  if (workspace) {
-    uint64_t need = 0;
-    c.done(entry.gated_workspace_bytes(&shape, c.code, 0, &need));
-    ws = c.block(workspace, need, "workspace", "hold what the call needs");
-  }
+  void *const stream = c.stream(integer(a[8]));
+  void *const ws = c.scratch(
+      workspace, stream, [&](uint64_t *need) { return entry.gated_workspace_bytes(&shape, c.code, 0, need); });
   c.done(entry.gated(c.ctx, &shape, c.code, x.data_ptr(), &w, ptr(residual), &o, y.data_ptr(),
-                     bytes ? saved.data_ptr() : nullptr, ws, c.stream(integer(a[8]))));
+                     bytes ? saved.data_ptr() : nullptr, ws, stream));
   return with_saved(y, saved, save);
 }
 
@@ -318,12 +331,10 @@ PyObject *gated_backward(PyObject *const *a) {
   o.out_stride = c.rows("d_out", dy, rows, g.channels);
   uint64_t bytes = 0;
   c.done(entry.gated_saved_bytes(&shape, c.code, &bytes));
-  void *kept = c.block(saved, bytes, "saved", "be what the forward pass returned"), *ws = nullptr;
-  if (workspace) {
-    uint64_t need = 0;
-    c.done(entry.gated_workspace_bytes(&shape, c.code, 1, &need));
-    ws = c.block(workspace, need, "workspace", "hold what the call needs");
-  }
+  void *kept = c.block(saved, bytes, "saved", "be what the forward pass returned");
+  void *const stream = c.stream(integer(a[8]));
+  void *const ws = c.scratch(
+      workspace, stream, [&](uint64_t *need) { return entry.gated_workspace_bytes(&shape, c.code, 1, need); });
   auto needed = [&](const char *name) {
     if (a[7] == Py_None) return true;
     PyObject *key = PyUnicode_FromString(name);
@@ -345,8 +356,7 @@ PyObject *gated_backward(PyObject *const *a) {
       d[i] = c.make(g.shape(i));
       *slots[i] = d[i].data_ptr();
     }
-  c.done(entry.gated_backward(c.ctx, &shape, c.code, dy.data_ptr(), x.data_ptr(), &w, kept, &o, &out, ws,
-                              c.stream(integer(a[8]))));
+  c.done(entry.gated_backward(c.ctx, &shape, c.code, dy.data_ptr(), x.data_ptr(), &w, kept, &o, &out, ws, stream));
   PyObject *r = PyDict_New();
   if (dx.defined()) put(r, "x", dx);
   for (int i = 0; i < 6; ++i)
@@ -382,14 +392,9 @@ PyObject *gradients(PyObject *const *a) {
       refuse("out has " + std::to_string(out.size()) + " tensors; expected " + std::to_string(in.size()));
   }
   const at::Tensor *workspace = optional_tensor(a[6], "workspace");
-  void *ws = nullptr;
-  if (workspace) {
-    uint64_t need = 0;
-    c.done(entry.norm_workspace_bytes(n, &need));
-    ws = c.block(workspace, need, "workspace", "hold what the call needs");
-  }
+  void *const stream = c.stream(integer(a[5]));
+  void *const ws = c.scratch(workspace, stream, [&](uint64_t *need) { return entry.norm_workspace_bytes(n, need); });
   const at::Tensor norm = c.make({});
-  void *stream = c.stream(integer(a[5]));
   float *np = static_cast<float *>(norm.data_ptr());
   if (a[4] == Py_None) {
     c.done(entry.gradient_norm(c.ctx, in.data(), n, np, ws, stream));

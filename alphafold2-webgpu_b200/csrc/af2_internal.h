@@ -467,7 +467,7 @@ class LayerScratch {
   af2_ctx *ctx_;
   cudaStream_t stream_;
   uint8_t *base_ = nullptr;
-  bool owned_ = false, capturing_ = false;
+  bool owned_ = false;
 };
 
 struct DenseForward {

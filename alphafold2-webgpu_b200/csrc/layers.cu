@@ -33,19 +33,19 @@ af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
       return cuda_fail(ctx_, e, "create the layer scratch's event");
     }
   }
-  // inside a stream capture the order between streams is the graph's, not this context's
+  // A graph would keep the buffer's address, which the next call that needs more frees, and nothing would
+  // order its replays with other calls.
   if (!lasting(stream_)) {
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     if (cudaError_t e = cudaStreamIsCapturing(stream_, &capture); e != cudaSuccess)
       return cuda_fail(ctx_, e, "query the stream's capture");
-    capturing_ = capture != cudaStreamCaptureStatusNone;
+    if (capture != cudaStreamCaptureStatusNone)
+      return fail(ctx_, AF2_ERR_UNSUPPORTED, "a call inside a stream capture cannot use the context's scratch; pass a "
+                                             "workspace that the graph's owner keeps");
   }
   const bool grow = ctx_->layer_scratch.bytes < bytes;
-  if (grow && capturing_)
-    return fail(ctx_, AF2_ERR_UNSUPPORTED, "the context's scratch cannot grow inside a stream capture; pass a "
-                                           "workspace, or make the same call once before the capture");
   const cudaStream_t last = ctx_->layer_stream;
-  if (!capturing_ && last && (grow || last != stream_)) {
+  if (last && (grow || last != stream_)) {
     if (lasting(last))
       if (cudaError_t e = cudaEventRecord(ctx_->layer_done, last); e != cudaSuccess)
         return cuda_fail(ctx_, e, "record the layer scratch's use");
@@ -63,7 +63,7 @@ af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
 }
 
 af2_status LayerScratch::release() {
-  if (!owned_ || capturing_) return AF2_OK;
+  if (!owned_) return AF2_OK;
   ctx_->layer_stream = stream_;
   if (lasting(stream_)) return AF2_OK;
   if (cudaError_t e = cudaEventRecord(ctx_->layer_done, stream_); e != cudaSuccess)

@@ -674,7 +674,9 @@ AF2_API af2_status af2_dense_workspace_bytes(const af2_linear_shape *shape, int 
  * NULL, or af2_dense_saved_bytes() bytes, 256-byte aligned, for the backward
  * pass.  options NULL: contiguous rows, no activation.  workspace NULL =
  * context-owned (calls on different streams are then ordered among
- * themselves), else af2_dense_workspace_bytes() bytes, 256-byte aligned.
+ * themselves; inside a stream capture a call that needs scratch is refused
+ * with AF2_ERR_UNSUPPORTED), else af2_dense_workspace_bytes() bytes, 256-byte
+ * aligned.
  */
 AF2_API af2_status af2_dense(af2_ctx *ctx, const af2_linear_shape *shape, int dtype, const void *x,
                              const void *weight, const void *bias, const void *residual,

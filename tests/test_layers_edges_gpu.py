@@ -1,9 +1,12 @@
 """The learned layers at their edges: the caller's scratch, streams and captures, values far from one.
 Tolerances as in test_layers_gpu.py, but where a test states its own."""
+import ctypes
+
 import pytest
 import torch
 
 import af2cuda
+from af2cuda import _lib
 import layer_reference as ref
 from test_layers_gpu import BF16, DTYPES, F16, F32, close, dense_case, gated_case
 
@@ -69,3 +72,63 @@ def test_few_rows_whose_depth_is_shared(device, inner, columns, dtype):
                                          activation="silu") for _ in range(100)]
     close("y", outs[0], want, dtype)
     assert all(torch.equal(y, outs[0]) for y in outs)
+
+
+# ---- streams and captures ---------------------------------------------------------------------------
+
+
+def test_captured_without_a_workspace(device):
+    """What a graph holds stays its own: neither a larger call, which replaces the context's scratch, nor
+    calls on another stream between the replays touch it."""
+    s = gated_case(700, 130, 390, F32, seed=1100)
+    want = ref.gated(s["x"], s["weights"], None, "gelu", s["d_out"])
+
+    def step():
+        y, saved = af2cuda.encode_gated_transition_tensors(device, s["x"], s["weights"], activation="gelu", save=True)
+        grads = af2cuda.encode_gated_transition_backward_tensors(device, s["d_out"], s["x"], s["weights"], saved=saved,
+                                                                 activation="gelu")
+        norm = af2cuda.encode_gradient_norm_tensors(device, list(grads.values()))
+        return {"y": y, **grads}, norm
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, norm = step()
+    large = gated_case(9000, 264, 1032, F32, seed=1110)
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        for t in (*got.values(), norm):
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            y = af2cuda.encode_gated_transition_tensors(device, large["x"], large["weights"])
+        torch.cuda.synchronize()
+        for k in got:
+            close(k, got[k], want[k], F32)
+        exact = sum(got[k].double().square().sum().item() for k in got if k != "y") ** 0.5
+        assert abs(norm.item() - exact) <= 2.0**-23 * exact
+    close("y", y, ref.gated(large["x"], large["weights"], None, "silu")["y"], F32)
+
+
+def test_the_contexts_scratch_is_refused_in_a_capture(device):
+    s = dense_case(700, 130, 390, F32, seed=1120)
+    out = torch.empty_like(s["residual"])
+    shape = _lib.LinearShape(700, 130, 390)
+
+    def call(stream):
+        return _lib.lib().af2_dense(device.handle, ctypes.byref(shape), _lib.AF2_F32, s["x"].data_ptr(),
+                                    s["weight"].data_ptr(), None, None, None, out.data_ptr(), None, None, stream)
+
+    assert call(1) == _lib.AF2_OK
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        status = call(torch.cuda.current_stream().cuda_stream)
+        out.add_(1)
+    assert status == _lib.AF2_ERR_UNSUPPORTED
+    assert "workspace" in _lib.lib().af2_last_error(device.handle).decode()
+    graph.replay()
+    torch.cuda.synchronize()
+    close("y", out, ref.dense(s["x"], s["weight"], None, None, "none")["y"] + 1, F32)
