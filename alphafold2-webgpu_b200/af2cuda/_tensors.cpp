@@ -8,9 +8,11 @@
 // addresses, so that one loaded libaf2cuda.so serves all of the package.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -74,6 +76,11 @@ struct Call {
   int code = 0;
   at::ScalarType type = at::kFloat;
 
+  explicit Call(PyObject *const *args)
+      : ctx(reinterpret_cast<af2_ctx *>(PyLong_AsUnsignedLongLong(args[0]))),
+        ordinal(static_cast<int>(PyLong_AsLong(args[1]))) {
+    if (PyErr_Occurred()) throw Failed();
+  }
   void set_type(const at::Tensor &t) {
     code = dtype_code(t);
     type = t.scalar_type();
@@ -118,11 +125,20 @@ struct Call {
     return t->data_ptr();
   }
   // -1: torch's current stream (its default stream by cudaStreamLegacy's handle: the null one means
-  // the context's own stream to the library); else a handle.
-  void *stream(long long handle) const {
-    if (handle != -1) return reinterpret_cast<void *>(handle);
-    cudaStream_t s = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(ordinal)).stream();
-    return s ? static_cast<void *>(s) : reinterpret_cast<void *>(uintptr_t(1));
+  // the context's own stream to the library); else a handle.  Comes before the call's allocations: a block
+  // that torch hands out on its current stream may still be read there by what was queued before, and no
+  // other stream waits for that.  A named stream's tensors are allocated on it; for the context's own (0),
+  // which torch's allocator does not know, the host waits.
+  std::optional<c10::cuda::CUDAStreamGuard> named;
+  void *use_stream(long long handle) {
+    const auto device = static_cast<c10::DeviceIndex>(ordinal);
+    const cudaStream_t current = c10::cuda::getCurrentCUDAStream(device).stream();
+    if (handle == -1) return current ? static_cast<void *>(current) : reinterpret_cast<void *>(uintptr_t(1));
+    if (handle != 0)
+      named.emplace(c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(handle), device));
+    else if (!capturing(current))
+      C10_CUDA_CHECK(cudaStreamSynchronize(current));
+    return reinterpret_cast<void *>(handle);
   }
   // Scratch: the caller's; else none (the context's is used), but while the stream is being captured a block
   // from torch's allocator, which keeps it for the graph as it keeps the outputs.  query(bytes) asks for the
@@ -154,13 +170,6 @@ struct Call {
   }
 };
 
-Call call_of(PyObject *const *args) {
-  Call c;
-  c.ctx = reinterpret_cast<af2_ctx *>(PyLong_AsUnsignedLongLong(args[0]));
-  c.ordinal = static_cast<int>(PyLong_AsLong(args[1]));
-  if (PyErr_Occurred()) throw Failed();
-  return c;
-}
 long long integer(PyObject *o) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) throw Failed();
@@ -182,7 +191,8 @@ void put(PyObject *dict, const char *key, const at::Tensor &t) {
 
 // handle, ordinal, x, weight, bias, residual, activation, out, save, stream, workspace
 PyObject *dense(PyObject *const *a) {
-  Call c = call_of(a);
+  Call c(a);
+  void *const stream = c.use_stream(integer(a[9]));
   const at::Tensor &x = tensor_of(a[2], "x"), &w = tensor_of(a[3], "weight");
   const at::Tensor *bias = optional_tensor(a[4], "bias"), *residual = optional_tensor(a[5], "residual"),
                    *given = optional_tensor(a[7], "out"), *workspace = optional_tensor(a[10], "workspace");
@@ -205,7 +215,6 @@ PyObject *dense(PyObject *const *a) {
     c.done(entry.dense_saved_bytes(&shape, c.code, act, &bytes));
     saved = c.bytes(bytes);
   }
-  void *const stream = c.stream(integer(a[9]));
   void *const ws = c.scratch(
       workspace, stream, [&](uint64_t *need) { return entry.dense_workspace_bytes(&shape, c.code, act, 0, need); });
   c.done(entry.dense(c.ctx, &shape, c.code, x.data_ptr(), wp, bp, ptr(residual), &o, y.data_ptr(),
@@ -215,7 +224,8 @@ PyObject *dense(PyObject *const *a) {
 
 // handle, ordinal, d_out, x, weight, saved, bias, activation, need x, need weight, stream, workspace
 PyObject *dense_backward(PyObject *const *a) {
-  Call c = call_of(a);
+  Call c(a);
+  void *const stream = c.use_stream(integer(a[10]));
   const at::Tensor &dy = tensor_of(a[2], "d_out"), &x = tensor_of(a[3], "x"), &w = tensor_of(a[4], "weight");
   const at::Tensor *saved = optional_tensor(a[5], "saved"), *workspace = optional_tensor(a[11], "workspace");
   const int act = static_cast<int>(integer(a[7]));
@@ -232,7 +242,6 @@ PyObject *dense_backward(PyObject *const *a) {
     c.done(entry.dense_saved_bytes(&shape, c.code, act, &bytes));
     kept = c.block(saved, bytes, "saved", "be what the forward pass returned");
   }
-  void *const stream = c.stream(integer(a[10]));
   void *const ws = c.scratch(
       workspace, stream, [&](uint64_t *need) { return entry.dense_workspace_bytes(&shape, c.code, act, 1, need); });
   at::Tensor dx, dw, db;
@@ -287,7 +296,8 @@ GatedTensors gated_tensors(const Call &c, PyObject *dict, af2_gated_weights *w) 
 
 // handle, ordinal, x, weights, residual, activation, out, save, stream, workspace
 PyObject *gated(PyObject *const *a) {
-  Call c = call_of(a);
+  Call c(a);
+  void *const stream = c.use_stream(integer(a[8]));
   const at::Tensor &x = tensor_of(a[2], "x");
   const at::Tensor *residual = optional_tensor(a[4], "residual"), *given = optional_tensor(a[6], "out"),
                    *workspace = optional_tensor(a[9], "workspace");
@@ -308,7 +318,6 @@ PyObject *gated(PyObject *const *a) {
     c.done(entry.gated_saved_bytes(&shape, c.code, &bytes));
     saved = c.bytes(bytes);
   }
-  void *const stream = c.stream(integer(a[8]));
   void *const ws = c.scratch(
       workspace, stream, [&](uint64_t *need) { return entry.gated_workspace_bytes(&shape, c.code, 0, need); });
   c.done(entry.gated(c.ctx, &shape, c.code, x.data_ptr(), &w, ptr(residual), &o, y.data_ptr(),
@@ -318,7 +327,8 @@ PyObject *gated(PyObject *const *a) {
 
 // handle, ordinal, d_out, x, weights, saved, activation, need (None or a container of names), stream, workspace
 PyObject *gated_backward(PyObject *const *a) {
-  Call c = call_of(a);
+  Call c(a);
+  void *const stream = c.use_stream(integer(a[8]));
   const at::Tensor &dy = tensor_of(a[2], "d_out"), &x = tensor_of(a[3], "x");
   const at::Tensor *saved = optional_tensor(a[5], "saved"), *workspace = optional_tensor(a[9], "workspace");
   const int act = static_cast<int>(integer(a[6]));
@@ -332,7 +342,6 @@ PyObject *gated_backward(PyObject *const *a) {
   uint64_t bytes = 0;
   c.done(entry.gated_saved_bytes(&shape, c.code, &bytes));
   void *kept = c.block(saved, bytes, "saved", "be what the forward pass returned");
-  void *const stream = c.stream(integer(a[8]));
   void *const ws = c.scratch(
       workspace, stream, [&](uint64_t *need) { return entry.gated_workspace_bytes(&shape, c.code, 1, need); });
   auto needed = [&](const char *name) {
@@ -382,7 +391,8 @@ std::vector<af2_tensor_ref> refs(const Call &c, PyObject *list, const char *name
 
 // handle, ordinal, gradients (a list), out (a list or None), max_norm (None: the norm alone), stream, workspace
 PyObject *gradients(PyObject *const *a) {
-  Call c = call_of(a);
+  Call c(a);
+  void *const stream = c.use_stream(integer(a[5]));
   const std::vector<af2_tensor_ref> in = refs(c, a[2], "gradient");
   const int64_t n = static_cast<int64_t>(in.size());
   std::vector<af2_tensor_ref> out;
@@ -392,7 +402,6 @@ PyObject *gradients(PyObject *const *a) {
       refuse("out has " + std::to_string(out.size()) + " tensors; expected " + std::to_string(in.size()));
   }
   const at::Tensor *workspace = optional_tensor(a[6], "workspace");
-  void *const stream = c.stream(integer(a[5]));
   void *const ws = c.scratch(workspace, stream, [&](uint64_t *need) { return entry.norm_workspace_bytes(n, need); });
   const at::Tensor norm = c.make({});
   float *np = static_cast<float *>(norm.data_ptr());

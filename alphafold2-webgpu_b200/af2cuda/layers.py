@@ -8,7 +8,8 @@ Every tensor of a call has one type (float32, float16 or bfloat16); weights
 are [in, out] and used as they are stored, so they may change between calls.
 Activations, residuals and outputs are [rows, width] with any row stride of at
 least the width.  Calls run on torch's current stream unless ``stream`` names
-another (a raw CUDA stream handle; 0 is the device context's own stream).
+another (a raw CUDA stream handle; 0 is the device context's own stream); a
+named stream does not wait for the current one, so the inputs must be ready on it.
 
 No counterpart in the reference, whose weights are fixed and whose transition
 is ReLU (src/evoformer/transition.ts); the weights' names follow its
@@ -64,15 +65,17 @@ def _activation_code(activation: str) -> int:
 
 
 def _on_stream(tensors, device: Device, stream: int) -> None:
-    """Keeps new tensors that were written on a stream other than torch's current one from reuse
-    until it has passed."""
+    """Keeps tensors that were written on a named stream from reuse until it, and torch's current stream,
+    where the caller will read them, have passed.  (New ones were allocated on the named stream.)"""
     if stream == 0:  # the context's own stream: torch's allocator cannot follow it
         device.sync()
         return
     import torch
-    side = torch.cuda.ExternalStream(stream, device=torch.device("cuda", device.ordinal))
+    where = torch.device("cuda", device.ordinal)
+    streams = (torch.cuda.ExternalStream(stream, device=where), torch.cuda.current_stream(where))
     for t in tensors:
-        t.record_stream(side)
+        for s in streams:
+            t.record_stream(s)
 
 
 def dense_saved_bytes(rows: int, inner: int, columns: int, dtype, activation: str = "none") -> int:

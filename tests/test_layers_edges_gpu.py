@@ -132,3 +132,39 @@ def test_the_contexts_scratch_is_refused_in_a_capture(device):
     graph.replay()
     torch.cuda.synchronize()
     close("y", out, ref.dense(s["x"], s["weight"], None, None, "none")["y"] + 1, F32)
+
+
+def test_a_named_streams_outputs_do_not_reuse_what_is_still_read(device):
+    """Memory freed on torch's current stream, whose last reader there is still queued, is not what a call
+    on another stream writes its outputs to."""
+    s = dense_case(4096, 64, 1024, F32, seed=1130)
+    want = ref.dense(s["x"], s["weight"], None, None, "none")["y"]
+    side = torch.cuda.Stream()
+    for stream in (side.cuda_stream, 0):
+        kept = torch.zeros(4096, 1024, device="cuda")
+        freed = torch.full((4096, 1024), 3.0, device="cuda")
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)
+        kept.copy_(freed)
+        del freed
+        y = af2cuda.encode_dense_tensors(device, s["x"], s["weight"], stream=stream)
+        torch.cuda.synchronize()
+        assert bool((kept == 3.0).all()), stream
+        close("y", y, want, F32)
+
+
+def test_a_named_streams_outputs_live_until_the_current_stream_has_read_them(device):
+    s = dense_case(4096, 64, 1024, F32, seed=1140)
+    side, current = torch.cuda.Stream(), torch.cuda.current_stream()
+    kept, other = torch.zeros(4096, 1024, device="cuda"), torch.full_like(s["weight"], 9.0)
+    torch.cuda.synchronize()
+    y = af2cuda.encode_dense_tensors(device, s["x"], s["weight"], stream=side.cuda_stream)
+    want = ref.dense(s["x"], s["weight"], None, None, "none")["y"]
+    current.wait_stream(side)
+    torch.cuda._sleep(100_000_000)
+    kept.copy_(y)
+    del y
+    for _ in range(3):
+        af2cuda.encode_dense_tensors(device, s["x"], other, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    close("y", kept, want, F32)
