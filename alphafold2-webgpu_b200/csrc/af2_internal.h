@@ -10,6 +10,7 @@
 #include <vector>
 
 #include "../../include/af2cuda.h"
+#include "scratch_order.h"
 
 namespace af2 {
 
@@ -124,12 +125,11 @@ struct af2_ctx {
   // af2_set_weight_cache: prepared weights kept per weights pointer and shape, made once
   bool weight_cache = false;
   std::vector<af2::CachedWeights> cached_weights;
-  // scratch of the layers with learned weights, the stream of its last use, and an event behind
-  // that use (LayerScratch)
+  // scratch of the layers with learned weights, its last use, and an event behind that use (LayerScratch)
   af2::DeviceBuffer layer_scratch;
   std::vector<af2::LayerMap> layer_maps;  // descriptors by their shapes (layer_map_3d)
   cudaEvent_t layer_done = nullptr;
-  cudaStream_t layer_stream = nullptr;
+  af2::ScratchUse layer_use;
 };
 
 namespace af2 {
@@ -467,6 +467,7 @@ class LayerScratch {
   af2_ctx *ctx_;
   cudaStream_t stream_;
   uint8_t *base_ = nullptr;
+  ScratchUse use_;
   bool owned_ = false;
 };
 

@@ -44,17 +44,19 @@ af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
                                              "workspace that the graph's owner keeps");
   }
   const bool grow = ctx_->layer_scratch.bytes < bytes;
-  const cudaStream_t last = ctx_->layer_stream;
-  if (last && (grow || last != stream_)) {
-    if (lasting(last))
-      if (cudaError_t e = cudaEventRecord(ctx_->layer_done, last); e != cudaSuccess)
-        return cuda_fail(ctx_, e, "record the layer scratch's use");
-    // earlier calls may still use the buffer: this one follows them, or the host does before it is freed
-    if (cudaError_t e = grow ? cudaEventSynchronize(ctx_->layer_done)
-                             : cudaStreamWaitEvent(stream_, ctx_->layer_done, 0);
-        e != cudaSuccess)
-      return cuda_fail(ctx_, e, "order the layer scratch between streams");
-  }
+  use_ = {stream_, 0, lasting(stream_)};
+  if (!use_.lasting)
+    if (cudaError_t e = cudaStreamGetId(stream_, &use_.id); e != cudaSuccess)
+      return cuda_fail(ctx_, e, "query the stream's id");
+  // earlier calls may still use the buffer: this one follows them, or the host does before it is freed
+  const cudaError_t ordered = order_scratch(
+      ctx_->layer_use, use_, grow,
+      [&](const void *last) {
+        return cudaEventRecord(ctx_->layer_done, static_cast<cudaStream_t>(const_cast<void *>(last)));
+      },
+      [&] { return cudaStreamWaitEvent(stream_, ctx_->layer_done, 0); },
+      [&] { return cudaEventSynchronize(ctx_->layer_done); });
+  if (ordered != cudaSuccess) return cuda_fail(ctx_, ordered, "order the layer scratch between streams");
   if (grow)
     if (af2_status st = ensure(ctx_, ctx_->layer_scratch, bytes, "layer scratch"); st != AF2_OK) return st;
   base_ = static_cast<uint8_t *>(ctx_->layer_scratch.ptr);
@@ -64,8 +66,8 @@ af2_status LayerScratch::acquire(void *workspace, size_t bytes) {
 
 af2_status LayerScratch::release() {
   if (!owned_) return AF2_OK;
-  ctx_->layer_stream = stream_;
-  if (lasting(stream_)) return AF2_OK;
+  ctx_->layer_use = use_;
+  if (use_.lasting) return AF2_OK;
   if (cudaError_t e = cudaEventRecord(ctx_->layer_done, stream_); e != cudaSuccess)
     return cuda_fail(ctx_, e, "record the layer scratch's use");
   return AF2_OK;

@@ -168,3 +168,28 @@ def test_a_named_streams_outputs_live_until_the_current_stream_has_read_them(dev
         af2cuda.encode_dense_tensors(device, s["x"], other, stream=side.cuda_stream)
     torch.cuda.synchronize()
     close("y", kept, want, F32)
+
+
+def test_streams_that_come_and_go_share_the_scratch_safely(device):
+    """Each call on a new stream, destroyed with the work pending: handles come back, streams do not."""
+    runtime = ctypes.CDLL("libcudart.so.12")  # the one that torch has loaded
+    runtime.cudaStreamDestroy.argtypes = [ctypes.c_size_t]
+    cases = [gated_case(700, 130, 260, F32, seed=1150 + i) for i in range(2)]
+    want = [ref.gated(s["x"], s["weights"], None, "silu")["y"] for s in cases]
+    outs = [torch.empty_like(cases[0]["x"]) for _ in range(16)]
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        stream = ctypes.c_size_t()
+        assert runtime.cudaStreamCreateWithFlags(ctypes.byref(stream), 1) == 0
+        s = cases[i % 2]
+        shape = _lib.TransitionShape(700, 130, 260)
+        w = _lib.GatedWeights(*[s["weights"][k].data_ptr() for k in ("gateWeight", "gateBias", "valueWeight", "valueBias",
+                                                                     "outputWeight", "outputBias")])
+        o = _lib.LayerOptions(3, 0, 130, 130, 130, 130)
+        _lib.check(_lib.lib().af2_gated_transition(device.handle, ctypes.byref(shape), _lib.AF2_F32, s["x"].data_ptr(),
+                                                   ctypes.byref(w), None, ctypes.byref(o), out.data_ptr(), None, None,
+                                                   stream.value), device.handle)
+        assert runtime.cudaStreamDestroy(stream.value) == 0
+    torch.cuda.synchronize()
+    for i, y in enumerate(outs):
+        close("y", y, want[i % 2], F32)

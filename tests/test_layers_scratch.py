@@ -1,5 +1,6 @@
 """CPU tests of the learned layers' scratch: the size queries against what the passes count
-(tests/layer_scratch_check.cpp, linked with the library's objects)."""
+(tests/layer_scratch_check.cpp, linked with the library's objects), the order of its uses against
+fakes (tests/scratch_order_check.cpp)."""
 import importlib.util
 import shutil
 import subprocess
@@ -29,5 +30,15 @@ def test_queries_cover_every_part_of_the_gradients(tmp_path):
                     *map(str, sorted((PKG / "csrc" / "_build").glob("*.o"))), "-o", str(exe),
                     f"-L{cuda / 'lib64'}", "-lcudart_static", "-ldl", "-lrt", "-pthread"], check=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stdout + res.stderr
+    assert res.stdout.strip() == "ok"
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_order_between_uses_of_the_scratch(tmp_path):
+    exe = tmp_path / "scratch_order_check"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(PKG / "csrc"), str(ROOT / "tests" / "scratch_order_check.cpp"),
+                    "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert res.returncode == 0, res.stdout + res.stderr
     assert res.stdout.strip() == "ok"
