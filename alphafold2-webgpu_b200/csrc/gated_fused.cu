@@ -59,7 +59,7 @@ struct Args {
   unsigned int *err;
 };
 
-// 2^x for x in [-126, 60] without the multi-function unit: x = n + f, |f| <= 1/2, 2^f by the
+// 2^x for x in [-126, 63] without the multi-function unit: x = n + f, |f| <= 1/2, 2^f by the
 // polynomial of degree 4 with the least largest relative error there (2.6e-6), n added to its exponent.
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   const float2 magic = f2(12582912.f);  // 1.5 * 2^23: the sum's low bits are the rounded integer
@@ -76,10 +76,8 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
 // silu of two values, sigmoid2_fast with the exponential on the FMA pipe
 __device__ __forceinline__ float2 silu2_poly(float2 z) {
   const float2 x = f2mul(z, f2(-1.4426950408889634f));
-  const float2 e = ex2_poly2(make_float2(fmaxf(fminf(x.x, 60.f), -126.f), fmaxf(fminf(x.y, 60.f), -126.f)));
-  const float2 d = f2add(e, f2(1.f));
-  const float r = rcp_approx(d.x * d.y);
-  return f2mul(z, f2mul(f2(r), make_float2(d.y, d.x)));
+  const float2 e = ex2_poly2(make_float2(fmaxf(fminf(x.x, 63.f), -126.f), fmaxf(fminf(x.y, 63.f), -126.f)));
+  return f2mul(z, shared_reciprocal(f2add(e, f2(1.f))));
 }
 
 // silu of two values for bf16, one instruction of the multi-function unit each: z / 2 (1 + tanh(z / 2)).

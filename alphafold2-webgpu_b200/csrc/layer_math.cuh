@@ -11,8 +11,10 @@
 // tensors, within a few units of f32's last place; FAST = true, for 16-bit ones,
 // relative error below 2^-16 where the value matters to them.
 //   - FAST: two sigmoids share one reciprocal: with d = 1 + e^-z, 1 / d0 =
-//     d1 / (d0 d1).  The exponent is held below 2^60 so that the product cannot
-//     overflow; a sigmoid below 2^-60 (z < -41) is 2^-60.
+//     d1 / (d0 d1).  The exponential is held below 2^63 so that the product cannot
+//     overflow, and 2^-62 is taken off the sigmoid, with 0 as the least: far out it
+//     is 0, not the bound, which a z of the type's lowest value would make large of.
+//     What that takes off a sigmoid is 2^-16 of it at z = -32.
 //   - Phi(-u) = e^(-u^2 / 2) t Q(t), t = 1 / (1 + c u), u >= 0: the form of
 //     Hastings' approximations, Q fitted to Phi(-u) e^(u^2 / 2) / t on u in [0, 14]
 //     for the least largest relative error (degree 5, c = 0.31: 4.7e-6; degree 8,
@@ -36,12 +38,15 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// The sigmoids of two values; a NaN gives 2^-60 (its product with z is NaN again).
+// The sigmoids with the denominators d.
+__device__ __forceinline__ float2 shared_reciprocal(float2 d) {
+  const float r = rcp_approx(d.x * d.y);
+  return make_float2(__saturatef(fmaf(r, d.y, -0x1p-62f)), __saturatef(fmaf(r, d.x, -0x1p-62f)));
+}
+// The sigmoids of two values; a NaN gives 0 (its product with z is NaN again).
 __device__ __forceinline__ float2 sigmoid2_fast(float2 z) {
   const float2 x = f2mul(z, f2(-1.4426950408889634f));
-  const float2 d = f2add(make_float2(ex2_approx(fminf(x.x, 60.f)), ex2_approx(fminf(x.y, 60.f))), f2(1.f));
-  const float r = rcp_approx(d.x * d.y);
-  return f2mul(f2(r), make_float2(d.y, d.x));
+  return shared_reciprocal(f2add(make_float2(ex2_approx(fminf(x.x, 63.f)), ex2_approx(fminf(x.y, 63.f))), f2(1.f)));
 }
 
 // Phi and, for the slope, e^(-z^2 / 2).

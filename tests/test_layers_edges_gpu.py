@@ -193,3 +193,57 @@ def test_streams_that_come_and_go_share_the_scratch_safely(device):
     torch.cuda.synchronize()
     for i, y in enumerate(outs):
         close("y", y, want[i % 2], F32)
+
+
+# ---- values far from one ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["relu", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("rows", [3, 40, 600])
+def test_gates_shut_by_the_lowest_value(device, rows, act, dtype):
+    """A bias of the type's lowest value shuts some hidden channels: their activation is 0, and what
+    stands beside them is as it would be alone."""
+    lowest = torch.finfo(dtype).min
+    for channels in (64, 200):
+        s = gated_case(rows, channels, 264, dtype, seed=1200)
+        s["weights"]["gateBias"][::3] = lowest
+        w = s["weights"]
+        want = ref.gated(s["x"], w, None, act, s["d_out"])
+        y = af2cuda.encode_gated_transition_tensors(device, s["x"], w, activation=act)
+        close("y alone", y, want["y"], dtype)
+        y, saved = af2cuda.encode_gated_transition_tensors(device, s["x"], w, activation=act, save=True)
+        grads = af2cuda.encode_gated_transition_backward_tensors(device, s["d_out"], s["x"], w, saved=saved, activation=act)
+        for k, v in {"y": y, **grads}.items():
+            close(k, v, want[k], dtype)
+            if k in ("gateBias", "valueBias", "gateWeight", "valueWeight"):
+                assert not v[..., ::3].any(), k
+    d = dense_case(rows, 96, 136, dtype, seed=1210)
+    d["bias"][::3] = lowest
+    want = ref.dense(d["x"], d["weight"], d["bias"], None, act, d["d_out"])
+    y = af2cuda.encode_dense_tensors(device, d["x"], d["weight"], bias=d["bias"], activation=act)
+    close("y alone", y, want["y"], dtype)
+    y, saved = af2cuda.encode_dense_tensors(device, d["x"], d["weight"], bias=d["bias"], activation=act, save=True)
+    grads = af2cuda.encode_dense_backward_tensors(device, d["d_out"], d["x"], d["weight"], saved=saved, bias=True, activation=act)
+    for k, v in {"y": y, **grads}.items():
+        close(k, v, want[k], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+def test_infinite_and_nan_pre_activations(device, act, dtype):
+    """Through biases: each column is what the formula makes of it, the columns beside it what they were."""
+    for rows in (4, 500):
+        d = dense_case(rows, 64, 80, dtype, seed=1220)
+        clean = af2cuda.encode_dense_tensors(device, d["x"], d["weight"], bias=d["bias"], activation=act)
+        for value in (float("inf"), float("-inf"), float("nan")):
+            bias = d["bias"].clone()
+            bias[[0, 17, 33]] = value
+            limit = ref.act(act, torch.tensor(value, dtype=torch.float64)).item()
+            for save in (False, True):
+                y = af2cuda.encode_dense_tensors(device, d["x"], d["weight"], bias=bias, activation=act, save=save)
+                y = y[0] if save else y
+                other = [c for c in range(80) if c not in (0, 17, 33)]
+                close("the others", y[:, other], clean[:, other].double(), dtype)
+                got = y[:, [0, 17, 33]]
+                assert bool(torch.isnan(got).all() if limit != limit else (got == limit).all()), (value, save)
