@@ -12,10 +12,12 @@
 //
 // What bounds it.  Per chunk and SM the tensor core takes 768 clocks (512 + 256)
 // and the activations 8192 values: with one exponential and half a reciprocal
-// each the multi-function unit would take 768 clocks too: bf16 takes one tanh a
-// value (512), f16 every second pair's exponential on the FMA pipe (512 and that).
-// 262144 rows of 128 -> 512 -> 128 in bf16: 97 us alone, 62 of them at cuBLAS's
-// rate for the products (107 repeated, under the power cap).
+// each the multi-function unit would take 768 clocks too, so every second pair's
+// exponentials run on the FMA pipe (512 and that).  (silu as z / 2 (1 + tanh(z / 2)),
+// one instruction of that unit a value, took 95 us below, but tanh.approx's 2^-11
+// is 1 % of silu at z = -4 and 10 % at -6.)
+// 262144 rows of 128 -> 512 -> 128 in bf16: 109 us alone, 62 of them at cuBLAS's
+// rate for the products (104 repeated, f16 108).
 #include <algorithm>
 #include <type_traits>
 
@@ -78,15 +80,6 @@ __device__ __forceinline__ float2 silu2_poly(float2 z) {
   const float2 x = f2mul(z, f2(-1.4426950408889634f));
   const float2 e = ex2_poly2(make_float2(fmaxf(fminf(x.x, 63.f), -126.f), fmaxf(fminf(x.y, 63.f), -126.f)));
   return f2mul(z, shared_reciprocal(f2add(e, f2(1.f))));
-}
-
-// silu of two values for bf16, one instruction of the multi-function unit each: z / 2 (1 + tanh(z / 2)).
-// tanh.approx is within 2^-11 of itself, so the result is within 2^-11 of |z| / 2: below a third of a
-// bf16 rounding where z > 0, and beside values of that size where z < 0 (at z = -4 1 % of a value
-// that is 2 % of |z|).
-__device__ __forceinline__ float2 silu2_tanh(float2 z) {
-  const float2 half = f2mul(z, f2(0.5f));
-  return f2fma(half, make_float2(tanhf_approx(half.x), tanhf_approx(half.y)), half);
 }
 
 // The chunks of a CTA's tiles in order; a tile starts at chunk (tile mod chunks), so that the CTAs do
@@ -350,9 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             float2 a;
-            if constexpr (ACT == AF2_ACTIVATION_SILU && BF16)
-              a = silu2_tanh(gz[i]);
-            else if constexpr (ACT == AF2_ACTIVATION_SILU)
+            if constexpr (ACT == AF2_ACTIVATION_SILU)
               a = i ? silu2_poly(gz[i]) : activate2<ACT, true>(gz[i]);
             else
               a = activate2<ACT, true>(gz[i]);

@@ -247,3 +247,40 @@ def test_infinite_and_nan_pre_activations(device, act, dtype):
                 close("the others", y[:, other], clean[:, other].double(), dtype)
                 got = y[:, [0, 17, 33]]
                 assert bool(torch.isnan(got).all() if limit != limit else (got == limit).all()), (value, save)
+
+
+def bare_gate(rows, width, dtype, low, high):
+    """A gated transition whose hidden activations are act(x), one by one: the gate and output weights are
+    identities, the value is 1, and x goes from low to high."""
+    x = torch.linspace(low, high, rows * width, device="cuda").to(dtype).view(rows, width)
+    one = torch.eye(width, device="cuda").to(dtype)
+    return x, {"gateWeight": one, "valueWeight": torch.zeros_like(one), "valueBias": torch.ones_like(one[0]),
+               "outputWeight": one}
+
+
+def exact_act(kind, z):
+    """ref.act in f64 with its last places on the negative side: Phi(z) from erfc, since 1 + erf cancels."""
+    return z * torch.erfc(-z * 0.5**0.5) / 2 if kind == "gelu" else ref.act(kind, z)
+
+
+def elements_close(name, got, want, relative, dtype):
+    """Within `relative` of each element, and half of f16's smallest step."""
+    err = (got.double() - want).abs() - (2.0**-25 if dtype == F16 else 0.0)
+    worst = (err / want.abs().clamp(min=1e-300)).max().item()
+    assert worst <= relative, f"{name}: an element is off by {worst:.3e} of its size"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act,low", [("sigmoid", -30.0), ("silu", -30.0), ("gelu", -10.0)])
+@pytest.mark.parametrize("rows,width", [(4, 64), (700, 64), (5000, 128), (700, 200)])
+def test_activations_element_by_element(device, rows, width, act, low, dtype):
+    """No positive gate hides the error of a negative one.  Each element is rounded once (the output's
+    product copies it), and the activations of 16-bit tensors are within 2^-16."""
+    x, w = bare_gate(rows, width, dtype, low, 12.0)
+    want = exact_act(act, x.double())
+    alone = af2cuda.encode_gated_transition_tensors(device, x, w, activation=act)
+    elements_close("y alone", alone, want, ref.ROUNDOFF[dtype] + 2.0**-16, dtype)
+    kept, _ = af2cuda.encode_gated_transition_tensors(device, x, w, activation=act, save=True)
+    elements_close("y", kept, want, ref.ROUNDOFF[dtype] + 2.0**-16, dtype)
+    d = af2cuda.encode_dense_tensors(device, x, w["gateWeight"], activation=act)
+    elements_close("dense", d, want, ref.ROUNDOFF[dtype] + 2.0**-16, dtype)
