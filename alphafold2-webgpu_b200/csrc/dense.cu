@@ -179,7 +179,7 @@ inline RowGrid row_grid(int64_t rows, int64_t width) {
 // load(row, column, in) for DEPTH rows a thread, then use(row, column, in, sums) for them: the loads of
 // one are held up neither by the other's stores nor by its arithmetic.  Then sums[s] over the block's rows
 // go to partial[x][s][pitch], in a fixed order.
-template <typename T, int SETS, int DEPTH, int STREAMS, typename Load, typename Use>
+template <typename In, int SETS, int DEPTH, typename Load, typename Use>
 __device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, const RowGrid &grid, float *partial,
                                                int64_t pitch, Load &&load, Use &&use) {
   const unsigned y = blockIdx.x / grid.down, x = blockIdx.x - y * grid.down;
@@ -190,7 +190,7 @@ __device__ __forceinline__ void for_row_groups(int64_t rows, int64_t width, cons
   if (c < width && ty < grid.at_once) {
     const int end = static_cast<int>(min(rows - r0, static_cast<int64_t>(grid.group)));
     for (int r = ty; r < end; r += DEPTH * grid.at_once) {
-      Raw8<T> in[DEPTH][STREAMS];
+      In in[DEPTH];
 #pragma unroll
       for (int i = 0; i < DEPTH; ++i)
         if (r + i * grid.at_once < end) load(r0 + r + i * grid.at_once, c, in[i]);
@@ -224,30 +224,33 @@ template <typename T>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T *src, int64_t stride, int64_t rows, int64_t width,
                                                          const RowGrid grid, float *partial, int64_t pitch) {
   dependency_wait();
-  for_row_groups<T, 1, 4, 1>(
+  for_row_groups<Raw8<T>, 1, 4>(
       rows, width, grid, partial, pitch,
-      [&](int64_t r, int64_t c, Raw8<T>(&in)[1]) { load_raw8<T>(src + r * stride + c, columns_of(width, c), in[0]); },
-      [&](int64_t, int64_t, const Raw8<T>(&in)[1], float (&sums)[1][8]) {
+      [&](int64_t r, int64_t c, Raw8<T> &in) { load_raw8<T>(src + r * stride + c, columns_of(width, c), in); },
+      [&](int64_t, int64_t, const Raw8<T> &in, float (&sums)[1][8]) {
         float x[8];
-        values8<T>(in[0], x);
+        values8<T>(in, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) sums[0][i] += x[i];
       });
 }
 
-// Eight saved values (16-bit types: slopes).
+// What a slope is kept in (SavedPlanes).
 template <typename T>
-__device__ __forceinline__ void load_saved8(const SavedPlanes &s, int plane, int64_t r, int64_t c, Raw8<T> &x) {
-  const int64_t at = plane * s.stride + r * s.pitch + c;
-  if constexpr (sizeof(T) == 4)
+using Kept = std::conditional_t<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat16, float>;
+// Eight saved slopes.
+template <typename T>
+__device__ __forceinline__ void load_slopes8(const SavedPlanes &s, int64_t r, int64_t c, Raw8<Kept<T>> &x) {
+  const int64_t at = r * s.pitch + c;
+  if constexpr (sizeof(Kept<T>) == 4)
     load_raw8<float>(s.f32 + at, 8, x);
   else
     load_raw8<T>(reinterpret_cast<const T *>(s.half + at), 8, x);
 }
 template <typename T>
-__device__ __forceinline__ void slopes8(const Raw8<T> &r, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    values8<T>(r, x);
+__device__ __forceinline__ void slopes8(const Raw8<Kept<T>> &r, float (&x)[8]) {
+  if constexpr (sizeof(Kept<T>) == 4) {
+    values8<float>(r, x);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -268,19 +271,23 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
   dependency_wait();
   const unsigned own = grid.down * grid.across;
   if (blockIdx.x >= own) return pack_groups<T>(copies, blockIdx.x - own, gridDim.x - own);
-  constexpr int STREAMS = SLOPE ? 2 : 1, DEPTH = sizeof(T) == 4 ? 2 : 4;
-  for_row_groups<T, 1, DEPTH, STREAMS>(
+  constexpr int DEPTH = sizeof(T) == 4 ? 2 : 4;
+  struct In {
+    Raw8<T> dy;
+    Raw8<Kept<T>> slope;
+  };
+  for_row_groups<In, 1, DEPTH>(
       rows, width, grid, partial, pitch,
-      [&](int64_t r, int64_t c, Raw8<T>(&in)[STREAMS]) {
-        load_raw8<T>(dy + r * dy_stride + c, columns_of(width, c), in[0]);
-        if constexpr (SLOPE) load_saved8<T>(saved, 0, r, c, in[1]);
+      [&](int64_t r, int64_t c, In &in) {
+        load_raw8<T>(dy + r * dy_stride + c, columns_of(width, c), in.dy);
+        if constexpr (SLOPE) load_slopes8<T>(saved, r, c, in.slope);
       },
-      [&](int64_t r, int64_t c, const Raw8<T>(&in)[STREAMS], float (&sums)[1][8]) {
+      [&](int64_t r, int64_t c, const In &in, float (&sums)[1][8]) {
         float d[8];
-        values8<T>(in[0], d);
+        values8<T>(in.dy, d);
         if constexpr (SLOPE) {
           float z[8];
-          slopes8<T>(in[1], z);
+          slopes8<T>(in.slope, z);
           const int n = columns_of(width, c);
 #pragma unroll
           for (int i = 0; i < 8; ++i) d[i] = i < n ? d[i] * z[i] : 0.f;  // (past the width nothing was saved)
@@ -290,6 +297,9 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
         store_operand8<T>(dz, r * dz_pitch + c, dz_piece, d);
       });
 }
+
+// Whether `count` saved factors are kept in f32 (SavedPlanes).
+bool planes_are_f32(int dtype, int count) { return dtype == AF2_F32 || (dtype == AF2_F16 && count == 1); }
 
 // ---- one pass of a layer --------------------------------------------------------------
 
@@ -388,7 +398,7 @@ class Pass {
     SavedPlanes s;
     s.pitch = saved_pitch(width);
     s.stride = rows * s.pitch;
-    if (f32()) {
+    if (planes_are_f32(dtype_, count)) {
       s.f32 = static_cast<float *>(saved);
     } else {
       s.half = static_cast<uint16_t *>(saved);
@@ -490,7 +500,7 @@ class Pass {
 
 uint64_t planes_bytes(int64_t rows, int64_t width, int dtype, int count) {
   const uint64_t n = static_cast<uint64_t>(count) * rows * saved_pitch(width);
-  if (dtype == AF2_F32) return part(4 * n);
+  if (planes_are_f32(dtype, count)) return part(4 * n);
   return part(2 * n) + (count > 1 ? part(align_up(rows, 32) * saved_pitch(width) / 8) : 0);
 }
 uint64_t hidden_bytes(int64_t rows, int64_t hidden, int dtype) {

@@ -10,7 +10,8 @@
 //   largest of a block is in [2^14, 2^15): nothing overflows, and what is
 //   2^-28 of the largest still has its 11 bits.
 //
-//   f16 (rounds to 2^-11): sign, 3 bits of exponent, 12 of mantissa, to 2^-13,
+//   f16 (rounds to 2^-11): a dense layer's slopes are kept in f32 (16 bits hold
+//   either f16's precision or its range).  The gated transition's factors: sign, 3 bits of exponent, 12 of mantissa, to 2^-13,
 //   scaled so that the largest has exponent 6 of 7 (rounding may carry to 7):
 //   full precision for six binades, below them steps of 2^-17 of the largest's
 //   binade, as f16 itself ends 2^-14 below one.  In f32 terms: the value times
@@ -83,19 +84,6 @@ struct Factor<__half> {
   }
   static __device__ __forceinline__ float scale(uint32_t e) { return __uint_as_float(e < 254u ? e << 23 : 0x7fffffffu); }
   static __device__ __forceinline__ float2 value(uint32_t w, float scale) { return f2mul(decode(w), f2(scale)); }
-  // A slope: at most 1.13 in size; a NaN is kept as the largest code.
-  static __device__ __forceinline__ uint32_t slope(float2 v) {
-    uint32_t w = codes(f2mul(v, f2(kDown)));
-    if (v.x != v.x) w |= 0x7fffu;
-    if (v.y != v.y) w |= 0x7fff0000u;
-    return w;
-  }
-  static __device__ __forceinline__ float2 slope_value(uint32_t w) {
-    float2 v = decode(w);
-    if ((w & 0x7fffu) == 0x7fffu) v.x = __uint_as_float(0x7fffffffu);
-    if ((w & 0x7fff0000u) == 0x7fff0000u) v.y = __uint_as_float(0x7fffffffu);
-    return v;
-  }
 };
 
 }  // namespace af2

@@ -803,11 +803,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         // turn, the second where the first holds slopes (f32: the two halves of the warp's only block of
         // columns).
         const bool keep = (KIND == kOutSave || KIND == kOutRows) && p.save;
+        const bool staged = keep && std::is_same<OT, __nv_bfloat16>::value;  // (f32 slopes leave from each lane)
         auto fetch = [&](int b, int at) {
           if (lane == 0) {
             bulk_wait_read_all();
             mbar_arrive_expect_tx(load(ew, at & 1), F32 ? 4096 : 2048);
-            const uint32_t to = block_addr + (F32 ? 0 : 2048 * (keep ? 1 : at & 1));
+            const uint32_t to = block_addr + (F32 ? 0 : 2048 * (staged ? 1 : at & 1));
             tma_load_3d(to, &maps.residual, load(ew, at & 1), n0 + b * 32, r0, 0);
             if (F32) tma_load_3d(to + 2048, &maps.residual, load(ew, at & 1), n0 + b * 32 + 16, r0, 0);
           }
@@ -940,7 +941,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const int c0 = n0 + b * 32;
           uint32_t r[32];
           tmem_ld32(taddr + b * 32, r);
-          if (tma_residual && !keep && b + step < end) fetch(b + step, loads + 1);
+          if (tma_residual && !staged && b + step < end) fetch(b + step, loads + 1);
           float(&y)[32] = reinterpret_cast<float(&)[32]>(r);
           const int cols = min(32, p.n - c0);
           const OT *bias = PLAIN || partial ? nullptr : static_cast<const OT *>(p.bias[tile.z]);
@@ -959,9 +960,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
           }
           if (!PLAIN && !partial && p.activation != AF2_ACTIVATION_NONE) {
-            if (keep) {  // the slopes, through the first block
-              if (lane == 0) bulk_wait_read_all();
-              __syncwarp();
+            if (keep) {  // the slopes: f32 along each lane's row, or 16 bits through the first block
+              if (staged) {
+                if (lane == 0) bulk_wait_read_all();
+                __syncwarp();
+              }
               with_activation(p.activation, [&](auto act) {
                 constexpr int ACT = decltype(act)::value;
 #pragma unroll
@@ -974,15 +977,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     y[8 * c + 2 * i] = v2.x;
                     y[8 * c + 2 * i + 1] = v2.y;
                   }
-                  *piece16(block, lane, c) = make_uint4(Factor<OT>::slope(s[0]), Factor<OT>::slope(s[1]),
-                                                        Factor<OT>::slope(s[2]), Factor<OT>::slope(s[3]));
+                  if constexpr (std::is_same<OT, __nv_bfloat16>::value) {
+                    *piece16(block, lane, c) = make_uint4(Factor<OT>::slope(s[0]), Factor<OT>::slope(s[1]),
+                                                          Factor<OT>::slope(s[2]), Factor<OT>::slope(s[3]));
+                  } else if (m < p.m) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[2 * i] = __float_as_uint(s[i].x), w[2 * i + 1] = __float_as_uint(s[i].y);
+                    store_sector(p.saved_f32 + m * p.saved_pitch + c0 + 8 * c, w);
+                  }
                 }
               });
-              fence_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_3d(&maps.half, block_addr, c0, r0, 0);
-                bulk_commit();
+              if (staged) {
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  tma_store_3d(&maps.half, block_addr, c0, r0, 0);
+                  bulk_commit();
+                }
               }
             } else {
               with_activation(p.activation, [&](auto act) {
@@ -1010,7 +1022,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             continue;
           }
           // the block that the result leaves from, with the residual in it where there is one
-          const uint32_t at = 2048u * (keep || lane_residual ? 1 : tma_residual ? loads & 1 : stores++ & 1);
+          const uint32_t at = 2048u * (staged || lane_residual ? 1 : tma_residual ? loads & 1 : stores++ & 1);
           uint8_t *const dst = block + at;
           if (tma_residual) {
             ok = warp_wait(load(ew, loads & 1), (loads >> 1) & 1, abort_flag, launch.err, kErrWaitEpilogue);
@@ -1018,7 +1030,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               if (lane == 0) {
                 mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
                 ++loads;
-                if (!keep && b + step < end) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
+                if (!staged && b + step < end) mbar_wait_drain(load(ew, loads & 1), (loads >> 1) & 1, launch.err);
               }
               break;
             }
@@ -1061,7 +1073,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                  p.out_stride, rows, cols, lane);
             __syncwarp();
           }
-          if (tma_residual && keep && b + step < end) fetch(b + step, loads);
+          if (tma_residual && staged && b + step < end) fetch(b + step, loads);
           if (lane_residual && b + step < end) bring(b + step);
         }
         }
@@ -1161,11 +1173,12 @@ __device__ __forceinline__ void reduce(const ReduceArgs &p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j >= cols) break;
-      if constexpr (sizeof(OT) == 2) {
+      if constexpr (std::is_same<OT, __nv_bfloat16>::value) {
         if (p.saved_half)
           p.saved_half[m * p.saved_pitch + c0 + j] = static_cast<uint16_t>(Factor<OT>::slope(f2(slope[j])));
+      } else {
+        if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c0 + j] = slope[j];
       }
-      if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c0 + j] = slope[j];
       out[j] = from_f32<OT>(y[j] + r[j]);
     }
   }
