@@ -254,7 +254,7 @@ __device__ __forceinline__ void slopes8(const Raw8<Kept<T>> &r, float (&x)[8]) {
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 v = Factor<T>::slope_value(r.w[i]);
+      const float2 v = slope_values(r.w[i]);
       x[2 * i] = v.x;
       x[2 * i + 1] = v.y;
     }
@@ -297,9 +297,6 @@ __global__ void __launch_bounds__(256) dense_slope_kernel(const T *dy, int64_t d
         store_operand8<T>(dz, r * dz_pitch + c, dz_piece, d);
       });
 }
-
-// Whether `count` saved factors are kept in f32 (SavedPlanes).
-bool planes_are_f32(int dtype, int count) { return dtype == AF2_F32 || (dtype == AF2_F16 && count == 1); }
 
 // ---- one pass of a layer --------------------------------------------------------------
 
@@ -398,7 +395,7 @@ class Pass {
     SavedPlanes s;
     s.pitch = saved_pitch(width);
     s.stride = rows * s.pitch;
-    if (planes_are_f32(dtype_, count)) {
+    if (dtype_ != AF2_BF16) {
       s.f32 = static_cast<float *>(saved);
     } else {
       s.half = static_cast<uint16_t *>(saved);
@@ -500,7 +497,7 @@ class Pass {
 
 uint64_t planes_bytes(int64_t rows, int64_t width, int dtype, int count) {
   const uint64_t n = static_cast<uint64_t>(count) * rows * saved_pitch(width);
-  if (planes_are_f32(dtype, count)) return part(4 * n);
+  if (dtype != AF2_BF16) return part(4 * n);
   return part(2 * n) + (count > 1 ? part(align_up(rows, 32) * saved_pitch(width) / 8) : 0);
 }
 uint64_t hidden_bytes(int64_t rows, int64_t hidden, int dtype) {

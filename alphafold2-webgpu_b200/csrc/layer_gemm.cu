@@ -58,17 +58,20 @@ constexpr int kPairs = 74;  // CTA pairs of a B200; only the choice of tiles and
 enum Kind { kOut, kOutSave, kOutRows, kProducts, kGate, kGateSave, kGateBackward };
 
 // Stages of the operand ring and bytes of one epilogue warp's staging: 32 x 32 blocks of 16 bits
-// (2 KB), two of them (GateBackward: one of each factor); three where h and two factors leave
+// (2 KB), two of them (GateBackward: one of each factor); three where h and two bf16 factors leave
 // together, paid for with a stage.
 // f32: a stage has a step's three terms, A's [3][128 x 32] and B's behind them; the staged blocks
 // are 32 x 16.
-template <int KIND, int BN, bool F32>
+template <typename T>
+constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+template <int KIND, int BN, typename OT>
 struct Shape {
+  static constexpr bool F32 = sizeof(OT) == 4;
   static constexpr int STEP = F32 ? 32 : BK;
   static constexpr uint32_t A_TERM = BM * STEP * 2, B_TERM = (BN / 2) * STEP * 2;
   static constexpr uint32_t OFF_B = (F32 ? 3 : 1) * A_TERM;
   static constexpr uint32_t STAGE_BYTES = OFF_B + (F32 ? 3 : 1) * B_TERM;
-  static constexpr uint32_t SLOT_BYTES = KIND == kGateSave && !F32 ? 6144 : 4096;
+  static constexpr uint32_t SLOT_BYTES = KIND == kGateSave && kBf16<OT> ? 6144 : 4096;
   static constexpr int STAGES = (229376 - EPI_WARPS * SLOT_BYTES) / STAGE_BYTES;
   static constexpr uint32_t OFF_STAGE = STAGES * STAGE_BYTES;
   static constexpr uint32_t OFF_BAR = OFF_STAGE + EPI_WARPS * SLOT_BYTES;
@@ -305,7 +308,7 @@ template <int KIND, typename OT, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     layer_gemm_kernel(const __grid_constant__ Launch<KIND == kProducts ? kMaxProducts : 1> launch) {
   constexpr int LIMIT = KIND == kProducts ? kMaxProducts : 1;
-  using S = Shape<KIND, BN, sizeof(OT) == 4>;
+  using S = Shape<KIND, BN, OT>;
   constexpr bool GATE = KIND == kGate || KIND == kGateSave;
   constexpr bool F32 = sizeof(OT) == 4;
   constexpr int STAGES = S::STAGES;
@@ -613,6 +616,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           for (int i = 0; i < 16; ++i) sums[i] = sums[16 + i];
         }
         if (!ok) break;
+      } else if constexpr (KIND == kGateBackward && !kBf16<OT>) {
+        // f16: dg = dh p and dv = dh a with the saved factors p = v act'(g) and a = act(g) in f32, 16 columns at
+        // a time: the factors come into the warp's blocks, dg and dv leave from each lane along its row.
+        auto fetch = [&](int c) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(load(ew, 0), 4096);
+            tma_load_3d(block_addr, &maps.half, load(ew, 0), c, r0, 0);
+            tma_load_3d(block_addr + 2048, &maps.half, load(ew, 0), c, r0, 1);
+          }
+        };
+        if (first < end) fetch(n0 + first * 32);
+        if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) {
+          if (first < end && lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, launch.err);
+          break;
+        }
+        tc_fence_after();
+        int half = 0;
+#pragma unroll 1
+        for (int b = first; b < end;) {
+          const int at = b * 32 + 16 * half, c0 = n0 + at;
+          uint32_t dh[16];
+          tmem_ld16(taddr + at, dh);
+          ok = warp_wait(load(ew, 0), loads & 1, abort_flag, launch.err, kErrWaitEpilogue);
+          if (!ok) {
+            if (lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, launch.err);
+            break;
+          }
+          ++loads;
+          float d[32];  // p and a, then dg and dv
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float4 u = *reinterpret_cast<const float4 *>(piece16(block + (c >> 2) * 2048, lane, c & 3));
+            d[4 * c] = u.x, d[4 * c + 1] = u.y, d[4 * c + 2] = u.z, d[4 * c + 3] = u.w;
+          }
+          fence_async_smem();
+          __syncwarp();  // every lane has read p and a
+          if (half == 0 && c0 + 16 < p.n) {
+            half = 1;
+          } else {
+            half = 0;
+            b += step;
+          }
+          if (b < end) fetch(n0 + b * 32 + 16 * half);
+          tmem_ld_wait();
+#pragma unroll
+          for (int set = 0; set < 2; ++set) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float *x = d + 16 * set + 2 * i;
+              const float2 f = f2mul(make_float2(x[0], x[1]),
+                                     make_float2(__uint_as_float(dh[2 * i]), __uint_as_float(dh[2 * i + 1])));
+              x[0] = f.x, x[1] = f.y;
+              w[i] = pack2_t<OT>(f.x, f.y);
+            }
+            if (m < p.m) store_sector(static_cast<OT *>(p.out[set]) + m * p.out_stride + c0, w);
+          }
+          if (p.column_partial) {
+            const float sum = lane_sums(d, lane);
+            p.column_partial[(static_cast<int64_t>(r0 >> 5) * 2 + (lane >> 4)) * p.saved_pitch + c0 + (lane & 15)] = sum;
+          }
+        }
+        if (!ok) break;
       } else if constexpr (KIND == kGateBackward) {
         // dg = dh p and dv = dh a with the saved factors p = v act'(g) and a = act(g).  A block's
         // factors come into the warp's two blocks and the products leave from the same place.
@@ -645,14 +711,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             float d[32];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {  // 8 columns each
-              const float scale = Factor<OT>::scale((scales >> (16 * plane + 8 * (c >> 1))) & 0xffu);
+              const float scale = factor_scale((scales >> (16 * plane + 8 * (c >> 1))) & 0xffu);
               uint4 *piece = piece16(block + plane * 2048, lane, c);
               const uint4 u = *piece;
               uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float2 dh = make_float2(__uint_as_float(v[8 * c + 2 * i]), __uint_as_float(v[8 * c + 2 * i + 1]));
-                const float2 f = f2mul(Factor<OT>::value(w[i], scale), dh);
+                const float2 f = f2mul(factor_values(w[i], scale), dh);
                 w[i] = pack2_t<OT>(f.x, f.y);
                 d[8 * c + 2 * i] = f.x;
                 d[8 * c + 2 * i + 1] = f.y;
@@ -676,6 +742,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         if (!ok) break;
       } else if constexpr (GATE) {
         // h = act(g) v; columns [0, BN / 2) of the accumulator are g, the others v
+        constexpr bool CODES = KIND == kGateSave && kBf16<OT>;  // factors leave through blocks of their own
         if (!warp_wait(acc_full(buf), acc_phase, abort_flag, launch.err, kErrWaitEpilogue)) break;
         tc_fence_after();
         if constexpr (F32) {
@@ -727,7 +794,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll 1
         for (int b = first; b < end; b += step) {
           const int c0 = n0 + b * 32;
-          const uint32_t at = KIND == kGateSave ? 0 : (stores++ & 1) * 2048;
+          const uint32_t at = CODES ? 0 : (stores++ & 1) * 2048;
           uint32_t scales = 0;
 #pragma unroll
           for (int part = 0; part < 2; ++part) {  // 16 columns each
@@ -756,13 +823,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 const float2 hz = f2mul(af[i], vz);
                 h[i] = pack2_t<OT>(hz.x, hz.y);
               }
-              if constexpr (KIND == kGateSave)
-                scales |= Factor<OT>::block(pf, pw) << (8 * part) | Factor<OT>::block(af, aw) << (16 + 8 * part);
+              if constexpr (CODES) {
+                scales |= factor_block(pf, pw) << (8 * part) | factor_block(af, aw) << (16 + 8 * part);
+              } else if constexpr (KIND == kGateSave) {  // f32, from each lane along its row
+                if (m < p.m)
+#pragma unroll
+                  for (int set = 0; set < 2; ++set)
+#pragma unroll
+                    for (int c = 0; c < 8; c += 4) {
+                      const float2 *f = (set ? af : pf) + c;
+                      uint32_t w[8];
+#pragma unroll
+                      for (int i = 0; i < 4; ++i) w[2 * i] = __float_as_uint(f[i].x), w[2 * i + 1] = __float_as_uint(f[i].y);
+                      store_sector(p.saved_f32 + set * p.saved_stride + m * p.saved_pitch + c0 + part * 16 + 2 * c, w);
+                    }
+              }
             });
             if (part == 0) {
               // the blocks are free once what left from them before has been read
               if (lane == 0) {
-                if (KIND == kGateSave)
+                if (CODES)
                   bulk_wait_read_all();
                 else
                   bulk_wait_read_but_one();
@@ -773,7 +853,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             for (int c = 0; c < 2; ++c) {
               const int pc = part * 2 + c;
               *piece16(block + at, lane, pc) = make_uint4(h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
-              if constexpr (KIND == kGateSave) {
+              if constexpr (CODES) {
                 *piece16(block + 2048, lane, pc) = make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]);
                 *piece16(block + 4096, lane, pc) = make_uint4(aw[4 * c], aw[4 * c + 1], aw[4 * c + 2], aw[4 * c + 3]);
               }
@@ -783,13 +863,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           __syncwarp();
           if (lane == 0) {
             tma_store_3d(&maps.out[0], block_addr + at, c0, r0, 0);
-            if constexpr (KIND == kGateSave) {
+            if constexpr (CODES) {
               tma_store_3d(&maps.half, block_addr + 2048, c0, r0, 0);
               tma_store_3d(&maps.half, block_addr + 4096, c0, r0, 1);
             }
             bulk_commit();
           }
-          if constexpr (KIND == kGateSave) p.saved_scale[(c0 >> 5) * p.scale_rows + m] = scales;
+          if constexpr (CODES) p.saved_scale[(c0 >> 5) * p.scale_rows + m] = scales;
         }
       } else {
         // out = act(acc + bias) (+ residual)
@@ -803,7 +883,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         // turn, the second where the first holds slopes (f32: the two halves of the warp's only block of
         // columns).
         const bool keep = (KIND == kOutSave || KIND == kOutRows) && p.save;
-        const bool staged = keep && std::is_same<OT, __nv_bfloat16>::value;  // (f32 slopes leave from each lane)
+        const bool staged = keep && kBf16<OT>;  // (f32 slopes leave from each lane)
         auto fetch = [&](int b, int at) {
           if (lane == 0) {
             bulk_wait_read_all();
@@ -977,9 +1057,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     y[8 * c + 2 * i] = v2.x;
                     y[8 * c + 2 * i + 1] = v2.y;
                   }
-                  if constexpr (std::is_same<OT, __nv_bfloat16>::value) {
-                    *piece16(block, lane, c) = make_uint4(Factor<OT>::slope(s[0]), Factor<OT>::slope(s[1]),
-                                                          Factor<OT>::slope(s[2]), Factor<OT>::slope(s[3]));
+                  if constexpr (kBf16<OT>) {
+                    *piece16(block, lane, c) = make_uint4(slope_codes(s[0]), slope_codes(s[1]),
+                                                          slope_codes(s[2]), slope_codes(s[3]));
                   } else if (m < p.m) {
                     uint32_t w[8];
 #pragma unroll
@@ -1173,9 +1253,9 @@ __device__ __forceinline__ void reduce(const ReduceArgs &p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j >= cols) break;
-      if constexpr (std::is_same<OT, __nv_bfloat16>::value) {
+      if constexpr (kBf16<OT>) {
         if (p.saved_half)
-          p.saved_half[m * p.saved_pitch + c0 + j] = static_cast<uint16_t>(Factor<OT>::slope(f2(slope[j])));
+          p.saved_half[m * p.saved_pitch + c0 + j] = static_cast<uint16_t>(slope_codes(f2(slope[j])));
       } else {
         if (p.saved_f32) p.saved_f32[m * p.saved_pitch + c0 + j] = slope[j];
       }
@@ -1250,7 +1330,7 @@ int launch_pairs(const af2_ctx *ctx, int tiles) { return std::min(tiles, std::ma
 
 template <int KIND, typename OT, int BN>
 af2_status launch(af2_ctx *ctx, Launch<KIND == kProducts ? kMaxProducts : 1> &l, cudaStream_t stream) {
-  constexpr uint32_t smem = Shape<KIND, BN, sizeof(OT) == 4>::BYTES;
+  constexpr uint32_t smem = Shape<KIND, BN, OT>::BYTES;
   auto kernel = layer_gemm_kernel<KIND, OT, BN>;
   static std::atomic<uint64_t> allowed{0};  // devices on which this kernel has its shared memory
   const uint64_t bit = uint64_t(1) << (ctx->device & 63);
@@ -1590,8 +1670,9 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
       if (g.bias[i] && reinterpret_cast<uintptr_t>(g.bias[i]) % 16 != 0) p.vector_bias = 0;
       if (i < outs && !aligned16(g.out[i], g.out_stride, out_bytes)) p.tma_out = 0;
     }
-    const bool terms = g.epilogue != kEpilogueOut && out_bytes == 4;  // written by the lanes
-    if (p.tma_out && !terms)
+    const bool by_lanes = g.epilogue == kEpilogueGateBackward ? g.saved.f32 != nullptr
+                                                               : g.epilogue == kEpilogueGate && out_bytes == 4;
+    if (p.tma_out && !by_lanes)
       for (int i = 0; i < outs; ++i)
         maps_ok &= layer_map_3d(ctx, &maps.out[i], map_type(g.out_dtype), g.out[i], g.n, g.m, 1, g.out_stride * out_bytes,
                                  g.out_stride * out_bytes, out_bytes == 4 ? 16 : 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -1605,7 +1686,7 @@ af2_status describe(af2_ctx *ctx, const LayerGemm &g, int64_t first_tile, Produc
       maps_ok &= layer_map_3d(ctx, &maps.half, CU_TENSOR_MAP_DATA_TYPE_UINT16, g.saved.half, g.saved.pitch, g.m,
                                g.epilogue == kEpilogueOut ? 1 : 2, g.saved.pitch * 2, g.saved.stride * 2, 32, 32, 1,
                                CU_TENSOR_MAP_SWIZZLE_64B);
-    if (g.epilogue == kEpilogueGateBackward && out_bytes == 4)
+    if (g.epilogue == kEpilogueGateBackward && g.saved.f32)
       maps_ok &= layer_map_3d(ctx, &maps.half, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, g.saved.f32, g.n, g.m, 2, g.saved.pitch * 4,
                                g.saved.stride * 4, 16, 32, 1, CU_TENSOR_MAP_SWIZZLE_64B);
     p.column_partial = g.column_partial;
@@ -1654,11 +1735,13 @@ af2_status layer_gemm_launch(af2_ctx *ctx, const LayerGemm *g, int count, cudaSt
       if (g->epilogue == kEpilogueGateBackward)
         return dtype == AF2_F32 ? launch_bn<kGateBackward, float>(ctx, bn, l, stream)
                                 : launch_16<kGateBackward>(ctx, dtype, bn, l, stream);
-      if (g->epilogue == kEpilogueGate)
-        return dtype == AF2_F32 ? (g->saved.f32 ? launch_bn<kGateSave, float>(ctx, bn, l, stream)
-                                                : launch_bn<kGate, float>(ctx, bn, l, stream))
-               : g->saved.half  ? launch_16<kGateSave>(ctx, dtype, bn, l, stream)
-                             : launch_16<kGate>(ctx, dtype, bn, l, stream);
+      if (g->epilogue == kEpilogueGate) {
+        const bool save = l.product[0].args.save;
+        return dtype == AF2_F32 ? (save ? launch_bn<kGateSave, float>(ctx, bn, l, stream)
+                                        : launch_bn<kGate, float>(ctx, bn, l, stream))
+               : save ? launch_16<kGateSave>(ctx, dtype, bn, l, stream)
+                      : launch_16<kGate>(ctx, dtype, bn, l, stream);
+      }
       const Args &p = l.product[0].args;
       auto out = [&](auto kind) {
         constexpr int KIND = decltype(kind)::value;

@@ -24,7 +24,7 @@ enum GemmEpilogue {
 };
 
 // Factors kept for the backward pass, rows of `pitch` elements; the second factor's plane `stride`
-// elements after the first's.  The f32 type, and f16 for a dense layer's slopes, keep f32 in `f32`.  Else 16 bits
+// elements after the first's.  f32 and f16 tensors keep f32 in `f32`.  bf16 ones keep 16 bits
 // (layer_factor.cuh) in `half`; the gated transition's factors, of any size, with an exponent byte for
 // every 16 columns of a row, four of them (two factors x two halves) as a word per row and 32 columns in
 // `scale` [pitch / 32][scale_rows].

@@ -314,3 +314,32 @@ def test_slopes_element_by_element(device, rows, width, scale, act, low, high, d
     allowed = (ref.ROUNDOFF[dtype] + kept + 2.0**-18) * slope.abs() + 2.0**-16 * terms
     allowed = scale * (allowed + least) + (2.0**-25 if dtype == F16 else 0.0)
     assert bool((err <= allowed).all()), (err / allowed).max().item()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,width", [(4, 64), (700, 64), (3000, 77), (1000, 264)])
+@pytest.mark.parametrize("outlier", [1.0, 300.0, 4096.0])
+def test_factors_beside_outliers_element_by_element(device, rows, width, outlier, dtype):
+    """The gated transition's two factors in every column, one of which in eight is `outlier` times the
+    others: through identity weights dx is dg, or dv.  Their products are rounded once, the activations'
+    arithmetic is within 2^-16 of the terms, and bf16 keeps a factor to 2^-11."""
+    rounded = ref.ROUNDOFF[dtype] + 2.0**-18 + (2.0**-11 if dtype == BF16 else 0.0)
+    tiny = 2.0**-25 if dtype == F16 else 0.0
+    x, w = bare_gate(rows, width, dtype, -8.0, 5.0)
+    d_out = torch.full_like(x, 0.75)
+    size = torch.ones(width, device="cuda").to(dtype)
+    size[::8] = outlier
+    w["valueBias"] = size  # v
+    _, saved = af2cuda.encode_gated_transition_tensors(device, x, w, save=True)
+    got = af2cuda.encode_gated_transition_backward_tensors(device, d_out, x, w, saved=saved)["x"]
+    slope, terms = exact_slope("silu", x.double())
+    want = 0.75 * size.double() * slope
+    allowed = rounded * want.abs() + 2.0**-16 * 0.75 * size.double() * terms + tiny
+    assert bool(((got.double() - want).abs() <= allowed).all()), "dg"
+    # a = the gate's bias, v = x
+    w = {"gateWeight": torch.zeros_like(w["gateWeight"]), "gateBias": size / 3, "valueWeight": w["gateWeight"],
+         "outputWeight": w["outputWeight"]}
+    _, saved = af2cuda.encode_gated_transition_tensors(device, x, w, activation="none", save=True)
+    got = af2cuda.encode_gated_transition_backward_tensors(device, d_out, x, w, saved=saved, activation="none")["x"]
+    want = 0.75 * (size / 3).double().expand_as(got)
+    assert bool(((got.double() - want).abs() <= rounded * want.abs() + tiny).all()), "dv"
