@@ -8,8 +8,12 @@
 //
 // Two elements at a time, because the epilogues that call it are bound by the
 // multi-function unit and by issue slots.  Two forms: FAST = false, for f32
-// tensors, within a few units of f32's last place; FAST = true, for 16-bit ones,
-// relative error below 2^-16 where the value matters to them.
+// tensors, within some ten units of f32's last place, on the negative side too;
+// FAST = true, for 16-bit ones, relative error below 2^-16 where the value
+// matters to them.
+//   - f32: an exponential's argument is a rounded product, whose error grows with it
+//     (|z| 2^-24 of e^-z, z^2 2^-24 of e^(-z^2 / 2)): fma gives the product's
+//     rest, and the exponential is multiplied by 1 + ln 2 of that.
 //   - FAST: two sigmoids share one reciprocal: with d = 1 + e^-z, 1 / d0 =
 //     d1 / (d0 d1).  The exponential is held below 2^63 so that the product cannot
 //     overflow, and 2^-62 is taken off the sigmoid, with 0 as the least: far out it
@@ -49,11 +53,31 @@ __device__ __forceinline__ float2 sigmoid2_fast(float2 z) {
   return shared_reciprocal(f2add(make_float2(ex2_approx(fminf(x.x, 63.f)), ex2_approx(fminf(x.y, 63.f))), f2(1.f)));
 }
 
+// 2^(x - over), `over` within x's rounding (none where x is out of f32's range of powers).
+__device__ __forceinline__ float ex2_less(float x, float over) {
+  return ex2_approx(x) * fmaf(fabsf(x) < 160.f ? over : 0.f, -0.69314718f, 1.f);
+}
+constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.9259630e-8f;  // and what its rounding left
+
+// The sigmoids of two values to f32's accuracy.
+__device__ __forceinline__ float2 sigmoid2_f32(float2 z) {
+  const float2 x = f2mul(z, f2(-kLog2e));
+  const float2 over = f2fma(z, f2(kLog2eRest), f2fma(z, f2(kLog2e), x));
+  return make_float2(rcp_approx(1.f + ex2_less(x.x, over.x)), rcp_approx(1.f + ex2_less(x.y, over.y)));
+}
+
 // Phi and, for the slope, e^(-z^2 / 2).
 template <bool FAST>
 __device__ __forceinline__ float2 normal_cdf2(float2 z, float2 &e) {
-  const float2 arg = f2mul(f2mul(z, z), f2(-0.72134752044448170f));
-  e = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
+  const float2 square = f2mul(z, z), arg = f2mul(square, f2(-kLog2e / 2));
+  if constexpr (FAST) {
+    e = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
+  } else {
+    float2 over = f2fma(square, f2(kLog2e / 2), arg);
+    over = f2fma(square, f2(kLog2eRest / 2), over);
+    over = f2fma(make_float2(fmaf(z.x, z.x, -square.x), fmaf(z.y, z.y, -square.y)), f2(kLog2e / 2), over);
+    e = make_float2(ex2_less(arg.x, over.x), ex2_less(arg.y, over.y));
+  }
   const float2 d = f2fma(make_float2(fabsf(z.x), fabsf(z.y)), f2(FAST ? 0.31f : 0.265f), f2(1.f));
   const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
   float2 q;
@@ -83,9 +107,9 @@ __device__ __forceinline__ float relu(float z) { return z > 0.f ? z : (z != z ? 
 template <int ACT, bool FAST>
 __device__ __forceinline__ float2 activate2(float2 z) {
   if constexpr (ACT == AF2_ACTIVATION_RELU) return make_float2(relu(z.x), relu(z.y));
-  if constexpr (ACT == AF2_ACTIVATION_SIGMOID) return make_float2(sigmoidf(z.x), sigmoidf(z.y));
-  if constexpr (ACT == AF2_ACTIVATION_SILU)
-    return f2mul(z, FAST ? sigmoid2_fast(z) : make_float2(sigmoidf(z.x), sigmoidf(z.y)));
+  if constexpr (ACT == AF2_ACTIVATION_SIGMOID)
+    return FAST ? make_float2(sigmoidf(z.x), sigmoidf(z.y)) : sigmoid2_f32(z);
+  if constexpr (ACT == AF2_ACTIVATION_SILU) return f2mul(z, FAST ? sigmoid2_fast(z) : sigmoid2_f32(z));
   if constexpr (ACT == AF2_ACTIVATION_GELU) {
     float2 e;
     return f2mul(z, normal_cdf2<FAST>(z, e));
@@ -108,7 +132,9 @@ __device__ __forceinline__ void activate_slope2(float2 z, float2 &value, float2 
     value = f2mul(z, cdf);
     slope = f2fma(f2mul(z, f2(0.39894228040143268f)), e, cdf);
   } else {
-    const float2 s = FAST && ACT == AF2_ACTIVATION_SILU ? sigmoid2_fast(z) : make_float2(sigmoidf(z.x), sigmoidf(z.y));
+    const float2 s = !FAST                         ? sigmoid2_f32(z)
+                     : ACT == AF2_ACTIVATION_SILU ? sigmoid2_fast(z)
+                                                  : make_float2(sigmoidf(z.x), sigmoidf(z.y));
     const float2 rest = f2fma(s, f2(-1.f), f2(1.f));
     if constexpr (ACT == AF2_ACTIVATION_SIGMOID) {
       value = s;

@@ -343,3 +343,18 @@ def test_factors_beside_outliers_element_by_element(device, rows, width, outlier
     got = af2cuda.encode_gated_transition_backward_tensors(device, d_out, x, w, saved=saved, activation="none")["x"]
     want = 0.75 * (size / 3).double().expand_as(got)
     assert bool(((got.double() - want).abs() <= rounded * want.abs() + tiny).all()), "dv"
+
+
+@pytest.mark.parametrize("act,low,units", [("sigmoid", -60.0, 12), ("silu", -60.0, 13), ("gelu", -12.0, 22)])
+@pytest.mark.parametrize("rows,width", [(4, 64), (700, 64), (3000, 77), (700, 200)])
+def test_f32_activations_element_by_element(device, rows, width, act, low, units):
+    """In units of 2^-24 of the element: the hardware's exponential 4 and reciprocal 2, one for each
+    operation beside them (gelu's polynomial has nine), two for the copies through identity weights."""
+    x, w = bare_gate(rows, width, F32, low, 12.0)
+    want = exact_act(act, x.double())
+    alone = af2cuda.encode_gated_transition_tensors(device, x, w, activation=act)
+    elements_close("y alone", alone, want, units * 2.0**-24, F32)
+    kept, _ = af2cuda.encode_gated_transition_tensors(device, x, w, activation=act, save=True)
+    elements_close("y", kept, want, units * 2.0**-24, F32)
+    d = af2cuda.encode_dense_tensors(device, x, w["gateWeight"], activation=act)
+    elements_close("dense", d, want, units * 2.0**-24, F32)
