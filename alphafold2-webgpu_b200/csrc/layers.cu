@@ -10,6 +10,7 @@
 #include <cmath>
 #include <new>
 #include <string>
+#include <vector>
 
 #include "af2_internal.h"
 
@@ -225,6 +226,42 @@ af2_status check_set(af2_ctx *ctx, const af2_tensor_ref *t, int64_t count, const
       wrong = " is not aligned to its element type";
     if (!wrong.empty())
       return fail(ctx, AF2_ERR_INVALID_ARGUMENT, std::string(what) + " " + std::to_string(i) + wrong);
+  }
+  return AF2_OK;
+}
+
+// What is written overlaps nothing else that is written, and no tensor but, as the same memory, its own:
+// blocks scale their parts of the set in no order.  (Sets come sorted by address more often than not.)
+af2_status check_overlaps(af2_ctx *ctx, const af2_tensor_ref *tensors, const af2_tensor_ref *outputs, int64_t count) {
+  struct Span {
+    uintptr_t begin, end;
+    int64_t index;
+  };
+  auto spans = [&](const af2_tensor_ref *t) {
+    std::vector<Span> s;
+    s.reserve(static_cast<size_t>(count));
+    for (int64_t i = 0; i < count; ++i) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(t[i].data);
+      if (t[i].count > 0) s.push_back({at, at + t[i].count * element_bytes(t[i].dtype), i});
+    }
+    auto before = [](const Span &a, const Span &b) { return a.begin < b.begin; };
+    if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
+    return s;
+  };
+  const std::vector<Span> written = spans(outputs ? outputs : tensors);
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i].begin < written[i - 1].end)
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT,
+                  std::string(outputs ? "outputs " : "tensors ") + std::to_string(written[i - 1].index) + " and " +
+                      std::to_string(written[i].index) + " overlap");
+  if (!outputs) return AF2_OK;
+  size_t first = 0;  // written spans in order do not overlap: their ends are in order too
+  for (const Span &t : spans(tensors)) {
+    while (first < written.size() && written[first].end <= t.begin) ++first;
+    for (size_t i = first; i < written.size() && written[i].begin < t.end; ++i)
+      if (written[i].index != t.index || written[i].begin != t.begin)
+        return fail(ctx, AF2_ERR_INVALID_ARGUMENT,
+                    "output " + std::to_string(written[i].index) + " overlaps tensor " + std::to_string(t.index));
   }
   return AF2_OK;
 }
@@ -469,6 +506,7 @@ static af2_status gradient_call(af2_ctx *ctx, const af2_tensor_ref *tensors, con
           return fail(ctx, AF2_ERR_INVALID_ARGUMENT,
                       "output " + std::to_string(i) + " differs from its tensor in size or type");
     }
+    if (clip && (st = check_overlaps(ctx, tensors, outputs, count)) != AF2_OK) return st;
     if ((st = check_block(ctx, workspace, "workspace")) != AF2_OK) return st;
     cudaSetDevice(ctx->device);
     const cudaStream_t cs = stream_of(ctx, stream);

@@ -759,7 +759,8 @@ AF2_API af2_status af2_gradient_norm(af2_ctx *ctx, const af2_tensor_ref *tensors
  * 1e-6)), computed in f32 and rounded once to the output's type.  outputs:
  * NULL scales in place (and writes nothing when the factor is 1), else
  * `count` refs of the same counts and types, each the same memory as its input or
- * disjoint from every input.  A NaN norm makes every element NaN, an infinite one
+ * disjoint from every input.  What is written may not overlap (a tensor that
+ * occurs twice is refused).  A NaN norm makes every element NaN, an infinite one
  * makes the finite elements zero.  max_norm must be finite and not negative.
  */
 AF2_API af2_status af2_clip_gradients(af2_ctx *ctx, const af2_tensor_ref *tensors, const af2_tensor_ref *outputs,

@@ -358,3 +358,34 @@ def test_f32_activations_element_by_element(device, rows, width, act, low, units
     elements_close("y", kept, want, units * 2.0**-24, F32)
     d = af2cuda.encode_dense_tensors(device, x, w["gateWeight"], activation=act)
     elements_close("dense", d, want, units * 2.0**-24, F32)
+
+
+# ---- sets of tensors ---------------------------------------------------------------------------------
+
+
+def test_overlapping_tensors_are_refused_where_they_are_written(device):
+    """Blocks scale their parts of a set in no order: what two of them would write is refused."""
+    flat = torch.randn(4000, device="cuda")
+    a, b, c = flat[:1000], flat[1000:2500], flat[2500:]
+    clip = af2cuda.encode_clip_gradients_tensors
+    before = flat.clone()
+    for bad in ([a, a], [a, b, a], [flat, c], [c, flat], [a, flat[999:1001]], [b, a, flat[2400:2600]]):
+        with pytest.raises(af2cuda.RangeError, match="overlap"):
+            clip(device, bad, 1.0)
+    with pytest.raises(af2cuda.RangeError, match="overlap"):
+        clip(device, [a, torch.randn(1000, device="cuda")], 1.0, out=[flat[:1000], flat[500:1500]])
+    with pytest.raises(af2cuda.RangeError, match="output 1 overlaps tensor 0"):
+        clip(device, [a, torch.randn(1000, device="cuda")], 1.0, out=[torch.empty(1000, device="cuda"), a])
+    with pytest.raises(af2cuda.RangeError, match="output 0 overlaps tensor 0"):
+        clip(device, [a], 1.0, out=[flat[1:1001]])
+    assert torch.equal(flat, before)
+    # read twice and written apart; in any order; in place by name; nothing at all
+    outs = [torch.empty(1000, device="cuda") for _ in range(2)]
+    norm = clip(device, [a, a], 1.0, out=outs)
+    assert abs(norm.item() - 2**0.5 * before[:1000].double().norm().item()) <= 1e-5 * norm.item()
+    assert torch.equal(outs[0], outs[1])
+    empty = flat[:0]
+    norm = clip(device, [c, empty, a, b, empty], 1.0, out=[c, empty, a, b, empty])
+    assert abs(norm.item() - before.double().norm().item()) <= 1e-5 * norm.item()
+    assert torch.allclose(flat, before / norm, rtol=1e-5)
+    assert abs(af2cuda.encode_gradient_norm_tensors(device, [a, a]).item() - 2**0.5 * a.norm().item()) <= 1e-5
