@@ -175,6 +175,11 @@ long long integer(PyObject *o) {
   if (v == -1 && PyErr_Occurred()) throw Failed();
   return v;
 }
+bool truth(PyObject *o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Failed();
+  return v == 1;
+}
 void *ptr(const at::Tensor *t) { return t ? t->data_ptr() : nullptr; }
 PyObject *wrap(const at::Tensor &t) { return THPVariable_Wrap(t); }
 
@@ -197,7 +202,7 @@ PyObject *dense(PyObject *const *a) {
   const at::Tensor *bias = optional_tensor(a[4], "bias"), *residual = optional_tensor(a[5], "residual"),
                    *given = optional_tensor(a[7], "out"), *workspace = optional_tensor(a[10], "workspace");
   const int act = static_cast<int>(integer(a[6]));
-  const bool save = PyObject_IsTrue(a[8]);
+  const bool save = truth(a[8]);
   if (w.dim() != 2) refuse("weight has shape " + shape_text(w.sizes()) + "; expected (inner, columns)");
   const int64_t inner = w.size(0), columns = w.size(1);
   c.set_type(x);
@@ -245,9 +250,9 @@ PyObject *dense_backward(PyObject *const *a) {
   void *const ws = c.scratch(
       workspace, stream, [&](uint64_t *need) { return entry.dense_workspace_bytes(&shape, c.code, act, 1, need); });
   at::Tensor dx, dw, db;
-  if (PyObject_IsTrue(a[8])) dx = c.make({rows, inner});
-  if (PyObject_IsTrue(a[9])) dw = c.make({inner, columns});
-  if (PyObject_IsTrue(a[6])) db = c.make({columns});
+  if (truth(a[8])) dx = c.make({rows, inner});
+  if (truth(a[9])) dw = c.make({inner, columns});
+  if (truth(a[6])) db = c.make({columns});
   auto at_of = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
   c.done(entry.dense_backward(c.ctx, &shape, c.code, dy.data_ptr(), x.data_ptr(), wp, kept, &o, at_of(dx), at_of(dw),
                               at_of(db), ws, stream));
@@ -302,7 +307,7 @@ PyObject *gated(PyObject *const *a) {
   const at::Tensor *residual = optional_tensor(a[4], "residual"), *given = optional_tensor(a[6], "out"),
                    *workspace = optional_tensor(a[9], "workspace");
   const int act = static_cast<int>(integer(a[5]));
-  const bool save = PyObject_IsTrue(a[7]);
+  const bool save = truth(a[7]);
   c.set_type(x);
   af2_gated_weights w{};
   const GatedTensors g = gated_tensors(c, a[3], &w);

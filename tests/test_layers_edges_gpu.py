@@ -389,3 +389,17 @@ def test_overlapping_tensors_are_refused_where_they_are_written(device):
     assert abs(norm.item() - before.double().norm().item()) <= 1e-5 * norm.item()
     assert torch.allclose(flat, before / norm, rtol=1e-5)
     assert abs(af2cuda.encode_gradient_norm_tensors(device, [a, a]).item() - 2**0.5 * a.norm().item()) <= 1e-5
+
+
+# ---- arguments -----------------------------------------------------------------------------------------
+
+
+def test_options_without_a_truth_value_are_errors(device):
+    """The bias itself where the backward pass asks whether there is one."""
+    d = dense_case(20, 16, 24, BF16, seed=1300)
+    with pytest.raises(RuntimeError, match="[Aa]mbiguous"):
+        af2cuda.encode_dense_backward_tensors(device, d["d_out"], d["x"], d["weight"], bias=d["bias"])
+    with pytest.raises(RuntimeError, match="[Aa]mbiguous"):
+        af2cuda.encode_dense_tensors(device, d["x"], d["weight"], save=d["bias"])
+    got = af2cuda.encode_dense_backward_tensors(device, d["d_out"], d["x"], d["weight"], bias=True)
+    close("bias", got["bias"], d["d_out"].double().sum(0), BF16)
