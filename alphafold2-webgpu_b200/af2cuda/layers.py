@@ -30,6 +30,7 @@ _BOUND = ("af2_dense_saved_bytes", "af2_dense_workspace_bytes", "af2_dense", "af
           "af2_gated_transition_saved_bytes", "af2_gated_transition_workspace_bytes", "af2_gated_transition",
           "af2_gated_transition_backward", "af2_gradient_norm_workspace_bytes", "af2_gradient_norm",
           "af2_clip_gradients")
+_BOTH = ("x", "weight")
 _tensors = None
 
 
@@ -62,6 +63,14 @@ def _activation_code(activation: str) -> int:
     if code is None:
         raise _lib.RangeError(f"activation must be one of {', '.join(ACTIVATIONS)}; received {activation}")
     return code
+
+
+def _needed(need, known) -> set:
+    names = {need} if isinstance(need, str) else set(need)
+    if not names <= set(known):
+        raise _lib.RangeError(f"need names {', '.join(sorted(map(str, names - set(known))))}; "
+                              f"expected some of {', '.join(known)}")
+    return names
 
 
 def _on_stream(tensors, device: Device, stream: int) -> None:
@@ -123,10 +132,12 @@ def encode_dense_tensors(device: Device, x, weight, *, bias=None, residual=None,
 
 
 def encode_dense_backward_tensors(device: Device, d_out, x, weight, *, saved=None, bias: bool = False,
-                                  activation: str = "none", need=("x", "weight"), stream: Optional[int] = None,
+                                  activation: str = "none", need=_BOTH, stream: Optional[int] = None,
                                   workspace=None) -> dict:
     """Gradients of encode_dense_tensors for d_out [rows, columns]: {"x", "weight"}, those of them
     that `need` names, and "bias" with bias=True.  The residual's gradient is d_out itself."""
+    if need is not _BOTH:
+        need = _needed(need, ("x", "weight", "bias") if bias else _BOTH)
     grads = (_tensors or _native()).dense_backward(device.handle.value, device.ordinal, d_out, x, weight, saved, bias,
                                                    _activation_code(activation), "x" in need, "weight" in need,
                                                    -1 if stream is None else stream, workspace)
@@ -153,7 +164,9 @@ def encode_gated_transition_backward_tensors(device: Device, d_out, x, weights: 
                                              activation: str = "silu", need=None, stream: Optional[int] = None,
                                              workspace=None) -> dict:
     """Gradients of encode_gated_transition_tensors for d_out [rows, channels]: "x" and every
-    weight given, by its name, or those that `need` names.  The residual's gradient is d_out itself."""
+    weight given, by its name, or those of them that `need` names.  The residual's gradient is d_out itself."""
+    if need is not None:
+        need = _needed(need, ("x", *GATED_WEIGHTS))
     grads = (_tensors or _native()).gated_backward(device.handle.value, device.ordinal, d_out, x, weights, saved,
                                                    _activation_code(activation), need,
                                                    -1 if stream is None else stream, workspace)

@@ -403,3 +403,16 @@ def test_options_without_a_truth_value_are_errors(device):
         af2cuda.encode_dense_tensors(device, d["x"], d["weight"], save=d["bias"])
     got = af2cuda.encode_dense_backward_tensors(device, d["d_out"], d["x"], d["weight"], bias=True)
     close("bias", got["bias"], d["d_out"].double().sum(0), BF16)
+
+
+def test_one_need_by_its_name(device):
+    d = dense_case(20, 16, 24, BF16, seed=1310)
+    assert list(af2cuda.encode_dense_backward_tensors(device, d["d_out"], d["x"], d["weight"], need="weight")) == ["weight"]
+    got = af2cuda.encode_dense_backward_tensors(device, d["d_out"], d["x"], d["weight"], bias=True, need=["bias", "x"])
+    assert sorted(got) == ["bias", "x"]
+    s = gated_case(20, 16, 24, BF16, seed=1320)
+    _, saved = af2cuda.encode_gated_transition_tensors(device, s["x"], s["weights"], save=True)
+    for need in ("x", "gateBias", ["valueWeight", "outputBias"], iter(["x", "outputWeight"])):
+        names = [need] if isinstance(need, str) else need if isinstance(need, list) else ["x", "outputWeight"]
+        got = af2cuda.encode_gated_transition_backward_tensors(device, s["d_out"], s["x"], s["weights"], saved=saved, need=need)
+        assert sorted(got) == sorted(names)
