@@ -181,6 +181,10 @@ bool truth(PyObject *o) {
   return v == 1;
 }
 void *ptr(const at::Tensor *t) { return t ? t->data_ptr() : nullptr; }
+// A tensor of the caller's was written: what autograd has saved of it shows as stale.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 PyObject *wrap(const at::Tensor &t) { return THPVariable_Wrap(t); }
 
 // (y, saved) or y.
@@ -224,6 +228,7 @@ PyObject *dense(PyObject *const *a) {
       workspace, stream, [&](uint64_t *need) { return entry.dense_workspace_bytes(&shape, c.code, act, 0, need); });
   c.done(entry.dense(c.ctx, &shape, c.code, x.data_ptr(), wp, bp, ptr(residual), &o, y.data_ptr(),
                      bytes ? saved.data_ptr() : nullptr, ws, stream));
+  if (given) written(*given);
   return with_saved(y, saved, save);
 }
 
@@ -327,6 +332,7 @@ PyObject *gated(PyObject *const *a) {
       workspace, stream, [&](uint64_t *need) { return entry.gated_workspace_bytes(&shape, c.code, 0, need); });
   c.done(entry.gated(c.ctx, &shape, c.code, x.data_ptr(), &w, ptr(residual), &o, y.data_ptr(),
                      bytes ? saved.data_ptr() : nullptr, ws, stream));
+  if (given) written(*given);
   return with_saved(y, saved, save);
 }
 
@@ -416,6 +422,8 @@ PyObject *gradients(PyObject *const *a) {
     const double limit = PyFloat_AsDouble(a[4]);
     if (PyErr_Occurred()) throw Failed();
     c.done(entry.clip_gradients(c.ctx, in.data(), a[3] != Py_None ? out.data() : nullptr, n, limit, np, ws, stream));
+    PyObject *list = a[a[3] != Py_None ? 3 : 2];
+    for (Py_ssize_t i = 0; i < static_cast<Py_ssize_t>(n); ++i) written(THPVariable_Unpack(PyList_GET_ITEM(list, i)));
   }
   return wrap(norm);
 }

@@ -30,7 +30,8 @@ def encode_gradient_norm_tensors(device: Device, gradients: Sequence, *, stream:
 def encode_clip_gradients_tensors(device: Device, gradients: Sequence, max_norm: float, *, out: Optional[Sequence] = None,
                                   stream: Optional[int] = None, workspace=None):
     """Scales every tensor by min(1, max_norm / (norm + 1e-6)), in place or into the tensors of
-    `out` (same sizes and types), and returns the norm before clipping, an f32 scalar on the device."""
+    `out` (same sizes and types), and returns the norm before clipping, an f32 scalar on the device.
+    Autograd does not record it.  Tensors that overlap where they are written are refused."""
     max_norm = float(max_norm)
     if not (max_norm >= 0 and math.isfinite(max_norm)):
         raise _lib.RangeError(f"max_norm must be finite and not negative; received {max_norm}")

@@ -10,6 +10,8 @@ Activations, residuals and outputs are [rows, width] with any row stride of at
 least the width.  Calls run on torch's current stream unless ``stream`` names
 another (a raw CUDA stream handle; 0 is the device context's own stream); a
 named stream does not wait for the current one, so the inputs must be ready on it.
+Autograd does not record the calls: results are detached, also from tensors that
+require gradients, and the backward passes are called by hand.
 
 No counterpart in the reference, whose weights are fixed and whose transition
 is ReLU (src/evoformer/transition.ts); the weights' names follow its

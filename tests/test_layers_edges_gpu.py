@@ -416,3 +416,29 @@ def test_one_need_by_its_name(device):
         names = [need] if isinstance(need, str) else need if isinstance(need, list) else ["x", "outputWeight"]
         got = af2cuda.encode_gated_transition_backward_tensors(device, s["d_out"], s["x"], s["weights"], saved=saved, need=need)
         assert sorted(got) == sorted(names)
+
+
+def test_written_tensors_show_it_to_autograd(device):
+    """What a call writes counts as written in place: a backward pass of torch's that saved it refuses."""
+    d = dense_case(20, 16, 24, F32, seed=1330)
+    out = torch.ones(20, 24, device="cuda")
+    factor = torch.ones(20, 24, device="cuda", requires_grad=True)
+    product = (out * factor).sum()
+    af2cuda.encode_dense_tensors(device, d["x"], d["weight"], out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    s = gated_case(20, 16, 24, F32, seed=1340)
+    residual = s["residual"].clone()
+    version = residual._version
+    af2cuda.encode_gated_transition_tensors(device, s["x"], s["weights"], residual=residual, out=residual)
+    assert residual._version > version
+    a, b, c = (torch.ones(50, device="cuda") for _ in range(3))
+    versions = [t._version for t in (a, b, c)]
+    af2cuda.encode_clip_gradients_tensors(device, [a], 1.0, out=[b])
+    af2cuda.encode_clip_gradients_tensors(device, [c], 1.0)
+    assert [t._version for t in (a, b, c)] == [versions[0], versions[1] + 1, versions[2] + 1]
+    with torch.inference_mode():
+        t = torch.ones(20, 24, device="cuda")
+        af2cuda.encode_dense_tensors(device, d["x"], d["weight"], out=t)
+    af2cuda.encode_dense_tensors(device, d["x"], d["weight"], out=t)
+    close("y", t, ref.dense(d["x"], d["weight"], None, None, "none")["y"], F32)
