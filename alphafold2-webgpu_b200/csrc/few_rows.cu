@@ -219,9 +219,7 @@ af2_status few_rows_launch(af2_ctx *ctx, const FewRows &f, cudaStream_t stream) 
          f.out_stride, static_cast<int>(f.rows), static_cast<int>(f.inner), static_cast<int>(f.columns), f.activation, 1,
          f.follows};
   const int blocks = (p.columns + COLS - 1) / COLS;
-  // the depth over more blocks while the SMs are not all busy and each keeps 128 weight rows
-  const int groups = static_cast<int>((f.rows + 3) / 4);
-  while (p.splits < 8 && blocks * groups * p.splits * 2 <= ctx->sm_count && p.inner / (p.splits * 2) >= 128) p.splits *= 2;
+  p.splits = few_rows_splits((f.rows + 3) / 4 * blocks, f.inner, ctx->sm_count);
   LaunchScope scope(ctx, stream, kProfLayerGemm);
   cudaError_t e = cudaSuccess;
   with_element(f.dtype, [&](auto *tag) {

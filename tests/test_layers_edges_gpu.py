@@ -442,3 +442,18 @@ def test_written_tensors_show_it_to_autograd(device):
         af2cuda.encode_dense_tensors(device, d["x"], d["weight"], out=t)
     af2cuda.encode_dense_tensors(device, d["x"], d["weight"], out=t)
     close("y", t, ref.dense(d["x"], d["weight"], None, None, "none")["y"], F32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,inner,columns", [(2, 8192, 512), (16, 4096, 1024), (16, 1024, 1024), (40, 20001, 33),
+                                                (200, 16384, 32), (256, 256, 32), (5, 40, 5000)])
+def test_dense_layers_deep_and_wide_for_few_rows(device, rows, inner, columns, dtype):
+    """On both sides of the choice between the kernels."""
+    d = dense_case(rows, inner, columns, dtype, seed=1350)
+    y = af2cuda.encode_dense_tensors(device, d["x"], d["weight"], bias=d["bias"], residual=d["residual"], activation="silu")
+    close("y", y, ref.dense(d["x"], d["weight"], d["bias"], d["residual"], "silu")["y"], dtype)
+    size = af2cuda.dense_workspace_bytes(rows, inner, columns, dtype, "silu")
+    scratch, intact = guarded(size)
+    y = af2cuda.encode_dense_tensors(device, d["x"], d["weight"], activation="silu", workspace=scratch)
+    close("y", y, ref.dense(d["x"], d["weight"], None, None, "silu")["y"], dtype)
+    assert intact()

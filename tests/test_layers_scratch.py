@@ -1,6 +1,6 @@
 """CPU tests of the learned layers' scratch: the size queries against what the passes count
 (tests/layer_scratch_check.cpp, linked with the library's objects), the order of its uses against
-fakes (tests/scratch_order_check.cpp)."""
+fakes (tests/scratch_order_check.cpp), and the choice between kernels (tests/few_rows_check.cpp)."""
 import importlib.util
 import shutil
 import subprocess
@@ -39,6 +39,17 @@ def test_order_between_uses_of_the_scratch(tmp_path):
     exe = tmp_path / "scratch_order_check"
     subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(PKG / "csrc"), str(ROOT / "tests" / "scratch_order_check.cpp"),
                     "-o", str(exe)], check=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0, res.stdout + res.stderr
+    assert res.stdout.strip() == "ok"
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_choice_of_the_kernel_for_few_rows(tmp_path):
+    cuda = Path(_build_module().nvcc()).resolve().parent.parent
+    exe = tmp_path / "few_rows_check"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(PKG / "csrc"), "-isystem", str(cuda / "include"),
+                    str(ROOT / "tests" / "few_rows_check.cpp"), "-o", str(exe)], check=True)
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert res.returncode == 0, res.stdout + res.stderr
     assert res.stdout.strip() == "ok"
