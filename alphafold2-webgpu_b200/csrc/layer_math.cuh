@@ -2,7 +2,7 @@
 // their slopes, in f32.
 //
 //   relu:    max(z, 0);  1 where z > 0
-//   sigmoid: s;          s (1 - s)            s = 1 / (1 + e^-z)
+//   sigmoid: s;          s (1 - s)            s = 1 / (1 + e^-z), 1 - s = e^-z s
 //   silu:    z s;        s (1 + z (1 - s))
 //   gelu:    z Phi(z);   Phi(z) + z phi(z)    Phi, phi of the standard normal
 //
@@ -59,11 +59,19 @@ __device__ __forceinline__ float ex2_less(float x, float over) {
 }
 constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.9259630e-8f;  // and what its rounding left
 
+// e^-z of two values.
+template <bool FAST>
+__device__ __forceinline__ float2 exp_of_minus(float2 z) {
+  const float2 x = f2mul(z, f2(-kLog2e));
+  if constexpr (FAST) return make_float2(ex2_approx(x.x), ex2_approx(x.y));
+  const float2 over = f2fma(z, f2(kLog2eRest), f2fma(z, f2(kLog2e), x));
+  return make_float2(ex2_less(x.x, over.x), ex2_less(x.y, over.y));
+}
+
 // The sigmoids of two values to f32's accuracy.
 __device__ __forceinline__ float2 sigmoid2_f32(float2 z) {
-  const float2 x = f2mul(z, f2(-kLog2e));
-  const float2 over = f2fma(z, f2(kLog2eRest), f2fma(z, f2(kLog2e), x));
-  return make_float2(rcp_approx(1.f + ex2_less(x.x, over.x)), rcp_approx(1.f + ex2_less(x.y, over.y)));
+  const float2 e = exp_of_minus<false>(z);
+  return make_float2(rcp_approx(1.f + e.x), rcp_approx(1.f + e.y));
 }
 
 // Phi and, for the slope, e^(-z^2 / 2).
@@ -132,16 +140,16 @@ __device__ __forceinline__ void activate_slope2(float2 z, float2 &value, float2 
     value = f2mul(z, cdf);
     slope = f2fma(f2mul(z, f2(0.39894228040143268f)), e, cdf);
   } else {
-    const float2 s = !FAST                         ? sigmoid2_f32(z)
-                     : ACT == AF2_ACTIVATION_SILU ? sigmoid2_fast(z)
-                                                  : make_float2(sigmoidf(z.x), sigmoidf(z.y));
-    const float2 rest = f2fma(s, f2(-1.f), f2(1.f));
     if constexpr (ACT == AF2_ACTIVATION_SIGMOID) {
-      value = s;
-      slope = f2mul(s, rest);
+      const float2 e = exp_of_minus<FAST>(z);
+      value = make_float2(rcp_approx(1.f + e.x), rcp_approx(1.f + e.y));
+      // 1 - s, which cancels where z is large, is e^-z s
+      slope = f2mul(value, make_float2(z.x > 0.f ? e.x * value.x : 1.f - value.x,
+                                       z.y > 0.f ? e.y * value.y : 1.f - value.y));
     } else {
+      const float2 s = FAST ? sigmoid2_fast(z) : sigmoid2_f32(z);
       value = f2mul(z, s);
-      slope = f2mul(s, f2fma(z, rest, f2(1.f)));
+      slope = f2mul(s, f2fma(z, f2fma(s, f2(-1.f), f2(1.f)), f2(1.f)));
     }
   }
 }

@@ -457,3 +457,26 @@ def test_dense_layers_deep_and_wide_for_few_rows(device, rows, inner, columns, d
     y = af2cuda.encode_dense_tensors(device, d["x"], d["weight"], activation="silu", workspace=scratch)
     close("y", y, ref.dense(d["x"], d["weight"], None, None, "silu")["y"], dtype)
     assert intact()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act,low,high", [("sigmoid", 0.0, 24.0), ("sigmoid", -24.0, 0.0), ("silu", -24.0, 24.0),
+                                          ("gelu", -6.0, 6.0)])
+@pytest.mark.parametrize("rows,width", [(700, 64), (3000, 77)])
+def test_slopes_at_both_ends(device, rows, width, act, low, high, dtype):
+    """As test_slopes_element_by_element, for sigmoid's positive side and for f32 too: there the slope's
+    terms are within 24 units of 2^-24."""
+    x, w = bare_gate(rows, width, dtype, low, high)
+    scale = 2.0**14
+    _, saved = af2cuda.encode_dense_tensors(device, x, w["gateWeight"], activation=act, save=True)
+    got = af2cuda.encode_dense_backward_tensors(device, torch.full_like(x, scale), x, w["gateWeight"], saved=saved,
+                                                activation=act)["x"]
+    slope, terms = exact_slope(act, x.double())
+    if act == "sigmoid":
+        terms = slope
+    kept, least = (2.0**-11, 2.0**-39) if dtype == BF16 else (0.0, 0.0)
+    rounded = ref.ROUNDOFF[dtype] + kept + 2.0**-18 if dtype != F32 else 0.0
+    allowed = rounded * slope.abs() + (24 * 2.0**-24 if dtype == F32 else 2.0**-16) * terms + least
+    allowed = scale * allowed + (2.0**-25 if dtype == F16 else 0.0)
+    err = (got.double() - scale * slope).abs()
+    assert bool((err <= allowed).all()), (err / allowed).max().item()
