@@ -482,7 +482,6 @@ class Pass {
   void check(cudaError_t e, const char *what) {
     if (e != cudaSuccess && status == AF2_OK) status = cuda_fail(ctx_, e, what);
   }
-  cudaStream_t stream() const { return stream_; }
 
  private:
   af2_ctx *ctx_;

@@ -640,10 +640,13 @@ AF2_API af2_status af2_linear(af2_ctx *ctx, const af2_linear_shape *shape, const
  * weights are fixed.
  *
  * Arithmetic: 16-bit tensors are multiplied as they are, f32 tensors to f32
- * accuracy; sums, biases, activations and the residual are f32, rounded once
- * to `dtype`.  The hidden activations of a 16-bit gated transition and the
- * gradients at its pre-activations are rounded to `dtype` where they become a
- * product's operand.
+ * accuracy (where one holds an infinity or a NaN, the sums that it enters are
+ * infinite or NaN, which of them may differ between sizes); sums, biases,
+ * activations and the residual are f32, rounded once to `dtype`.  The hidden
+ * activations of a 16-bit gated transition and the gradients at a layer's
+ * pre-activations are rounded to `dtype` where they become a product's
+ * operand.  What a forward pass saves of its activations is f32, for bf16 11
+ * significant bits.
  *
  * rows = 0 is valid: outputs of no rows are not touched, and the gradients of
  * the weights are zero.  Outputs must not overlap inputs, except that out may
