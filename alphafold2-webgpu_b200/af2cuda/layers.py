@@ -151,7 +151,7 @@ def encode_dense_backward_tensors(device: Device, d_out, x, weight, *, saved=Non
 def encode_gated_transition_tensors(device: Device, x, weights: dict, *, residual=None, activation: str = "silu",
                                     out=None, save: bool = False, stream: Optional[int] = None, workspace=None):
     """out = (act(x gateWeight + gateBias) * (x valueWeight + valueBias)) outputWeight + outputBias
-    (+ residual): x, residual and out [rows, channels] (out may be the residual), gateWeight and
+    (+ residual): x, residual and out [rows, channels] (out may be the residual, and x), gateWeight and
     valueWeight [channels, hidden], outputWeight [hidden, channels]; the biases may be absent.
     Returns out, or with save=True (out, saved) for encode_gated_transition_backward_tensors."""
     result = (_tensors or _native()).gated(device.handle.value, device.ordinal, x, weights, residual,

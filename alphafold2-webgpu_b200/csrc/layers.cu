@@ -133,6 +133,49 @@ af2_status check_block(af2_ctx *ctx, const void *ptr, const char *name) {
   return AF2_OK;
 }
 
+// `rows` rows of `width` elements, `stride` from one to the next.
+struct Rows {
+  const void *ptr;
+  int64_t rows, width, stride;
+};
+
+// Whether two tensors of one type share an element: exact for equal strides and where one has no gaps;
+// otherwise (two with gaps of different sizes) not looked into.
+bool overlap(const Rows &a, const Rows &b, size_t size) {
+  if (!a.ptr || !b.ptr || a.rows == 0 || b.rows == 0) return false;
+  const int64_t pa = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.ptr) / size),
+                pb = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.ptr) / size);
+  const int64_t end_a = pa + (a.rows - 1) * a.stride + a.width, end_b = pb + (b.rows - 1) * b.stride + b.width;
+  if (pa >= end_b || pb >= end_a) return false;
+  auto has_gaps = [](const Rows &r) { return r.rows > 1 && r.stride != r.width; };
+  // a row of r that reaches past `from` and begins before `to`
+  auto row_between = [](const Rows &r, int64_t p, int64_t from, int64_t to) {
+    const int64_t before = from - p - r.width;  // rows that begin at p + k stride <= p + before end at or before `from`
+    const int64_t first = before < 0 ? 0 : before / r.stride + 1;
+    return first < r.rows && p + first * r.stride < to;
+  };
+  if (!has_gaps(a)) return row_between(b, pb, pa, end_a);
+  if (!has_gaps(b)) return row_between(a, pa, pb, end_b);
+  if (a.stride != b.stride) return false;
+  // rows k of a and k - q, k - q - 1 of b are neighbours
+  int64_t q = (pb - pa) / a.stride, column = (pb - pa) % a.stride;
+  if (column < 0) column += a.stride, --q;
+  auto meet = [&](int64_t shift) { return shift < a.rows && shift + b.rows > 0; };
+  return (column < a.width && meet(q)) || (column + b.width > a.stride && meet(q + 1));
+}
+
+// Blocks write `out` while others read: it may overlap no input, but be the same rows as one of `same`.
+template <int M, int N>
+af2_status check_out(af2_ctx *ctx, const Rows &out, const Rows (&same)[M], const Rows (&inputs)[N], int dtype) {
+  const size_t size = element_bytes(dtype);
+  for (const Rows &in : inputs)
+    if (overlap(out, in, size)) return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "out overlaps an input");
+  for (const Rows &in : same)
+    if (overlap(out, in, size) && !(out.ptr == in.ptr && (out.stride == in.stride || out.rows == 1)))
+      return fail(ctx, AF2_ERR_INVALID_ARGUMENT, "out overlaps an input without being it");
+  return AF2_OK;
+}
+
 struct Strides {
   int activation = AF2_ACTIVATION_NONE;
   int64_t x = 0, residual = 0, out = 0, d_x = 0;
@@ -323,6 +366,10 @@ af2_status af2_dense(af2_ctx *ctx, const af2_linear_shape *shape, int dtype, con
     if ((st = check_block(ctx, saved, "saved")) != AF2_OK || (st = check_block(ctx, workspace, "workspace")) != AF2_OK)
       return st;
     if (!some) return AF2_OK;
+    const int64_t rows = shape->rows, in = shape->inner, columns = shape->columns;
+    const Rows same[] = {{residual, rows, columns, s.residual}};
+    const Rows inputs[] = {{x, rows, in, s.x}, {weight, in, columns, columns}, {bias, 1, columns, columns}};
+    if ((st = check_out(ctx, {out, rows, columns, s.out}, same, inputs, dtype)) != AF2_OK) return st;
     cudaSetDevice(ctx->device);
     const DenseForward p{shape->rows, shape->inner, shape->columns, dtype, s.activation, x,   weight,
                          bias,        residual,     s.x,            s.residual, s.out,  out, saved};
@@ -430,6 +477,16 @@ af2_status af2_gated_transition(af2_ctx *ctx, const af2_transition_shape *shape,
     if ((st = check_block(ctx, saved, "saved")) != AF2_OK || (st = check_block(ctx, workspace, "workspace")) != AF2_OK)
       return st;
     if (!some) return AF2_OK;
+    const int64_t rows = shape->rows, c = shape->channels, h = shape->hidden_channels;
+    // (x is read into the hidden activations before the same rows of out are written, whichever kernel runs)
+    const Rows same[] = {{residual, rows, c, s.residual}, {x, rows, c, s.x}};
+    const Rows inputs[] = {{weights->gate_weight, c, h, h},
+                           {weights->gate_bias, 1, h, h},
+                           {weights->value_weight, c, h, h},
+                           {weights->value_bias, 1, h, h},
+                           {weights->output_weight, h, c, c},
+                           {weights->output_bias, 1, c, c}};
+    if ((st = check_out(ctx, {out, rows, c, s.out}, same, inputs, dtype)) != AF2_OK) return st;
     cudaSetDevice(ctx->device);
     const GatedForward p{shape->rows, shape->channels, shape->hidden_channels, dtype, s.activation, x,
                          residual,    *weights,        s.x,                    s.residual, s.out,   out, saved};

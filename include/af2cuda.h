@@ -650,7 +650,8 @@ AF2_API af2_status af2_linear(af2_ctx *ctx, const af2_linear_shape *shape, const
  *
  * rows = 0 is valid: outputs of no rows are not touched, and the gradients of
  * the weights are zero.  Outputs must not overlap inputs, except that out may
- * be the residual itself.
+ * be the residual itself, and af2_gated_transition's x itself (an `out` that
+ * overlaps otherwise is refused).
  */
 typedef struct af2_layer_options {
     int32_t activation; /* af2_activation; of the gate in af2_gated_transition */

@@ -480,3 +480,44 @@ def test_slopes_at_both_ends(device, rows, width, act, low, high, dtype):
     allowed = scale * allowed + (2.0**-25 if dtype == F16 else 0.0)
     err = (got.double() - scale * slope).abs()
     assert bool((err <= allowed).all()), (err / allowed).max().item()
+
+
+def test_outputs_that_overlap_inputs_are_refused(device):
+    """Blocks write an output while others read: in place works where each row is read before it is written."""
+    dense, gated = af2cuda.encode_dense_tensors, af2cuda.encode_gated_transition_tensors
+    flat = torch.randn(4000, device="cuda").to(BF16)
+    x, w = flat[:1600].view(100, 16), torch.randn(16, 16, device="cuda").to(BF16)
+    for bad in (x, flat[1500:3100].view(100, 16), flat[1:1601].view(100, 16)):
+        with pytest.raises(af2cuda.RangeError, match="out overlaps"):
+            dense(device, x, w, out=bad)
+    with pytest.raises(af2cuda.RangeError, match="out overlaps"):
+        dense(device, flat[2000:3600].view(100, 16), x[:16], out=x)
+    with pytest.raises(af2cuda.RangeError, match="out overlaps"):
+        dense(device, flat[2000:3600].view(100, 16), w, bias=x[99], out=x)
+    with pytest.raises(af2cuda.RangeError, match="without being it"):
+        dense(device, flat[2000:3600].view(100, 16), w, residual=flat[16:1616].view(100, 16), out=x)
+    # the halves of one buffer's rows, rows between rows, and what only touches
+    both = torch.randn(100, 32, device="cuda").to(BF16)
+    want = ref.dense(both[:, :16], w, None, None, "none")["y"]
+    close("halves", dense(device, both[:, :16], w, out=both[:, 16:]), want, BF16)
+    with pytest.raises(af2cuda.RangeError, match="out overlaps"):
+        dense(device, both[:, :16], w, out=both[:, 15:31])
+    with pytest.raises(af2cuda.RangeError, match="out overlaps"):
+        dense(device, both[:99, 16:], w, out=both[1:, 10:26])
+    close("rows", dense(device, both[::2, :16], w, out=both[1::2, :16]),
+          ref.dense(both[::2, :16], w, None, None, "none")["y"], BF16)
+    close("next to it", dense(device, x, w, out=flat[1600:3200].view(100, 16)),
+          ref.dense(x, w, None, None, "none")["y"], BF16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,channels,hidden", [(3, 64, 128), (700, 64, 128), (20000, 128, 512), (700, 200, 264),
+                                                  (700, 77, 130)])
+def test_gated_transition_in_place(device, rows, channels, hidden, dtype):
+    s = gated_case(rows, channels, hidden, dtype, seed=1360)
+    want = ref.gated(s["x"], s["weights"], s["x"], "silu")["y"]
+    alone = af2cuda.encode_gated_transition_tensors(device, s["x"], s["weights"], residual=s["x"])
+    x = s["x"].clone()
+    af2cuda.encode_gated_transition_tensors(device, x, s["weights"], residual=x, out=x)
+    close("y", x, want, dtype)
+    assert torch.equal(x, alone)
