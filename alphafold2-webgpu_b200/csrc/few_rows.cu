@@ -9,7 +9,7 @@
 // of blocks shares the depth and adds up through distributed shared memory, in
 // rank order.  The launch that follows another (the transition's second
 // product) reads its first weights before it waits for the one before it.  One row of
-// that transition: 11.1 us for both launches; 1024 -> 1024 alone 3.8.
+// that transition: 11.1 us for both launches; 1024 -> 1024 alone 4.8, with the call.
 #include <algorithm>
 #include <type_traits>
 

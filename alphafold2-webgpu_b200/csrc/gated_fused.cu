@@ -15,9 +15,9 @@
 // each the multi-function unit would take 768 clocks too, so every second pair's
 // exponentials run on the FMA pipe (512 and that).  (silu as z / 2 (1 + tanh(z / 2)),
 // one instruction of that unit a value, took 95 us below, but tanh.approx's 2^-11
-// is 1 % of silu at z = -4 and 10 % at -6.)
-// 262144 rows of 128 -> 512 -> 128 in bf16: 109 us alone, 62 of them at cuBLAS's
-// rate for the products (104 repeated, f16 108).
+// is up to 1 % of silu at z = -4 and 10 % at -6.)
+// 262144 rows of 128 -> 512 -> 128 in bf16: 98 to 109 us in a burst, 62 of them at
+// cuBLAS's rate for the products (103 to 121 repeated, as the power cap has it).
 #include <algorithm>
 #include <type_traits>
 

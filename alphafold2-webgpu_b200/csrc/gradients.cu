@@ -7,10 +7,11 @@
 // takes a contiguous range of them: it sums their squares, the grid meets, every
 // block adds all blocks' sums in the same order (no atomics: the result depends
 // on the sizes alone) and scales its own chunks, the last read first, because
-// those are still in L2.  What bounds it is memory: a set is read once for the
-// norm, and again, as far as it has left the 126 MB of L2, for the scaling: 201 MB
-// of bf16 scaled in 101 us, 6 TB/s of the 604 MB moved; the norm of 0.8 MB 4.7 us,
-// a launch and the grid's meeting.
+// those are still in L2.  A set is read once for the norm, and again, as far as it
+// has left the 126 MB of L2, for the scaling: 201 MB of bf16 take 107 us, 93 in a
+// launch alone, whose 452 MB of DRAM traffic are 59 % of that memory's rate (69 us),
+// so that memory is not all that bounds it; the norm of 0.8 MB 6.2 us, a launch and
+// the grid's meeting.
 //
 // Squares are summed in f64.  Eight elements at a time are first summed in f32,
 // whose rounding (2^-24 of the eight) is far below f32's own once the sums of
