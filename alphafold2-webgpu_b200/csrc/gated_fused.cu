@@ -393,7 +393,11 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
         break;
       }
       tc_fence_after();
-      if (res && !warp_wait(load(ow), loads++ & 1, abort_flag, p.err, kErrWaitEpilogue)) break;
+      if (res && !warp_wait(load(ow), loads & 1, abort_flag, p.err, kErrWaitEpilogue)) {
+        if (lane == 0) mbar_wait_drain(load(ow), loads & 1, p.err);
+        break;
+      }
+      loads += res;
       // the next tile's second products wait for this read: all blocks first, then the stores
       const uint32_t d2 = tmem + (static_cast<uint32_t>(q * 32) << 16) + COL_D2 + col0;
       uint32_t v[2][16];

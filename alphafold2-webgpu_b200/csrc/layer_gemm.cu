@@ -704,9 +704,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           uint32_t v[32];
           tmem_ld32(taddr + b * 32, v);
           const uint32_t scales = p.saved_scale[(c0 >> 5) * p.scale_rows + m];
-          ok = warp_wait(load(ew, 0), loads++ & 1, abort_flag, launch.err, kErrWaitEpilogue);
+          ok = warp_wait(load(ew, 0), loads & 1, abort_flag, launch.err, kErrWaitEpilogue);
           tmem_ld_wait();
-          if (!ok) break;
+          if (!ok) {
+            if (lane == 0) mbar_wait_drain(load(ew, 0), loads & 1, launch.err);
+            break;
+          }
+          ++loads;
 #pragma unroll
           for (int plane = 0; plane < 2; ++plane) {
             float d[32];
