@@ -2,7 +2,7 @@
 // libaf2cuda.so's C ABI: argument checks, outputs and the stream, in C++
 // because a step has hundreds of tensors and its smallest calls take less time
 // on the GPU than an interpreted check of their arguments (a dense layer of one
-// row: 4.8 us there, 11 us in Python; clipping 384 tensors: 27 and 394 us).
+// row: 4.8 us there, 11 us in Python; clipping 384 tensors: 25 and 394 us).
 //
 // The module links nothing of the library: bind() takes the entry points'
 // addresses, so that one loaded libaf2cuda.so serves all of the package.
