@@ -11,13 +11,15 @@
 // for each, read as they are stored (MN-major).
 //
 // What bounds it.  Per chunk and SM the tensor core takes 768 clocks (512 + 256)
-// and the activations 8192 values: with one exponential and half a reciprocal
-// each the multi-function unit would take 768 clocks too, so every second pair's
-// exponentials run on the FMA pipe (512 and that).  (silu as z / 2 (1 + tanh(z / 2)),
-// one instruction of that unit a value, took 95 us below, but tanh.approx's 2^-11
-// is up to 1 % of silu at z = -4 and 10 % at -6.)
-// 262144 rows of 128 -> 512 -> 128 in bf16: 98 to 109 us in a burst, 62 of them at
-// cuBLAS's rate for the products (103 to 121 repeated, as the power cap has it).
+// and the activations 8192 values: with one exponential and half a reciprocal each
+// the multi-function unit takes 768 clocks too, beside it; neither is full (tensor
+// 49 %, that unit 51 %, issue slots 59 % on 75776 rows), and what the gate warps wait
+// for most is their accumulator.  (Every second pair's
+// exponentials as a polynomial on the FMA pipe: 119 us where this takes 114, every
+// fourth 115.  silu as z / 2 (1 + tanh(z / 2)), one instruction of that unit a value:
+// 110, but tanh.approx's 2^-11 is up to 1 % of silu at z = -4 and 10 % at -6.)
+// 262144 rows of 128 -> 512 -> 128 in bf16: 94 us in a burst, 62 of them at cuBLAS's
+// rate for the products (98 to 114 repeated, as the power cap has it; f16 102).
 #include <algorithm>
 #include <type_traits>
 
@@ -60,27 +62,6 @@ struct Args {
   int channels, hidden, chunks, tiles, activation, has_residual;
   unsigned int *err;
 };
-
-// 2^x for x in [-126, 63] without the multi-function unit: x = n + f, |f| <= 1/2, 2^f by the
-// polynomial of degree 4 with the least largest relative error there (2.6e-6), n added to its exponent.
-__device__ __forceinline__ float2 ex2_poly2(float2 x) {
-  const float2 magic = f2(12582912.f);  // 1.5 * 2^23: the sum's low bits are the rounded integer
-  const float2 t = f2add(x, magic);
-  const float2 f = f2fma(f2add(t, f2(-12582912.f)), f2(-1.f), x);
-  float2 p = f2fma(f2(0.009570102207362652f), f, f2(0.05591786280274391f));
-  p = f2fma(p, f, f2(0.240247443318367f));
-  p = f2fma(p, f, f2(0.6931217908859253f));
-  p = f2fma(p, f, f2(0.9999992847442627f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
-
-// silu of two values, sigmoid2_fast with the exponential on the FMA pipe
-__device__ __forceinline__ float2 silu2_poly(float2 z) {
-  const float2 x = f2mul(z, f2(-1.4426950408889634f));
-  const float2 e = ex2_poly2(make_float2(fmaxf(fminf(x.x, 63.f), -126.f), fmaxf(fminf(x.y, 63.f), -126.f)));
-  return f2mul(z, shared_reciprocal(f2add(e, f2(1.f))));
-}
 
 // The chunks of a CTA's tiles in order; a tile starts at chunk (tile mod chunks), so that the CTAs do
 // not all read the same weights at once.
@@ -342,12 +323,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_fused_kernel(const __grid_co
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float2 a;
-            if constexpr (ACT == AF2_ACTIVATION_SILU)
-              a = i ? silu2_poly(gz[i]) : activate2<ACT, true>(gz[i]);
-            else
-              a = activate2<ACT, true>(gz[i]);
-            a = f2mul(a, vz[i]);
+            const float2 a = f2mul(activate2<ACT, true>(gz[i]), vz[i]);
             h[2 * i4 + i] = pack2_t<T>(a.x, a.y);
           }
         }
